@@ -447,6 +447,129 @@ int lik_quantize_fp8(const void* x, int32_t dtype, int64_t rows, int32_t dim, ui
                      void* workspace, size_t workspace_bytes, lik_stream_t stream);
 
 /*
+ * Operators of the encoder in front of the projection head. Rows are token
+ * vectors with a contiguous last dimension; strides count elements.
+ */
+
+/*
+ * Layer norm of x [rows, dim], with a residual of sum = round(x + residual)
+ * (sum [rows, dim] is written and is what is normalised; null without one):
+ *   y = (s - mean(s)) / sqrt(var(s) + eps) * weight + bias
+ * dtype bf16 / fp16 / fp32; weight and bias (null: none) in it or in fp32.
+ * y is contiguous. stats (optional) [rows, 2]: mean and 1 / sqrt(var + eps) for the
+ * backward pass. dim <= 8192 (LIK_ERR_UNSUPPORTED above).
+ */
+int lik_layer_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, int32_t dtype,
+                   int64_t rows, int32_t dim, const void* weight, const void* bias, int32_t weight_dtype, float eps,
+                   void* y, void* sum, float* stats, lik_stream_t stream);
+/*
+ * Its gradients: grad_x [rows, dim] (contiguous; of x and of the residual alike)
+ * = the norm's from grad_y, plus grad_sum (null: none); grad_weight and grad_bias
+ * [dim] in weight_dtype (null: not wanted). sum is what was normalised. Sums
+ * over rows are taken in a fixed order.
+ */
+size_t lik_layer_norm_backward_workspace_size(int32_t dtype, int64_t rows, int32_t dim);
+int lik_layer_norm_backward(const void* grad_y, int64_t grad_y_stride, const void* grad_sum, int64_t grad_sum_stride,
+                            const void* sum, int64_t sum_stride, const float* stats, int32_t dtype, int64_t rows,
+                            int32_t dim, const void* weight, int32_t weight_dtype, void* grad_x, void* grad_weight,
+                            void* grad_bias, void* workspace, size_t workspace_bytes, lik_stream_t stream);
+
+/*
+ * Gated feed-forward block of x [rows, dim]:
+ *   out = (act(x Wg^T) * (x Wu^T)) w_out^T + residual
+ * w_in [2 hidden, dim]: Wg, then Wu; w_out [dim, hidden]; activation 0: gelu
+ * (erf), 1: gelu by tanh, 2: silu; bf16 / fp16. dim and hidden are multiples of 8,
+ * every row starts on 16 bytes. out [rows, dim] and hidden_act [rows, hidden]
+ * (act * up, always written) are contiguous; gate_up (optional) fp32 [rows,
+ * 2 hidden] keeps both projections for the backward pass.
+ */
+int lik_gated_ffn(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int32_t dim, int32_t hidden,
+                  const void* w_in, int64_t w_in_stride, const void* w_out, int64_t w_out_stride, const void* residual,
+                  int64_t residual_stride, int32_t activation, void* out, void* hidden_act, float* gate_up,
+                  lik_stream_t stream);
+/*
+ * Its gradients from grad [rows, dim] and what the forward kept: grad_x [rows, dim],
+ * grad_w_in [2 hidden, dim], grad_w_out [dim, hidden], contiguous, each null if
+ * not wanted (the residual's is grad itself). rows >= 1.
+ */
+size_t lik_gated_ffn_backward_workspace_size(int32_t dtype, int64_t rows, int32_t dim, int32_t hidden);
+int lik_gated_ffn_backward(const void* grad, int64_t grad_stride, const void* x, int64_t x_stride, int32_t dtype,
+                           int64_t rows, int32_t dim, int32_t hidden, const void* w_in, int64_t w_in_stride,
+                           const void* w_out, int64_t w_out_stride, const void* hidden_act, const float* gate_up,
+                           int32_t activation, void* grad_x, void* grad_w_in, void* grad_w_out, void* workspace,
+                           size_t workspace_bytes, lik_stream_t stream);
+
+/*
+ * Attention of heads query heads over kv_heads key / value heads (heads a
+ * multiple of kv_heads; query head h reads key head h / (heads / kv_heads)), bf16 /
+ * fp16, dim a multiple of 8 up to 128, every row on 16 bytes:
+ *   out_i = sum_j softmax_j(scale q_i k_j) v_j over the kept j
+ * padded: row l of sequence i and head h at data + i*stride_n + l*stride_l + h*stride_h,
+ *   masks (optional, up to 2^18 tokens) are int8 keep flags as in lik_seqs_t;
+ * packed: cu_q and cu_k [n + 1], rows [q_rows] and [k_rows]; q_len and k_len
+ *   bound the longest sequence.
+ * Query i keeps key j of its sequence where i - left <= j <= i + right (-1:
+ * unbounded; positions count from the sequence's start) and the masks keep both. A
+ * query that keeps no key gives zeros. scale > 0.
+ */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  int32_t dtype;
+  int32_t heads;
+  int32_t kv_heads;
+  int32_t dim;
+  int64_t n;
+  int64_t q_len;
+  int64_t k_len;
+  int64_t q_stride_n;
+  int64_t q_stride_l;
+  int64_t q_stride_h;
+  int64_t k_stride_n;
+  int64_t k_stride_l;
+  int64_t k_stride_h;
+  int64_t v_stride_n;
+  int64_t v_stride_l;
+  int64_t v_stride_h;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  int64_t q_rows;
+  int64_t k_rows;
+  const int8_t* q_mask;
+  int64_t q_mask_stride_n;
+  int64_t q_mask_stride_l;
+  const int8_t* k_mask;
+  int64_t k_mask_stride_n;
+  int64_t k_mask_stride_l;
+  int32_t left;
+  int32_t right;
+  float scale;
+} lik_attention_t;
+
+/*
+ * out [n, q_len, heads, dim] (packed: [q_rows, heads, dim]), contiguous, in the
+ * inputs' type. lse (optional) fp32 [heads, n * q_len] (packed: [heads, q_rows]): the
+ * rows' softmax statistics for the backward pass (log2 of the sum of 2^(scale
+ * log2(e) q k); +inf for a query that keeps no key). Packed rows that belong to
+ * no sequence are left as they are.
+ */
+size_t lik_attention_workspace_size(const lik_attention_t* a);
+int lik_attention(const lik_attention_t* a, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                  lik_stream_t stream);
+/*
+ * Its gradients from out, lse and grad (out's shape, strides grad_stride_*; dim
+ * contiguous, 16-byte rows): grad_q like out, grad_k and grad_v contiguous
+ * [n, k_len, kv_heads, dim] (packed: [k_rows, kv_heads, dim]); zeros in masked
+ * rows. The probabilities are computed again from lse; sums are taken in a
+ * fixed order.
+ */
+size_t lik_attention_backward_workspace_size(const lik_attention_t* a);
+int lik_attention_backward(const lik_attention_t* a, const void* out, const float* lse, const void* grad,
+                           int64_t grad_stride_n, int64_t grad_stride_l, int64_t grad_stride_h, void* grad_q,
+                           void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes, lik_stream_t stream);
+
+/*
  * Allocation-free scoring. No counterpart in the reference: this entry point
  * is for callers that cannot allocate device memory (code under HIP graph
  * capture, tight serving loops, harnesses that forbid hipMalloc). It scores

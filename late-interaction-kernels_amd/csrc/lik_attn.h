@@ -1,0 +1,193 @@
+// What the attention kernels share: parameters, the sequences and their masks,
+// tiles of rows in LDS.
+//
+//   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i k_j) / sum over the kept j
+// A pair (i, j) of one sequence is kept where both masks keep its rows and
+// i - left <= j <= i + right. A row without a kept key gives o = 0 and no gradient.
+//
+// Every product is a 32 x 32 MFMA whose columns are the rows that a wavefront owns
+// (queries in the forward and the gradient of q, keys in the gradients of k and v)
+// and whose rows are the other side's, streamed through LDS 64 at a time. A lane
+// then holds 16 scores of ONE column: maximum and sum of the softmax are in-lane plus
+// one exchange between the wavefront's halves, and the probabilities, rounded and
+// packed, are the next product's operand as they lie (the accumulator's order of
+// rows only permutes that product's sum, and the transposing LDS reads of the other
+// operand follow the same order).
+#pragma once
+#include "lik_enc.h"
+
+namespace lik {
+namespace enc {
+
+struct AttRows {  // rows of one operand: byte strides
+  const char* data;
+  int64_t sn, sl, sh;
+};
+
+struct AttP {
+  AttRows q, k, v, g;  // g: gradient of the output
+  const int32_t *cu_q, *cu_k;
+  int64_t q_rows, k_rows;  // packed: rows in memory
+  const int8_t *qm, *km;
+  int64_t qm_sn, qm_sl, km_sn, km_sl;
+  int64_t q_len, k_len, q_total;  // q_total: rows of the output per head
+  int n, heads, group, dim;       // group: query heads of one key head
+  int left, right;                // INT32_MAX: unbounded
+  float scale, c;                 // c = scale log2 e
+  char* out;                      // [q_total][heads][dim]
+  float* lse;                     // [heads][q_total]: log2 of the sum of 2^(c q k); +inf where nothing is kept
+  float* delta;                   // [heads][q_total]: sum_d g o
+  char *gq, *gk, *gv;             // contiguous gradients
+  float* gmax;                    // fp16: [kMaxParts] largest |g| of a share of the rows each
+  float* part_o;                  // forward split over keys: [split][q_total][heads][dim] fp32
+  float* part_lse;                // [split][heads][q_total]
+  int splits, tiles;              // q tiles (k tiles) of a sequence
+};
+
+constexpr int kNone = 0x7fffffff;
+
+// A sequence's rows: first row, length.
+struct Span {
+  int64_t row;
+  int len;
+};
+__device__ __forceinline__ Span span_of(const int32_t* cu, int64_t rows, int64_t len, int i) {
+  if (!cu) return {i * len, (int)len};
+  // offsets outside the rows in memory are cut off
+  int64_t a = cu[i], b = cu[i + 1];
+  a = a < 0 ? 0 : a > rows ? rows : a;
+  b = b < a ? a : b > rows ? rows : b;
+  const int64_t l = b - a < len ? b - a : len;
+  return {a, (int)l};
+}
+
+// Keep bits of a mask row (len tokens) into LDS, 32 tokens a word; returns the
+// last kept token + 1 and whether every token before it is kept. All 256 threads.
+struct Kept {
+  int extent;
+  bool holes;
+};
+__device__ __forceinline__ Kept scan_mask(uint32_t* bits, const int8_t* mask, int64_t stride, int len, int* s_kept) {
+  const int tid = threadIdx.x;
+  if (tid < 2) s_kept[tid] = 0;
+  __syncthreads();
+  int last = 0, count = 0;
+  for (int t0 = 0; t0 < len; t0 += 256) {
+    const int t = t0 + tid;
+    const bool on = t < len && mask[t * stride] != 0;
+    const uint64_t b = __ballot(on);
+    if ((tid & 63) == 0) {
+      bits[t >> 5] = (uint32_t)b;
+      bits[(t >> 5) + 1] = (uint32_t)(b >> 32);
+      count += __popcll(b);
+      if (b) last = t + 64 - __clzll(b);
+    }
+  }
+  if ((tid & 63) == 0) {
+    atomicMax(&s_kept[0], last);
+    atomicAdd(&s_kept[1], count);
+  }
+  __syncthreads();
+  return {s_kept[0], s_kept[1] != s_kept[0]};
+}
+// words of keep bits that scan_mask writes for len tokens
+inline uint32_t mask_words(int64_t len) { return (uint32_t)((len + 255) / 256 * 8); }
+constexpr int64_t kMaskMost = 1 << 18;  // tokens whose keep bits fit LDS beside the tiles
+
+// The kernels' sizes by the head dimension: k steps of 16, blocks of 32, bytes of a row in LDS.
+template <int DC>
+struct Dim {
+  static constexpr int KS = DC * 2, DB = DC, PITCH = DC <= 2 ? 128 : 256;
+  static constexpr int SPR = PITCH / 16, TILE = 64 * PITCH, NI = TILE / 1024 / 4;
+};
+
+// 64 rows into LDS by four wavefronts; row r at r * PITCH, chunks swizzled.
+// limit: rows that exist; bits (null: all): keep bits of the rows from row 0 of the tile.
+template <int DC>
+__device__ __forceinline__ void issue_rows(uint32_t lds, const char* base, int64_t ld, int dim, int limit,
+                                           const uint32_t* bits, int wv, int lane) {
+  using D = Dim<DC>;
+  const u32x4 desc = raw_desc(base, 0xffffff00u);
+#pragma unroll
+  for (int i = 0; i < D::NI; ++i) {
+    const int slot = (wv * D::NI + i) * 64 + lane, r = slot / D::SPR, c = (slot % D::SPR) ^ lds_swz(r);
+    bool on = c * 8 < dim && r < limit;
+    if (bits) on = on && ((bits[r >> 5] >> (r & 31)) & 1u);
+    dma16(lds + (wv * D::NI + i) * 1024, on ? (uint32_t)(r * ld + c * 16) : kOob, desc);
+  }
+}
+// MFMA operand of 32 rows from row0, elements 16 ks + 8 (lane / 32) ..
+template <int DC>
+__device__ __forceinline__ u32x4 row_frag(uint32_t lds, int row0, int ks, int lane) {
+  const int r = row0 + (lane & 31);
+  return lds_b128(lds + r * Dim<DC>::PITCH + (((ks * 2 + (lane >> 5)) ^ lds_swz(r)) << 4));
+}
+// The same rows across: lane l has element 32 db + l % 32 of rows
+// row0 + 4 (l / 32) + {0..3, 8..11}, the order in which accumulators hold rows.
+template <int DC>
+__device__ __forceinline__ u32x4 col_frag(uint32_t lds, int row0, int db, int lane) {
+  const int i = lane & 15, col = db * 32 + (lane & 16) + 4 * (i & 3);
+  const int r0 = row0 + 4 * (lane >> 5) + (i >> 2), r1 = r0 + 8;
+  const u32x2 lo = lds_tr(lds + r0 * Dim<DC>::PITCH + (((col >> 3) ^ lds_swz(r0)) << 4) + ((col & 4) << 1));
+  const u32x2 hi = lds_tr(lds + r1 * Dim<DC>::PITCH + (((col >> 3) ^ lds_swz(r1)) << 4) + ((col & 4) << 1));
+  return u32x4{lo[0], lo[1], hi[0], hi[1]};
+}
+// This lane's column operand of a row in memory (null: zeros): elements 16 ks + 8 (lane / 32) ..
+template <int DC>
+__device__ __forceinline__ void load_cols(u32x4* f, const char* row, int dim, int lane) {
+#pragma unroll
+  for (int ks = 0; ks < Dim<DC>::KS; ++ks) {
+    const int e = ks * 16 + 8 * (lane >> 5);
+    f[ks] = row && e < dim ? *(const u32x4*)(row + e * 2) : u32x4{0u, 0u, 0u, 0u};
+  }
+}
+
+// other half's value of x
+__device__ __forceinline__ float swap_half(float x) {
+  const uint32_t b = __float_as_uint(x);
+  const auto s = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  return __uint_as_float((threadIdx.x & 32) ? (uint32_t)s[0] : (uint32_t)s[1]);
+}
+
+// Keep word of the 32 rows [t, t + 32) of a sequence of len rows, shifted so that this
+// lane's accumulator element i has bit 8 (i / 4) + i % 4.
+__device__ __forceinline__ uint32_t lane_word(const uint32_t* bits, int t, int len, int lane) {
+  const int left = len - t;
+  uint32_t w = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
+  if (bits && left > 0) w &= bits[t >> 5];
+  return w >> (4 * (lane >> 5));
+}
+__device__ __forceinline__ constexpr int acc_row(int i) { return 8 * (i / 4) + i % 4; }
+
+// Four consecutive elements of accumulator quads 2 j and 2 j + 1 as 16-bit pairs
+// to eight consecutive ones a lane: half h then holds elements 16 j + 8 h + 0..7.
+__device__ __forceinline__ u32x4 join_halves(uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1) {
+  const auto s0 = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
+  const auto s1 = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
+  return u32x4{(uint32_t)s0[0], (uint32_t)s1[0], (uint32_t)s0[1], (uint32_t)s1[1]};
+}
+// One column's DB x 32 elements times f to its row in memory (dim elements).
+template <int EK, int DC>
+__device__ __forceinline__ void store_cols(char* row, const f32x16* acc, float f, int dim, int lane, bool on) {
+#pragma unroll
+  for (int db = 0; db < DC; ++db)
+#pragma unroll
+    for (int q = 0; q < 4; q += 2) {
+      const f32x16& a = acc[db];
+      const u32x4 o = join_halves(pack2<EK>(a[q * 4] * f, a[q * 4 + 1] * f), pack2<EK>(a[q * 4 + 2] * f, a[q * 4 + 3] * f),
+                                  pack2<EK>(a[q * 4 + 4] * f, a[q * 4 + 5] * f),
+                                  pack2<EK>(a[q * 4 + 6] * f, a[q * 4 + 7] * f));
+      const int e = db * 32 + 8 * q + 8 * (lane >> 5);
+      if (on && e < dim) *(u32x4*)(row + e * 2) = o;
+    }
+}
+
+// 16-byte rows; 64 of them within a lane's 32-bit offset
+inline bool att_rows_ok(const void* d, int64_t sn, int64_t sl, int64_t sh) {
+  return (uintptr_t)d % 16 == 0 && sn % 8 == 0 && sl % 8 == 0 && sh % 8 == 0 && sl >= 0 && sl < (1 << 24);
+}
+// Checks the arguments that both directions share and fills the parameters; false: nothing to do, or rc is an error.
+bool attention_shape(const lik_attention_t* a, AttP& p, int& rc);
+
+}  // namespace enc
+}  // namespace lik

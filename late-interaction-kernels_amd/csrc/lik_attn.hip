@@ -1,0 +1,359 @@
+// Attention, forward. One pass over the keys with the running maximum and sum of
+// the softmax; the layout of the products is described in lik_attn.h.
+#include "lik_attn.h"
+
+namespace lik {
+namespace enc {
+namespace {
+
+// A workgroup of four wavefronts owns 128 QB queries of one head, a wavefront 32 QB
+// of them as MFMA columns, and walks the keys that any of them keeps, 64 at a
+// time, in two LDS buffers: the next tile is loaded while this one is used.
+//   scores  S^T[key][query] = K Q^T   (K rows from LDS, Q in registers)
+//   output  O^T[d][query]  += V^T P^T (V by transposing LDS reads, P as it lies)
+template <int EK, int DC, int QB>
+__global__ void __launch_bounds__(256) attention_kernel(const AttP p) {
+  using D = Dim<DC>;
+  __shared__ __attribute__((aligned(1024))) char s_tile[2][2 * D::TILE];
+  __shared__ int s_kept[2];
+  extern __shared__ uint32_t s_bits[];
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // tiles of one key head's queries follow each other on one XCD: they share its keys in L2
+  uint32_t t = xcd_tile(blockIdx.x, gridDim.x);
+  const int split = (int)(t % (uint32_t)p.splits);
+  t /= (uint32_t)p.splits;
+  const int tile = (int)(t % (uint32_t)p.tiles);
+  t /= (uint32_t)p.tiles;
+  const int head = (int)(t % (uint32_t)p.heads), seq = (int)(t / (uint32_t)p.heads);
+  const int kvh = head / p.group;
+  const Span qs = span_of(p.cu_q, p.q_rows, p.q_len, seq), ks = span_of(p.cu_k, p.k_rows, p.k_len, seq);
+  const int q0 = tile * 128 * QB;
+  if (q0 >= qs.len) return;  // (all threads)
+
+  // the lane's queries: column l32 of each of the wavefront's QB blocks
+  int qpos[QB];
+  bool qon[QB];
+  u32x4 qf[QB][D::KS];
+  const char* qbase = p.q.data + (p.cu_q ? qs.row * p.q.sl : seq * p.q.sn) + head * p.q.sh;
+#pragma unroll
+  for (int b = 0; b < QB; ++b) {
+    qpos[b] = q0 + (wv * QB + b) * 32 + l32;
+    qon[b] = qpos[b] < qs.len && (!p.qm || p.qm[seq * p.qm_sn + qpos[b] * p.qm_sl] != 0);
+    load_cols<DC>(qf[b], qon[b] ? qbase + qpos[b] * p.q.sl : nullptr, p.dim, lane);
+  }
+  bool any = qon[0];
+#pragma unroll
+  for (int b = 1; b < QB; ++b) any |= qon[b];
+  any = __ballot(any) != 0;  // this wavefront has a query
+
+  // keys: the kept extent, then what the window leaves to this workgroup, then this split's share
+  int klen = ks.len;
+  bool holes = false;
+  if (p.km) {
+    const Kept kept = scan_mask(s_bits, p.km + seq * p.km_sn, p.km_sl, klen, s_kept);
+    klen = kept.extent;
+    holes = kept.holes;
+  }
+  const int q_end = (q0 + 128 * QB < qs.len ? q0 + 128 * QB : qs.len) - 1;  // last query of the workgroup
+  int kb = p.left == kNone || q0 - p.left < 0 ? 0 : (q0 - p.left) & ~63;
+  int ke = p.right == kNone || (int64_t)q_end + p.right + 1 >= klen ? klen : q_end + p.right + 1;
+  if (p.splits > 1) {
+    const int tiles = ke > kb ? (ke - kb + 63) / 64 : 0, per = (tiles + p.splits - 1) / p.splits;
+    kb += split * per * 64;
+    ke = kb + per * 64 < ke ? kb + per * 64 : ke;
+  }
+  if (__syncthreads_or(any) == 0) ke = kb;  // no query of this tile is kept
+
+  const char* kbase = p.k.data + (p.cu_k ? ks.row * p.k.sl : seq * p.k.sn) + kvh * p.k.sh;
+  const char* vbase = p.v.data + (p.cu_k ? ks.row * p.v.sl : seq * p.v.sn) + kvh * p.v.sh;
+  const uint32_t lds[2] = {lds_addr(s_tile[0]), lds_addr(s_tile[1])};
+  auto issue = [&](uint32_t at, int kt) {
+    const uint32_t* bits = holes ? s_bits + (kt >> 5) : nullptr;
+    issue_rows<DC>(at, kbase + kt * p.k.sl, p.k.sl, p.dim, klen - kt, bits, wv, lane);
+    issue_rows<DC>(at + D::TILE, vbase + kt * p.v.sl, p.v.sl, p.dim, klen - kt, bits, wv, lane);
+  };
+
+  f32x16 o[QB][DC];
+  float top[QB], sum[QB];
+#pragma unroll
+  for (int b = 0; b < QB; ++b) {
+    top[b] = -INFINITY;
+    sum[b] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DC; ++d) o[b][d] = f32x16{};
+  }
+  const int wq0 = q0 + wv * QB * 32, wq1 = wq0 + QB * 32 - 1;  // the wavefront's queries
+  if (kb < ke) issue(lds[0], kb);
+  int buf = 0;
+  for (int kt = kb; kt < ke; kt += 64, buf ^= 1) {
+    // this tile is complete, and every wavefront is done with the other buffer
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (kt + 64 < ke) issue(buf ? lds[0] : lds[1], kt + 64);
+    if (!any || (p.right != kNone && kt > wq1 + p.right) || (p.left != kNone && kt + 63 < wq0 - p.left)) continue;
+    const uint32_t at = buf ? lds[1] : lds[0];
+    const bool whole = kt + 64 <= klen && !holes && (p.right == kNone || kt + 63 <= wq0 + p.right) &&
+                       (p.left == kNone || kt >= wq1 - p.left);
+    f32x16 s[QB][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int b = 0; b < QB; ++b) s[b][u] = f32x16{};
+#pragma unroll
+      for (int k = 0; k < D::KS; ++k) {
+        const u32x4 kf = row_frag<DC>(at, u * 32, k, lane);
+#pragma unroll
+        for (int b = 0; b < QB; ++b) s[b][u] = mfma16<EK>(s[b][u], kf, qf[b][k]);
+      }
+    }
+    if (!whole) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t w = lane_word(holes ? s_bits : nullptr, kt + u * 32, klen, lane);
+#pragma unroll
+        for (int b = 0; b < QB; ++b) {
+          const int ahead = kt + u * 32 + 4 * (lane >> 5) - qpos[b];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int a = ahead + acc_row(i);
+            const bool on = ((w >> acc_row(i)) & 1u) && a <= p.right && (p.left == kNone || a >= -p.left);
+            s[b][u][i] = on ? s[b][u][i] : -INFINITY;
+          }
+        }
+      }
+    }
+    u32x4 pf[QB][4];
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+      float m = s[b][0][0];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m = fmaxf(m, s[b][u][i]);
+      m = fmaxf(fmaxf(m, swap_half(m)), top[b]);
+      const float mc = m == -INFINITY ? 0.f : m * p.c;
+      const float alpha = exp2f(fmaf(top[b], p.c, -mc));
+      top[b] = m;
+      float add = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float e = exp2f(fmaf(s[b][u][i], p.c, -mc));
+          s[b][u][i] = e;
+          add += e;
+        }
+      sum[b] = fmaf(sum[b], alpha, add);
+#pragma unroll
+      for (int d = 0; d < DC; ++d) o[b][d] *= alpha;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          pf[b][k][e] = pack2<EK>(s[b][k / 2][(k % 2) * 8 + 2 * e], s[b][k / 2][(k % 2) * 8 + 2 * e + 1]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int d = 0; d < DC; ++d) {
+        const u32x4 vf = col_frag<DC>(at + D::TILE, k * 16, d, lane);
+#pragma unroll
+        for (int b = 0; b < QB; ++b) o[b][d] = mfma16<EK>(o[b][d], vf, pf[b][k]);
+      }
+  }
+
+#pragma unroll
+  for (int b = 0; b < QB; ++b) {
+    const float total = sum[b] + swap_half(sum[b]);
+    const bool on = qpos[b] < qs.len, kept = qon[b] && total != 0.f;
+    const float inv = kept ? 1.0f / total : 0.f;
+    const float lse = kept ? fmaf(top[b], p.c, log2f(total)) : INFINITY;
+    const int64_t row = qs.row + qpos[b];
+    if (p.splits > 1) {
+      // this split's mean of the values, and its statistics
+      if (on && lane < 32) p.part_lse[((int64_t)split * p.heads + head) * p.q_total + row] = kept ? lse : -INFINITY;
+      float* at = p.part_o + (((int64_t)split * p.q_total + row) * p.heads + head) * p.dim;
+#pragma unroll
+      for (int d = 0; d < DC; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int e = d * 32 + 8 * q + 4 * (lane >> 5);
+          if (on && e < p.dim)
+            *(f32x4*)(at + e) = f32x4{o[b][d][q * 4] * inv, o[b][d][q * 4 + 1] * inv, o[b][d][q * 4 + 2] * inv,
+                                      o[b][d][q * 4 + 3] * inv};
+        }
+    } else {
+      if (p.lse && on && lane < 32) p.lse[(int64_t)head * p.q_total + row] = lse;
+      if (!kept)
+#pragma unroll
+        for (int d = 0; d < DC; ++d) o[b][d] = f32x16{};
+      store_cols<EK, DC>(p.out + (row * p.heads + head) * p.dim * 2, o[b], inv, p.dim, lane, on);
+    }
+  }
+}
+
+// Joins the splits of a row: sum_s 2^(lse_s - lse) o_s. Four elements a thread.
+template <int EK>
+__global__ void __launch_bounds__(256) attention_join_kernel(const AttP p) {
+  const int per = p.dim / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= p.q_total * p.heads * per) return;
+  const int e = (int)(i % per) * 4;
+  const int64_t rh = i / per, row = rh / p.heads;
+  if (p.cu_q && (row < p.cu_q[0] || row >= p.cu_q[p.n])) return;  // in no sequence
+  const int head = (int)(rh % p.heads);
+  float top = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) top = max_nan(top, p.part_lse[((int64_t)s * p.heads + head) * p.q_total + row]);
+  f32x4 a = {};
+  float total = 0.f;
+  if (top != -INFINITY)
+    for (int s = 0; s < p.splits; ++s) {
+      const float w = exp2f(p.part_lse[((int64_t)s * p.heads + head) * p.q_total + row] - top);
+      total += w;
+      const f32x4 x = *(const f32x4*)(p.part_o + (((int64_t)s * p.q_total + row) * p.heads + head) * p.dim + e);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) a[k] = fmaf(w, x[k], a[k]);
+    }
+  const float inv = top != -INFINITY ? 1.0f / total : 0.f;
+  if (p.lse && e == 0) p.lse[(int64_t)head * p.q_total + row] = top != -INFINITY ? top + log2f(total) : INFINITY;
+  *(u32x2*)(p.out + (rh * p.dim + e) * 2) =
+      u32x2{pack2<EK>(a[0] * inv, a[1] * inv), pack2<EK>(a[2] * inv, a[3] * inv)};
+}
+
+}  // namespace
+
+namespace {
+
+// Splits of the keys: where the tiles of queries do not fill the 256 CUs and the
+// keys are long, down to 256 keys a split.
+int key_splits(const AttP& p, int64_t wgs) {
+  if (p.left != kNone && p.right != kNone) return 1;  // a window is short
+  int64_t s = 512 / (wgs < 1 ? 1 : wgs);
+  const int64_t most = p.k_len / 256;
+  if (s > most) s = most;
+  return s < 2 ? 1 : (int)s;
+}
+void forward_shape(AttP& p) {
+  p.tiles = (int)((p.q_len + 127) / 128);
+  p.splits = key_splits(p, (int64_t)p.n * p.heads * p.tiles);
+}
+size_t forward_ws(const AttP& p) {
+  if (p.splits < 2) return 0;
+  return align256((size_t)p.splits * p.q_total * p.heads * p.dim * 4) +
+         align256((size_t)p.splits * p.q_total * p.heads * 4) + 256;
+}
+
+template <int EK, int DC>
+int launch_forward(const AttP& p, hipStream_t s) {
+  const int64_t grid = (int64_t)p.n * p.heads * p.tiles * p.splits;
+  if (grid > 0x7fffffff) return LIK_ERR_UNSUPPORTED;
+  launch_kernel(attention_kernel<EK, DC, 1>, dim3((unsigned)grid), dim3(256), p.km ? mask_words(p.k_len) * 4 : 0u, s, p);
+  if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
+  if (p.splits > 1) {
+    const int64_t m = p.q_total * p.heads * (p.dim / 4);
+    launch_kernel(attention_join_kernel<EK>, dim3((unsigned)((m + 255) / 256)), dim3(256), 0u, s, p);
+    if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
+  }
+  return LIK_OK;
+}
+
+template <int EK>
+int run_forward(const AttP& p, hipStream_t s) {
+  if (p.dim <= 32) return launch_forward<EK, 1>(p, s);
+  if (p.dim <= 64) return launch_forward<EK, 2>(p, s);
+  if (p.dim <= 96) return launch_forward<EK, 3>(p, s);
+  return launch_forward<EK, 4>(p, s);
+}
+
+}  // namespace
+
+// Checks the arguments that both directions share and fills the parameters;
+// false: nothing to do, or rc is an error.
+bool attention_shape(const lik_attention_t* a, AttP& p, int& rc) {
+  rc = LIK_ERR_INVALID;
+  if (!a || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads || a->dim < 1 || a->n < 0 || a->q_len < 0 ||
+      a->k_len < 0 || !(a->scale > 0.f) || !(a->scale < INFINITY) || !a->cu_q != !a->cu_k || a->left < -1 || a->right < -1)
+    return false;
+  if (a->cu_q && (a->q_mask || a->k_mask || a->q_rows < 0 || a->k_rows < 0)) return false;
+  rc = LIK_ERR_UNSUPPORTED;
+  if ((a->dtype != LIK_BF16 && a->dtype != LIK_F16) || a->dim % 8 || a->dim > 128 || a->q_len > (1 << 30) ||
+      a->k_len > (1 << 30) || a->n > 0x7fffffff)
+    return false;
+  if ((a->k_mask && a->k_len > kMaskMost) || (a->q_mask && a->q_len > kMaskMost)) return false;
+  p.q_total = a->cu_q ? a->q_rows : a->n * a->q_len;
+  rc = LIK_OK;
+  if (a->n == 0 || p.q_total == 0) return false;
+  const bool keys = (a->cu_k ? a->k_rows : a->n * a->k_len) > 0;
+  if (!a->q || (keys && (!a->k || !a->v))) {
+    rc = LIK_ERR_INVALID;
+    return false;
+  }
+  if (!att_rows_ok(a->q, a->q_stride_n, a->q_stride_l, a->q_stride_h) ||
+      !att_rows_ok(a->k, a->k_stride_n, a->k_stride_l, a->k_stride_h) ||
+      !att_rows_ok(a->v, a->v_stride_n, a->v_stride_l, a->v_stride_h)) {
+    rc = LIK_ERR_UNSUPPORTED;
+    return false;
+  }
+  p.q = {(const char*)a->q, a->q_stride_n * 2, a->q_stride_l * 2, a->q_stride_h * 2};
+  p.k = {(const char*)a->k, a->k_stride_n * 2, a->k_stride_l * 2, a->k_stride_h * 2};
+  p.v = {(const char*)a->v, a->v_stride_n * 2, a->v_stride_l * 2, a->v_stride_h * 2};
+  p.cu_q = a->cu_q;
+  p.cu_k = a->cu_k;
+  p.q_rows = a->q_rows;
+  p.k_rows = a->k_rows;
+  p.qm = a->q_mask;
+  p.km = a->k_mask;
+  p.qm_sn = a->q_mask_stride_n;
+  p.qm_sl = a->q_mask_stride_l;
+  p.km_sn = a->k_mask_stride_n;
+  p.km_sl = a->k_mask_stride_l;
+  p.q_len = a->q_len;
+  p.k_len = a->k_len;
+  p.n = (int)a->n;
+  p.heads = a->heads;
+  p.group = a->heads / a->kv_heads;
+  p.dim = a->dim;
+  p.left = a->left < 0 || a->left >= (1 << 30) ? kNone : a->left;
+  p.right = a->right < 0 || a->right >= (1 << 30) ? kNone : a->right;
+  p.scale = a->scale;
+  p.c = a->scale * 1.4426950408889634f;
+  return true;
+}
+
+}  // namespace enc
+}  // namespace lik
+
+using namespace lik;
+using namespace lik::enc;
+
+extern "C" {
+
+size_t lik_attention_workspace_size(const lik_attention_t* a) {
+  AttP p{};
+  int rc;
+  if (!attention_shape(a, p, rc)) return 0;
+  forward_shape(p);
+  return forward_ws(p);
+}
+
+int lik_attention(const lik_attention_t* a, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                  lik_stream_t stream) {
+  AttP p{};
+  int rc;
+  if (!attention_shape(a, p, rc)) return rc;
+  if (!out) return LIK_ERR_INVALID;
+  if ((uintptr_t)out % 16) return LIK_ERR_UNSUPPORTED;
+  forward_shape(p);
+  if (p.splits > 1) {
+    if (!workspace || workspace_bytes < forward_ws(p)) return LIK_ERR_WORKSPACE;
+    char* ws = align256(workspace);
+    p.part_o = (float*)ws;
+    p.part_lse = (float*)(ws + align256((size_t)p.splits * p.q_total * p.heads * p.dim * 4));
+  }
+  p.out = (char*)out;
+  p.lse = lse;
+  return a->dtype == LIK_BF16 ? run_forward<EK_BF16>(p, (hipStream_t)stream)
+                              : run_forward<EK_F16>(p, (hipStream_t)stream);
+}
+
+}  // extern "C"

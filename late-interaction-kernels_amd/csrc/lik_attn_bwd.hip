@@ -1,0 +1,462 @@
+// Attention, backward. With p from the scores and the kept statistics,
+//   dv_j = sum_i p_ij g_i,  ds_ij = p_ij (g_i v_j - delta_i),  delta_i = sum_d g_i o_i
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i
+// Two kernels, each with the sums of its own rows in registers: one walks the keys for
+// the gradient of q, one the queries (of every head that shares the key head) for
+// those of k and v. Both compute the scores and g v again: seven products where
+// one kernel with the gradient of q in memory would take five, but no atomics (the
+// same bits every time) and no fp32 gradient of q to clear, add to and convert.
+// p and ds are rounded once to the 16-bit type, as the products' operands have to be.
+// fp16 would lose small gradients there: g is scaled by the power of two that
+// brings its largest element to 1/2 .. 1, and the sums are scaled back.
+#include "lik_attn.h"
+
+namespace lik {
+namespace enc {
+namespace {
+
+constexpr int kMaxParts = 256;
+
+// delta, and for fp16 the largest |g| of this workgroup's rows. 16 lanes a row.
+template <int EK>
+__global__ void __launch_bounds__(256) attention_delta_kernel(const AttP p) {
+  const int lane = threadIdx.x & 15;
+  const int64_t items = p.q_total * p.heads;
+  float big = 0.f;
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4; i < items; i += (int64_t)gridDim.x * 16) {
+    const int64_t row = i / p.heads;
+    const int head = (int)(i % p.heads);
+    const int64_t seq = p.cu_q ? 0 : row / p.q_len, pos = p.cu_q ? row : row % p.q_len;
+    float d = 0.f;
+    if (lane * 8 < p.dim && (!p.qm || p.qm[seq * p.qm_sn + pos * p.qm_sl] != 0)) {
+      const u32x4 g = *(const u32x4*)(p.g.data + seq * p.g.sn + pos * p.g.sl + head * p.g.sh + lane * 16);
+      const u32x4 o = *(const u32x4*)(p.out + i * p.dim * 2 + lane * 16);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float a, b, x, y;
+        unpack2<EK>(g[k], a, b);
+        unpack2<EK>(o[k], x, y);
+        d = fmaf(a, x, d);
+        d = fmaf(b, y, d);
+        if constexpr (EK == EK_F16) big = fmaxf(big, fmaxf(fabsf(a), fabsf(b)));
+      }
+    }
+#pragma unroll
+    for (int s = 1; s < 16; s <<= 1) d += __shfl_xor(d, s);
+    if (lane == 0) p.delta[(int64_t)head * p.q_total + row] = d;
+  }
+  if constexpr (EK == EK_F16) {
+    __shared__ float s_big[4];
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) big = fmaxf(big, __shfl_xor(big, s));
+    if ((threadIdx.x & 63) == 0) s_big[threadIdx.x >> 6] = big;
+    __syncthreads();
+    if (threadIdx.x == 0) p.gmax[blockIdx.x] = fmaxf(fmaxf(s_big[0], s_big[1]), fmaxf(s_big[2], s_big[3]));
+  }
+}
+
+// The power of two that scales ds (fp16); s_big: 4 floats of LDS. All threads.
+template <int EK>
+__device__ __forceinline__ float grad_scale(const AttP& p, int parts, float* s_big) {
+  if constexpr (EK != EK_F16) return 1.0f;
+  float big = (int)threadIdx.x < parts ? p.gmax[threadIdx.x] : 0.f;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) big = fmaxf(big, __shfl_xor(big, s));
+  if ((threadIdx.x & 63) == 0) s_big[threadIdx.x >> 6] = big;
+  __syncthreads();
+  big = fmaxf(fmaxf(s_big[0], s_big[1]), fmaxf(s_big[2], s_big[3]));
+  if (!(big > 0.f) || !(big < INFINITY)) return 1.0f;
+  int e;
+  frexpf(big, &e);  // big = m 2^e, m in 1/2 .. 1
+  return ldexpf(1.0f, -e);
+}
+
+// Gradient of q: the forward's walk over the keys (K rows also by transposing
+// reads, V rows in LDS), dq^T[d][query] += K^T ds^T.
+template <int EK, int DC, int QB>
+__global__ void __launch_bounds__(256) attention_dq_kernel(const AttP p, int parts) {
+  using D = Dim<DC>;
+  __shared__ __attribute__((aligned(1024))) char s_tile[2][2 * D::TILE];
+  __shared__ int s_kept[2];
+  __shared__ float s_big[4];
+  extern __shared__ uint32_t s_bits[];
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  uint32_t t = xcd_tile(blockIdx.x, gridDim.x);
+  const int tile = (int)(t % (uint32_t)p.tiles);
+  t /= (uint32_t)p.tiles;
+  const int head = (int)(t % (uint32_t)p.heads), seq = (int)(t / (uint32_t)p.heads);
+  const int kvh = head / p.group;
+  const Span qs = span_of(p.cu_q, p.q_rows, p.q_len, seq), ks = span_of(p.cu_k, p.k_rows, p.k_len, seq);
+  const int q0 = tile * 128 * QB;
+  if (q0 >= qs.len) return;
+  const float gs = grad_scale<EK>(p, parts, s_big);
+
+  int qpos[QB];
+  float lse[QB], delta[QB];
+  u32x4 qf[QB][D::KS], gf[QB][D::KS];
+  const char* qbase = p.q.data + (p.cu_q ? qs.row * p.q.sl : seq * p.q.sn) + head * p.q.sh;
+  const char* gbase = p.g.data + (p.cu_q ? qs.row * p.g.sl : seq * p.g.sn) + head * p.g.sh;
+  bool any = false;
+#pragma unroll
+  for (int b = 0; b < QB; ++b) {
+    qpos[b] = q0 + (wv * QB + b) * 32 + l32;
+    const int64_t at = (int64_t)head * p.q_total + qs.row + qpos[b];
+    lse[b] = qpos[b] < qs.len ? p.lse[at] : INFINITY;
+    const bool on = lse[b] != INFINITY;  // +inf: past the end, masked, or without a key
+    delta[b] = on ? p.delta[at] : 0.f;
+    load_cols<DC>(qf[b], on ? qbase + qpos[b] * p.q.sl : nullptr, p.dim, lane);
+    load_cols<DC>(gf[b], on ? gbase + qpos[b] * p.g.sl : nullptr, p.dim, lane);
+    any |= on;
+  }
+  any = __ballot(any) != 0;
+
+  int klen = ks.len;
+  bool holes = false;
+  if (p.km) {
+    const Kept kept = scan_mask(s_bits, p.km + seq * p.km_sn, p.km_sl, klen, s_kept);
+    klen = kept.extent;
+    holes = kept.holes;
+  }
+  const int q_end = (q0 + 128 * QB < qs.len ? q0 + 128 * QB : qs.len) - 1;
+  const int kb = p.left == kNone || q0 - p.left < 0 ? 0 : (q0 - p.left) & ~63;
+  int ke = p.right == kNone || (int64_t)q_end + p.right + 1 >= klen ? klen : q_end + p.right + 1;
+  if (__syncthreads_or(any) == 0) ke = kb;
+
+  const char* kbase = p.k.data + (p.cu_k ? ks.row * p.k.sl : seq * p.k.sn) + kvh * p.k.sh;
+  const char* vbase = p.v.data + (p.cu_k ? ks.row * p.v.sl : seq * p.v.sn) + kvh * p.v.sh;
+  const uint32_t lds[2] = {lds_addr(s_tile[0]), lds_addr(s_tile[1])};
+  auto issue = [&](uint32_t at, int kt) {
+    const uint32_t* bits = holes ? s_bits + (kt >> 5) : nullptr;
+    issue_rows<DC>(at, kbase + kt * p.k.sl, p.k.sl, p.dim, klen - kt, bits, wv, lane);
+    issue_rows<DC>(at + D::TILE, vbase + kt * p.v.sl, p.v.sl, p.dim, klen - kt, bits, wv, lane);
+  };
+
+  f32x16 acc[QB][DC];
+#pragma unroll
+  for (int b = 0; b < QB; ++b)
+#pragma unroll
+    for (int d = 0; d < DC; ++d) acc[b][d] = f32x16{};
+  const int wq0 = q0 + wv * QB * 32, wq1 = wq0 + QB * 32 - 1;
+  if (kb < ke) issue(lds[0], kb);
+  int buf = 0;
+  for (int kt = kb; kt < ke; kt += 64, buf ^= 1) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (kt + 64 < ke) issue(buf ? lds[0] : lds[1], kt + 64);
+    if (!any || (p.right != kNone && kt > wq1 + p.right) || (p.left != kNone && kt + 63 < wq0 - p.left)) continue;
+    const uint32_t at = buf ? lds[1] : lds[0];
+    const bool whole = kt + 64 <= klen && !holes && (p.right == kNone || kt + 63 <= wq0 + p.right) &&
+                       (p.left == kNone || kt >= wq1 - p.left);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      f32x16 s[QB], dp[QB];
+#pragma unroll
+      for (int b = 0; b < QB; ++b) s[b] = dp[b] = f32x16{};
+#pragma unroll
+      for (int k = 0; k < D::KS; ++k) {
+        const u32x4 kf = row_frag<DC>(at, u * 32, k, lane);
+        const u32x4 vf = row_frag<DC>(at + D::TILE, u * 32, k, lane);
+#pragma unroll
+        for (int b = 0; b < QB; ++b) {
+          s[b] = mfma16<EK>(s[b], kf, qf[b][k]);
+          dp[b] = mfma16<EK>(dp[b], vf, gf[b][k]);
+        }
+      }
+      if (!whole) {
+        const uint32_t w = lane_word(holes ? s_bits : nullptr, kt + u * 32, klen, lane);
+#pragma unroll
+        for (int b = 0; b < QB; ++b) {
+          const int ahead = kt + u * 32 + 4 * (lane >> 5) - qpos[b];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int a = ahead + acc_row(i);
+            const bool on = ((w >> acc_row(i)) & 1u) && a <= p.right && (p.left == kNone || a >= -p.left);
+            s[b][i] = on ? s[b][i] : -INFINITY;
+          }
+        }
+      }
+      u32x4 df[QB][2];
+#pragma unroll
+      for (int b = 0; b < QB; ++b) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float e = exp2f(fmaf(s[b][i], p.c, -lse[b]));
+          s[b][i] = e * (EK == EK_F16 ? (dp[b][i] - delta[b]) * gs : dp[b][i] - delta[b]);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) df[b][k][e] = pack2<EK>(s[b][k * 8 + 2 * e], s[b][k * 8 + 2 * e + 1]);
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int d = 0; d < DC; ++d) {
+          const u32x4 kf = col_frag<DC>(at, u * 32 + k * 16, d, lane);
+#pragma unroll
+          for (int b = 0; b < QB; ++b) acc[b][d] = mfma16<EK>(acc[b][d], kf, df[b][k]);
+        }
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < QB; ++b)
+    store_cols<EK, DC>(p.gq + ((qs.row + qpos[b]) * p.heads + head) * p.dim * 2, acc[b], p.scale / gs, p.dim, lane,
+                       qpos[b] < qs.len);
+}
+
+// Gradients of k and v: a wavefront owns 32 KB keys as MFMA columns, K and V in
+// registers, and walks the queries of the group's heads, 64 at a time.
+//   P[query][key] from S = Q K^T;  dv^T[d][key] += G^T P;  dp = G V^T;  dk^T[d][key] += Q^T ds
+template <int EK, int DC, int KB>
+__global__ void __launch_bounds__(256) attention_dkv_kernel(const AttP p, int parts) {
+  using D = Dim<DC>;
+  __shared__ __attribute__((aligned(1024))) char s_tile[2][2 * D::TILE];
+  __shared__ __attribute__((aligned(16))) float s_stat[2][2][64];
+  __shared__ int s_kept[2];
+  __shared__ float s_big[4];
+  extern __shared__ uint32_t s_bits[];
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  uint32_t t = xcd_tile(blockIdx.x, gridDim.x);
+  const int tile = (int)(t % (uint32_t)p.tiles);
+  t /= (uint32_t)p.tiles;
+  const int kv_heads = p.heads / p.group;
+  const int kvh = (int)(t % (uint32_t)kv_heads), seq = (int)(t / (uint32_t)kv_heads);
+  const Span qs = span_of(p.cu_q, p.q_rows, p.q_len, seq), ks = span_of(p.cu_k, p.k_rows, p.k_len, seq);
+  const int k0 = tile * 128 * KB;
+  if (k0 >= ks.len) return;
+  const float gs = grad_scale<EK>(p, parts, s_big);
+
+  int kpos[KB];
+  bool kon[KB];
+  u32x4 kf[KB][D::KS], vf[KB][D::KS];
+  const char* kbase = p.k.data + (p.cu_k ? ks.row * p.k.sl : seq * p.k.sn) + kvh * p.k.sh;
+  const char* vbase = p.v.data + (p.cu_k ? ks.row * p.v.sl : seq * p.v.sn) + kvh * p.v.sh;
+  bool any = false;
+#pragma unroll
+  for (int b = 0; b < KB; ++b) {
+    kpos[b] = k0 + (wv * KB + b) * 32 + l32;
+    kon[b] = kpos[b] < ks.len && (!p.km || p.km[seq * p.km_sn + kpos[b] * p.km_sl] != 0);
+    load_cols<DC>(kf[b], kon[b] ? kbase + kpos[b] * p.k.sl : nullptr, p.dim, lane);
+    load_cols<DC>(vf[b], kon[b] ? vbase + kpos[b] * p.v.sl : nullptr, p.dim, lane);
+    any |= kon[b];
+  }
+  any = __ballot(any) != 0;
+
+  int qlen = qs.len;
+  bool holes = false;
+  if (p.qm) {
+    const Kept kept = scan_mask(s_bits, p.qm + seq * p.qm_sn, p.qm_sl, qlen, s_kept);
+    qlen = kept.extent;
+    holes = kept.holes;
+  }
+  // queries that keep one of these keys: key - right <= query <= key + left
+  const int k_end = (k0 + 128 * KB < ks.len ? k0 + 128 * KB : ks.len) - 1;
+  const int qb = p.right == kNone || k0 - p.right < 0 ? 0 : (k0 - p.right) & ~63;
+  int qe = p.left == kNone || (int64_t)k_end + p.left + 1 >= qlen ? qlen : k_end + p.left + 1;
+  if (__syncthreads_or(any) == 0) qe = qb;
+  const int steps = qe > qb ? (qe - qb + 63) / 64 : 0;  // of one head
+
+  const uint32_t lds[2] = {lds_addr(s_tile[0]), lds_addr(s_tile[1])};
+  const char* q0 = p.q.data + (p.cu_q ? qs.row * p.q.sl : seq * p.q.sn);
+  const char* g0 = p.g.data + (p.cu_q ? qs.row * p.g.sl : seq * p.g.sn);
+  auto issue = [&](uint32_t at, int head, int qt) {
+    const uint32_t* bits = holes ? s_bits + (qt >> 5) : nullptr;
+    issue_rows<DC>(at, q0 + head * p.q.sh + qt * p.q.sl, p.q.sl, p.dim, qlen - qt, bits, wv, lane);
+    issue_rows<DC>(at + D::TILE, g0 + head * p.g.sh + qt * p.g.sl, p.g.sl, p.dim, qlen - qt, bits, wv, lane);
+  };
+  // threads 0..63: a query's statistic (+inf past the end: p = 0), 64..127: its delta
+  auto stat = [&](int head, int qt) {
+    float x = 0.f;
+    if (tid < 128) {
+      const int pos = qt + (tid & 63);
+      const int64_t at = (int64_t)head * p.q_total + qs.row + pos;
+      x = pos < qlen ? (tid < 64 ? p.lse[at] : p.delta[at]) : tid < 64 ? INFINITY : 0.f;
+    }
+    return x;
+  };
+
+  f32x16 dk[KB][DC], dv[KB][DC];
+#pragma unroll
+  for (int b = 0; b < KB; ++b)
+#pragma unroll
+    for (int d = 0; d < DC; ++d) dk[b][d] = dv[b][d] = f32x16{};
+  const int wk0 = k0 + wv * KB * 32, wk1 = wk0 + KB * 32 - 1;  // the wavefront's keys
+  const int total = steps * p.group;
+  int head = kvh * p.group, qt = qb;
+  if (total) {
+    const float x = stat(head, qt);
+    issue(lds[0], head, qt);
+    if (tid < 128) s_stat[0][tid >> 6][tid & 63] = x;
+  }
+  int buf = 0;
+  for (int it = 0; it < total; ++it, buf ^= 1) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const int now = qt;
+    qt += 64;
+    if (qt >= qe) {
+      qt = qb;
+      ++head;
+    }
+    float next = 0.f;
+    if (it + 1 < total) {
+      next = stat(head, qt);
+      issue(buf ? lds[0] : lds[1], head, qt);
+    }
+    const bool skip = !any || (p.left != kNone && now > wk1 + p.left) || (p.right != kNone && now + 63 < wk0 - p.right);
+    if (!skip) {
+      const uint32_t at = buf ? lds[1] : lds[0];
+      const bool whole =
+          (p.left == kNone || now + 63 <= wk0 + p.left) && (p.right == kNone || now >= wk1 - p.right);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        f32x16 s[KB], dp[KB];
+#pragma unroll
+        for (int b = 0; b < KB; ++b) s[b] = dp[b] = f32x16{};
+#pragma unroll
+        for (int k = 0; k < D::KS; ++k) {
+          const u32x4 qf = row_frag<DC>(at, u * 32, k, lane);
+          const u32x4 gf = row_frag<DC>(at + D::TILE, u * 32, k, lane);
+#pragma unroll
+          for (int b = 0; b < KB; ++b) {
+            s[b] = mfma16<EK>(s[b], qf, kf[b][k]);
+            dp[b] = mfma16<EK>(dp[b], gf, vf[b][k]);
+          }
+        }
+        if (!whole) {
+#pragma unroll
+          for (int b = 0; b < KB; ++b) {
+            const int ahead = kpos[b] - (now + u * 32 + 4 * (lane >> 5));
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int a = ahead - acc_row(i);
+              const bool on = a <= p.right && (p.left == kNone || a >= -p.left);
+              s[b][i] = on ? s[b][i] : -INFINITY;
+            }
+          }
+        }
+        u32x4 pf[KB][2], df[KB][2];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 ls = *(const f32x4*)&s_stat[buf][0][u * 32 + 8 * q + 4 * (lane >> 5)];
+          const f32x4 dl = *(const f32x4*)&s_stat[buf][1][u * 32 + 8 * q + 4 * (lane >> 5)];
+#pragma unroll
+          for (int b = 0; b < KB; ++b) {
+            float e[4], ds[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              e[i] = exp2f(fmaf(s[b][q * 4 + i], p.c, -ls[i]));
+              const float x = dp[b][q * 4 + i] - dl[i];
+              ds[i] = e[i] * (EK == EK_F16 ? x * gs : x);
+            }
+            pf[b][q / 2][(q % 2) * 2] = pack2<EK>(e[0], e[1]);
+            pf[b][q / 2][(q % 2) * 2 + 1] = pack2<EK>(e[2], e[3]);
+            df[b][q / 2][(q % 2) * 2] = pack2<EK>(ds[0], ds[1]);
+            df[b][q / 2][(q % 2) * 2 + 1] = pack2<EK>(ds[2], ds[3]);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int d = 0; d < DC; ++d) {
+            const u32x4 gc = col_frag<DC>(at + D::TILE, u * 32 + k * 16, d, lane);
+            const u32x4 qc = col_frag<DC>(at, u * 32 + k * 16, d, lane);
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+              dv[b][d] = mfma16<EK>(dv[b][d], gc, pf[b][k]);
+              dk[b][d] = mfma16<EK>(dk[b][d], qc, df[b][k]);
+            }
+          }
+      }
+    }
+    if (it + 1 < total && tid < 128) s_stat[buf ^ 1][tid >> 6][tid & 63] = next;
+  }
+#pragma unroll
+  for (int b = 0; b < KB; ++b) {
+    if (!kon[b])  // masked keys have no gradient (their lanes ran on zero rows)
+#pragma unroll
+      for (int d = 0; d < DC; ++d) dk[b][d] = dv[b][d] = f32x16{};
+    const int64_t at = ((ks.row + kpos[b]) * kv_heads + kvh) * p.dim * 2;
+    store_cols<EK, DC>(p.gk + at, dk[b], p.scale / gs, p.dim, lane, kpos[b] < ks.len);
+    store_cols<EK, DC>(p.gv + at, dv[b], 1.0f, p.dim, lane, kpos[b] < ks.len);
+  }
+}
+
+template <int EK, int DC>
+int launch_backward(AttP p, hipStream_t s) {
+  const int64_t items = p.q_total * p.heads;
+  int64_t wgs = (items + 15) / 16;
+  if (EK == EK_F16 && wgs > kMaxParts) wgs = kMaxParts;
+  if (wgs > 1 << 16) wgs = 1 << 16;
+  launch_kernel(attention_delta_kernel<EK>, dim3((unsigned)wgs), dim3(256), 0u, s, p);
+  if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
+  const int parts = (int)wgs;
+  p.tiles = (int)((p.q_len + 127) / 128);
+  int64_t grid = (int64_t)p.n * p.heads * p.tiles;
+  if (grid > 0x7fffffff) return LIK_ERR_UNSUPPORTED;
+  if (p.gq) {
+    launch_kernel(attention_dq_kernel<EK, DC, 1>, dim3((unsigned)grid), dim3(256), p.km ? mask_words(p.k_len) * 4 : 0u, s,
+                  p, parts);
+    if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
+  }
+  p.tiles = (int)((p.k_len + 127) / 128);
+  grid = (int64_t)p.n * (p.heads / p.group) * p.tiles;
+  if (grid > 0x7fffffff) return LIK_ERR_UNSUPPORTED;
+  if (p.gk && grid) {
+    launch_kernel(attention_dkv_kernel<EK, DC, 1>, dim3((unsigned)grid), dim3(256), p.qm ? mask_words(p.q_len) * 4 : 0u,
+                  s, p, parts);
+    if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
+  }
+  return LIK_OK;
+}
+
+template <int EK>
+int run_backward(const AttP& p, hipStream_t s) {
+  if (p.dim <= 32) return launch_backward<EK, 1>(p, s);
+  if (p.dim <= 64) return launch_backward<EK, 2>(p, s);
+  if (p.dim <= 96) return launch_backward<EK, 3>(p, s);
+  return launch_backward<EK, 4>(p, s);
+}
+
+size_t backward_ws(const AttP& p) { return align256((size_t)p.q_total * p.heads * 4) + kMaxParts * 4 + 256; }
+
+}  // namespace
+}  // namespace enc
+}  // namespace lik
+
+using namespace lik;
+using namespace lik::enc;
+
+extern "C" {
+
+size_t lik_attention_backward_workspace_size(const lik_attention_t* a) {
+  AttP p{};
+  int rc;
+  return attention_shape(a, p, rc) ? backward_ws(p) : 0;
+}
+
+int lik_attention_backward(const lik_attention_t* a, const void* out, const float* lse, const void* grad,
+                           int64_t grad_stride_n, int64_t grad_stride_l, int64_t grad_stride_h, void* grad_q,
+                           void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes, lik_stream_t stream) {
+  AttP p{};
+  int rc;
+  if (!attention_shape(a, p, rc)) return rc != LIK_OK ? rc : LIK_ERR_INVALID;  // no query: nothing writes grad_k
+  if (!out || !lse || !grad || !grad_k != !grad_v) return LIK_ERR_INVALID;
+  if (!att_rows_ok(grad, grad_stride_n, grad_stride_l, grad_stride_h) || (uintptr_t)out % 16 ||
+      (uintptr_t)grad_q % 16 || (uintptr_t)grad_k % 16 || (uintptr_t)grad_v % 16)
+    return LIK_ERR_UNSUPPORTED;
+  if (!workspace || workspace_bytes < backward_ws(p)) return LIK_ERR_WORKSPACE;
+  char* ws = align256(workspace);
+  p.delta = (float*)ws;
+  p.gmax = (float*)(ws + align256((size_t)p.q_total * p.heads * 4));
+  p.out = (char*)const_cast<void*>(out);
+  p.lse = const_cast<float*>(lse);
+  p.g = {(const char*)grad, grad_stride_n * 2, grad_stride_l * 2, grad_stride_h * 2};
+  p.gq = (char*)grad_q;
+  p.gk = (char*)grad_k;
+  p.gv = (char*)grad_v;
+  return a->dtype == LIK_BF16 ? run_backward<EK_BF16>(p, (hipStream_t)stream)
+                              : run_backward<EK_F16>(p, (hipStream_t)stream);
+}
+
+}  // extern "C"

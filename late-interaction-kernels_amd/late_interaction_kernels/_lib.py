@@ -80,6 +80,16 @@ EXPORTED_SYMBOLS = (
     "lik_quantize_fp8_workspace_size",
     "lik_seqlens_cover",
     "lik_seqlens_cover_each",
+    "lik_layer_norm",
+    "lik_layer_norm_backward",
+    "lik_layer_norm_backward_workspace_size",
+    "lik_gated_ffn",
+    "lik_gated_ffn_backward",
+    "lik_gated_ffn_backward_workspace_size",
+    "lik_attention",
+    "lik_attention_workspace_size",
+    "lik_attention_backward",
+    "lik_attention_backward_workspace_size",
 )
 
 _p = ctypes.c_void_p
@@ -129,6 +139,45 @@ class LikPlaidDocs(ctypes.Structure):
         ("bucket_weights", _p),
         ("n_buckets", _i32),
         ("nbits", _i32),
+    ]
+
+
+class LikAttention(ctypes.Structure):
+    """Mirror of ``lik_attention_t``."""
+
+    _fields_ = [
+        ("q", _p),
+        ("k", _p),
+        ("v", _p),
+        ("dtype", _i32),
+        ("heads", _i32),
+        ("kv_heads", _i32),
+        ("dim", _i32),
+        ("n", _i64),
+        ("q_len", _i64),
+        ("k_len", _i64),
+        ("q_stride_n", _i64),
+        ("q_stride_l", _i64),
+        ("q_stride_h", _i64),
+        ("k_stride_n", _i64),
+        ("k_stride_l", _i64),
+        ("k_stride_h", _i64),
+        ("v_stride_n", _i64),
+        ("v_stride_l", _i64),
+        ("v_stride_h", _i64),
+        ("cu_q", _p),
+        ("cu_k", _p),
+        ("q_rows", _i64),
+        ("k_rows", _i64),
+        ("q_mask", _p),
+        ("q_mask_stride_n", _i64),
+        ("q_mask_stride_l", _i64),
+        ("k_mask", _p),
+        ("k_mask_stride_n", _i64),
+        ("k_mask_stride_l", _i64),
+        ("left", _i32),
+        ("right", _i32),
+        ("scale", ctypes.c_float),
     ]
 
 
@@ -242,6 +291,29 @@ def load() -> ctypes.CDLL:
     lib.lik_quantize_fp8_workspace_size.restype = ctypes.c_size_t
     lib.lik_quantize_fp8.argtypes = [_p, _i32, _i64, _i32, ctypes.c_uint32, _p, _p, _p, ctypes.c_size_t, _p]
     lib.lik_quantize_fp8.restype = ctypes.c_int
+    lib.lik_layer_norm.argtypes = [_p, _i64, _p, _i64, _i32, _i64, _i32, _p, _p, _i32, ctypes.c_float, _p, _p, _p, _p]
+    lib.lik_layer_norm.restype = ctypes.c_int
+    lib.lik_layer_norm_backward_workspace_size.argtypes = [_i32, _i64, _i32]
+    lib.lik_layer_norm_backward_workspace_size.restype = ctypes.c_size_t
+    lib.lik_layer_norm_backward.argtypes = [_p, _i64, _p, _i64, _p, _i64, _p, _i32, _i64, _i32, _p, _i32, _p, _p, _p,
+                                            _p, ctypes.c_size_t, _p]
+    lib.lik_layer_norm_backward.restype = ctypes.c_int
+    lib.lik_gated_ffn.argtypes = [_p, _i64, _i32, _i64, _i32, _i32, _p, _i64, _p, _i64, _p, _i64, _i32, _p, _p, _p, _p]
+    lib.lik_gated_ffn.restype = ctypes.c_int
+    lib.lik_gated_ffn_backward_workspace_size.argtypes = [_i32, _i64, _i32, _i32]
+    lib.lik_gated_ffn_backward_workspace_size.restype = ctypes.c_size_t
+    lib.lik_gated_ffn_backward.argtypes = [_p, _i64, _p, _i64, _i32, _i64, _i32, _i32, _p, _i64, _p, _i64, _p, _p, _i32,
+                                           _p, _p, _p, _p, ctypes.c_size_t, _p]
+    lib.lik_gated_ffn_backward.restype = ctypes.c_int
+    lib.lik_attention_workspace_size.argtypes = [P(LikAttention)]
+    lib.lik_attention_workspace_size.restype = ctypes.c_size_t
+    lib.lik_attention.argtypes = [P(LikAttention), _p, _p, _p, ctypes.c_size_t, _p]
+    lib.lik_attention.restype = ctypes.c_int
+    lib.lik_attention_backward_workspace_size.argtypes = [P(LikAttention)]
+    lib.lik_attention_backward_workspace_size.restype = ctypes.c_size_t
+    lib.lik_attention_backward.argtypes = [P(LikAttention), _p, _p, _p, _i64, _i64, _i64, _p, _p, _p, _p,
+                                           ctypes.c_size_t, _p]
+    lib.lik_attention_backward.restype = ctypes.c_int
     _lib = lib
     return lib
 
