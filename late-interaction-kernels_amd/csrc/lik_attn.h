@@ -99,6 +99,11 @@ template <int DC>
 struct Dim {
   static constexpr int KS = DC * 2, DB = DC, PITCH = DC <= 2 ? 128 : 256;
   static constexpr int SPR = PITCH / 16, TILE = 64 * PITCH, NI = TILE / 1024 / 4;
+  // 16-byte chunk c of row r lies at chunk c ^ swz(r): 16 consecutive rows at one chunk (row-wise reads)
+  // cover the 64 banks, and so do any four rows of an aligned group at 64 bytes each (transposing reads).
+  __device__ __forceinline__ static int swz(int r) {
+    return PITCH == 128 ? ((r & 2) << 1) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
+  }
 };
 
 // 64 rows into LDS by four wavefronts; row r at r * PITCH, chunks swizzled.
@@ -110,7 +115,7 @@ __device__ __forceinline__ void issue_rows(uint32_t lds, const char* base, int64
   const u32x4 desc = raw_desc(base, 0xffffff00u);
 #pragma unroll
   for (int i = 0; i < D::NI; ++i) {
-    const int slot = (wv * D::NI + i) * 64 + lane, r = slot / D::SPR, c = (slot % D::SPR) ^ lds_swz(r);
+    const int slot = (wv * D::NI + i) * 64 + lane, r = slot / D::SPR, c = (slot % D::SPR) ^ D::swz(r);
     bool on = c * 8 < dim && r < limit;
     if (bits) on = on && ((bits[r >> 5] >> (r & 31)) & 1u);
     dma16(lds + (wv * D::NI + i) * 1024, on ? (uint32_t)(r * ld + c * 16) : kOob, desc);
@@ -119,17 +124,19 @@ __device__ __forceinline__ void issue_rows(uint32_t lds, const char* base, int64
 // MFMA operand of 32 rows from row0, elements 16 ks + 8 (lane / 32) ..
 template <int DC>
 __device__ __forceinline__ u32x4 row_frag(uint32_t lds, int row0, int ks, int lane) {
+  using D = Dim<DC>;
   const int r = row0 + (lane & 31);
-  return lds_b128(lds + r * Dim<DC>::PITCH + (((ks * 2 + (lane >> 5)) ^ lds_swz(r)) << 4));
+  return lds_b128(lds + r * Dim<DC>::PITCH + (((ks * 2 + (lane >> 5)) ^ D::swz(r)) << 4));
 }
 // The same rows across: lane l has element 32 db + l % 32 of rows
 // row0 + 4 (l / 32) + {0..3, 8..11}, the order in which accumulators hold rows.
 template <int DC>
 __device__ __forceinline__ u32x4 col_frag(uint32_t lds, int row0, int db, int lane) {
+  using D = Dim<DC>;
   const int i = lane & 15, col = db * 32 + (lane & 16) + 4 * (i & 3);
   const int r0 = row0 + 4 * (lane >> 5) + (i >> 2), r1 = r0 + 8;
-  const u32x2 lo = lds_tr(lds + r0 * Dim<DC>::PITCH + (((col >> 3) ^ lds_swz(r0)) << 4) + ((col & 4) << 1));
-  const u32x2 hi = lds_tr(lds + r1 * Dim<DC>::PITCH + (((col >> 3) ^ lds_swz(r1)) << 4) + ((col & 4) << 1));
+  const u32x2 lo = lds_tr(lds + r0 * Dim<DC>::PITCH + (((col >> 3) ^ D::swz(r0)) << 4) + ((col & 4) << 1));
+  const u32x2 hi = lds_tr(lds + r1 * Dim<DC>::PITCH + (((col >> 3) ^ D::swz(r1)) << 4) + ((col & 4) << 1));
   return u32x4{lo[0], lo[1], hi[0], hi[1]};
 }
 // This lane's column operand of a row in memory (null: zeros): elements 16 ks + 8 (lane / 32) ..

@@ -81,12 +81,6 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
 }
 
-// 16-byte chunk c of LDS row r lies at chunk c ^ lds_swz(r) (rows of at least
-// eight chunks): eight consecutive rows then cover all banks at one chunk (row-wise
-// 16-byte reads), and any four consecutive rows of an aligned group cover them
-// with two neighbouring chunks each (the transposing reads below).
-__device__ __forceinline__ int lds_swz(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
-
 // Transposing LDS read: in each group of 16 lanes, lane i names 4 consecutive
 // 16-bit elements of row i / 4 (columns 4 (i % 4) ..); lane j gets column j of
 // the four rows.

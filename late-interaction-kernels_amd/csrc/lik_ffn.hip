@@ -9,10 +9,10 @@
 //             dg = dh u act'(g), du = dh act(g), side by side as [rows][2 hidden]
 //             dx = [dg du] [Wg; Wu]        B across k
 //             dw_in = [dg du]^T x, dw_out = gy^T h   A and B across k, k = rows
-// Sums over k are fp32 (MFMA accumulators, fp32 partial sums where k is split).
-// h, dg and du are rounded once to the 16-bit type, as the next product's operands
-// have to be; g and u are kept in fp32 for the backward, so that dg and du carry no
-// second rounding.
+// Sums over k are fp32 (MFMA accumulators, fp32 partial sums where k is split). h, dg and du are rounded
+// once to the 16-bit type, as the next product's operands have to be. g and u are kept for the backward so
+// that dg and du carry next to no other rounding: of bf16 calls in fp16 (11 bits against the 8 of dg and
+// du) divided by 16, which holds up to 1.0e6, of fp16 calls in fp32.
 #include "lik_enc.h"
 
 namespace lik {
@@ -20,20 +20,22 @@ namespace enc {
 namespace {
 
 enum { ACT_GELU = 0, ACT_GELU_TANH = 1, ACT_SILU = 2 };
-enum { EPI_STORE = 0, EPI_GLU = 1, EPI_GLU_BWD = 2, EPI_PART = 3 };
+enum { EPI_STORE = 0, EPI_GLU = 1, EPI_GLU_BWD = 2 };
 
 struct GemmP {
   const char* a;  // A(m, k): m * a_ld + k, or across k: k * a_ld + m (elements of 2 bytes)
   const char* b;
   int64_t a_ld, b_ld;  // bytes
   int m, n, k;
-  int k_per;           // k of one split (a multiple of 64)
-  int tiles_m, tiles_n, splits;
-  char* out;           // [m][n] 16-bit, row stride out_ld bytes; EPI_PART: fp32 [split][m][n]
+  int tiles_n, full;   // the first `full` tiles are one workgroup's each,
+  int tail, splits;    // the `tail` others are `splits` workgroups' each,
+  int k_per;           // of k_per (a multiple of 64) of k
+  float* part;         // their sums [tail][splits][a tile in the accumulators' order]
+  char* out;           // [m][n] 16-bit, row stride out_ld bytes; EPI_GLU_BWD: [m][2 hidden]
   int64_t out_ld;
   const char* res;     // EPI_STORE: added before the rounding; null: none
   int64_t res_ld;
-  float* gu;           // EPI_GLU: [m][2 hidden] kept g and u (null: not kept); EPI_GLU_BWD: read
+  char* gu;            // EPI_GLU: [m][2 hidden] kept g and u (null: not kept); EPI_GLU_BWD: read
   int hidden;
   int act;
 };
@@ -42,30 +44,46 @@ struct GemmP {
 template <bool SLOPE>
 __device__ __forceinline__ float act_of(int act, float x, float& slope) {
   if (act == ACT_SILU) {
-    const float s = 1.0f / (1.0f + __expf(-x));
+    const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-x));
     if (SLOPE) slope = s * (1.0f + x * (1.0f - s));
     return x * s;
   }
   if (act == ACT_GELU_TANH) {
     // (1 + tanh u) / 2 = sigmoid(2 u), u = sqrt(2 / pi) (x + 0.044715 x^3)
     const float x2 = x * x;
-    const float s = 1.0f / (1.0f + __expf(-1.5957691216f * x * fmaf(0.044715f, x2, 1.0f)));
+    const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-1.5957691216f * x * fmaf(0.044715f, x2, 1.0f)));
     if (SLOPE) slope = s * (1.0f + x * (1.0f - s) * 1.5957691216f * fmaf(0.134145f, x2, 1.0f));
     return x * s;
   }
-  const float cdf = 0.5f * (1.0f + erff(x * 0.70710678118f));
-  if (SLOPE) slope = fmaf(x, 0.39894228040f * __expf(-0.5f * x * x), cdf);
+  // cdf(-|x|) = erfc(|x| / sqrt 2) / 2 = poly(s) exp(-x^2 / 2), s = 1 / (1 + p |x| / sqrt 2): Abramowitz and
+  // Stegun 7.1.26, absolute error of erf 1.5e-7, far under the 16-bit outputs' rounding; the exponential is the
+  // slope's too (the library's erff costs three times as many instructions).
+  const float z = fabsf(x), s = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118f, z, 1.0f));
+  const float e = __expf(-0.5f * x * x);
+  float q = fmaf(1.061405429f, s, -1.453152027f);
+  q = fmaf(q, s, 1.421413741f);
+  q = fmaf(q, s, -0.284496736f);
+  q = fmaf(q, s, 0.254829592f);
+  const float tail = 0.5f * q * s * e;
+  const float cdf = x < 0.f ? tail : 1.0f - tail;
+  if (SLOPE) slope = fmaf(x, 0.39894228040f * e, cdf);
   return x * cdf;
 }
 
 // One operand's tile of T rows (m or n) by 64 k in LDS, 128 bytes a row of T:
 // along k: [T][64], 8 chunks a row; across k: [64][T], T / 8 chunks a row.
+constexpr int BK = 64;
+
 template <int T, bool X, int NW>
 struct Stage {
-  static constexpr int BYTES = T * 128;
-  static constexpr int NI = T / 8 / NW;  // 1 KB loads of a wavefront
-  static_assert(T % (8 * NW) == 0, "");
+  static constexpr int BYTES = T * BK * 2;
+  static constexpr int NI = BYTES / 1024 / NW;  // 1 KB loads of a wavefront
+  static_assert(BYTES % (1024 * NW) == 0 && T % 128 == 0, "");
 
+  // 16-byte chunk c of row r lies at chunk c ^ swz(r), so that reads cover the 64 banks evenly: along
+  // k 16 consecutive rows (two to 256 bytes) at one chunk; across k (rows of whole 256 bytes) four
+  // consecutive rows at 64 bytes each.
+  __device__ __forceinline__ static int swz(int r) { return X ? (r & 3) << 2 : (r >> 1) & 7; }
   // Lane offsets of the wavefront's loads from the tile's origin, kOob past the matrix' edge.
   // `rows`: rows (along k) or columns (across k) the tile has; glu: rows 32..63 of each 64 are up rows.
   __device__ __forceinline__ static void offsets(uint32_t* off, int wv, int lane, int64_t ld, int rows, bool glu,
@@ -74,85 +92,257 @@ struct Stage {
     for (int i = 0; i < NI; ++i) {
       const int slot = (wv * NI + i) * 64 + lane;
       if constexpr (X) {
-        const int r = slot / (T / 8), c = (slot % (T / 8)) ^ lds_swz(r);
+        const int r = slot / (T / 8), c = (slot % (T / 8)) ^ swz(r);
         off[i] = c * 8 < rows ? (uint32_t)(r * ld + c * 16) : kOob;
       } else {
-        const int r = slot / 8, c = (slot % 8) ^ lds_swz(r);
+        const int r = slot / 8, c = (slot % 8) ^ swz(r);
         const int at = glu ? (r / 64) * 32 + r % 32 : r;
         off[i] = at < rows ? (uint32_t)((at + (glu && (r & 32) ? (int64_t)hidden : 0)) * ld + c * 16) : kOob;
       }
     }
   }
-  // k_left: k of this step that exist (at most 64)
-  __device__ __forceinline__ static void issue(uint32_t lds, const uint32_t* off, int wv, int lane, const char* base,
-                                               uint32_t bytes, int k_left) {
-    const u32x4 desc = raw_desc(base, bytes);
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      uint32_t o = off[i];
+  // load i of a step of which k_left k exist (at most BK)
+  __device__ __forceinline__ static void issue(uint32_t lds, const uint32_t* off, int i, int wv, int lane,
+                                               const u32x4& desc, int k_left) {
+    uint32_t o = off[i];
+    if (k_left < BK) {
       const int slot = (wv * NI + i) * 64 + lane;
       if constexpr (X) {
-        if (k_left < 64 && slot / (T / 8) >= k_left) o = kOob;
+        if (slot / (T / 8) >= k_left) o = kOob;
       } else {
-        if (k_left < 64 && (int)((slot % 8) ^ lds_swz(slot / 8)) * 8 >= k_left) o = kOob;
+        if (((slot % 8) ^ swz(slot / 8)) * 8 >= k_left) o = kOob;
       }
-      dma16(lds + (wv * NI + i) * 1024, o, desc);
+    }
+    dma16(lds + (wv * NI + i) * 1024, o, desc);
+  }
+  // Lane addresses (from the buffer's origin) of the wavefront's MFMA operands: block j is 32 rows from
+  // row0 + 32 j, row0 a multiple of 32; lane l has row l % 32, k = 16 ks + 8 (l / 32) + 0..7.
+  // Along k: one 16-byte read, a[ks]. Across k: two transposing reads (k + 0..3, k + 4..7), a[j].
+  __device__ __forceinline__ static void bases(uint32_t* a, int row0, int lane) {
+    const int h = lane >> 5;
+    if constexpr (X) {
+      const int i = lane & 15, k = 8 * h + (i >> 2);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int col = row0 + 32 * j + (lane & 16) + 4 * (i & 3);
+        a[j] = k * (T * 2) + (((col >> 3) ^ swz(k)) << 4) + ((col & 4) << 1);
+      }
+    } else {
+      const int r = row0 + (lane & 31);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) a[ks] = r * 128 + (((ks * 2 + h) ^ swz(r)) << 4);
     }
   }
-  // MFMA operand of 32 rows from row0, k step ks (16 k): lane l has row l % 32, k = 8 (l / 32) + 0..7.
-  __device__ __forceinline__ static u32x4 frag(uint32_t lds, int row0, int ks, int lane) {
+  __device__ __forceinline__ static u32x4 frag(const uint32_t* a, uint32_t lds, int j, int ks) {
     if constexpr (X) {
-      const int i = lane & 15, h = lane >> 5;
-      const int col = row0 + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
-      const int k0 = ks * 16 + 8 * h + (i >> 2);
-      const u32x2 lo = lds_tr(lds + k0 * (T * 2) + (((col >> 3) ^ lds_swz(k0)) << 4) + ((col & 4) << 1));
-      const u32x2 hi = lds_tr(lds + (k0 + 4) * (T * 2) + (((col >> 3) ^ lds_swz(k0 + 4)) << 4) + ((col & 4) << 1));
+      const u32x2 lo = lds_tr(a[j] + lds + ks * 16 * (T * 2)), hi = lds_tr(a[j] + lds + (ks * 16 + 4) * (T * 2));
       return u32x4{lo[0], lo[1], hi[0], hi[1]};
     } else {
-      const int r = row0 + (lane & 31), c = ks * 2 + (lane >> 5);
-      return lds_b128(lds + r * 128 + ((c ^ lds_swz(r)) << 4));
+      return lds_b128(a[ks] + lds + j * 32 * 128);
     }
   }
 };
 
-// Four consecutive n of accumulator quads 2j and 2j + 1, as 16-bit pairs, to
+// Four consecutive n of accumulator quads 2 j and 2 j + 1, as 16-bit pairs, to
 // eight consecutive n per lane (the wavefront's halves exchange): lane half h
-// then holds n = 16 j + 8 h + 0..7 of its m.
+// then holds n = 16 j + 8 h + 0..7 of its m. split_halves is the inverse.
 __device__ __forceinline__ u32x4 join_halves(uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1) {
   const auto s0 = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
   const auto s1 = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
   return u32x4{(uint32_t)s0[0], (uint32_t)s1[0], (uint32_t)s0[1], (uint32_t)s1[1]};
 }
+__device__ __forceinline__ u32x4 split_halves(const u32x4& x) {
+  const auto s0 = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false);
+  const auto s1 = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
+  return u32x4{(uint32_t)s0[0], (uint32_t)s1[0], (uint32_t)s0[1], (uint32_t)s1[1]};
+}
+template <int EK>
+__device__ __forceinline__ void unpack8(const u32x4& x, float* v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) unpack2<EK>(x[i], v[2 * i], v[2 * i + 1]);
+}
 
+// The kept g and u: bytes of a value, and eight of them (n + 8 h + 0..7 of quads 2 j, 2 j + 1).
+template <int EK>
+struct Kept {
+  static constexpr int B = EK == EK_BF16 ? 2 : 4;
+  static constexpr float DOWN = 0.0625f, UP = 16.0f;
+};
+
+// What the epilogue of a 32 x 32 block reads: the residual, or g and u.
+template <int EK, int EPI>
+struct Extra {
+  u32x4 x[EPI == EPI_GLU_BWD ? (EK == EK_BF16 ? 4 : 8) : 2];
+};
+// Lane (l32, h) of a block's accumulators holds m = l32 and n = 8 q + 4 h + e of quad q, element e. The block
+// starts at column n (a hidden column for both GLU epilogues); columns come in groups of 8.
+template <int EK, int EPI>
+__device__ __forceinline__ void load_extra(const GemmP& p, Extra<EK, EPI>& ex, int m, int n, int h) {
+  if constexpr (EPI == EPI_STORE) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      ex.x[j] = u32x4{0u, 0u, 0u, 0u};
+      const int c = n + 16 * j + 8 * h;
+      if (p.res && m < p.m && c < p.n) ex.x[j] = *(const u32x4*)(p.res + m * p.res_ld + c * 2);
+    }
+  } else if constexpr (EPI == EPI_GLU_BWD && EK == EK_BF16) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      ex.x[2 * j] = ex.x[2 * j + 1] = u32x4{0u, 0u, 0u, 0u};
+      const int c = n + 16 * j + 8 * h;
+      if (m < p.m && c < p.hidden) {
+        const char* at = p.gu + ((int64_t)m * 2 * p.hidden + c) * 2;
+        ex.x[2 * j] = *(const u32x4*)at;
+        ex.x[2 * j + 1] = *(const u32x4*)(at + (int64_t)p.hidden * 2);
+      }
+    }
+  } else if constexpr (EPI == EPI_GLU_BWD) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      ex.x[2 * q] = ex.x[2 * q + 1] = u32x4{0u, 0u, 0u, 0u};
+      const int c = n + 8 * q + 4 * h;
+      if (m < p.m && n + 8 * q < p.hidden) {
+        const char* at = p.gu + ((int64_t)m * 2 * p.hidden + c) * 4;
+        ex.x[2 * q] = *(const u32x4*)at;
+        ex.x[2 * q + 1] = *(const u32x4*)(at + (int64_t)p.hidden * 4);
+      }
+    }
+  }
+}
+// c0: the block's sums (EPI_GLU: of the gate), c1: EPI_GLU only, the up projection's.
+// NJ: groups of 16 columns.
+template <int EK, int EPI, int NJ = 2>
+__device__ __forceinline__ void finish_block(const GemmP& p, const f32x16& c0, const f32x16& c1,
+                                             const Extra<EK, EPI>& ex, int m, int n, int h) {
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {  // quads 2 j, 2 j + 1: 16 columns
+    const int c = n + 16 * j + 8 * h;
+    const bool on = m < p.m && c < (EPI == EPI_STORE ? p.n : p.hidden);
+    if constexpr (EPI == EPI_STORE) {
+      float v[8];
+      unpack8<EK>(split_halves(ex.x[j]), v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += c0[8 * j + e];
+      const u32x4 o =
+          join_halves(pack2<EK>(v[0], v[1]), pack2<EK>(v[2], v[3]), pack2<EK>(v[4], v[5]), pack2<EK>(v[6], v[7]));
+      if (on) *(u32x4*)(p.out + m * p.out_ld + c * 2) = o;
+    } else if constexpr (EPI == EPI_GLU) {
+      float v[8], none;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = act_of<false>(p.act, c0[8 * j + e], none) * c1[8 * j + e];
+      const u32x4 o =
+          join_halves(pack2<EK>(v[0], v[1]), pack2<EK>(v[2], v[3]), pack2<EK>(v[4], v[5]), pack2<EK>(v[6], v[7]));
+      if (on) *(u32x4*)(p.out + m * p.out_ld + c * 2) = o;
+      if (p.gu) {
+        if constexpr (EK == EK_BF16) {
+          constexpr float d = Kept<EK>::DOWN;
+          u32x4 g, u;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            g[e] = pack2<EK_F16>(c0[8 * j + 2 * e] * d, c0[8 * j + 2 * e + 1] * d);
+            u[e] = pack2<EK_F16>(c1[8 * j + 2 * e] * d, c1[8 * j + 2 * e + 1] * d);
+          }
+          g = join_halves(g[0], g[1], g[2], g[3]);
+          u = join_halves(u[0], u[1], u[2], u[3]);
+          char* at = p.gu + ((int64_t)m * 2 * p.hidden + c) * 2;
+          if (on) {
+            *(u32x4*)at = g;
+            *(u32x4*)(at + (int64_t)p.hidden * 2) = u;
+          }
+        } else {
+#pragma unroll
+          for (int q = 2 * j; q < 2 * j + 2; ++q)
+            if (m < p.m && n + 8 * q < p.hidden) {
+              char* at = p.gu + ((int64_t)m * 2 * p.hidden + n + 8 * q + 4 * h) * 4;
+              *(f32x4*)at = f32x4{c0[4 * q], c0[4 * q + 1], c0[4 * q + 2], c0[4 * q + 3]};
+              *(f32x4*)(at + (int64_t)p.hidden * 4) = f32x4{c1[4 * q], c1[4 * q + 1], c1[4 * q + 2], c1[4 * q + 3]};
+            }
+        }
+      }
+    } else {
+      float g[8], u[8], dg[8], du[8];
+      if constexpr (EK == EK_BF16) {
+        unpack8<EK_F16>(split_halves(ex.x[2 * j]), g);
+        unpack8<EK_F16>(split_halves(ex.x[2 * j + 1]), u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          g[e] *= Kept<EK>::UP;
+          u[e] *= Kept<EK>::UP;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          g[e] = __uint_as_float(ex.x[4 * j + 2 * (e / 4)][e % 4]);
+          u[e] = __uint_as_float(ex.x[4 * j + 2 * (e / 4) + 1][e % 4]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float dh = c0[8 * j + e];
+        float slope;
+        du[e] = dh * act_of<true>(p.act, g[e], slope);
+        dg[e] = dh * u[e] * slope;
+      }
+      const u32x4 og = join_halves(pack2<EK>(dg[0], dg[1]), pack2<EK>(dg[2], dg[3]), pack2<EK>(dg[4], dg[5]),
+                                   pack2<EK>(dg[6], dg[7]));
+      const u32x4 ou = join_halves(pack2<EK>(du[0], du[1]), pack2<EK>(du[2], du[3]), pack2<EK>(du[4], du[5]),
+                                   pack2<EK>(du[6], du[7]));
+      if (on) {
+        char* o = p.out + m * p.out_ld + c * 2;
+        *(u32x4*)o = og;
+        *(u32x4*)(o + (int64_t)p.hidden * 2) = ou;
+      }
+    }
+  }
+}
+
+// A workgroup of WM x WN wavefronts owns a TM x TN tile and walks k in steps of 64 (whole 128-byte lines of
+// either layout), four k steps of 16 each; the operands of one are read from LDS while the one before is
+// multiplied. A has three LDS buffers and B two (all 160 KB at 256 x 256): before a step's last k step its
+// buffers have been read, there the next step's are waited for and B's loads of the step after it start;
+// A's start one k step later and are in flight across the wait, so that requests never run dry.
 template <int EK, bool XA, bool XB, int TM, int TN, int WM, int WN, int EPI>
 __global__ void __launch_bounds__(WM* WN * 64) gemm_kernel(const GemmP p) {
   constexpr int NW = WM * WN, MB = TM / WM / 32, NB = TN / WN / 32;
   using SA = Stage<TM, XA, NW>;
   using SB = Stage<TN, XB, NW>;
   constexpr bool GLU = EPI == EPI_GLU;
-  __shared__ __attribute__((aligned(1024))) char s_tile[2][SA::BYTES + SB::BYTES];
+  __shared__ __attribute__((aligned(1024))) char s_tile[3 * SA::BYTES + 2 * SB::BYTES];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wv % WM, wn = wv / WM;
-  uint32_t t = xcd_tile(blockIdx.x, gridDim.x);
-  const int split = (int)(t / (uint32_t)(p.tiles_m * p.tiles_n));
-  t %= (uint32_t)(p.tiles_m * p.tiles_n);
+  const bool whole = (int)blockIdx.x < p.full;
+  const int at = (int)blockIdx.x - p.full, split = whole ? 0 : at / p.tail;
+  const uint32_t t = whole ? xcd_tile(blockIdx.x, (uint32_t)p.full) : (uint32_t)(p.full + at % p.tail);
   const int tm = (int)(t / (uint32_t)p.tiles_n), tn = (int)(t % (uint32_t)p.tiles_n);
   const int m0 = tm * TM, n0 = GLU ? tn * (TN / 2) : tn * TN;  // GLU: n0 counts hidden columns
-  const int k0 = split * p.k_per, k1 = k0 + p.k_per < p.k ? k0 + p.k_per : p.k;
+  const int k0 = split * p.k_per, k1 = whole || k0 + p.k_per > p.k ? p.k : k0 + p.k_per;
+  const int steps = (k1 - k0 + BK - 1) / BK;
 
   uint32_t offa[SA::NI], offb[SB::NI];
   SA::offsets(offa, wv, lane, p.a_ld, p.m - m0, false, 0);
   SB::offsets(offb, wv, lane, p.b_ld, (GLU ? p.hidden : p.n) - n0, GLU, p.hidden);
-  const uint32_t lds0 = lds_addr(s_tile[0]), lds1 = lds_addr(s_tile[1]);
-  auto issue = [&](uint32_t lds, int k) {
-    const int left = k1 - k;
-    if constexpr (XA) SA::issue(lds, offa, wv, lane, p.a + (int64_t)k * p.a_ld + (int64_t)m0 * 2, 0xffffff00u, left);
-    else SA::issue(lds, offa, wv, lane, p.a + (int64_t)m0 * p.a_ld + (int64_t)k * 2, 0xffffff00u, left);
-    if constexpr (XB)
-      SB::issue(lds + SA::BYTES, offb, wv, lane, p.b + (int64_t)k * p.b_ld + (int64_t)n0 * 2, 0xffffff00u, left);
-    else
-      SB::issue(lds + SA::BYTES, offb, wv, lane, p.b + (int64_t)n0 * p.b_ld + (int64_t)k * 2, 0xffffff00u, left);
+  const uint32_t lds0 = lds_addr(s_tile);
+  uint32_t ra[4], rb[4];
+  SA::bases(ra, wm * (TM / WM), lane);
+  SB::bases(rb, wn * (TN / WN), lane);
+  // A's loads of step i go into buffer i % 3, B's into i % 2; a step past the end loads nothing but counts alike
+  const uint32_t ldb = lds0 + 3 * SA::BYTES;
+  auto k_of = [&](int i) { return k0 + i * BK; };
+  auto desc_a = [&](int i) {
+    const int64_t k = k_of(i);
+    return raw_desc(XA ? p.a + k * p.a_ld + (int64_t)m0 * 2 : p.a + (int64_t)m0 * p.a_ld + k * 2,
+                    k < k1 ? 0xffffff00u : 0u);
+  };
+  auto desc_b = [&](int i) {
+    const int64_t k = k_of(i);
+    return raw_desc(XB ? p.b + k * p.b_ld + (int64_t)n0 * 2 : p.b + (int64_t)n0 * p.b_ld + k * 2,
+                    k < k1 ? 0xffffff00u : 0u);
+  };
+  u32x4 fa[2][MB], fb[2][NB];
+  auto read = [&](int set, uint32_t la, uint32_t lb, int ks, int j) {
+    if (j < MB) fa[set][j] = SA::frag(ra, la, j, ks);
+    else fb[set][j - MB] = SB::frag(rb, lb, j - MB, ks);
   };
 
   f32x16 acc[NB][MB];
@@ -160,189 +350,258 @@ __global__ void __launch_bounds__(WM* WN * 64) gemm_kernel(const GemmP p) {
   for (int i = 0; i < NB; ++i)
 #pragma unroll
     for (int j = 0; j < MB; ++j) acc[i][j] = f32x16{};
-  issue(lds0, k0);
-  int buf = 0;
-  for (int k = k0; k < k1; k += 64, buf ^= 1) {
-    // this step's tile is complete, and every wavefront is done with the other buffer
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    const uint32_t lds = buf ? lds1 : lds0;
-    if (k + 64 < k1) issue(buf ? lds0 : lds1, k + 64);
+  // One k step: the MFMAs of operand set `set`, and spread between them the reads of the other set
+  // (k step ks of buffers la, lb) and `loads` loads.
+  auto k_step = [&](auto SET, uint32_t la, uint32_t lb, int ks, auto LOADS, auto load) {
+    constexpr int set = decltype(SET)::value;
+    constexpr int S = NB * MB, R = MB + NB, OPS = R + decltype(LOADS)::value;
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      u32x4 fa[MB], fb[NB];
+    for (int s = 0; s < S; ++s) {
+      acc[s / MB][s % MB] = mfma16<EK>(acc[s / MB][s % MB], fb[set][s / MB], fa[set][s % MB]);
 #pragma unroll
-      for (int j = 0; j < MB; ++j) fa[j] = SA::frag(lds, wm * (TM / WM) + j * 32, ks, lane);
-#pragma unroll
-      for (int i = 0; i < NB; ++i) fb[i] = SB::frag(lds + SA::BYTES, wn * (TN / WN) + i * 32, ks, lane);
-#pragma unroll
-      for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int j = 0; j < MB; ++j) acc[i][j] = mfma16<EK>(acc[i][j], fb[i], fa[j]);
+      for (int o = s * OPS / S; o < (s + 1) * OPS / S; ++o) {
+        if (o < R) read(set ^ 1, la, lb, ks, o);
+        else load(o - R);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
+  };
+  using std::integral_constant;
+  constexpr integral_constant<int, 0> S0{}, NONE{};
+  constexpr integral_constant<int, 1> S1{};
+  constexpr integral_constant<int, SA::NI> LA{};
+  constexpr integral_constant<int, SB::NI> LB{};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const u32x4 da = desc_a(i), db = desc_b(i);
+#pragma unroll
+    for (int j = 0; j < SA::NI; ++j) SA::issue(lds0 + i * SA::BYTES, offa, j, wv, lane, da, k1 - k_of(i));
+#pragma unroll
+    for (int j = 0; j < SB::NI; ++j) SB::issue(ldb + i * SB::BYTES, offb, j, wv, lane, db, k1 - k_of(i));
   }
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(SA::NI + SB::NI) : "memory");
+#pragma unroll
+  for (int j = 0; j < MB + NB; ++j) read(0, lds0, ldb, 0, j);
+  uint32_t a0 = lds0, a1 = lds0 + SA::BYTES, a2 = lds0 + 2 * SA::BYTES, b0 = ldb, b1 = ldb + SB::BYTES;
+  for (int i = 0; i < steps; ++i) {
+    const int left = k1 - k_of(i + 2);
+    const u32x4 da = desc_a(i + 2), db = desc_b(i + 2);
+    k_step(S0, a0, b0, 1, LA, [&](int j) { SA::issue(a2, offa, j, wv, lane, da, left); });
+    k_step(S1, a0, b0, 2, NONE, [&](int) {});
+    k_step(S0, a0, b0, 3, NONE, [&](int) {});
+    // the next step's buffers are complete, and every wavefront has read all of this step's
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(SA::NI) : "memory");
+    k_step(S1, a1, b1, 0, LB, [&](int j) { SB::issue(b0, offb, j, wv, lane, db, left); });
+    const uint32_t a = a0, b = b0;
+    a0 = a1, a1 = a2, a2 = a;
+    b0 = b1, b1 = b;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load is in flight to LDS when the workgroup ends
 
-  // Epilogue. Lane (l32, h) of acc[i][j] holds m = l32 and n = 8 q + 4 h + e of quad q, element e.
+  if (!whole) {
+    float* out = p.part + (((int64_t)(at % p.tail) * p.splits + split) * NW + wv) * (NB * MB * 1024) + lane * 4;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int j = 0; j < MB; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *(f32x4*)(out + ((i * MB + j) * 4 + q) * 256) =
+              f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    return;
+  }
   const int l32 = lane & 31, h = lane >> 5;
+  constexpr int PAIR = GLU ? 2 : 1;  // column blocks of one output block
 #pragma unroll
   for (int j = 0; j < MB; ++j) {
-    const int m = m0 + wm * (TM / WM) + j * 32 + l32;
-    if constexpr (EPI == EPI_STORE) {
+    const int m = m0 + wm * (TM / WM) + j * 32 + l32, n = n0 + wn * (TN / WN / PAIR);
+    // a row's loads before its first store (g and u of fp16 calls take twice the registers: block by block)
+    constexpr int AHEAD = EK == EK_F16 && EPI == EPI_GLU_BWD ? 1 : NB / PAIR;
 #pragma unroll
-      for (int i = 0; i < NB; ++i)
+    for (int i0 = 0; i0 < NB / PAIR; i0 += AHEAD) {
+      Extra<EK, EPI> ex[AHEAD];
 #pragma unroll
-        for (int q = 0; q < 4; q += 2) {
-          const int n = n0 + wn * (TN / WN) + i * 32 + 8 * q;  // this pair of quads: 16 columns
-          float v[8];
+      for (int i = 0; i < AHEAD; ++i) load_extra<EK, EPI>(p, ex[i], m, n + (i0 + i) * 32, h);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = acc[i][j][q * 4 + e];
-          if (p.res) {
-            // the lane's own quads: columns n + 4 h and n + 8 + 4 h
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-              if (m < p.m && n + 8 * u < p.n) {
-                const u32x2 r = *(const u32x2*)(p.res + m * p.res_ld + (n + 8 * u + 4 * h) * 2);
-                float a, b;
-                unpack2<EK>(r[0], a, b);
-                v[4 * u] += a;
-                v[4 * u + 1] += b;
-                unpack2<EK>(r[1], a, b);
-                v[4 * u + 2] += a;
-                v[4 * u + 3] += b;
-              }
-          }
-          const u32x4 o = join_halves(pack2<EK>(v[0], v[1]), pack2<EK>(v[2], v[3]), pack2<EK>(v[4], v[5]),
-                                      pack2<EK>(v[6], v[7]));
-          if (m < p.m && n + 8 * h < p.n) *(u32x4*)(p.out + m * p.out_ld + (n + 8 * h) * 2) = o;
-        }
-    } else if constexpr (EPI == EPI_PART) {
-#pragma unroll
-      for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int n = n0 + wn * (TN / WN) + i * 32 + 8 * q + 4 * h;
-          const f32x4 o = {acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]};
-          if (m < p.m && n < p.n) *(f32x4*)(p.out + (((int64_t)split * p.m + m) * p.n + n) * 4) = o;
-        }
-    } else if constexpr (EPI == EPI_GLU) {
-      static_assert(EPI != EPI_GLU || NB % 2 == 0, "gate and up blocks in pairs");
-#pragma unroll
-      for (int i = 0; i < NB; i += 2)
-#pragma unroll
-        for (int q = 0; q < 4; q += 2) {
-          const int f = n0 + wn * (TN / WN / 2) + (i / 2) * 32 + 8 * q;
-          float v[8], none;
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            v[e] = act_of<false>(p.act, acc[i][j][q * 4 + e], none) * acc[i + 1][j][q * 4 + e];
-          if (p.gu) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-              if (m < p.m && f + 8 * u < p.hidden) {
-                float* g = p.gu + (int64_t)m * 2 * p.hidden + f + 8 * u + 4 * h;
-                const int s = (q + u) * 4;
-                *(f32x4*)g = f32x4{acc[i][j][s], acc[i][j][s + 1], acc[i][j][s + 2], acc[i][j][s + 3]};
-                *(f32x4*)(g + p.hidden) =
-                    f32x4{acc[i + 1][j][s], acc[i + 1][j][s + 1], acc[i + 1][j][s + 2], acc[i + 1][j][s + 3]};
-              }
-          }
-          const u32x4 o = join_halves(pack2<EK>(v[0], v[1]), pack2<EK>(v[2], v[3]), pack2<EK>(v[4], v[5]),
-                                      pack2<EK>(v[6], v[7]));
-          if (m < p.m && f + 8 * h < p.hidden) *(u32x4*)(p.out + m * p.out_ld + (f + 8 * h) * 2) = o;
-        }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; q += 2) {
-          const int f = n0 + wn * (TN / WN) + i * 32 + 8 * q;
-          float dg[8], du[8];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            f32x4 g = {}, up = {};
-            if (m < p.m && f + 8 * u < p.hidden) {
-              const float* at = p.gu + (int64_t)m * 2 * p.hidden + f + 8 * u + 4 * h;
-              g = *(const f32x4*)at;
-              up = *(const f32x4*)(at + p.hidden);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float dh = acc[i][j][(q + u) * 4 + e];
-              float slope;
-              du[4 * u + e] = dh * act_of<true>(p.act, g[e], slope);
-              dg[4 * u + e] = dh * up[e] * slope;
-            }
-          }
-          const u32x4 og = join_halves(pack2<EK>(dg[0], dg[1]), pack2<EK>(dg[2], dg[3]), pack2<EK>(dg[4], dg[5]),
-                                       pack2<EK>(dg[6], dg[7]));
-          const u32x4 ou = join_halves(pack2<EK>(du[0], du[1]), pack2<EK>(du[2], du[3]), pack2<EK>(du[4], du[5]),
-                                       pack2<EK>(du[6], du[7]));
-          if (m < p.m && f + 8 * h < p.hidden) {
-            char* o = p.out + m * p.out_ld + (f + 8 * h) * 2;
-            *(u32x4*)o = og;
-            *(u32x4*)(o + (int64_t)p.hidden * 2) = ou;
-          }
-        }
+      for (int i = 0; i < AHEAD; ++i)
+        finish_block<EK, EPI>(p, acc[(i0 + i) * PAIR][j], acc[(i0 + i) * PAIR + PAIR - 1][j], ex[i], m,
+                              n + (i0 + i) * 32, h);
     }
   }
 }
 
-// out = the sum of the splits' fp32 partial sums, rounded once; four elements a thread.
-template <int EK>
-__global__ void __launch_bounds__(256) sum_parts_kernel(const float* part, int splits, int64_t n4, char* out) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n4) return;
-  f32x4 a = *(const f32x4*)(part + i * 4);
-  for (int s = 1; s < splits; ++s) {
-    const f32x4 b = *(const f32x4*)(part + ((int64_t)s * n4 + i) * 4);
+// The tail's epilogue: a workgroup adds the splits of one block of every wavefront in order.
+template <int EK, int TM, int TN, int WM, int WN, int EPI>
+__global__ void __launch_bounds__(WM* WN * 64) gemm_finish_kernel(const GemmP p) {
+  constexpr int NW = WM * WN, MB = TM / WM / 32, NB = TN / WN / 32, PAIR = EPI == EPI_GLU ? 2 : 1;
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, wm = wv % WM, wn = wv / WM, h = lane >> 5;
+  int u = (int)blockIdx.x;
+  const int j = u % MB;
+  u /= MB;
+  const int i = u % (NB / PAIR) * PAIR;
+  u /= NB / PAIR;
+  const int t = p.full + u, tm = t / p.tiles_n, tn = t % p.tiles_n;
+  const int m = tm * TM + wm * (TM / WM) + j * 32 + (lane & 31);
+  const int n = tn * (TN / PAIR) + wn * (TN / WN / PAIR) + i / PAIR * 32;
+  Extra<EK, EPI> ex;
+  load_extra<EK, EPI>(p, ex, m, n, h);
+  f32x16 c[PAIR];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) a[e] += b[e];
-  }
-  *(u32x2*)(out + i * 8) = u32x2{pack2<EK>(a[0], a[1]), pack2<EK>(a[2], a[3])};
+  for (int b = 0; b < PAIR; ++b) c[b] = f32x16{};
+  const float* in = p.part + ((int64_t)u * p.splits * NW + wv) * (NB * MB * 1024) + lane * 4;
+#pragma unroll 2
+  for (int s = 0; s < p.splits; ++s, in += NW * NB * MB * 1024)
+#pragma unroll
+    for (int b = 0; b < PAIR; ++b)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 x = *(const f32x4*)(in + (((i + b) * MB + j) * 4 + q) * 256);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[b][4 * q + e] += x[e];
+      }
+  finish_block<EK, EPI>(p, c[0], c[PAIR - 1], ex, m, n, h);
 }
 
-constexpr int kTM = 256, kTN = 256;
+// Few rows: the weights are read once for all of them and little else happens, so the call is bound by how many
+// loads are in flight. A workgroup owns 32 weight rows (EPI_GLU: 16 gate and the 16 up rows of the same columns,
+// which meet in one lane's accumulators) and 32 MB rows of x, its eight wavefronts an eighth of k each: operands
+// go from memory to registers as they lie, the eight sums meet in LDS and are added in order.
+template <int EK, int EPI, int MB>
+__global__ void __launch_bounds__(512) few_rows_kernel(const GemmP p) {
+  constexpr int NW = 8, U = MB <= 2 ? 6 : 3;
+  __shared__ __attribute__((aligned(16))) float s_sum[NW][MB][4][64][4];
+  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = (int)blockIdx.x * (EPI == EPI_GLU ? 16 : 32), m0 = (int)blockIdx.y * 32 * MB;
+  const int n = EPI == EPI_GLU ? n0 + (l32 & 15) : n0 + l32;
+  const int row = EPI == EPI_GLU && l32 >= 16 ? p.hidden + n : n;
+  const uint32_t boff = n < (EPI == EPI_GLU ? p.hidden : p.n) ? (uint32_t)(row * p.b_ld) : kOob;
+  uint32_t aoff[MB];
+#pragma unroll
+  for (int j = 0; j < MB; ++j) aoff[j] = m0 + j * 32 + l32 < p.m ? (uint32_t)((j * 32 + l32) * p.a_ld) : kOob;
+  const __amdgpu_buffer_rsrc_t rb =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p.b), (short)0, (int)0xffffff00u, 0x00020000);
+  const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<char*>(p.a + (int64_t)m0 * p.a_ld), (short)0, (int)0xffffff00u, 0x00020000);
+  f32x16 acc[MB];
+#pragma unroll
+  for (int j = 0; j < MB; ++j) acc[j] = f32x16{};
+  const int all = (p.k + 15) / 16, per = (all + NW - 1) / NW;
+  const int end = (wv + 1) * per < all ? (wv + 1) * per : all;
+  for (int ks = wv * per; ks < end; ks += U) {
+    u32x4 fb[U], fa[U][MB];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int e = (ks + u) * 16 + 8 * h;
+      const bool on = ks + u < end && e < p.k;
+      fb[u] = __builtin_amdgcn_raw_buffer_load_b128(rb, on && boff != kOob ? boff + e * 2 : kOob, 0, 0);
+#pragma unroll
+      for (int j = 0; j < MB; ++j)
+        fa[u][j] = __builtin_amdgcn_raw_buffer_load_b128(ra, on && aoff[j] != kOob ? aoff[j] + e * 2 : kOob, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < MB; ++j) acc[j] = mfma16<EK>(acc[j], fb[u], fa[u][j]);
+  }
+#pragma unroll
+  for (int j = 0; j < MB; ++j)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *(f32x4*)s_sum[wv][j][q][lane] = f32x4{acc[j][4 * q], acc[j][4 * q + 1], acc[j][4 * q + 2], acc[j][4 * q + 3]};
+  __syncthreads();
+  if (wv >= MB) return;
+  const int m = m0 + wv * 32 + l32;
+  Extra<EK, EPI> ex;
+  load_extra<EK, EPI>(p, ex, m, n0, h);
+  f32x16 c = {};
+#pragma unroll
+  for (int w = 0; w < NW; ++w)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 x = *(const f32x4*)s_sum[w][wv][q][lane];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c[4 * q + e] += x[e];
+    }
+  if constexpr (EPI == EPI_GLU) {
+    f32x16 up = {};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) up[e] = c[8 + e];
+    finish_block<EK, EPI, 1>(p, c, up, ex, m, n0, h);
+  } else {
+    finish_block<EK, EPI>(p, c, c, ex, m, n0, h);
+  }
+}
+
+constexpr int kTM = 256, kTN = 256, kCUs = 256;
+// Rows up to which few_rows_kernel takes the forward's products.
+constexpr int kFewRows = 256;
+
+template <int EK, int EPI>
+int launch_few_rows(const GemmP& p, hipStream_t s) {
+  const unsigned nb = EPI == EPI_GLU ? (p.hidden + 15) / 16 : (p.n + 31) / 32;
+  if (p.m <= 32)
+    launch_kernel(few_rows_kernel<EK, EPI, 1>, dim3(nb), dim3(512), 0u, s, p);
+  else if (p.m <= 64)
+    launch_kernel(few_rows_kernel<EK, EPI, 2>, dim3(nb), dim3(512), 0u, s, p);
+  else
+    launch_kernel(few_rows_kernel<EK, EPI, 4>, dim3(nb, (p.m + 127) / 128), dim3(512), 0u, s, p);
+  return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;
+}
+
+// Tiles run in rounds of one workgroup a CU. What is left after the whole rounds would take another round on
+// a few CUs; instead k of each of those tiles is split over several workgroups, whose fp32 sums a second
+// kernel adds. Costs in us as measured at 256 x 256 tiles: 1.8 a step of 64 k (all CUs busy), 8 for the
+// second launch, and the partial sums' 256 KB a workgroup written and read at about 4.5 TB/s.
+struct Shape {
+  int tiles_n, full, tail, splits, k_per;
+};
+Shape gemm_shape(int64_t m, int64_t n_tiles, int64_t k) {
+  const int64_t tiles = (m + kTM - 1) / kTM * n_tiles, steps = (k + BK - 1) / BK;
+  Shape s{(int)n_tiles, (int)tiles, 0, 1, (int)(steps * BK)};
+  const int64_t left = tiles % kCUs;
+  if (left == 0) return s;
+  double best = 1.8 * steps;
+  for (int64_t sp = 2; sp <= steps / 2 && left * sp <= 4 * kCUs; ++sp) {
+    const int64_t per = (steps + sp - 1) / sp, real = (steps + per - 1) / per;
+    if (real != sp) continue;
+    const double cost = 1.8 * per * ((left * sp + kCUs - 1) / kCUs) + 8 + 0.12 * left * sp;
+    if (cost < best) {
+      best = cost;
+      s = {(int)n_tiles, (int)(tiles - left), (int)left, (int)sp, (int)(per * BK)};
+    }
+  }
+  return s;
+}
+size_t part_bytes(const Shape& s) { return (size_t)s.tail * s.splits * kTM * kTN * 4; }
+int64_t n_tiles(int64_t n) { return (n + kTN - 1) / kTN; }
+int64_t glu_tiles(int64_t hidden) { return (hidden + kTN / 2 - 1) / (kTN / 2); }
 
 template <int EK, bool XA, bool XB, int EPI>
-int launch_gemm(GemmP p, hipStream_t s) {
-  const int n = EPI == EPI_GLU ? 2 * p.hidden : p.n;
-  p.tiles_m = (p.m + kTM - 1) / kTM;
-  p.tiles_n = EPI == EPI_GLU ? (p.hidden + kTN / 2 - 1) / (kTN / 2) : (n + kTN - 1) / kTN;
-  launch_kernel(gemm_kernel<EK, XA, XB, kTM, kTN, 4, 2, EPI>, dim3((unsigned)(p.tiles_m * p.tiles_n * p.splits)),
-                dim3(512), 0u, s, p);
-  return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;
-}
-
-// Weight gradients have few tiles and a long k (the rows): k is split so that the
-// tiles fill the 256 CUs, in steps of 64 k.
-struct Splits {
-  int splits, k_per;
-};
-Splits weight_splits(int m, int n, int64_t k) {
-  const int tiles = ((m + kTM - 1) / kTM) * ((n + kTN - 1) / kTN);
-  int64_t want = 256 / tiles;
-  const int64_t most = (k + 511) / 512;
-  if (want > most) want = most;
-  if (want < 1) want = 1;
-  const int64_t per = ((k + want - 1) / want + 63) / 64 * 64;
-  return {(int)((k + per - 1) / per), (int)per};
-}
-
-template <int EK>
-int weight_grad(GemmP p, char* out, float* part, hipStream_t s) {
-  const Splits sp = weight_splits(p.m, p.n, p.k);
-  p.splits = sp.splits;
-  p.k_per = sp.k_per;
-  if (sp.splits == 1) {
-    p.out = out;
-    p.out_ld = (int64_t)p.n * 2;
-    return launch_gemm<EK, true, true, EPI_STORE>(p, s);
+int launch_gemm(GemmP p, float* part, hipStream_t s) {
+  if constexpr (!XA && !XB)
+    if (p.m <= kFewRows) return launch_few_rows<EK, EPI>(p, s);
+  const Shape sh = gemm_shape(p.m, EPI == EPI_GLU ? glu_tiles(p.hidden) : n_tiles(p.n), p.k);
+  p.tiles_n = sh.tiles_n;
+  p.full = sh.full;
+  p.tail = sh.tail;
+  p.splits = sh.splits;
+  p.k_per = sh.k_per;
+  p.part = part;
+  launch_kernel(gemm_kernel<EK, XA, XB, kTM, kTN, 4, 2, EPI>, dim3((unsigned)(sh.full + sh.tail * sh.splits)), dim3(512),
+                0u, s, p);
+  if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
+  if (sh.tail) {
+    constexpr int blocks = kTM / 4 / 32 * (kTN / 2 / 32) / (EPI == EPI_GLU ? 2 : 1);
+    launch_kernel(gemm_finish_kernel<EK, kTM, kTN, 4, 2, EPI>, dim3((unsigned)(sh.tail * blocks)), dim3(512), 0u, s, p);
+    if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
   }
-  p.out = (char*)part;
-  if (const int rc = launch_gemm<EK, true, true, EPI_PART>(p, s)) return rc;
-  const int64_t n4 = (int64_t)p.m * p.n / 4;
-  launch_kernel(sum_parts_kernel<EK>, dim3((unsigned)((n4 + 255) / 256)), dim3(256), 0u, s, (const float*)part,
-                sp.splits, n4, out);
-  return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;
+  return LIK_OK;
+}
+
+size_t most(size_t a, size_t b) { return a > b ? a : b; }
+size_t ffn_ws(int64_t rows, int d, int f) {
+  return most(part_bytes(gemm_shape(rows, glu_tiles(f), d)), part_bytes(gemm_shape(rows, n_tiles(d), f))) + 256;
 }
 
 struct FfnBwdWs {
@@ -351,11 +610,10 @@ struct FfnBwdWs {
 FfnBwdWs ffn_bwd_ws(int64_t rows, int d, int f) {
   FfnBwdWs w;
   w.dgu = 0;
-  const Splits a = weight_splits(2 * f, d, rows), b = weight_splits(d, f, rows);
-  const size_t pa = a.splits > 1 ? (size_t)a.splits * 2 * f * d * 4 : 0;
-  const size_t pb = b.splits > 1 ? (size_t)b.splits * d * f * 4 : 0;
   w.part = align256((size_t)rows * 2 * f * 2);
-  w.total = w.part + (pa > pb ? pa : pb) + 256;
+  w.total = w.part + 256 +
+            most(most(part_bytes(gemm_shape(rows, n_tiles(f), d)), part_bytes(gemm_shape(rows, n_tiles(d), 2 * f))),
+                 most(part_bytes(gemm_shape(2 * f, n_tiles(d), rows)), part_bytes(gemm_shape(d, n_tiles(f), rows))));
   return w;
 }
 
@@ -364,6 +622,8 @@ int ffn_check(int32_t dtype, int64_t rows, int32_t d, int32_t f, int32_t act) {
   if (rows < 0 || d < 8 || f < 8 || act < ACT_GELU || act > ACT_SILU) return LIK_ERR_INVALID;
   // 16-byte chunks of k; rows of weights and tokens within a 32-bit tile offset
   if (d % 8 || f % 8 || d > (1 << 20) || f > (1 << 20) || rows > 0x7fffff00) return LIK_ERR_UNSUPPORTED;
+  const int64_t most_n = (2ll * f > d ? 2ll * f : d) / 128 + 1;  // workgroups of a launch, in 31 bits
+  if ((rows / 256 + 1) * most_n > (1 << 30)) return LIK_ERR_UNSUPPORTED;
   return LIK_OK;
 }
 // 16-byte rows; a tile of 256, and `more` rows before it, within a lane's 32-bit offset
@@ -375,9 +635,8 @@ bool rows16(const void* p, int64_t stride, int64_t more = 0) {
 template <int EK>
 int ffn_forward(const void* x, int64_t x_ld, int64_t rows, int d, int f, const void* w_in, int64_t wi_ld,
                 const void* w_out, int64_t wo_ld, const void* res, int64_t res_ld, int act, void* out, void* h,
-                float* gu, hipStream_t s) {
+                void* gu, float* part, hipStream_t s) {
   GemmP p{};
-  p.splits = 1;
   p.act = act;
   p.hidden = f;
   p.m = (int)rows;
@@ -386,33 +645,32 @@ int ffn_forward(const void* x, int64_t x_ld, int64_t rows, int d, int f, const v
   p.b = (const char*)w_in;
   p.b_ld = wi_ld * 2;
   p.n = f;
-  p.k = p.k_per = d;
+  p.k = d;
   p.out = (char*)h;
   p.out_ld = (int64_t)f * 2;
-  p.gu = gu;
-  if (const int rc = launch_gemm<EK, false, false, EPI_GLU>(p, s)) return rc;
+  p.gu = (char*)gu;
+  if (const int rc = launch_gemm<EK, false, false, EPI_GLU>(p, part, s)) return rc;
   p.a = (const char*)h;
   p.a_ld = (int64_t)f * 2;
   p.b = (const char*)w_out;
   p.b_ld = wo_ld * 2;
   p.n = d;
-  p.k = p.k_per = f;
+  p.k = f;
   p.out = (char*)out;
   p.out_ld = (int64_t)d * 2;
   p.res = (const char*)res;
   p.res_ld = res_ld * 2;
-  return launch_gemm<EK, false, false, EPI_STORE>(p, s);
+  return launch_gemm<EK, false, false, EPI_STORE>(p, part, s);
 }
 
 template <int EK>
 int ffn_backward(const void* g, int64_t g_ld, const void* x, int64_t x_ld, int64_t rows, int d, int f,
-                 const void* w_in, int64_t wi_ld, const void* w_out, int64_t wo_ld, const void* h, const float* gu,
+                 const void* w_in, int64_t wi_ld, const void* w_out, int64_t wo_ld, const void* h, const void* gu,
                  int act, void* gx, void* gw_in, void* gw_out, char* ws, hipStream_t s) {
   const FfnBwdWs w = ffn_bwd_ws(rows, d, f);
   char* dgu = ws + w.dgu;
   float* part = (float*)(ws + w.part);
   GemmP p{};
-  p.splits = 1;
   p.act = act;
   p.hidden = f;
   if (gx || gw_in) {
@@ -422,11 +680,11 @@ int ffn_backward(const void* g, int64_t g_ld, const void* x, int64_t x_ld, int64
     p.b = (const char*)w_out;
     p.b_ld = wo_ld * 2;
     p.n = f;
-    p.k = p.k_per = d;
+    p.k = d;
     p.out = dgu;
     p.out_ld = (int64_t)f * 4;
-    p.gu = const_cast<float*>(gu);
-    if (const int rc = launch_gemm<EK, false, true, EPI_GLU_BWD>(p, s)) return rc;
+    p.gu = (char*)const_cast<void*>(gu);
+    if (const int rc = launch_gemm<EK, false, true, EPI_GLU_BWD>(p, part, s)) return rc;
   }
   if (gx) {
     p.a = dgu;
@@ -434,10 +692,10 @@ int ffn_backward(const void* g, int64_t g_ld, const void* x, int64_t x_ld, int64
     p.b = (const char*)w_in;
     p.b_ld = wi_ld * 2;
     p.n = d;
-    p.k = p.k_per = 2 * f;
+    p.k = 2 * f;
     p.out = (char*)gx;
     p.out_ld = (int64_t)d * 2;
-    if (const int rc = launch_gemm<EK, false, true, EPI_STORE>(p, s)) return rc;
+    if (const int rc = launch_gemm<EK, false, true, EPI_STORE>(p, part, s)) return rc;
   }
   p.k = (int)rows;
   if (gw_in) {
@@ -447,7 +705,9 @@ int ffn_backward(const void* g, int64_t g_ld, const void* x, int64_t x_ld, int64
     p.a_ld = (int64_t)f * 4;
     p.b = (const char*)x;
     p.b_ld = x_ld * 2;
-    if (const int rc = weight_grad<EK>(p, (char*)gw_in, part, s)) return rc;
+    p.out = (char*)gw_in;
+    p.out_ld = (int64_t)d * 2;
+    if (const int rc = launch_gemm<EK, true, true, EPI_STORE>(p, part, s)) return rc;
   }
   if (gw_out) {
     p.m = d;
@@ -456,7 +716,9 @@ int ffn_backward(const void* g, int64_t g_ld, const void* x, int64_t x_ld, int64
     p.a_ld = g_ld * 2;
     p.b = (const char*)h;
     p.b_ld = (int64_t)f * 2;
-    if (const int rc = weight_grad<EK>(p, (char*)gw_out, part, s)) return rc;
+    p.out = (char*)gw_out;
+    p.out_ld = (int64_t)f * 2;
+    if (const int rc = launch_gemm<EK, true, true, EPI_STORE>(p, part, s)) return rc;
   }
   return LIK_OK;
 }
@@ -470,19 +732,25 @@ using namespace lik::enc;
 
 extern "C" {
 
+size_t lik_gated_ffn_workspace_size(int32_t dtype, int64_t rows, int32_t dim, int32_t hidden) {
+  if (ffn_check(dtype, rows, dim, hidden, ACT_GELU) != LIK_OK || rows == 0) return 0;
+  return ffn_ws(rows, dim, hidden);
+}
+
 int lik_gated_ffn(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int32_t dim, int32_t hidden,
                   const void* w_in, int64_t w_in_stride, const void* w_out, int64_t w_out_stride, const void* residual,
-                  int64_t residual_stride, int32_t activation, void* out, void* hidden_act, float* gate_up,
-                  lik_stream_t stream) {
+                  int64_t residual_stride, int32_t activation, void* out, void* hidden_act, void* gate_up,
+                  void* workspace, size_t workspace_bytes, lik_stream_t stream) {
   if (const int rc = ffn_check(dtype, rows, dim, hidden, activation)) return rc;
   if (rows == 0) return LIK_OK;
   if (!x || !w_in || !w_out || !out || !hidden_act) return LIK_ERR_INVALID;
   if (!rows16(x, x_stride) || !rows16(w_in, w_in_stride, hidden) || !rows16(w_out, w_out_stride) || !rows16(out, 0) ||
       !rows16(hidden_act, 0) || !rows16(gate_up, 0) || (residual && !rows16(residual, residual_stride)))
     return LIK_ERR_UNSUPPORTED;
+  if (!workspace || workspace_bytes < ffn_ws(rows, dim, hidden)) return LIK_ERR_WORKSPACE;
   const auto fn = dtype == LIK_BF16 ? ffn_forward<EK_BF16> : ffn_forward<EK_F16>;
   return fn(x, x_stride, rows, dim, hidden, w_in, w_in_stride, w_out, w_out_stride, residual, residual_stride,
-            activation, out, hidden_act, gate_up, (hipStream_t)stream);
+            activation, out, hidden_act, gate_up, (float*)align256(workspace), (hipStream_t)stream);
 }
 
 size_t lik_gated_ffn_backward_workspace_size(int32_t dtype, int64_t rows, int32_t dim, int32_t hidden) {
@@ -492,7 +760,7 @@ size_t lik_gated_ffn_backward_workspace_size(int32_t dtype, int64_t rows, int32_
 
 int lik_gated_ffn_backward(const void* grad, int64_t grad_stride, const void* x, int64_t x_stride, int32_t dtype,
                            int64_t rows, int32_t dim, int32_t hidden, const void* w_in, int64_t w_in_stride,
-                           const void* w_out, int64_t w_out_stride, const void* hidden_act, const float* gate_up,
+                           const void* w_out, int64_t w_out_stride, const void* hidden_act, const void* gate_up,
                            int32_t activation, void* grad_x, void* grad_w_in, void* grad_w_out, void* workspace,
                            size_t workspace_bytes, lik_stream_t stream) {
   if (const int rc = ffn_check(dtype, rows, dim, hidden, activation)) return rc;

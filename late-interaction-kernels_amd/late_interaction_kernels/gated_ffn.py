@@ -15,6 +15,8 @@ import torch.nn.functional as F
 from . import _lib
 from .autograd import _needs_grad
 
+# what the forward keeps both projections in: more bits than the gradients' rounding (bf16's are scaled into fp16)
+_KEPT = {torch.bfloat16: torch.float16, torch.float16: torch.float32}
 ACTIVATIONS = {"gelu": 0, "gelu_tanh": 1, "silu": 2}
 
 
@@ -23,13 +25,18 @@ def _forward(x2, w_in, w_out, r2, act, want_kept):
     f = w_out.shape[1]
     out = torch.empty(rows, d, dtype=x2.dtype, device=x2.device)
     h = torch.empty(rows, f, dtype=x2.dtype, device=x2.device)
-    gu = torch.empty(rows, 2 * f, dtype=torch.float32, device=x2.device) if want_kept else None
+    gu = None
+    if want_kept:
+        gu = torch.empty(rows, 2 * f, dtype=_KEPT[x2.dtype], device=x2.device)
     if rows:
+        lib, code = _lib.load(), _lib.DTYPE_CODE[x2.dtype]
+        nbytes = lib.lik_gated_ffn_workspace_size(code, rows, d, f)
+        ws = _lib.workspace(nbytes, x2.device)
         with _lib.on_device(x2.device):
-            rc = _lib.load().lik_gated_ffn(
-                x2.data_ptr(), x2.stride(0), _lib.DTYPE_CODE[x2.dtype], rows, d, f, w_in.data_ptr(), w_in.stride(0),
-                w_out.data_ptr(), w_out.stride(0), _lib.ptr(r2), 0 if r2 is None else r2.stride(0), act,
-                out.data_ptr(), h.data_ptr(), _lib.ptr(gu), _lib.stream_of(x2))
+            rc = lib.lik_gated_ffn(
+                x2.data_ptr(), x2.stride(0), code, rows, d, f, w_in.data_ptr(), w_in.stride(0), w_out.data_ptr(),
+                w_out.stride(0), _lib.ptr(r2), 0 if r2 is None else r2.stride(0), act, out.data_ptr(), h.data_ptr(),
+                _lib.ptr(gu), _lib.ptr(ws), nbytes, _lib.stream_of(x2))
         _lib.check(rc, "lik_gated_ffn")
     return out, h, gu
 
