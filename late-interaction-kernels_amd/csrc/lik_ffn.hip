@@ -41,33 +41,45 @@ struct GemmP {
 };
 
 // act(x) and its derivative
-template <bool SLOPE>
-__device__ __forceinline__ float act_of(int act, float x, float& slope) {
-  if (act == ACT_SILU) {
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ float act_of(float x, float& slope) {
+  if constexpr (ACT == ACT_SILU) {
     const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-x));
     if (SLOPE) slope = s * (1.0f + x * (1.0f - s));
     return x * s;
-  }
-  if (act == ACT_GELU_TANH) {
+  } else if constexpr (ACT == ACT_GELU_TANH) {
     // (1 + tanh u) / 2 = sigmoid(2 u), u = sqrt(2 / pi) (x + 0.044715 x^3)
     const float x2 = x * x;
     const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-1.5957691216f * x * fmaf(0.044715f, x2, 1.0f)));
     if (SLOPE) slope = s * (1.0f + x * (1.0f - s) * 1.5957691216f * fmaf(0.134145f, x2, 1.0f));
     return x * s;
+  } else {
+    // cdf(-|x|) = erfc(|x| / sqrt 2) / 2 = poly(s) exp(-x^2 / 2), s = 1 / (1 + p |x| / sqrt 2): Abramowitz and
+    // Stegun 7.1.26, absolute error of erf 1.5e-7, far under the 16-bit outputs' rounding; the exponential is
+    // the slope's too (the library's erff costs three times as many instructions).
+    const float z = fabsf(x), s = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118f, z, 1.0f));
+    const float e = __expf(-0.5f * x * x);
+    float q = fmaf(1.061405429f, s, -1.453152027f);
+    q = fmaf(q, s, 1.421413741f);
+    q = fmaf(q, s, -0.284496736f);
+    q = fmaf(q, s, 0.254829592f);
+    const float tail = 0.5f * q * s * e;
+    const float cdf = x < 0.f ? tail : 1.0f - tail;
+    if (SLOPE) slope = fmaf(x, 0.39894228040f * e, cdf);
+    return x * cdf;
   }
-  // cdf(-|x|) = erfc(|x| / sqrt 2) / 2 = poly(s) exp(-x^2 / 2), s = 1 / (1 + p |x| / sqrt 2): Abramowitz and
-  // Stegun 7.1.26, absolute error of erf 1.5e-7, far under the 16-bit outputs' rounding; the exponential is the
-  // slope's too (the library's erff costs three times as many instructions).
-  const float z = fabsf(x), s = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118f, z, 1.0f));
-  const float e = __expf(-0.5f * x * x);
-  float q = fmaf(1.061405429f, s, -1.453152027f);
-  q = fmaf(q, s, 1.421413741f);
-  q = fmaf(q, s, -0.284496736f);
-  q = fmaf(q, s, 0.254829592f);
-  const float tail = 0.5f * q * s * e;
-  const float cdf = x < 0.f ? tail : 1.0f - tail;
-  if (SLOPE) slope = fmaf(x, 0.39894228040f * e, cdf);
-  return x * cdf;
+}
+// Eight at a time, so that one value's chain of instructions fills the other's waits.
+template <bool SLOPE>
+__device__ __forceinline__ void act8(int act, const float* x, float* y, float* slope) {
+  float none;
+  auto all = [&](auto A) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = act_of<decltype(A)::value, SLOPE>(x[e], SLOPE ? slope[e] : none);
+  };
+  if (act == ACT_SILU) all(std::integral_constant<int, ACT_SILU>{});
+  else if (act == ACT_GELU_TANH) all(std::integral_constant<int, ACT_GELU_TANH>{});
+  else all(std::integral_constant<int, ACT_GELU>{});
 }
 
 // One operand's tile of T rows (m or n) by 64 k in LDS, 128 bytes a row of T:
@@ -227,9 +239,12 @@ __device__ __forceinline__ void finish_block(const GemmP& p, const f32x16& c0, c
           join_halves(pack2<EK>(v[0], v[1]), pack2<EK>(v[2], v[3]), pack2<EK>(v[4], v[5]), pack2<EK>(v[6], v[7]));
       if (on) *(u32x4*)(p.out + m * p.out_ld + c * 2) = o;
     } else if constexpr (EPI == EPI_GLU) {
-      float v[8], none;
+      float g[8], v[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = act_of<false>(p.act, c0[8 * j + e], none) * c1[8 * j + e];
+      for (int e = 0; e < 8; ++e) g[e] = c0[8 * j + e];
+      act8<false>(p.act, g, v, nullptr);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= c1[8 * j + e];
       const u32x4 o =
           join_halves(pack2<EK>(v[0], v[1]), pack2<EK>(v[2], v[3]), pack2<EK>(v[4], v[5]), pack2<EK>(v[6], v[7]));
       if (on) *(u32x4*)(p.out + m * p.out_ld + c * 2) = o;
@@ -276,12 +291,13 @@ __device__ __forceinline__ void finish_block(const GemmP& p, const f32x16& c0, c
           u[e] = __uint_as_float(ex.x[4 * j + 2 * (e / 4) + 1][e % 4]);
         }
       }
+      float a[8], slope[8];
+      act8<true>(p.act, g, a, slope);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float dh = c0[8 * j + e];
-        float slope;
-        du[e] = dh * act_of<true>(p.act, g[e], slope);
-        dg[e] = dh * u[e] * slope;
+        du[e] = dh * a[e];
+        dg[e] = dh * u[e] * slope[e];
       }
       const u32x4 og = join_halves(pack2<EK>(dg[0], dg[1]), pack2<EK>(dg[2], dg[3]), pack2<EK>(dg[4], dg[5]),
                                    pack2<EK>(dg[6], dg[7]));
