@@ -12,7 +12,7 @@ namespace {
 //   scores  S^T[key][query] = K Q^T   (K rows from LDS, Q in registers)
 //   output  O^T[d][query]  += V^T P^T (V by transposing LDS reads, P as it lies)
 template <int EK, int DC, int QB>
-__global__ void __launch_bounds__(256) attention_kernel(const AttP p) {
+__global__ void __launch_bounds__(256, 2) attention_kernel(const AttP p) {
   using D = Dim<DC>;
   __shared__ __attribute__((aligned(1024))) char s_tile[2][2 * D::TILE];
   __shared__ int s_kept[2];
@@ -132,14 +132,14 @@ __global__ void __launch_bounds__(256) attention_kernel(const AttP p) {
         for (int i = 0; i < 16; ++i) m = fmaxf(m, s[b][u][i]);
       m = fmaxf(fmaxf(m, swap_half(m)), top[b]);
       const float mc = m == -INFINITY ? 0.f : m * p.c;
-      const float alpha = exp2f(fmaf(top[b], p.c, -mc));
+      const float alpha = __builtin_amdgcn_exp2f(fmaf(top[b], p.c, -mc));
       top[b] = m;
       float add = 0.f;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float e = exp2f(fmaf(s[b][u][i], p.c, -mc));
+          const float e = __builtin_amdgcn_exp2f(fmaf(s[b][u][i], p.c, -mc));
           s[b][u][i] = e;
           add += e;
         }
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(256) attention_kernel(const AttP p) {
     const float total = sum[b] + swap_half(sum[b]);
     const bool on = qpos[b] < qs.len, kept = qon[b] && total != 0.f;
     const float inv = kept ? 1.0f / total : 0.f;
-    const float lse = kept ? fmaf(top[b], p.c, log2f(total)) : INFINITY;
+    const float lse = kept ? fmaf(top[b], p.c, __builtin_amdgcn_logf(total)) : INFINITY;
     const int64_t row = qs.row + qpos[b];
     if (p.splits > 1) {
       // this split's mean of the values, and its statistics
@@ -208,14 +208,14 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttP p) {
   float total = 0.f;
   if (top != -INFINITY)
     for (int s = 0; s < p.splits; ++s) {
-      const float w = exp2f(p.part_lse[((int64_t)s * p.heads + head) * p.q_total + row] - top);
+      const float w = __builtin_amdgcn_exp2f(p.part_lse[((int64_t)s * p.heads + head) * p.q_total + row] - top);
       total += w;
       const f32x4 x = *(const f32x4*)(p.part_o + (((int64_t)s * p.q_total + row) * p.heads + head) * p.dim + e);
 #pragma unroll
       for (int k = 0; k < 4; ++k) a[k] = fmaf(w, x[k], a[k]);
     }
   const float inv = top != -INFINITY ? 1.0f / total : 0.f;
-  if (p.lse && e == 0) p.lse[(int64_t)head * p.q_total + row] = top != -INFINITY ? top + log2f(total) : INFINITY;
+  if (p.lse && e == 0) p.lse[(int64_t)head * p.q_total + row] = top != -INFINITY ? top + __builtin_amdgcn_logf(total) : INFINITY;
   *(u32x2*)(p.out + (rh * p.dim + e) * 2) =
       u32x2{pack2<EK>(a[0] * inv, a[1] * inv), pack2<EK>(a[2] * inv, a[3] * inv)};
 }

@@ -74,7 +74,7 @@ __device__ __forceinline__ float grad_scale(const AttP& p, int parts, float* s_b
 // Gradient of q: the forward's walk over the keys (K rows also by transposing
 // reads, V rows in LDS), dq^T[d][query] += K^T ds^T.
 template <int EK, int DC, int QB>
-__global__ void __launch_bounds__(256) attention_dq_kernel(const AttP p, int parts) {
+__global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p, int parts) {
   using D = Dim<DC>;
   __shared__ __attribute__((aligned(1024))) char s_tile[2][2 * D::TILE];
   __shared__ int s_kept[2];
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(256) attention_dq_kernel(const AttP p, int par
       for (int b = 0; b < QB; ++b) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float e = exp2f(fmaf(s[b][i], p.c, -lse[b]));
+          const float e = __builtin_amdgcn_exp2f(fmaf(s[b][i], p.c, -lse[b]));
           s[b][i] = e * (EK == EK_F16 ? (dp[b][i] - delta[b]) * gs : dp[b][i] - delta[b]);
         }
 #pragma unroll
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(256) attention_dq_kernel(const AttP p, int par
 // registers, and walks the queries of the group's heads, 64 at a time.
 //   P[query][key] from S = Q K^T;  dv^T[d][key] += G^T P;  dp = G V^T;  dk^T[d][key] += Q^T ds
 template <int EK, int DC, int KB>
-__global__ void __launch_bounds__(256) attention_dkv_kernel(const AttP p, int parts) {
+__global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p, int parts) {
   using D = Dim<DC>;
   __shared__ __attribute__((aligned(1024))) char s_tile[2][2 * D::TILE];
   __shared__ __attribute__((aligned(16))) float s_stat[2][2][64];
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(256) attention_dkv_kernel(const AttP p, int pa
             float e[4], ds[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              e[i] = exp2f(fmaf(s[b][q * 4 + i], p.c, -ls[i]));
+              e[i] = __builtin_amdgcn_exp2f(fmaf(s[b][q * 4 + i], p.c, -ls[i]));
               const float x = dp[b][q * 4 + i] - dl[i];
               ds[i] = e[i] * (EK == EK_F16 ? x * gs : x);
             }
