@@ -42,9 +42,28 @@ struct AttP {
   float* part_o;                  // forward split over keys: [split][q_total][heads][dim] fp32
   float* part_lse;                // [split][heads][q_total]
   int splits, tiles;              // q tiles (k tiles) of a sequence
+  int chunk, wgs;                 // workgroups: `chunk` in a row go to one XCD; wgs of them have work
 };
 
 constexpr int kNone = 0x7fffffff;
+
+// Work item of this workgroup, or -1. Items of one key head share its keys in their XCD's L2 (workgroups go to the
+// XCDs in turn), so `chunk` items in a row go to one XCD; the chunks go round, because sequences differ in length.
+__device__ __forceinline__ int work_item(const AttP& p) {
+  const int x = (int)blockIdx.x & 7, j = (int)blockIdx.x >> 3;
+  const int64_t w = (int64_t)(j / p.chunk) * 8 * p.chunk + x * p.chunk + j % p.chunk;
+  return w < p.wgs ? (int)w : -1;
+}
+// A chunk is a key head's items, but at least eight chunks go to every XCD. Returns the grid (0: too large).
+inline unsigned work_grid(AttP& p, int64_t wgs, int64_t per_key_head) {
+  if (wgs > 0x3fffffff) return 0;
+  int64_t c = (wgs + 63) / 64;
+  if (c > per_key_head) c = per_key_head;
+  if (c < 1) c = 1;
+  p.chunk = (int)c;
+  p.wgs = (int)wgs;
+  return (unsigned)((wgs + 8 * c - 1) / (8 * c) * 8 * c);
+}
 
 // A sequence's rows: first row, length.
 struct Span {
@@ -156,15 +175,29 @@ __device__ __forceinline__ float swap_half(float x) {
   return __uint_as_float((threadIdx.x & 32) ? (uint32_t)s[0] : (uint32_t)s[1]);
 }
 
-// Keep word of the 32 rows [t, t + 32) of a sequence of len rows, shifted so that this
-// lane's accumulator element i has bit 8 (i / 4) + i % 4.
-__device__ __forceinline__ uint32_t lane_word(const uint32_t* bits, int t, int len, int lane) {
-  const int left = len - t;
-  uint32_t w = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
-  if (bits && left > 0) w &= bits[t >> 5];
-  return w >> (4 * (lane >> 5));
-}
 __device__ __forceinline__ constexpr int acc_row(int i) { return 8 * (i / 4) + i % 4; }
+
+// Sets the scores of a 32 x 32 block that are not kept to -inf. In this lane element i is row
+// t + 4 (lane / 32) + acc_row(i) of the streamed side. end: rows from there on are none; bits (null: all are
+// kept): their keep bits; window: element i is kept where 0 <= first + acc_row(i) <= span.
+__device__ __forceinline__ void mask_scores(f32x16& s, int t, int end, const uint32_t* bits, bool window, int first,
+                                            uint32_t span, int lane) {
+  const int h4 = 4 * (lane >> 5);
+  if (window) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = (uint32_t)(first + acc_row(i)) <= span ? s[i] : -INFINITY;
+  }
+  if (bits && t < end) {
+    const uint32_t w = bits[t >> 5] >> h4;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = (w & (1u << acc_row(i))) ? s[i] : -INFINITY;
+  }
+  if (t + 32 > end) {
+    const int left = end - t - h4;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = acc_row(i) < left ? s[i] : -INFINITY;
+  }
+}
 
 // Four consecutive elements of accumulator quads 2 j and 2 j + 1 as 16-bit pairs
 // to eight consecutive ones a lane: half h then holds elements 16 j + 8 h + 0..7.

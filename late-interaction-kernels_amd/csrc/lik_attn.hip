@@ -19,8 +19,9 @@ __global__ void __launch_bounds__(256, 2) attention_kernel(const AttP p) {
   extern __shared__ uint32_t s_bits[];
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // tiles of one key head's queries follow each other on one XCD: they share its keys in L2
-  uint32_t t = xcd_tile(blockIdx.x, gridDim.x);
+  const int item = work_item(p);
+  if (item < 0) return;
+  uint32_t t = (uint32_t)item;
   const int split = (int)(t % (uint32_t)p.splits);
   t /= (uint32_t)p.splits;
   const int tile = (int)(t % (uint32_t)p.tiles);
@@ -31,6 +32,28 @@ __global__ void __launch_bounds__(256, 2) attention_kernel(const AttP p) {
   const int q0 = tile * 128 * QB;
   if (q0 >= qs.len) return;  // (all threads)
 
+  const char* kbase = p.k.data + (p.cu_k ? ks.row * p.k.sl : seq * p.k.sn) + kvh * p.k.sh;
+  const char* vbase = p.v.data + (p.cu_k ? ks.row * p.v.sl : seq * p.v.sn) + kvh * p.v.sh;
+  const uint32_t lds[2] = {lds_addr(s_tile[0]), lds_addr(s_tile[1])};
+  int klen = ks.len;
+  bool holes = false;
+  auto issue = [&](uint32_t at, int kt) {
+    const uint32_t* bits = holes ? s_bits + (kt >> 5) : nullptr;
+    issue_rows<DC>(at, kbase + kt * p.k.sl, p.k.sl, p.dim, klen - kt, bits, wv, lane);
+    issue_rows<DC>(at + D::TILE, vbase + kt * p.v.sl, p.v.sl, p.dim, klen - kt, bits, wv, lane);
+  };
+
+  // The first tile's loads start before the keep bits are known (and again without the masked rows, if there
+  // are any): a short sequence's time is a chain of such latencies.
+  const int q_end = (q0 + 128 * QB < qs.len ? q0 + 128 * QB : qs.len) - 1;  // last query of the workgroup
+  int kb = p.left == kNone || q0 - p.left < 0 ? 0 : (q0 - p.left) & ~63;
+  int ke = p.right == kNone || (int64_t)q_end + p.right + 1 >= klen ? klen : q_end + p.right + 1;
+  if (p.splits > 1) {  // this split's share
+    const int tiles = ke > kb ? (ke - kb + 63) / 64 : 0, per = (tiles + p.splits - 1) / p.splits;
+    kb += split * per * 64;
+    ke = kb + per * 64 < ke ? kb + per * 64 : ke;
+  }
+  if (kb < ke) issue(lds[0], kb);
   // the lane's queries: column l32 of each of the wavefront's QB blocks
   int qpos[QB];
   bool qon[QB];
@@ -47,33 +70,22 @@ __global__ void __launch_bounds__(256, 2) attention_kernel(const AttP p) {
   for (int b = 1; b < QB; ++b) any |= qon[b];
   any = __ballot(any) != 0;  // this wavefront has a query
 
-  // keys: the kept extent, then what the window leaves to this workgroup, then this split's share
-  int klen = ks.len;
-  bool holes = false;
   if (p.km) {
     const Kept kept = scan_mask(s_bits, p.km + seq * p.km_sn, p.km_sl, klen, s_kept);
     klen = kept.extent;
     holes = kept.holes;
-  }
-  const int q_end = (q0 + 128 * QB < qs.len ? q0 + 128 * QB : qs.len) - 1;  // last query of the workgroup
-  int kb = p.left == kNone || q0 - p.left < 0 ? 0 : (q0 - p.left) & ~63;
-  int ke = p.right == kNone || (int64_t)q_end + p.right + 1 >= klen ? klen : q_end + p.right + 1;
-  if (p.splits > 1) {
-    const int tiles = ke > kb ? (ke - kb + 63) / 64 : 0, per = (tiles + p.splits - 1) / p.splits;
-    kb += split * per * 64;
-    ke = kb + per * 64 < ke ? kb + per * 64 : ke;
+    ke = ke < klen ? ke : klen;
+    if ((holes || (klen < ks.len && klen < kb + 64)) && kb < ke) {  // masked rows have to read as zeros
+      asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+      issue(lds[0], kb);
+    }
   }
   if (__syncthreads_or(any) == 0) ke = kb;  // no query of this tile is kept
 
-  const char* kbase = p.k.data + (p.cu_k ? ks.row * p.k.sl : seq * p.k.sn) + kvh * p.k.sh;
-  const char* vbase = p.v.data + (p.cu_k ? ks.row * p.v.sl : seq * p.v.sn) + kvh * p.v.sh;
-  const uint32_t lds[2] = {lds_addr(s_tile[0]), lds_addr(s_tile[1])};
-  auto issue = [&](uint32_t at, int kt) {
-    const uint32_t* bits = holes ? s_bits + (kt >> 5) : nullptr;
-    issue_rows<DC>(at, kbase + kt * p.k.sl, p.k.sl, p.dim, klen - kt, bits, wv, lane);
-    issue_rows<DC>(at + D::TILE, vbase + kt * p.v.sl, p.v.sl, p.dim, klen - kt, bits, wv, lane);
-  };
-
+  const bool window = p.left != kNone || p.right != kNone;
+  // a key is kept where 0 <= key - query + back <= reach
+  const int back = p.left == kNone ? 0x3fffffff : p.left;
+  const uint32_t reach = (uint32_t)back + (p.right == kNone ? 0x3fffffffu : (uint32_t)p.right);
   f32x16 o[QB][DC];
   float top[QB], sum[QB];
 #pragma unroll
@@ -84,7 +96,6 @@ __global__ void __launch_bounds__(256, 2) attention_kernel(const AttP p) {
     for (int d = 0; d < DC; ++d) o[b][d] = f32x16{};
   }
   const int wq0 = q0 + wv * QB * 32, wq1 = wq0 + QB * 32 - 1;  // the wavefront's queries
-  if (kb < ke) issue(lds[0], kb);
   int buf = 0;
   for (int kt = kb; kt < ke; kt += 64, buf ^= 1) {
     // this tile is complete, and every wavefront is done with the other buffer
@@ -108,19 +119,11 @@ __global__ void __launch_bounds__(256, 2) attention_kernel(const AttP p) {
     }
     if (!whole) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint32_t w = lane_word(holes ? s_bits : nullptr, kt + u * 32, klen, lane);
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int b = 0; b < QB; ++b) {
-          const int ahead = kt + u * 32 + 4 * (lane >> 5) - qpos[b];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int a = ahead + acc_row(i);
-            const bool on = ((w >> acc_row(i)) & 1u) && a <= p.right && (p.left == kNone || a >= -p.left);
-            s[b][u][i] = on ? s[b][u][i] : -INFINITY;
-          }
-        }
-      }
+        for (int b = 0; b < QB; ++b)
+          mask_scores(s[b][u], kt + u * 32, klen, holes ? s_bits : nullptr, window,
+                      kt + u * 32 + 4 * (lane >> 5) - qpos[b] + back, reach, lane);
     }
     u32x4 pf[QB][4];
 #pragma unroll
@@ -162,6 +165,7 @@ __global__ void __launch_bounds__(256, 2) attention_kernel(const AttP p) {
       }
   }
 
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load is in flight to LDS when the workgroup ends
 #pragma unroll
   for (int b = 0; b < QB; ++b) {
     const float total = sum[b] + swap_half(sum[b]);
@@ -244,10 +248,11 @@ size_t forward_ws(const AttP& p) {
 }
 
 template <int EK, int DC>
-int launch_forward(const AttP& p, hipStream_t s) {
-  const int64_t grid = (int64_t)p.n * p.heads * p.tiles * p.splits;
-  if (grid > 0x7fffffff) return LIK_ERR_UNSUPPORTED;
-  launch_kernel(attention_kernel<EK, DC, 1>, dim3((unsigned)grid), dim3(256), p.km ? mask_words(p.k_len) * 4 : 0u, s, p);
+int launch_forward(AttP p, hipStream_t s) {
+  const int64_t per = (int64_t)p.tiles * p.splits;
+  const unsigned grid = work_grid(p, per * p.n * p.heads, per * p.group);
+  if (!grid) return LIK_ERR_UNSUPPORTED;
+  launch_kernel(attention_kernel<EK, DC, 1>, dim3(grid), dim3(256), p.km ? mask_words(p.k_len) * 4 : 0u, s, p);
   if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
   if (p.splits > 1) {
     const int64_t m = p.q_total * p.heads * (p.dim / 4);

@@ -82,7 +82,9 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p, int 
   extern __shared__ uint32_t s_bits[];
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  uint32_t t = xcd_tile(blockIdx.x, gridDim.x);
+  const int item = work_item(p);
+  if (item < 0) return;
+  uint32_t t = (uint32_t)item;
   const int tile = (int)(t % (uint32_t)p.tiles);
   t /= (uint32_t)p.tiles;
   const int head = (int)(t % (uint32_t)p.heads), seq = (int)(t / (uint32_t)p.heads);
@@ -132,6 +134,9 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p, int 
     issue_rows<DC>(at + D::TILE, vbase + kt * p.v.sl, p.v.sl, p.dim, klen - kt, bits, wv, lane);
   };
 
+  const bool window = p.left != kNone || p.right != kNone;
+  const int back = p.left == kNone ? 0x3fffffff : p.left;
+  const uint32_t reach = (uint32_t)back + (p.right == kNone ? 0x3fffffffu : (uint32_t)p.right);
   f32x16 acc[QB][DC];
 #pragma unroll
   for (int b = 0; b < QB; ++b)
@@ -163,17 +168,10 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p, int 
         }
       }
       if (!whole) {
-        const uint32_t w = lane_word(holes ? s_bits : nullptr, kt + u * 32, klen, lane);
 #pragma unroll
-        for (int b = 0; b < QB; ++b) {
-          const int ahead = kt + u * 32 + 4 * (lane >> 5) - qpos[b];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int a = ahead + acc_row(i);
-            const bool on = ((w >> acc_row(i)) & 1u) && a <= p.right && (p.left == kNone || a >= -p.left);
-            s[b][i] = on ? s[b][i] : -INFINITY;
-          }
-        }
+        for (int b = 0; b < QB; ++b)
+          mask_scores(s[b], kt + u * 32, klen, holes ? s_bits : nullptr, window,
+                      kt + u * 32 + 4 * (lane >> 5) - qpos[b] + back, reach, lane);
       }
       u32x4 df[QB][2];
 #pragma unroll
@@ -217,7 +215,9 @@ __global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p, int
   extern __shared__ uint32_t s_bits[];
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  uint32_t t = xcd_tile(blockIdx.x, gridDim.x);
+  const int item = work_item(p);
+  if (item < 0) return;
+  uint32_t t = (uint32_t)item;
   const int tile = (int)(t % (uint32_t)p.tiles);
   t /= (uint32_t)p.tiles;
   const int kv_heads = p.heads / p.group;
@@ -276,6 +276,9 @@ __global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p, int
     return x;
   };
 
+  // a query keeps a key where 0 <= query - key + ahead <= reach
+  const int ahead = p.right == kNone ? 0x3fffffff : p.right;
+  const uint32_t reach = (uint32_t)ahead + (p.left == kNone ? 0x3fffffffu : (uint32_t)p.left);
   f32x16 dk[KB][DC], dv[KB][DC];
 #pragma unroll
   for (int b = 0; b < KB; ++b)
@@ -325,15 +328,8 @@ __global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p, int
         }
         if (!whole) {
 #pragma unroll
-          for (int b = 0; b < KB; ++b) {
-            const int ahead = kpos[b] - (now + u * 32 + 4 * (lane >> 5));
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int a = ahead - acc_row(i);
-              const bool on = a <= p.right && (p.left == kNone || a >= -p.left);
-              s[b][i] = on ? s[b][i] : -INFINITY;
-            }
-          }
+          for (int b = 0; b < KB; ++b)
+            mask_scores(s[b], 0, 64, nullptr, true, now + u * 32 + 4 * (lane >> 5) - kpos[b] + ahead, reach, lane);
         }
         u32x4 pf[KB][2], df[KB][2];
 #pragma unroll
@@ -392,18 +388,19 @@ int launch_backward(AttP p, hipStream_t s) {
   if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
   const int parts = (int)wgs;
   p.tiles = (int)((p.q_len + 127) / 128);
-  int64_t grid = (int64_t)p.n * p.heads * p.tiles;
-  if (grid > 0x7fffffff) return LIK_ERR_UNSUPPORTED;
+  unsigned grid = work_grid(p, (int64_t)p.tiles * p.n * p.heads, (int64_t)p.tiles * p.group);
+  if (!grid) return LIK_ERR_UNSUPPORTED;
   if (p.gq) {
-    launch_kernel(attention_dq_kernel<EK, DC, 1>, dim3((unsigned)grid), dim3(256), p.km ? mask_words(p.k_len) * 4 : 0u, s,
+    launch_kernel(attention_dq_kernel<EK, DC, 1>, dim3(grid), dim3(256), p.km ? mask_words(p.k_len) * 4 : 0u, s,
                   p, parts);
     if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
   }
   p.tiles = (int)((p.k_len + 127) / 128);
-  grid = (int64_t)p.n * (p.heads / p.group) * p.tiles;
-  if (grid > 0x7fffffff) return LIK_ERR_UNSUPPORTED;
+  wgs = (int64_t)p.n * (p.heads / p.group) * p.tiles;
+  grid = work_grid(p, wgs, p.tiles);
+  if (!grid && wgs) return LIK_ERR_UNSUPPORTED;
   if (p.gk && grid) {
-    launch_kernel(attention_dkv_kernel<EK, DC, 1>, dim3((unsigned)grid), dim3(256), p.qm ? mask_words(p.q_len) * 4 : 0u,
+    launch_kernel(attention_dkv_kernel<EK, DC, 1>, dim3(grid), dim3(256), p.qm ? mask_words(p.q_len) * 4 : 0u,
                   s, p, parts);
     if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
   }
