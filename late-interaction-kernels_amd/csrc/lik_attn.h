@@ -125,39 +125,60 @@ struct Dim {
   }
 };
 
-// 64 rows into LDS by four wavefronts; row r at r * PITCH, chunks swizzled.
-// limit: rows that exist; bits (null: all): keep bits of the rows from row 0 of the tile.
+// 64 rows of one operand into LDS by four wavefronts; row r at r * PITCH, chunks swizzled. The lane offsets
+// within a tile are kept; rows that do not exist (limit) or are not kept (bits, null: all are) read as zeros.
 template <int DC>
-__device__ __forceinline__ void issue_rows(uint32_t lds, const char* base, int64_t ld, int dim, int limit,
-                                           const uint32_t* bits, int wv, int lane) {
+struct Rows {
   using D = Dim<DC>;
-  const u32x4 desc = raw_desc(base, 0xffffff00u);
+  uint32_t off[D::NI];
+  __device__ __forceinline__ Rows(int64_t ld, int dim, int wv, int lane) {
 #pragma unroll
-  for (int i = 0; i < D::NI; ++i) {
-    const int slot = (wv * D::NI + i) * 64 + lane, r = slot / D::SPR, c = (slot % D::SPR) ^ D::swz(r);
-    bool on = c * 8 < dim && r < limit;
-    if (bits) on = on && ((bits[r >> 5] >> (r & 31)) & 1u);
-    dma16(lds + (wv * D::NI + i) * 1024, on ? (uint32_t)(r * ld + c * 16) : kOob, desc);
+    for (int i = 0; i < D::NI; ++i) {
+      const int slot = (wv * D::NI + i) * 64 + lane, r = slot / D::SPR, c = (slot % D::SPR) ^ D::swz(r);
+      off[i] = c * 8 < dim ? (uint32_t)r * (uint32_t)ld + c * 16 : kOob;
+    }
   }
-}
-// MFMA operand of 32 rows from row0, elements 16 ks + 8 (lane / 32) ..
+  __device__ __forceinline__ void issue(uint32_t lds, const char* base, int limit, const uint32_t* bits, int wv,
+                                        int lane) const {
+    const u32x4 desc = raw_desc(base, 0xffffff00u);
+    if (limit >= 64 && !bits) {
+#pragma unroll
+      for (int i = 0; i < D::NI; ++i) dma16(lds + (wv * D::NI + i) * 1024, off[i], desc);
+    } else {
+#pragma unroll
+      for (int i = 0; i < D::NI; ++i) {
+        const int r = ((wv * D::NI + i) * 64 + lane) / D::SPR;
+        bool on = r < limit;
+        if (bits) on = on && ((bits[r >> 5] >> (r & 31)) & 1u);
+        dma16(lds + (wv * D::NI + i) * 1024, on ? off[i] : kOob, desc);
+      }
+    }
+  }
+};
+// Lane addresses of the MFMA operands in a tile (tiles start on 1 KB): the swizzle makes the k step (row-wise)
+// and the block of 32 columns (across) an exclusive or, everything else an immediate offset.
+// row(): rows row0 .. row0 + 31, elements 16 ks + 8 (lane / 32) ..
+// col(): lane l has element 32 db + l % 32 of rows row0 + 4 (l / 32) + {0..3, 8..11}, the order in which
+// accumulators hold rows (row0 a multiple of 16).
 template <int DC>
-__device__ __forceinline__ u32x4 row_frag(uint32_t lds, int row0, int ks, int lane) {
+struct Frags {
   using D = Dim<DC>;
-  const int r = row0 + (lane & 31);
-  return lds_b128(lds + r * Dim<DC>::PITCH + (((ks * 2 + (lane >> 5)) ^ D::swz(r)) << 4));
-}
-// The same rows across: lane l has element 32 db + l % 32 of rows
-// row0 + 4 (l / 32) + {0..3, 8..11}, the order in which accumulators hold rows.
-template <int DC>
-__device__ __forceinline__ u32x4 col_frag(uint32_t lds, int row0, int db, int lane) {
-  using D = Dim<DC>;
-  const int i = lane & 15, col = db * 32 + (lane & 16) + 4 * (i & 3);
-  const int r0 = row0 + 4 * (lane >> 5) + (i >> 2), r1 = r0 + 8;
-  const u32x2 lo = lds_tr(lds + r0 * Dim<DC>::PITCH + (((col >> 3) ^ D::swz(r0)) << 4) + ((col & 4) << 1));
-  const u32x2 hi = lds_tr(lds + r1 * Dim<DC>::PITCH + (((col >> 3) ^ D::swz(r1)) << 4) + ((col & 4) << 1));
-  return u32x4{lo[0], lo[1], hi[0], hi[1]};
-}
+  uint32_t r, lo, hi;
+  __device__ __forceinline__ explicit Frags(int lane) {
+    const int l32 = lane & 31, h = lane >> 5, i = lane & 15, col = (lane & 16) + 4 * (i & 3), c0 = 4 * h + (i >> 2);
+    r = l32 * D::PITCH + ((h ^ D::swz(l32)) << 4);
+    lo = c0 * D::PITCH + (((col >> 3) ^ D::swz(c0)) << 4) + ((col & 4) << 1);
+    hi = (c0 + 8) * D::PITCH + (((col >> 3) ^ D::swz(c0 + 8)) << 4) + ((col & 4) << 1);
+  }
+  __device__ __forceinline__ u32x4 row(uint32_t tile, int row0, int ks) const {
+    return lds_b128(((tile + r) ^ (ks << 5)) + row0 * D::PITCH);
+  }
+  __device__ __forceinline__ u32x4 col(uint32_t tile, int row0, int db) const {
+    const u32x2 a = lds_tr(((tile + lo) ^ (db << 6)) + row0 * D::PITCH);
+    const u32x2 b = lds_tr(((tile + hi) ^ (db << 6)) + row0 * D::PITCH);
+    return u32x4{a[0], a[1], b[0], b[1]};
+  }
+};
 // This lane's column operand of a row in memory (null: zeros): elements 16 ks + 8 (lane / 32) ..
 template <int DC>
 __device__ __forceinline__ void load_cols(u32x4* f, const char* row, int dim, int lane) {
@@ -224,7 +245,7 @@ __device__ __forceinline__ void store_cols(char* row, const f32x16* acc, float f
 
 // 16-byte rows; 64 of them within a lane's 32-bit offset
 inline bool att_rows_ok(const void* d, int64_t sn, int64_t sl, int64_t sh) {
-  return (uintptr_t)d % 16 == 0 && sn % 8 == 0 && sl % 8 == 0 && sh % 8 == 0 && sl >= 0 && sl < (1 << 24);
+  return (uintptr_t)d % 16 == 0 && sn % 8 == 0 && sl % 8 == 0 && sh % 8 == 0 && sl >= 0 && sl < (1 << 24);  // (64 rows of up to 2^25 bytes)
 }
 // Checks the arguments that both directions share and fills the parameters; false: nothing to do, or rc is an error.
 bool attention_shape(const lik_attention_t* a, AttP& p, int& rc);

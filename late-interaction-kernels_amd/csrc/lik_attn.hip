@@ -12,7 +12,7 @@ namespace {
 //   scores  S^T[key][query] = K Q^T   (K rows from LDS, Q in registers)
 //   output  O^T[d][query]  += V^T P^T (V by transposing LDS reads, P as it lies)
 template <int EK, int DC, int QB>
-__global__ void __launch_bounds__(256, 2) attention_kernel(const AttP p) {
+__global__ void __launch_bounds__(256, DC <= 2 ? 4 : 2) attention_kernel(const AttP p) {
   using D = Dim<DC>;
   __shared__ __attribute__((aligned(1024))) char s_tile[2][2 * D::TILE];
   __shared__ int s_kept[2];
@@ -34,13 +34,15 @@ __global__ void __launch_bounds__(256, 2) attention_kernel(const AttP p) {
 
   const char* kbase = p.k.data + (p.cu_k ? ks.row * p.k.sl : seq * p.k.sn) + kvh * p.k.sh;
   const char* vbase = p.v.data + (p.cu_k ? ks.row * p.v.sl : seq * p.v.sn) + kvh * p.v.sh;
+  const Rows<DC> krows(p.k.sl, p.dim, wv, lane), vrows(p.v.sl, p.dim, wv, lane);
+  const Frags<DC> frags(lane);
   const uint32_t lds[2] = {lds_addr(s_tile[0]), lds_addr(s_tile[1])};
   int klen = ks.len;
   bool holes = false;
   auto issue = [&](uint32_t at, int kt) {
     const uint32_t* bits = holes ? s_bits + (kt >> 5) : nullptr;
-    issue_rows<DC>(at, kbase + kt * p.k.sl, p.k.sl, p.dim, klen - kt, bits, wv, lane);
-    issue_rows<DC>(at + D::TILE, vbase + kt * p.v.sl, p.v.sl, p.dim, klen - kt, bits, wv, lane);
+    krows.issue(at, kbase + kt * p.k.sl, klen - kt, bits, wv, lane);
+    vrows.issue(at + D::TILE, vbase + kt * p.v.sl, klen - kt, bits, wv, lane);
   };
 
   // The first tile's loads start before the keep bits are known (and again without the masked rows, if there
@@ -112,7 +114,7 @@ __global__ void __launch_bounds__(256, 2) attention_kernel(const AttP p) {
       for (int b = 0; b < QB; ++b) s[b][u] = f32x16{};
 #pragma unroll
       for (int k = 0; k < D::KS; ++k) {
-        const u32x4 kf = row_frag<DC>(at, u * 32, k, lane);
+        const u32x4 kf = frags.row(at, u * 32, k);
 #pragma unroll
         for (int b = 0; b < QB; ++b) s[b][u] = mfma16<EK>(s[b][u], kf, qf[b][k]);
       }
@@ -133,10 +135,18 @@ __global__ void __launch_bounds__(256, 2) attention_kernel(const AttP p) {
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) m = fmaxf(m, s[b][u][i]);
-      m = fmaxf(fmaxf(m, swap_half(m)), top[b]);
-      const float mc = m == -INFINITY ? 0.f : m * p.c;
-      const float alpha = __builtin_amdgcn_exp2f(fmaf(top[b], p.c, -mc));
-      top[b] = m;
+      m = fmaxf(m, swap_half(m));
+      // The reference maximum only moves when a score passes it by more than 2^8: until then the probabilities
+      // are up to 256 instead of 1, which no type's relative rounding sees, and the output needs no rescaling.
+      if (__ballot(fmaf(m, p.c, -8.0f) > top[b] * p.c) != 0) {
+        const float up = fmaxf(m, top[b]);
+        const float alpha = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((top[b] - up) * p.c);
+        top[b] = up;
+        sum[b] *= alpha;
+#pragma unroll
+        for (int d = 0; d < DC; ++d) o[b][d] *= alpha;
+      }
+      const float mc = top[b] == -INFINITY ? 0.f : top[b] * p.c;
       float add = 0.f;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -146,9 +156,7 @@ __global__ void __launch_bounds__(256, 2) attention_kernel(const AttP p) {
           s[b][u][i] = e;
           add += e;
         }
-      sum[b] = fmaf(sum[b], alpha, add);
-#pragma unroll
-      for (int d = 0; d < DC; ++d) o[b][d] *= alpha;
+      sum[b] += add;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -159,7 +167,7 @@ __global__ void __launch_bounds__(256, 2) attention_kernel(const AttP p) {
     for (int k = 0; k < 4; ++k)
 #pragma unroll
       for (int d = 0; d < DC; ++d) {
-        const u32x4 vf = col_frag<DC>(at + D::TILE, k * 16, d, lane);
+        const u32x4 vf = frags.col(at + D::TILE, k * 16, d);
 #pragma unroll
         for (int b = 0; b < QB; ++b) o[b][d] = mfma16<EK>(o[b][d], vf, pf[b][k]);
       }

@@ -127,11 +127,13 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p, int 
 
   const char* kbase = p.k.data + (p.cu_k ? ks.row * p.k.sl : seq * p.k.sn) + kvh * p.k.sh;
   const char* vbase = p.v.data + (p.cu_k ? ks.row * p.v.sl : seq * p.v.sn) + kvh * p.v.sh;
+  const Rows<DC> krows(p.k.sl, p.dim, wv, lane), vrows(p.v.sl, p.dim, wv, lane);
+  const Frags<DC> frags(lane);
   const uint32_t lds[2] = {lds_addr(s_tile[0]), lds_addr(s_tile[1])};
   auto issue = [&](uint32_t at, int kt) {
     const uint32_t* bits = holes ? s_bits + (kt >> 5) : nullptr;
-    issue_rows<DC>(at, kbase + kt * p.k.sl, p.k.sl, p.dim, klen - kt, bits, wv, lane);
-    issue_rows<DC>(at + D::TILE, vbase + kt * p.v.sl, p.v.sl, p.dim, klen - kt, bits, wv, lane);
+    krows.issue(at, kbase + kt * p.k.sl, klen - kt, bits, wv, lane);
+    vrows.issue(at + D::TILE, vbase + kt * p.v.sl, klen - kt, bits, wv, lane);
   };
 
   const bool window = p.left != kNone || p.right != kNone;
@@ -159,8 +161,8 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p, int 
       for (int b = 0; b < QB; ++b) s[b] = dp[b] = f32x16{};
 #pragma unroll
       for (int k = 0; k < D::KS; ++k) {
-        const u32x4 kf = row_frag<DC>(at, u * 32, k, lane);
-        const u32x4 vf = row_frag<DC>(at + D::TILE, u * 32, k, lane);
+        const u32x4 kf = frags.row(at, u * 32, k);
+        const u32x4 vf = frags.row(at + D::TILE, u * 32, k);
 #pragma unroll
         for (int b = 0; b < QB; ++b) {
           s[b] = mfma16<EK>(s[b], kf, qf[b][k]);
@@ -190,7 +192,7 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p, int 
       for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int d = 0; d < DC; ++d) {
-          const u32x4 kf = col_frag<DC>(at, u * 32 + k * 16, d, lane);
+          const u32x4 kf = frags.col(at, u * 32 + k * 16, d);
 #pragma unroll
           for (int b = 0; b < QB; ++b) acc[b][d] = mfma16<EK>(acc[b][d], kf, df[b][k]);
         }
@@ -257,13 +259,15 @@ __global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p, int
   if (__syncthreads_or(any) == 0) qe = qb;
   const int steps = qe > qb ? (qe - qb + 63) / 64 : 0;  // of one head
 
+  const Rows<DC> qrows(p.q.sl, p.dim, wv, lane), grows(p.g.sl, p.dim, wv, lane);
+  const Frags<DC> frags(lane);
   const uint32_t lds[2] = {lds_addr(s_tile[0]), lds_addr(s_tile[1])};
   const char* q0 = p.q.data + (p.cu_q ? qs.row * p.q.sl : seq * p.q.sn);
   const char* g0 = p.g.data + (p.cu_q ? qs.row * p.g.sl : seq * p.g.sn);
   auto issue = [&](uint32_t at, int head, int qt) {
     const uint32_t* bits = holes ? s_bits + (qt >> 5) : nullptr;
-    issue_rows<DC>(at, q0 + head * p.q.sh + qt * p.q.sl, p.q.sl, p.dim, qlen - qt, bits, wv, lane);
-    issue_rows<DC>(at + D::TILE, g0 + head * p.g.sh + qt * p.g.sl, p.g.sl, p.dim, qlen - qt, bits, wv, lane);
+    qrows.issue(at, q0 + head * p.q.sh + qt * p.q.sl, qlen - qt, bits, wv, lane);
+    grows.issue(at + D::TILE, g0 + head * p.g.sh + qt * p.g.sl, qlen - qt, bits, wv, lane);
   };
   // threads 0..63: a query's statistic (+inf past the end: p = 0), 64..127: its delta
   auto stat = [&](int head, int qt) {
@@ -318,8 +322,8 @@ __global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p, int
         for (int b = 0; b < KB; ++b) s[b] = dp[b] = f32x16{};
 #pragma unroll
         for (int k = 0; k < D::KS; ++k) {
-          const u32x4 qf = row_frag<DC>(at, u * 32, k, lane);
-          const u32x4 gf = row_frag<DC>(at + D::TILE, u * 32, k, lane);
+          const u32x4 qf = frags.row(at, u * 32, k);
+          const u32x4 gf = frags.row(at + D::TILE, u * 32, k);
 #pragma unroll
           for (int b = 0; b < KB; ++b) {
             s[b] = mfma16<EK>(s[b], qf, kf[b][k]);
@@ -355,8 +359,8 @@ __global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p, int
         for (int k = 0; k < 2; ++k)
 #pragma unroll
           for (int d = 0; d < DC; ++d) {
-            const u32x4 gc = col_frag<DC>(at + D::TILE, u * 32 + k * 16, d, lane);
-            const u32x4 qc = col_frag<DC>(at, u * 32 + k * 16, d, lane);
+            const u32x4 gc = frags.col(at + D::TILE, u * 32 + k * 16, d);
+            const u32x4 qc = frags.col(at, u * 32 + k * 16, d);
 #pragma unroll
             for (int b = 0; b < KB; ++b) {
               dv[b][d] = mfma16<EK>(dv[b][d], gc, pf[b][k]);
