@@ -553,22 +553,23 @@ typedef struct {
  * out [n, q_len, heads, dim] (packed: [q_rows, heads, dim]), contiguous, in the
  * inputs' type. lse (optional) fp32 [heads, n * q_len] (packed: [heads, q_rows]): the
  * rows' softmax statistics for the backward pass (log2 of the sum of 2^(scale
- * log2(e) q k); +inf for a query that keeps no key). Packed rows that belong to
- * no sequence are left as they are.
+ * log2(e) q k); +inf for a query that keeps no key). out_low (optional, out's shape):
+ * what the rounding took off out, for the backward pass. Packed rows that belong
+ * to no sequence are left as they are.
  */
 size_t lik_attention_workspace_size(const lik_attention_t* a);
-int lik_attention(const lik_attention_t* a, void* out, float* lse, void* workspace, size_t workspace_bytes,
-                  lik_stream_t stream);
+int lik_attention(const lik_attention_t* a, void* out, float* lse, int8_t* out_low, void* workspace,
+                  size_t workspace_bytes, lik_stream_t stream);
 /*
- * Its gradients from out, lse and grad (out's shape, strides grad_stride_*; dim
+ * Its gradients from out, lse, out_low and grad (out's shape, strides grad_stride_*; dim
  * contiguous, 16-byte rows): grad_q like out, grad_k and grad_v contiguous
  * [n, k_len, kv_heads, dim] (packed: [k_rows, kv_heads, dim]); zeros in masked
  * rows. The probabilities are computed again from lse; sums are taken in a
  * fixed order.
  */
 size_t lik_attention_backward_workspace_size(const lik_attention_t* a);
-int lik_attention_backward(const lik_attention_t* a, const void* out, const float* lse, const void* grad,
-                           int64_t grad_stride_n, int64_t grad_stride_l, int64_t grad_stride_h, void* grad_q,
+int lik_attention_backward(const lik_attention_t* a, const void* out, const float* lse, const int8_t* out_low,
+                           const void* grad, int64_t grad_stride_n, int64_t grad_stride_l, int64_t grad_stride_h, void* grad_q,
                            void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes, lik_stream_t stream);
 
 /*

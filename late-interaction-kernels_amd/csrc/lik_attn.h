@@ -35,10 +35,12 @@ struct AttP {
   int left, right;                // INT32_MAX: unbounded
   float scale, c;                 // c = scale log2 e
   char* out;                      // [q_total][heads][dim]
+  int8_t* low;                    // what the output's rounding took off, by element (below); null: not kept
   float* lse;                     // [heads][q_total]: log2 of the sum of 2^(c q k); +inf where nothing is kept
   float* delta;                   // [heads][q_total]: sum_d g o
   char *gq, *gk, *gv;             // contiguous gradients
-  float* gmax;                    // fp16: [kMaxParts] largest |g| of a share of the rows each
+  float* gmax;                    // fp16: [sequence][head][q tile]: largest |g|
+  int q_tiles;                    // backward: q tiles of a sequence
   float* part_o;                  // forward split over keys: [split][q_total][heads][dim] fp32
   float* part_lse;                // [split][heads][q_total]
   int splits, tiles;              // q tiles (k tiles) of a sequence
@@ -117,7 +119,7 @@ constexpr int64_t kMaskMost = 1 << 18;  // tokens whose keep bits fit LDS beside
 template <int DC>
 struct Dim {
   static constexpr int KS = DC * 2, DB = DC, PITCH = DC <= 2 ? 128 : 256;
-  static constexpr int SPR = PITCH / 16, TILE = 64 * PITCH, NI = TILE / 1024 / 4;
+  static constexpr int SPR = PITCH / 16, TILE = 64 * PITCH;
   // 16-byte chunk c of row r lies at chunk c ^ swz(r): 16 consecutive rows at one chunk (row-wise reads)
   // cover the 64 banks, and so do any four rows of an aligned group at 64 bytes each (transposing reads).
   __device__ __forceinline__ static int swz(int r) {
@@ -125,32 +127,33 @@ struct Dim {
   }
 };
 
-// 64 rows of one operand into LDS by four wavefronts; row r at r * PITCH, chunks swizzled. The lane offsets
+// N (64) rows of one operand into LDS by four wavefronts; row r at r * PITCH, chunks swizzled. The lane offsets
 // within a tile are kept; rows that do not exist (limit) or are not kept (bits, null: all are) read as zeros.
-template <int DC>
+template <int DC, int N = 64>
 struct Rows {
   using D = Dim<DC>;
-  uint32_t off[D::NI];
+  static constexpr int NI = N * D::PITCH / 1024 / 4;
+  uint32_t off[NI];
   __device__ __forceinline__ Rows(int64_t ld, int dim, int wv, int lane) {
 #pragma unroll
-    for (int i = 0; i < D::NI; ++i) {
-      const int slot = (wv * D::NI + i) * 64 + lane, r = slot / D::SPR, c = (slot % D::SPR) ^ D::swz(r);
+    for (int i = 0; i < NI; ++i) {
+      const int slot = (wv * NI + i) * 64 + lane, r = slot / D::SPR, c = (slot % D::SPR) ^ D::swz(r);
       off[i] = c * 8 < dim ? (uint32_t)r * (uint32_t)ld + c * 16 : kOob;
     }
   }
   __device__ __forceinline__ void issue(uint32_t lds, const char* base, int limit, const uint32_t* bits, int wv,
                                         int lane) const {
     const u32x4 desc = raw_desc(base, 0xffffff00u);
-    if (limit >= 64 && !bits) {
+    if (limit >= N && !bits) {
 #pragma unroll
-      for (int i = 0; i < D::NI; ++i) dma16(lds + (wv * D::NI + i) * 1024, off[i], desc);
+      for (int i = 0; i < NI; ++i) dma16(lds + (wv * NI + i) * 1024, off[i], desc);
     } else {
 #pragma unroll
-      for (int i = 0; i < D::NI; ++i) {
-        const int r = ((wv * D::NI + i) * 64 + lane) / D::SPR;
+      for (int i = 0; i < NI; ++i) {
+        const int r = ((wv * NI + i) * 64 + lane) / D::SPR;
         bool on = r < limit;
         if (bits) on = on && ((bits[r >> 5] >> (r & 31)) & 1u);
-        dma16(lds + (wv * D::NI + i) * 1024, on ? off[i] : kOob, desc);
+        dma16(lds + (wv * NI + i) * 1024, on ? off[i] : kOob, desc);
       }
     }
   }
@@ -220,6 +223,29 @@ __device__ __forceinline__ void mask_scores(f32x16& s, int t, int end, const uin
   }
 }
 
+// The output's rounding error as a byte: the difference of the fp32 results' bits before and after the
+// rounding, in steps of 2^LOW fp32 units (256 steps from half a unit of the 16-bit type below to half above).
+// delta = sum_d g o cancels against g v in the backward pass: with the byte o is as good as fp32 there.
+template <int EK>
+constexpr int kLow = EK == EK_F16 ? 5 : 8;
+template <int EK>
+__device__ __forceinline__ uint32_t low_byte1(float o) {  // in byte 1
+  const int most = 1 << (kLow<EK> + 7);
+  const int d = (int)(__float_as_uint(o) - __float_as_uint(el_to_f32<EK>(f32_to_el<EK>(o)))) + (1 << (kLow<EK> - 1));
+  return (uint32_t)(d < -most ? -most : d > most - 1 ? most - 1 : d) << (8 - kLow<EK>);
+}
+template <int EK>
+__device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d) {
+  const uint32_t ab = __builtin_amdgcn_perm(low_byte1<EK>(b), low_byte1<EK>(a), 0x0c0c0501u);
+  return __builtin_amdgcn_perm(low_byte1<EK>(d), low_byte1<EK>(c), 0x05010c0cu) | ab;
+}
+// The value again, to a 256th of its rounding error (k: which byte of low).
+template <int EK>
+__device__ __forceinline__ float with_low(float r, uint32_t low, int k) {
+  const int byte = (int)(low << (24 - 8 * k)) >> 24;
+  return __uint_as_float(__float_as_uint(r) + (uint32_t)(byte << kLow<EK>));
+}
+
 // Four consecutive elements of accumulator quads 2 j and 2 j + 1 as 16-bit pairs
 // to eight consecutive ones a lane: half h then holds elements 16 j + 8 h + 0..7.
 __device__ __forceinline__ u32x4 join_halves(uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1) {
@@ -240,6 +266,21 @@ __device__ __forceinline__ void store_cols(char* row, const f32x16* acc, float f
                                   pack2<EK>(a[q * 4 + 6] * f, a[q * 4 + 7] * f));
       const int e = db * 32 + 8 * q + 8 * (lane >> 5);
       if (on && e < dim) *(u32x4*)(row + e * 2) = o;
+    }
+}
+// The same elements' bytes.
+template <int EK, int DC>
+__device__ __forceinline__ void store_low(int8_t* row, const f32x16* acc, float f, int dim, int lane, bool on) {
+#pragma unroll
+  for (int db = 0; db < DC; ++db)
+#pragma unroll
+    for (int q = 0; q < 4; q += 2) {
+      const f32x16& a = acc[db];
+      const auto s = __builtin_amdgcn_permlane32_swap(
+          low_bytes<EK>(a[q * 4] * f, a[q * 4 + 1] * f, a[q * 4 + 2] * f, a[q * 4 + 3] * f),
+          low_bytes<EK>(a[q * 4 + 4] * f, a[q * 4 + 5] * f, a[q * 4 + 6] * f, a[q * 4 + 7] * f), false, false);
+      const int e = db * 32 + 8 * q + 8 * (lane >> 5);
+      if (on && e < dim) *(u32x2*)(row + e) = u32x2{(uint32_t)s[0], (uint32_t)s[1]};
     }
 }
 

@@ -200,6 +200,7 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 4 : 2) attention_kernel(const A
 #pragma unroll
         for (int d = 0; d < DC; ++d) o[b][d] = f32x16{};
       store_cols<EK, DC>(p.out + (row * p.heads + head) * p.dim * 2, o[b], inv, p.dim, lane, on);
+      if (p.low) store_low<EK, DC>(p.low + (row * p.heads + head) * p.dim, o[b], inv, p.dim, lane, on);
     }
   }
 }
@@ -230,6 +231,8 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttP p) {
   if (p.lse && e == 0) p.lse[(int64_t)head * p.q_total + row] = top != -INFINITY ? top + __builtin_amdgcn_logf(total) : INFINITY;
   *(u32x2*)(p.out + (rh * p.dim + e) * 2) =
       u32x2{pack2<EK>(a[0] * inv, a[1] * inv), pack2<EK>(a[2] * inv, a[3] * inv)};
+  if (p.low)
+    *(uint32_t*)(p.low + rh * p.dim + e) = low_bytes<EK>(a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
 }
 
 }  // namespace
@@ -349,13 +352,13 @@ size_t lik_attention_workspace_size(const lik_attention_t* a) {
   return forward_ws(p);
 }
 
-int lik_attention(const lik_attention_t* a, void* out, float* lse, void* workspace, size_t workspace_bytes,
+int lik_attention(const lik_attention_t* a, void* out, float* lse, int8_t* out_low, void* workspace, size_t workspace_bytes,
                   lik_stream_t stream) {
   AttP p{};
   int rc;
   if (!attention_shape(a, p, rc)) return rc;
   if (!out) return LIK_ERR_INVALID;
-  if ((uintptr_t)out % 16) return LIK_ERR_UNSUPPORTED;
+  if ((uintptr_t)out % 16 || (uintptr_t)out_low % 16) return LIK_ERR_UNSUPPORTED;
   forward_shape(p);
   if (p.splits > 1) {
     if (!workspace || workspace_bytes < forward_ws(p)) return LIK_ERR_WORKSPACE;
@@ -365,6 +368,7 @@ int lik_attention(const lik_attention_t* a, void* out, float* lse, void* workspa
   }
   p.out = (char*)out;
   p.lse = lse;
+  p.low = out_low;
   return a->dtype == LIK_BF16 ? run_forward<EK_BF16>(p, (hipStream_t)stream)
                               : run_forward<EK_F16>(p, (hipStream_t)stream);
 }

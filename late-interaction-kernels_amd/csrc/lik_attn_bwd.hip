@@ -8,63 +8,16 @@
 // same bits every time) and no fp32 gradient of q to clear, add to and convert.
 // p and ds are rounded once to the 16-bit type, as the products' operands have to be.
 // fp16 would lose small gradients there: g is scaled by the power of two that
-// brings its largest element to 1/2 .. 1, and the sums are scaled back.
+// brings its largest element to 1/2 .. 1 (of a wavefront's queries; of a key head's), and the sums are scaled
+// back.
 #include "lik_attn.h"
 
 namespace lik {
 namespace enc {
 namespace {
 
-constexpr int kMaxParts = 256;
-
-// delta, and for fp16 the largest |g| of this workgroup's rows. 16 lanes a row.
-template <int EK>
-__global__ void __launch_bounds__(256) attention_delta_kernel(const AttP p) {
-  const int lane = threadIdx.x & 15;
-  const int64_t items = p.q_total * p.heads;
-  float big = 0.f;
-  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4; i < items; i += (int64_t)gridDim.x * 16) {
-    const int64_t row = i / p.heads;
-    const int head = (int)(i % p.heads);
-    const int64_t seq = p.cu_q ? 0 : row / p.q_len, pos = p.cu_q ? row : row % p.q_len;
-    float d = 0.f;
-    if (lane * 8 < p.dim && (!p.qm || p.qm[seq * p.qm_sn + pos * p.qm_sl] != 0)) {
-      const u32x4 g = *(const u32x4*)(p.g.data + seq * p.g.sn + pos * p.g.sl + head * p.g.sh + lane * 16);
-      const u32x4 o = *(const u32x4*)(p.out + i * p.dim * 2 + lane * 16);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float a, b, x, y;
-        unpack2<EK>(g[k], a, b);
-        unpack2<EK>(o[k], x, y);
-        d = fmaf(a, x, d);
-        d = fmaf(b, y, d);
-        if constexpr (EK == EK_F16) big = fmaxf(big, fmaxf(fabsf(a), fabsf(b)));
-      }
-    }
-#pragma unroll
-    for (int s = 1; s < 16; s <<= 1) d += __shfl_xor(d, s);
-    if (lane == 0) p.delta[(int64_t)head * p.q_total + row] = d;
-  }
-  if constexpr (EK == EK_F16) {
-    __shared__ float s_big[4];
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) big = fmaxf(big, __shfl_xor(big, s));
-    if ((threadIdx.x & 63) == 0) s_big[threadIdx.x >> 6] = big;
-    __syncthreads();
-    if (threadIdx.x == 0) p.gmax[blockIdx.x] = fmaxf(fmaxf(s_big[0], s_big[1]), fmaxf(s_big[2], s_big[3]));
-  }
-}
-
-// The power of two that scales ds (fp16); s_big: 4 floats of LDS. All threads.
-template <int EK>
-__device__ __forceinline__ float grad_scale(const AttP& p, int parts, float* s_big) {
-  if constexpr (EK != EK_F16) return 1.0f;
-  float big = (int)threadIdx.x < parts ? p.gmax[threadIdx.x] : 0.f;
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) big = fmaxf(big, __shfl_xor(big, s));
-  if ((threadIdx.x & 63) == 0) s_big[threadIdx.x >> 6] = big;
-  __syncthreads();
-  big = fmaxf(fmaxf(s_big[0], s_big[1]), fmaxf(s_big[2], s_big[3]));
+// The power of two that brings a largest |g| of `big` to 1/2 .. 1 (1 for zeros, infinities and NaN).
+__device__ __forceinline__ float scale_for(float big) {
   if (!(big > 0.f) || !(big < INFINITY)) return 1.0f;
   int e;
   frexpf(big, &e);  // big = m 2^e, m in 1/2 .. 1
@@ -72,9 +25,10 @@ __device__ __forceinline__ float grad_scale(const AttP& p, int parts, float* s_b
 }
 
 // Gradient of q: the forward's walk over the keys (K rows also by transposing
-// reads, V rows in LDS), dq^T[d][query] += K^T ds^T.
+// reads, V rows in LDS), dq^T[d][query] += K^T ds^T. Its queries' delta, which the other kernel reads, comes
+// from the same registers.
 template <int EK, int DC, int QB>
-__global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p, int parts) {
+__global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p) {
   using D = Dim<DC>;
   __shared__ __attribute__((aligned(1024))) char s_tile[2][2 * D::TILE];
   __shared__ int s_kept[2];
@@ -91,8 +45,11 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p, int 
   const int kvh = head / p.group;
   const Span qs = span_of(p.cu_q, p.q_rows, p.q_len, seq), ks = span_of(p.cu_k, p.k_rows, p.k_len, seq);
   const int q0 = tile * 128 * QB;
-  if (q0 >= qs.len) return;
-  const float gs = grad_scale<EK>(p, parts, s_big);
+  float* gmax = EK == EK_F16 ? p.gmax + ((int64_t)seq * p.heads + head) * p.q_tiles + tile : nullptr;
+  if (q0 >= qs.len) {
+    if (EK == EK_F16 && tid == 0) *gmax = 0.f;
+    return;
+  }
 
   int qpos[QB];
   float lse[QB], delta[QB];
@@ -100,18 +57,47 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p, int 
   const char* qbase = p.q.data + (p.cu_q ? qs.row * p.q.sl : seq * p.q.sn) + head * p.q.sh;
   const char* gbase = p.g.data + (p.cu_q ? qs.row * p.g.sl : seq * p.g.sn) + head * p.g.sh;
   bool any = false;
+  float big = 0.f;
 #pragma unroll
   for (int b = 0; b < QB; ++b) {
     qpos[b] = q0 + (wv * QB + b) * 32 + l32;
     const int64_t at = (int64_t)head * p.q_total + qs.row + qpos[b];
     lse[b] = qpos[b] < qs.len ? p.lse[at] : INFINITY;
     const bool on = lse[b] != INFINITY;  // +inf: past the end, masked, or without a key
-    delta[b] = on ? p.delta[at] : 0.f;
     load_cols<DC>(qf[b], on ? qbase + qpos[b] * p.q.sl : nullptr, p.dim, lane);
     load_cols<DC>(gf[b], on ? gbase + qpos[b] * p.g.sl : nullptr, p.dim, lane);
+    const int64_t row = ((qs.row + qpos[b]) * p.heads + head) * p.dim;
+    u32x4 of[D::KS];
+    load_cols<DC>(of, on ? p.out + row * 2 : nullptr, p.dim, lane);
+    float d = 0.f;
+#pragma unroll
+    for (int k = 0; k < D::KS; ++k) {
+      const int e = k * 16 + 8 * (lane >> 5);
+      u32x2 low = {0u, 0u};
+      if (on && e < p.dim) low = *(const u32x2*)(p.low + row + e);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float g[2], o[2];
+        unpack2<EK>(gf[b][k][i / 2], g[0], g[1]);
+        unpack2<EK>(of[k][i / 2], o[0], o[1]);
+        d = fmaf(g[i % 2], with_low<EK>(o[i % 2], low[i / 4], i % 4), d);
+        if constexpr (EK == EK_F16) big = fmaxf(big, fabsf(g[i % 2]));
+      }
+    }
+    delta[b] = d + swap_half(d);
+    if (qpos[b] < qs.len && lane < 32) p.delta[at] = delta[b];
     any |= on;
   }
   any = __ballot(any) != 0;
+  float gs = 1.0f;  // of this wavefront's queries
+  if constexpr (EK == EK_F16) {
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) big = fmaxf(big, __shfl_xor(big, s));
+    if (lane == 0) s_big[wv] = big;
+    gs = scale_for(big);
+    __syncthreads();
+    if (tid == 0) *gmax = fmaxf(fmaxf(s_big[0], s_big[1]), fmaxf(s_big[2], s_big[3]));
+  }
 
   int klen = ks.len;
   bool holes = false;
@@ -123,7 +109,7 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p, int 
   const int q_end = (q0 + 128 * QB < qs.len ? q0 + 128 * QB : qs.len) - 1;
   const int kb = p.left == kNone || q0 - p.left < 0 ? 0 : (q0 - p.left) & ~63;
   int ke = p.right == kNone || (int64_t)q_end + p.right + 1 >= klen ? klen : q_end + p.right + 1;
-  if (__syncthreads_or(any) == 0) ke = kb;
+  if (__syncthreads_or(any) == 0 || !p.gq) ke = kb;
 
   const char* kbase = p.k.data + (p.cu_k ? ks.row * p.k.sl : seq * p.k.sn) + kvh * p.k.sh;
   const char* vbase = p.v.data + (p.cu_k ? ks.row * p.v.sl : seq * p.v.sn) + kvh * p.v.sh;
@@ -198,20 +184,26 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p, int 
         }
     }
   }
+  if (!p.gq) return;
 #pragma unroll
   for (int b = 0; b < QB; ++b)
     store_cols<EK, DC>(p.gq + ((qs.row + qpos[b]) * p.heads + head) * p.dim * 2, acc[b], p.scale / gs, p.dim, lane,
                        qpos[b] < qs.len);
 }
 
-// Gradients of k and v: a wavefront owns 32 KB keys as MFMA columns, K and V in
-// registers, and walks the queries of the group's heads, 64 at a time.
+// Gradients of k and v: a wavefront owns 32 KB keys as MFMA columns and walks the queries of the group's
+// heads, QT at a time. K and V are in registers; for head dims over 64 V's rows stay in LDS instead and the
+// steps are 32 queries (two wavefronts a SIMD then fit: 455 -> 250 us for 16 x 1030 causal rows, 16 / 4 heads).
 //   P[query][key] from S = Q K^T;  dv^T[d][key] += G^T P;  dp = G V^T;  dk^T[d][key] += Q^T ds
 template <int EK, int DC, int KB>
-__global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p, int parts) {
+__global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p) {
   using D = Dim<DC>;
-  __shared__ __attribute__((aligned(1024))) char s_tile[2][2 * D::TILE];
-  __shared__ __attribute__((aligned(16))) float s_stat[2][2][64];
+  constexpr bool VL = DC > 2;  // V in LDS
+  constexpr int QT = VL ? 32 : 64, TILE = D::PITCH * QT;
+  static_assert(!VL || KB == 1, "");
+  __shared__ __attribute__((aligned(1024))) char s_tile[2][2 * TILE];
+  __shared__ __attribute__((aligned(1024))) char s_v[VL ? 2 * D::TILE : 16];
+  __shared__ __attribute__((aligned(16))) float s_stat[2][2][QT];
   __shared__ int s_kept[2];
   __shared__ float s_big[4];
   extern __shared__ uint32_t s_bits[];
@@ -227,11 +219,21 @@ __global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p, int
   const Span qs = span_of(p.cu_q, p.q_rows, p.q_len, seq), ks = span_of(p.cu_k, p.k_rows, p.k_len, seq);
   const int k0 = tile * 128 * KB;
   if (k0 >= ks.len) return;
-  const float gs = grad_scale<EK>(p, parts, s_big);
+  float gs = 1.0f;
+  if constexpr (EK == EK_F16) {
+    const float* gm = p.gmax + ((int64_t)seq * p.heads + kvh * p.group) * p.q_tiles;
+    float big = 0.f;
+    for (int i = tid; i < p.group * p.q_tiles; i += 256) big = fmaxf(big, gm[i]);
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) big = fmaxf(big, __shfl_xor(big, s));
+    if (lane == 0) s_big[wv] = big;
+    __syncthreads();
+    gs = scale_for(fmaxf(fmaxf(s_big[0], s_big[1]), fmaxf(s_big[2], s_big[3])));
+  }
 
   int kpos[KB];
   bool kon[KB];
-  u32x4 kf[KB][D::KS], vf[KB][D::KS];
+  u32x4 kf[KB][D::KS], vf[KB][VL ? 1 : D::KS];
   const char* kbase = p.k.data + (p.cu_k ? ks.row * p.k.sl : seq * p.k.sn) + kvh * p.k.sh;
   const char* vbase = p.v.data + (p.cu_k ? ks.row * p.v.sl : seq * p.v.sn) + kvh * p.v.sh;
   bool any = false;
@@ -240,10 +242,16 @@ __global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p, int
     kpos[b] = k0 + (wv * KB + b) * 32 + l32;
     kon[b] = kpos[b] < ks.len && (!p.km || p.km[seq * p.km_sn + kpos[b] * p.km_sl] != 0);
     load_cols<DC>(kf[b], kon[b] ? kbase + kpos[b] * p.k.sl : nullptr, p.dim, lane);
-    load_cols<DC>(vf[b], kon[b] ? vbase + kpos[b] * p.v.sl : nullptr, p.dim, lane);
+    if constexpr (!VL) load_cols<DC>(vf[b], kon[b] ? vbase + kpos[b] * p.v.sl : nullptr, p.dim, lane);
     any |= kon[b];
   }
   any = __ballot(any) != 0;
+  if constexpr (VL) {  // (what masked rows hold stays in their own columns)
+    const Rows<DC> vrows(p.v.sl, p.dim, wv, lane);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      vrows.issue(lds_addr(s_v) + i * D::TILE, vbase + (k0 + 64 * i) * p.v.sl, ks.len - k0 - 64 * i, nullptr, wv, lane);
+  }
 
   int qlen = qs.len;
   bool holes = false;
@@ -257,9 +265,9 @@ __global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p, int
   const int qb = p.right == kNone || k0 - p.right < 0 ? 0 : (k0 - p.right) & ~63;
   int qe = p.left == kNone || (int64_t)k_end + p.left + 1 >= qlen ? qlen : k_end + p.left + 1;
   if (__syncthreads_or(any) == 0) qe = qb;
-  const int steps = qe > qb ? (qe - qb + 63) / 64 : 0;  // of one head
+  const int steps = qe > qb ? (qe - qb + QT - 1) / QT : 0;  // of one head
 
-  const Rows<DC> qrows(p.q.sl, p.dim, wv, lane), grows(p.g.sl, p.dim, wv, lane);
+  const Rows<DC, QT> qrows(p.q.sl, p.dim, wv, lane), grows(p.g.sl, p.dim, wv, lane);
   const Frags<DC> frags(lane);
   const uint32_t lds[2] = {lds_addr(s_tile[0]), lds_addr(s_tile[1])};
   const char* q0 = p.q.data + (p.cu_q ? qs.row * p.q.sl : seq * p.q.sn);
@@ -267,15 +275,15 @@ __global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p, int
   auto issue = [&](uint32_t at, int head, int qt) {
     const uint32_t* bits = holes ? s_bits + (qt >> 5) : nullptr;
     qrows.issue(at, q0 + head * p.q.sh + qt * p.q.sl, qlen - qt, bits, wv, lane);
-    grows.issue(at + D::TILE, g0 + head * p.g.sh + qt * p.g.sl, qlen - qt, bits, wv, lane);
+    grows.issue(at + TILE, g0 + head * p.g.sh + qt * p.g.sl, qlen - qt, bits, wv, lane);
   };
-  // threads 0..63: a query's statistic (+inf past the end: p = 0), 64..127: its delta
+  // threads 0..QT - 1: a query's statistic (+inf past the end: p = 0), QT..2 QT - 1: its delta
   auto stat = [&](int head, int qt) {
     float x = 0.f;
-    if (tid < 128) {
-      const int pos = qt + (tid & 63);
+    if (tid < 2 * QT) {
+      const int pos = qt + tid % QT;
       const int64_t at = (int64_t)head * p.q_total + qs.row + pos;
-      x = pos < qlen ? (tid < 64 ? p.lse[at] : p.delta[at]) : tid < 64 ? INFINITY : 0.f;
+      x = pos < qlen ? (tid < QT ? p.lse[at] : p.delta[at]) : tid < QT ? INFINITY : 0.f;
     }
     return x;
   };
@@ -294,13 +302,13 @@ __global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p, int
   if (total) {
     const float x = stat(head, qt);
     issue(lds[0], head, qt);
-    if (tid < 128) s_stat[0][tid >> 6][tid & 63] = x;
+    if (tid < 2 * QT) s_stat[0][tid / QT][tid % QT] = x;
   }
   int buf = 0;
   for (int it = 0; it < total; ++it, buf ^= 1) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     const int now = qt;
-    qt += 64;
+    qt += QT;
     if (qt >= qe) {
       qt = qb;
       ++head;
@@ -310,24 +318,24 @@ __global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p, int
       next = stat(head, qt);
       issue(buf ? lds[0] : lds[1], head, qt);
     }
-    const bool skip = !any || (p.left != kNone && now > wk1 + p.left) || (p.right != kNone && now + 63 < wk0 - p.right);
+    const bool skip = !any || (p.left != kNone && now > wk1 + p.left) || (p.right != kNone && now + QT - 1 < wk0 - p.right);
     if (!skip) {
       const uint32_t at = buf ? lds[1] : lds[0];
       const bool whole =
-          (p.left == kNone || now + 63 <= wk0 + p.left) && (p.right == kNone || now >= wk1 - p.right);
+          (p.left == kNone || now + QT - 1 <= wk0 + p.left) && (p.right == kNone || now >= wk1 - p.right);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < QT / 32; ++u) {
         f32x16 s[KB], dp[KB];
 #pragma unroll
         for (int b = 0; b < KB; ++b) s[b] = dp[b] = f32x16{};
 #pragma unroll
         for (int k = 0; k < D::KS; ++k) {
           const u32x4 qf = frags.row(at, u * 32, k);
-          const u32x4 gf = frags.row(at + D::TILE, u * 32, k);
+          const u32x4 gf = frags.row(at + TILE, u * 32, k);
 #pragma unroll
           for (int b = 0; b < KB; ++b) {
             s[b] = mfma16<EK>(s[b], qf, kf[b][k]);
-            dp[b] = mfma16<EK>(dp[b], gf, vf[b][k]);
+            dp[b] = mfma16<EK>(dp[b], gf, VL ? frags.row(lds_addr(s_v), wv * 32, k) : vf[b][VL ? 0 : k]);
           }
         }
         if (!whole) {
@@ -359,7 +367,7 @@ __global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p, int
         for (int k = 0; k < 2; ++k)
 #pragma unroll
           for (int d = 0; d < DC; ++d) {
-            const u32x4 gc = frags.col(at + D::TILE, u * 32 + k * 16, d);
+            const u32x4 gc = frags.col(at + TILE, u * 32 + k * 16, d);
             const u32x4 qc = frags.col(at, u * 32 + k * 16, d);
 #pragma unroll
             for (int b = 0; b < KB; ++b) {
@@ -369,8 +377,9 @@ __global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p, int
           }
       }
     }
-    if (it + 1 < total && tid < 128) s_stat[buf ^ 1][tid >> 6][tid & 63] = next;
+    if (it + 1 < total && tid < 2 * QT) s_stat[buf ^ 1][tid / QT][tid % QT] = next;
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // V's loads where there was no step
 #pragma unroll
   for (int b = 0; b < KB; ++b) {
     if (!kon[b])  // masked keys have no gradient (their lanes ran on zero rows)
@@ -384,31 +393,18 @@ __global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p, int
 
 template <int EK, int DC>
 int launch_backward(AttP p, hipStream_t s) {
-  const int64_t items = p.q_total * p.heads;
-  int64_t wgs = (items + 15) / 16;
-  if (EK == EK_F16 && wgs > kMaxParts) wgs = kMaxParts;
-  if (wgs > 1 << 16) wgs = 1 << 16;
-  launch_kernel(attention_delta_kernel<EK>, dim3((unsigned)wgs), dim3(256), 0u, s, p);
-  if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
-  const int parts = (int)wgs;
-  p.tiles = (int)((p.q_len + 127) / 128);
+  p.tiles = p.q_tiles;
   unsigned grid = work_grid(p, (int64_t)p.tiles * p.n * p.heads, (int64_t)p.tiles * p.group);
   if (!grid) return LIK_ERR_UNSUPPORTED;
-  if (p.gq) {
-    launch_kernel(attention_dq_kernel<EK, DC, 1>, dim3(grid), dim3(256), p.km ? mask_words(p.k_len) * 4 : 0u, s,
-                  p, parts);
-    if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
-  }
+  launch_kernel(attention_dq_kernel<EK, DC, 1>, dim3(grid), dim3(256), p.km ? mask_words(p.k_len) * 4 : 0u, s, p);
+  if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
   p.tiles = (int)((p.k_len + 127) / 128);
-  wgs = (int64_t)p.n * (p.heads / p.group) * p.tiles;
+  const int64_t wgs = (int64_t)p.n * (p.heads / p.group) * p.tiles;
+  if (!p.gk || !wgs) return LIK_OK;
   grid = work_grid(p, wgs, p.tiles);
-  if (!grid && wgs) return LIK_ERR_UNSUPPORTED;
-  if (p.gk && grid) {
-    launch_kernel(attention_dkv_kernel<EK, DC, 1>, dim3(grid), dim3(256), p.qm ? mask_words(p.q_len) * 4 : 0u,
-                  s, p, parts);
-    if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
-  }
-  return LIK_OK;
+  if (!grid) return LIK_ERR_UNSUPPORTED;
+  launch_kernel(attention_dkv_kernel<EK, DC, 1>, dim3(grid), dim3(256), p.qm ? mask_words(p.q_len) * 4 : 0u, s, p);
+  return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;
 }
 
 template <int EK>
@@ -419,7 +415,10 @@ int run_backward(const AttP& p, hipStream_t s) {
   return launch_backward<EK, 4>(p, s);
 }
 
-size_t backward_ws(const AttP& p) { return align256((size_t)p.q_total * p.heads * 4) + kMaxParts * 4 + 256; }
+int q_tiles(const AttP& p) { return (int)((p.q_len + 127) / 128); }
+size_t backward_ws(const AttP& p) {
+  return align256((size_t)p.q_total * p.heads * 4) + (size_t)p.n * p.heads * q_tiles(p) * 4 + 256;
+}
 
 }  // namespace
 }  // namespace enc
@@ -436,14 +435,15 @@ size_t lik_attention_backward_workspace_size(const lik_attention_t* a) {
   return attention_shape(a, p, rc) ? backward_ws(p) : 0;
 }
 
-int lik_attention_backward(const lik_attention_t* a, const void* out, const float* lse, const void* grad,
+int lik_attention_backward(const lik_attention_t* a, const void* out, const float* lse, const int8_t* out_low,
+                           const void* grad,
                            int64_t grad_stride_n, int64_t grad_stride_l, int64_t grad_stride_h, void* grad_q,
                            void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes, lik_stream_t stream) {
   AttP p{};
   int rc;
   if (!attention_shape(a, p, rc)) return rc != LIK_OK ? rc : LIK_ERR_INVALID;  // no query: nothing writes grad_k
-  if (!out || !lse || !grad || !grad_k != !grad_v) return LIK_ERR_INVALID;
-  if (!att_rows_ok(grad, grad_stride_n, grad_stride_l, grad_stride_h) || (uintptr_t)out % 16 ||
+  if (!out || !lse || !out_low || !grad || !grad_k != !grad_v) return LIK_ERR_INVALID;
+  if (!att_rows_ok(grad, grad_stride_n, grad_stride_l, grad_stride_h) || (uintptr_t)out % 16 || (uintptr_t)out_low % 16 ||
       (uintptr_t)grad_q % 16 || (uintptr_t)grad_k % 16 || (uintptr_t)grad_v % 16)
     return LIK_ERR_UNSUPPORTED;
   if (!workspace || workspace_bytes < backward_ws(p)) return LIK_ERR_WORKSPACE;
@@ -452,6 +452,8 @@ int lik_attention_backward(const lik_attention_t* a, const void* out, const floa
   p.gmax = (float*)(ws + align256((size_t)p.q_total * p.heads * 4));
   p.out = (char*)const_cast<void*>(out);
   p.lse = const_cast<float*>(lse);
+  p.low = const_cast<int8_t*>(out_low);
+  p.q_tiles = q_tiles(p);
   p.g = {(const char*)grad, grad_stride_n * 2, grad_stride_l * 2, grad_stride_h * 2};
   p.gq = (char*)grad_q;
   p.gk = (char*)grad_k;

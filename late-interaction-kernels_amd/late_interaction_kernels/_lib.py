@@ -311,11 +311,11 @@ def load() -> ctypes.CDLL:
     lib.lik_gated_ffn_backward.restype = ctypes.c_int
     lib.lik_attention_workspace_size.argtypes = [P(LikAttention)]
     lib.lik_attention_workspace_size.restype = ctypes.c_size_t
-    lib.lik_attention.argtypes = [P(LikAttention), _p, _p, _p, ctypes.c_size_t, _p]
+    lib.lik_attention.argtypes = [P(LikAttention), _p, _p, _p, _p, ctypes.c_size_t, _p]
     lib.lik_attention.restype = ctypes.c_int
     lib.lik_attention_backward_workspace_size.argtypes = [P(LikAttention)]
     lib.lik_attention_backward_workspace_size.restype = ctypes.c_size_t
-    lib.lik_attention_backward.argtypes = [P(LikAttention), _p, _p, _p, _i64, _i64, _i64, _p, _p, _p, _p,
+    lib.lik_attention_backward.argtypes = [P(LikAttention), _p, _p, _p, _p, _i64, _i64, _i64, _p, _p, _p, _p,
                                            ctypes.c_size_t, _p]
     lib.lik_attention_backward.restype = ctypes.c_int
     _lib = lib

@@ -42,37 +42,38 @@ def _args(q, k, v, meta, qm, km, cu_q, cu_k):
     return s
 
 
-def _forward(q, k, v, meta, qm, km, cu_q, cu_k, want_lse):
+def _forward(q, k, v, meta, qm, km, cu_q, cu_k, train):
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     rows = q.numel() // (q.shape[-1] * q.shape[-2])
-    lse = torch.empty(q.shape[-2], rows, dtype=torch.float32, device=q.device) if want_lse else None
+    lse = torch.empty(q.shape[-2], rows, dtype=torch.float32, device=q.device) if train else None
+    low = torch.empty(q.shape, dtype=torch.int8, device=q.device) if train else None
     if q.numel() == 0:
-        return out, lse
+        return out, lse, low
     a = _args(q, k, v, meta, qm, km, cu_q, cu_k)
     if a.n == 0 or a.q_len == 0:  # packed rows in no sequence
-        return out.zero_(), lse
+        return out.zero_(), lse, low
     lib = _lib.load()
     nbytes = lib.lik_attention_workspace_size(ctypes.byref(a))
     ws = _lib.workspace(nbytes, q.device)
     with _lib.on_device(q.device):
-        rc = lib.lik_attention(ctypes.byref(a), out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), nbytes,
-                               _lib.stream_of(q))
+        rc = lib.lik_attention(ctypes.byref(a), out.data_ptr(), _lib.ptr(lse), _lib.ptr(low), _lib.ptr(ws),
+                               nbytes, _lib.stream_of(q))
     _lib.check(rc, "lik_attention")
-    return out, lse
+    return out, lse, low
 
 
 class _AttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, meta, qm, km, cu_q, cu_k):
         q, k, v = (_lib.prepare_tokens(t) for t in (q, k, v))
-        out, lse = _forward(q, k, v, meta, qm, km, cu_q, cu_k, True)
-        ctx.save_for_backward(q, k, v, out, lse, qm, km, cu_q, cu_k)
+        out, lse, low = _forward(q, k, v, meta, qm, km, cu_q, cu_k, True)
+        ctx.save_for_backward(q, k, v, out, lse, low, qm, km, cu_q, cu_k)
         ctx.meta = meta
         return out
 
     @staticmethod
     def backward(ctx, grad):
-        q, k, v, out, lse, qm, km, cu_q, cu_k = ctx.saved_tensors
+        q, k, v, out, lse, low, qm, km, cu_q, cu_k = ctx.saved_tensors
         need_q, need_k, need_v = ctx.needs_input_grad[:3]
         a = _args(q, k, v, ctx.meta, qm, km, cu_q, cu_k)
         none = q.numel() == 0 or a.n == 0 or a.q_len == 0 or a.k_len == 0
@@ -88,7 +89,7 @@ class _AttentionFn(torch.autograd.Function):
             ws = _lib.workspace(nbytes, q.device)
             with _lib.on_device(q.device):
                 rc = lib.lik_attention_backward(
-                    ctypes.byref(a), out.data_ptr(), lse.data_ptr(), g.data_ptr(),
+                    ctypes.byref(a), out.data_ptr(), lse.data_ptr(), low.data_ptr(), g.data_ptr(),
                     0 if cu_q is not None else g.stride(0), g.stride(-3), g.stride(-2), _lib.ptr(gq), _lib.ptr(gk),
                     _lib.ptr(gv), _lib.ptr(ws), nbytes, _lib.stream_of(q))
             _lib.check(rc, "lik_attention_backward")
@@ -130,7 +131,7 @@ def _run(q, k, v, meta, qm, km, cu_q, cu_k):
         out = _AttentionFn.apply(q, k, v, meta, qm, km, cu_q, cu_k)
     else:
         q, k, v = (_lib.prepare_tokens(t) for t in (q, k, v))
-        out, _ = _forward(q, k, v, meta, qm, km, cu_q, cu_k, False)
+        out, _, _ = _forward(q, k, v, meta, qm, km, cu_q, cu_k, False)
     return out[..., :d] if d % 8 else out
 
 
