@@ -44,6 +44,7 @@ struct AttP {
   float* part_o;                  // forward split over keys: [split][q_total][heads][dim] fp32
   float* part_lse;                // [split][heads][q_total]
   int splits, tiles;              // q tiles (k tiles) of a sequence
+  bool few;                       // forward: attention_rows_kernel
   int chunk, wgs;                 // workgroups: `chunk` in a row go to one XCD; wgs of them have work
 };
 
@@ -127,12 +128,12 @@ struct Dim {
   }
 };
 
-// N (64) rows of one operand into LDS by four wavefronts; row r at r * PITCH, chunks swizzled. The lane offsets
+// N rows of one operand into LDS by NW wavefronts (wv: which of them this is); row r at r * PITCH, chunks swizzled. The lane offsets
 // within a tile are kept; rows that do not exist (limit) or are not kept (bits, null: all are) read as zeros.
-template <int DC, int N = 64>
+template <int DC, int N = 64, int NW = 4>
 struct Rows {
   using D = Dim<DC>;
-  static constexpr int NI = N * D::PITCH / 1024 / 4;
+  static constexpr int NI = N * D::PITCH / 1024 / NW;
   uint32_t off[NI];
   __device__ __forceinline__ Rows(int64_t ld, int dim, int wv, int lane) {
 #pragma unroll

@@ -6,6 +6,61 @@ namespace lik {
 namespace enc {
 namespace {
 
+// One step of the softmax on 32 NU scores of a lane's column: s to probabilities, packed as MFMA operands in pf;
+// top, sum and the output so far follow the running maximum.
+template <int EK, int DC, int NU>
+__device__ __forceinline__ void softmax_step(f32x16 (&s)[NU], f32x16 (&o)[DC], float& top, float& sum, float c,
+                                             u32x4 (&pf)[2 * NU]) {
+  float m = s[0][0];
+#pragma unroll
+  for (int u = 0; u < NU; ++u)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = fmaxf(m, s[u][i]);
+  m = fmaxf(m, swap_half(m));
+  // The reference maximum only moves when a score passes it by more than 2^8: until then the probabilities
+  // are up to 256 instead of 1, which no type's relative rounding sees, and the output needs no rescaling.
+  if (__ballot(fmaf(m, c, -8.0f) > top * c) != 0) {
+    const float up = fmaxf(m, top);
+    const float alpha = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((top - up) * c);
+    top = up;
+    sum *= alpha;
+#pragma unroll
+    for (int d = 0; d < DC; ++d) o[d] *= alpha;
+  }
+  const float mc = top == -INFINITY ? 0.f : top * c;
+  float add = 0.f;
+#pragma unroll
+  for (int u = 0; u < NU; ++u)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float e = __builtin_amdgcn_exp2f(fmaf(s[u][i], c, -mc));
+      s[u][i] = e;
+      add += e;
+    }
+  sum += add;
+#pragma unroll
+  for (int k = 0; k < 2 * NU; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) pf[k][e] = pack2<EK>(s[k / 2][(k % 2) * 8 + 2 * e], s[k / 2][(k % 2) * 8 + 2 * e + 1]);
+}
+
+// One split's share of a row's output: its mean of the values in fp32, and its statistic.
+template <int DC>
+__device__ __forceinline__ void store_part(const AttP& p, int split, int64_t row, int head, const f32x16 (&o)[DC],
+                                           float inv, float lse, int lane) {
+  if (lane < 32) p.part_lse[((int64_t)split * p.heads + head) * p.q_total + row] = lse;
+  float* at = p.part_o + (((int64_t)split * p.q_total + row) * p.heads + head) * p.dim;
+#pragma unroll
+  for (int d = 0; d < DC; ++d)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int e = d * 32 + 8 * q + 4 * (lane >> 5);
+      if (e < p.dim)
+        *(f32x4*)(at + e) =
+            f32x4{o[d][q * 4] * inv, o[d][q * 4 + 1] * inv, o[d][q * 4 + 2] * inv, o[d][q * 4 + 3] * inv};
+    }
+}
+
 // A workgroup of four wavefronts owns 128 QB queries of one head, a wavefront 32 QB
 // of them as MFMA columns, and walks the keys that any of them keeps, 64 at a
 // time, in two LDS buffers: the next tile is loaded while this one is used.
@@ -129,40 +184,7 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 4 : 2) attention_kernel(const A
     }
     u32x4 pf[QB][4];
 #pragma unroll
-    for (int b = 0; b < QB; ++b) {
-      float m = s[b][0][0];
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) m = fmaxf(m, s[b][u][i]);
-      m = fmaxf(m, swap_half(m));
-      // The reference maximum only moves when a score passes it by more than 2^8: until then the probabilities
-      // are up to 256 instead of 1, which no type's relative rounding sees, and the output needs no rescaling.
-      if (__ballot(fmaf(m, p.c, -8.0f) > top[b] * p.c) != 0) {
-        const float up = fmaxf(m, top[b]);
-        const float alpha = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((top[b] - up) * p.c);
-        top[b] = up;
-        sum[b] *= alpha;
-#pragma unroll
-        for (int d = 0; d < DC; ++d) o[b][d] *= alpha;
-      }
-      const float mc = top[b] == -INFINITY ? 0.f : top[b] * p.c;
-      float add = 0.f;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float e = __builtin_amdgcn_exp2f(fmaf(s[b][u][i], p.c, -mc));
-          s[b][u][i] = e;
-          add += e;
-        }
-      sum[b] += add;
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          pf[b][k][e] = pack2<EK>(s[b][k / 2][(k % 2) * 8 + 2 * e], s[b][k / 2][(k % 2) * 8 + 2 * e + 1]);
-    }
+    for (int b = 0; b < QB; ++b) softmax_step<EK, DC, 2>(s[b], o[b], top[b], sum[b], p.c, pf[b]);
 #pragma unroll
     for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -182,18 +204,7 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 4 : 2) attention_kernel(const A
     const float lse = kept ? fmaf(top[b], p.c, __builtin_amdgcn_logf(total)) : INFINITY;
     const int64_t row = qs.row + qpos[b];
     if (p.splits > 1) {
-      // this split's mean of the values, and its statistics
-      if (on && lane < 32) p.part_lse[((int64_t)split * p.heads + head) * p.q_total + row] = kept ? lse : -INFINITY;
-      float* at = p.part_o + (((int64_t)split * p.q_total + row) * p.heads + head) * p.dim;
-#pragma unroll
-      for (int d = 0; d < DC; ++d)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int e = d * 32 + 8 * q + 4 * (lane >> 5);
-          if (on && e < p.dim)
-            *(f32x4*)(at + e) = f32x4{o[b][d][q * 4] * inv, o[b][d][q * 4 + 1] * inv, o[b][d][q * 4 + 2] * inv,
-                                      o[b][d][q * 4 + 3] * inv};
-        }
+      if (on) store_part<DC>(p, split, row, head, o[b], inv, kept ? lse : -INFINITY, lane);
     } else {
       if (p.lse && on && lane < 32) p.lse[(int64_t)head * p.q_total + row] = lse;
       if (!kept)
@@ -205,52 +216,193 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 4 : 2) attention_kernel(const A
   }
 }
 
-// Joins the splits of a row: sum_s 2^(lse_s - lse) o_s. Four elements a thread.
+// Few queries over long keys: bound by reading K and V once, so every key head's queries (all heads of the
+// group, up to 32 QB rows) are one wavefront's MFMA columns, and every wavefront has keys of its own: 32 at a
+// time through two private LDS buffers, no barrier, 4 to 8 KB in flight for each of K and V. A wavefront's keys
+// are a split; attention_join_kernel adds them.
+template <int EK, int DC, int QB>
+__global__ void __launch_bounds__(256, DC <= 2 ? 2 : 1) attention_rows_kernel(const AttP p) {
+  using D = Dim<DC>;
+  constexpr int TILE = 32 * D::PITCH, NI = 2 * TILE / 1024;
+  __shared__ __attribute__((aligned(1024))) char s_ring[4][2][2 * TILE];
+  __shared__ int s_kept[2];
+  extern __shared__ uint32_t s_bits[];
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int item = work_item(p);
+  if (item < 0) return;
+  const int wsplits = p.splits / 4, kv_heads = p.heads / p.group;
+  uint32_t t = (uint32_t)item;
+  const int ws = (int)(t % (uint32_t)wsplits);
+  t /= (uint32_t)wsplits;
+  const int kvh = (int)(t % (uint32_t)kv_heads), seq = (int)(t / (uint32_t)kv_heads);
+  const Span qs = span_of(p.cu_q, p.q_rows, p.q_len, seq), ks = span_of(p.cu_k, p.k_rows, p.k_len, seq);
+  const int split = ws * 4 + wv, steps = (ks.len + 31) / 32, per = (steps + p.splits - 1) / p.splits;
+  const int first = ws * 4 * per * 32, kb = split * per * 32;  // the workgroup's first key, the wavefront's
+  const int last = first + 4 * per * 32 < ks.len ? first + 4 * per * 32 : ks.len;
+  int ke = kb + per * 32 < ks.len ? kb + per * 32 : ks.len;
+
+  const char* kbase = p.k.data + (p.cu_k ? ks.row * p.k.sl : seq * p.k.sn) + kvh * p.k.sh;
+  const char* vbase = p.v.data + (p.cu_k ? ks.row * p.v.sl : seq * p.v.sn) + kvh * p.v.sh;
+  const Rows<DC, 32, 1> krows(p.k.sl, p.dim, 0, lane), vrows(p.v.sl, p.dim, 0, lane);
+  const Frags<DC> frags(lane);
+  const uint32_t lds[2] = {lds_addr(s_ring[wv][0]), lds_addr(s_ring[wv][1])};
+  bool holes = false;
+  auto issue = [&](uint32_t at, int kt) {
+    const uint32_t* bits = holes ? s_bits + ((kt - first) >> 5) : nullptr;
+    krows.issue(at, kbase + kt * p.k.sl, ke - kt, bits, 0, lane);
+    vrows.issue(at + TILE, vbase + kt * p.v.sl, ke - kt, bits, 0, lane);
+  };
+  if (!p.km) {
+    if (kb < ke) issue(lds[0], kb);
+    if (kb + 32 < ke) issue(lds[1], kb + 32);
+  }
+  // column c: row c % q_len of head c / q_len of the group
+  int row[QB], head[QB];
+  bool on[QB];
+  u32x4 qf[QB][D::KS];
+  const char* qbase = p.q.data + (p.cu_q ? qs.row * p.q.sl : seq * p.q.sn);
+#pragma unroll
+  for (int b = 0; b < QB; ++b) {
+    const int c = b * 32 + l32;
+    row[b] = c % (int)p.q_len;
+    head[b] = kvh * p.group + c / (int)p.q_len;
+    on[b] = c < p.group * (int)p.q_len && row[b] < qs.len;
+    const bool q_on = on[b] && (!p.qm || p.qm[seq * p.qm_sn + row[b] * p.qm_sl] != 0);
+    load_cols<DC>(qf[b], q_on ? qbase + row[b] * p.q.sl + head[b] * p.q.sh : nullptr, p.dim, lane);
+    if (!q_on) row[b] = -1 - row[b];  // written as a row without keys
+  }
+  if (p.km) {  // the workgroup's own keys' bits
+    const Kept kept = scan_mask(s_bits, p.km + seq * p.km_sn + first * p.km_sl, p.km_sl, last > first ? last - first : 0,
+                                s_kept);
+    holes = kept.holes;
+    ke = ke < first + kept.extent ? ke : first + kept.extent;
+    if (kb < ke) issue(lds[0], kb);
+    if (kb + 32 < ke) issue(lds[1], kb + 32);
+  }
+
+  f32x16 o[QB][DC];
+  float top[QB], sum[QB];
+#pragma unroll
+  for (int b = 0; b < QB; ++b) {
+    top[b] = -INFINITY;
+    sum[b] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DC; ++d) o[b][d] = f32x16{};
+  }
+  int buf = 0;
+  for (int kt = kb; kt < ke; kt += 32, buf ^= 1) {
+    // this tile is complete (the next one's loads, if there is one, are younger)
+    if (kt + 32 < ke) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NI) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const uint32_t at = buf ? lds[1] : lds[0];
+    f32x16 s[QB][1];
+#pragma unroll
+    for (int b = 0; b < QB; ++b) s[b][0] = f32x16{};
+#pragma unroll
+    for (int k = 0; k < D::KS; ++k) {
+      const u32x4 kf = frags.row(at, 0, k);
+#pragma unroll
+      for (int b = 0; b < QB; ++b) s[b][0] = mfma16<EK>(s[b][0], kf, qf[b][k]);
+    }
+    u32x4 pf[QB][2];
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+      if (holes || kt + 32 > ke)
+        mask_scores(s[b][0], kt - first, ke - first, holes ? s_bits : nullptr, false, 0, 0u, lane);
+      softmax_step<EK, DC, 1>(s[b], o[b], top[b], sum[b], p.c, pf[b]);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int d = 0; d < DC; ++d) {
+        const u32x4 vf = frags.col(at + TILE, k * 16, d);
+#pragma unroll
+        for (int b = 0; b < QB; ++b) o[b][d] = mfma16<EK>(o[b][d], vf, pf[b][k]);
+      }
+    if (kt + 64 < ke) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this buffer has been read
+      issue(at, kt + 64);
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < QB; ++b) {
+    const float total = sum[b] + swap_half(sum[b]);
+    const bool kept = row[b] >= 0 && total != 0.f;
+    if (on[b])
+      store_part<DC>(p, split, qs.row + (row[b] < 0 ? -1 - row[b] : row[b]), head[b], o[b], kept ? 1.0f / total : 0.f,
+                     kept ? fmaf(top[b], p.c, __builtin_amdgcn_logf(total)) : -INFINITY, lane);
+  }
+}
+
+// Joins the splits of a row: sum_s 2^(lse_s - lse) o_s. A wavefront a row and head: its lanes take the splits'
+// statistics, then two elements each.
 template <int EK>
 __global__ void __launch_bounds__(256) attention_join_kernel(const AttP p) {
-  const int per = p.dim / 4;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= p.q_total * p.heads * per) return;
-  const int e = (int)(i % per) * 4;
-  const int64_t rh = i / per, row = rh / p.heads;
-  if (p.cu_q && (row < p.cu_q[0] || row >= p.cu_q[p.n])) return;  // in no sequence
+  __shared__ float s_w[4][64];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const int64_t rh = (int64_t)blockIdx.x * 4 + wv;
+  const int64_t row = rh / p.heads;
   const int head = (int)(rh % p.heads);
-  float top = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) top = max_nan(top, p.part_lse[((int64_t)s * p.heads + head) * p.q_total + row]);
-  f32x4 a = {};
-  float total = 0.f;
-  if (top != -INFINITY)
-    for (int s = 0; s < p.splits; ++s) {
-      const float w = __builtin_amdgcn_exp2f(p.part_lse[((int64_t)s * p.heads + head) * p.q_total + row] - top);
-      total += w;
-      const f32x4 x = *(const f32x4*)(p.part_o + (((int64_t)s * p.q_total + row) * p.heads + head) * p.dim + e);
+  bool on = row < p.q_total;
+  if (on && p.cu_q) on = row >= p.cu_q[0] && row < p.cu_q[p.n];  // else in no sequence
+  if (!on) return;
+  // (at most 64 splits)
+  const float l = lane < p.splits ? p.part_lse[((int64_t)lane * p.heads + head) * p.q_total + row] : -INFINITY;
+  float top = l;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) a[k] = fmaf(w, x[k], a[k]);
-    }
-  const float inv = top != -INFINITY ? 1.0f / total : 0.f;
-  if (p.lse && e == 0) p.lse[(int64_t)head * p.q_total + row] = top != -INFINITY ? top + __builtin_amdgcn_logf(total) : INFINITY;
-  *(u32x2*)(p.out + (rh * p.dim + e) * 2) =
-      u32x2{pack2<EK>(a[0] * inv, a[1] * inv), pack2<EK>(a[2] * inv, a[3] * inv)};
-  if (p.low)
-    *(uint32_t*)(p.low + rh * p.dim + e) = low_bytes<EK>(a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
+  for (int s = 1; s < 64; s <<= 1) top = max_nan(top, __shfl_xor(top, s));
+  const float w = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(l - top);
+  float total = w;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) total += __shfl_xor(total, s);
+  const float inv = top == -INFINITY ? 0.f : 1.0f / total;
+  if (p.lse && lane == 0)
+    p.lse[(int64_t)head * p.q_total + row] = top == -INFINITY ? INFINITY : top + __builtin_amdgcn_logf(total);
+  s_w[wv][lane] = w * inv;  // (a wavefront reads only what it wrote itself)
+  __builtin_amdgcn_wave_barrier();
+  const int e = 4 * (lane & 31);
+  if (e >= p.dim) return;
+  f32x4 a = {};
+  const float* in = p.part_o + rh * p.dim + e;
+  const int64_t step = p.q_total * p.heads * p.dim;
+#pragma unroll 4
+  for (int s = lane >> 5; s < p.splits; s += 2) {  // the halves take the even and the odd splits
+    const f32x4 x = *(const f32x4*)(in + s * step);
+    const float ws = s_w[wv][s];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) a[k] = fmaf(ws, x[k], a[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) a[k] += swap_half(a[k]);
+  if (lane < 32) {
+    *(u32x2*)(p.out + (rh * p.dim + e) * 2) = u32x2{pack2<EK>(a[0], a[1]), pack2<EK>(a[2], a[3])};
+    if (p.low) *(uint32_t*)(p.low + rh * p.dim + e) = low_bytes<EK>(a[0], a[1], a[2], a[3]);
+  }
 }
 
-}  // namespace
-
-namespace {
-
-// Splits of the keys: where the tiles of queries do not fill the 256 CUs and the
-// keys are long, down to 256 keys a split.
-int key_splits(const AttP& p, int64_t wgs) {
-  if (p.left != kNone && p.right != kNone) return 1;  // a window is short
-  int64_t s = 512 / (wgs < 1 ? 1 : wgs);
-  const int64_t most = p.k_len / 256;
-  if (s > most) s = most;
-  return s < 2 ? 1 : (int)s;
-}
+// Splits of the keys. Up to 64 rows a key head and no window: attention_rows_kernel, whose workgroups fill the
+// CUs once (LDS: two a CU up to head dim 64, else one), a wavefront 64 keys at least. More rows: where the tiles
+// of queries do not fill the 256 CUs and the keys are long, down to 256 keys a split.
 void forward_shape(AttP& p) {
   p.tiles = (int)((p.q_len + 127) / 128);
-  p.splits = key_splits(p, (int64_t)p.n * p.heads * p.tiles);
+  const bool window = p.left != kNone || p.right != kNone;
+  p.few = !window && p.q_len * p.group <= 64 && p.k_len >= 256;
+  int64_t s;
+  if (p.few) {
+    const int64_t units = (int64_t)p.n * (p.heads / p.group);
+    s = (p.dim <= 64 ? 512 : 256) / units;
+    const int64_t most = (p.k_len + 255) / 256;
+    if (s > most) s = most;
+    if (s > 16) s = 16;
+    p.splits = 4 * (int)(s < 1 ? 1 : s);
+    return;
+  }
+  const int64_t wgs = (int64_t)p.n * p.heads * p.tiles;
+  s = p.left != kNone && p.right != kNone ? 1 : 512 / wgs;  // (a window is short)
+  if (s > p.k_len / 256) s = p.k_len / 256;
+  if (s > 64) s = 64;
+  p.splits = s < 2 ? 1 : (int)s;
 }
 size_t forward_ws(const AttP& p) {
   if (p.splits < 2) return 0;
@@ -260,14 +412,25 @@ size_t forward_ws(const AttP& p) {
 
 template <int EK, int DC>
 int launch_forward(AttP p, hipStream_t s) {
-  const int64_t per = (int64_t)p.tiles * p.splits;
-  const unsigned grid = work_grid(p, per * p.n * p.heads, per * p.group);
-  if (!grid) return LIK_ERR_UNSUPPORTED;
-  launch_kernel(attention_kernel<EK, DC, 1>, dim3(grid), dim3(256), p.km ? mask_words(p.k_len) * 4 : 0u, s, p);
+  const uint32_t bits = p.km ? mask_words(p.k_len) * 4 : 0u;
+  if (p.few) {
+    const int64_t per = p.splits / 4;
+    const unsigned grid = work_grid(p, per * p.n * (p.heads / p.group), per);
+    if (!grid) return LIK_ERR_UNSUPPORTED;
+    if (p.q_len * p.group <= 32)
+      launch_kernel(attention_rows_kernel<EK, DC, 1>, dim3(grid), dim3(256), bits, s, p);
+    else
+      launch_kernel(attention_rows_kernel<EK, DC, 2>, dim3(grid), dim3(256), bits, s, p);
+  } else {
+    const int64_t per = (int64_t)p.tiles * p.splits;
+    const unsigned grid = work_grid(p, per * p.n * p.heads, per * p.group);
+    if (!grid) return LIK_ERR_UNSUPPORTED;
+    launch_kernel(attention_kernel<EK, DC, 1>, dim3(grid), dim3(256), bits, s, p);
+  }
   if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
   if (p.splits > 1) {
-    const int64_t m = p.q_total * p.heads * (p.dim / 4);
-    launch_kernel(attention_join_kernel<EK>, dim3((unsigned)((m + 255) / 256)), dim3(256), 0u, s, p);
+    const int64_t m = p.q_total * p.heads;
+    launch_kernel(attention_join_kernel<EK>, dim3((unsigned)((m + 3) / 4)), dim3(256), 0u, s, p);
     if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
   }
   return LIK_OK;
