@@ -224,7 +224,10 @@ def attention_varlen(
     cu_k = cu_q if cu_seqlens_k is cu_seqlens_q else _i32(cu_seqlens_k)
     given = [(cu, None if m is None else int(m), name) for cu, m, name in (
         (cu_q, max_seqlen_q, "max_seqlen_q"), (cu_k, max_seqlen_k, "max_seqlen_k"))]
-    assert_max_seqlens_cover(*given)
+    if cu_k is cu_q and None not in (given[0][1], given[1][1]):  # one array: the tighter bound covers both
+        assert_max_seqlens_cover(min(given, key=lambda g: g[1]))
+    else:
+        assert_max_seqlens_cover(*given)
     max_q, max_k = (seqlen_max(cu) if m is None else m for cu, m, _ in given)
     return _run(q, k, v, (left, right, scale, max_q, max_k), None, None, cu_q, cu_k)
 
