@@ -484,21 +484,21 @@ __global__ void __launch_bounds__(WM* WN * 64) gemm_finish_kernel(const GemmP p)
 // go from memory to registers as they lie, the eight sums meet in LDS and are added in order.
 template <int EK, int EPI, int MB>
 __global__ void __launch_bounds__(512) few_rows_kernel(const GemmP p) {
-  constexpr int NW = 8, U = MB <= 2 ? 6 : 3;
+  constexpr int NW = 8, U = 6;
   __shared__ __attribute__((aligned(16))) float s_sum[NW][MB][4][64][4];
   const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n0 = (int)blockIdx.x * (EPI == EPI_GLU ? 16 : 32), m0 = (int)blockIdx.y * 32 * MB;
+  const int n0 = (int)blockIdx.x * (EPI == EPI_GLU ? 16 : 32);
   const int n = EPI == EPI_GLU ? n0 + (l32 & 15) : n0 + l32;
   const int row = EPI == EPI_GLU && l32 >= 16 ? p.hidden + n : n;
   const uint32_t boff = n < (EPI == EPI_GLU ? p.hidden : p.n) ? (uint32_t)(row * p.b_ld) : kOob;
   uint32_t aoff[MB];
 #pragma unroll
-  for (int j = 0; j < MB; ++j) aoff[j] = m0 + j * 32 + l32 < p.m ? (uint32_t)((j * 32 + l32) * p.a_ld) : kOob;
+  for (int j = 0; j < MB; ++j) aoff[j] = j * 32 + l32 < p.m ? (uint32_t)((j * 32 + l32) * p.a_ld) : kOob;
   const __amdgpu_buffer_rsrc_t rb =
       __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p.b), (short)0, (int)0xffffff00u, 0x00020000);
   const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<char*>(p.a + (int64_t)m0 * p.a_ld), (short)0, (int)0xffffff00u, 0x00020000);
+      const_cast<char*>(p.a), (short)0, (int)0xffffff00u, 0x00020000);
   f32x16 acc[MB];
 #pragma unroll
   for (int j = 0; j < MB; ++j) acc[j] = f32x16{};
@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(512) few_rows_kernel(const GemmP p) {
       *(f32x4*)s_sum[wv][j][q][lane] = f32x4{acc[j][4 * q], acc[j][4 * q + 1], acc[j][4 * q + 2], acc[j][4 * q + 3]};
   __syncthreads();
   if (wv >= MB) return;
-  const int m = m0 + wv * 32 + l32;
+  const int m = wv * 32 + l32;
   Extra<EK, EPI> ex;
   load_extra<EK, EPI>(p, ex, m, n0, h);
   f32x16 c = {};
@@ -549,75 +549,90 @@ __global__ void __launch_bounds__(512) few_rows_kernel(const GemmP p) {
   }
 }
 
-constexpr int kTM = 256, kTN = 256, kCUs = 256;
-// Rows up to which few_rows_kernel takes the forward's products.
-constexpr int kFewRows = 256;
+constexpr int kCUs = 256;
+// Whether few_rows_kernel takes one of the forward's products: m rows by n weight rows of length k. Both
+// products together, few_rows_kernel against the 128 x 128 tiles: (768, 1152) 32 rows 13 against 20 us, 64 rows 17
+// against 20, 128 rows 25 against 20; (1024, 2624) 32 rows 20 against 25, 64 rows 28 against 25.
+bool few_rows(int64_t m, int64_t n, int64_t k) { return m <= 32 || (m <= 64 && n * k <= (1 << 21)); }
 
 template <int EK, int EPI>
 int launch_few_rows(const GemmP& p, hipStream_t s) {
   const unsigned nb = EPI == EPI_GLU ? (p.hidden + 15) / 16 : (p.n + 31) / 32;
   if (p.m <= 32)
     launch_kernel(few_rows_kernel<EK, EPI, 1>, dim3(nb), dim3(512), 0u, s, p);
-  else if (p.m <= 64)
-    launch_kernel(few_rows_kernel<EK, EPI, 2>, dim3(nb), dim3(512), 0u, s, p);
   else
-    launch_kernel(few_rows_kernel<EK, EPI, 4>, dim3(nb, (p.m + 127) / 128), dim3(512), 0u, s, p);
+    launch_kernel(few_rows_kernel<EK, EPI, 2>, dim3(nb), dim3(512), 0u, s, p);
   return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;
 }
 
-// Tiles run in rounds of one workgroup a CU. What is left after the whole rounds would take another round on
-// a few CUs; instead k of each of those tiles is split over several workgroups, whose fp32 sums a second
-// kernel adds. Costs in us as measured at 256 x 256 tiles: 1.8 a step of 64 k (all CUs busy), 8 for the
-// second launch, and the partial sums' 256 KB a workgroup written and read at about 4.5 TB/s.
+// Tiles of 256 x 256 (eight wavefronts, all of a CU's LDS) read the least for their work; tiles of 128 x 128 (four
+// wavefronts, two workgroups a CU) give four times as many workgroups where there are few. Tiles run in rounds of
+// the CUs. What is left after the whole rounds would take another round on a few CUs; instead k of each of those
+// tiles is split over several workgroups, whose fp32 sums a second kernel adds. The choice takes the least of
+// the costs in us, as measured: a step of 64 k, a round's start and epilogue, and for split tiles the second
+// launch and the partial sums written and read at about 4.5 TB/s.
 struct Shape {
-  int tiles_n, full, tail, splits, k_per;
+  int tile, tiles_n, full, tail, splits, k_per;
+  double cost;
 };
-Shape gemm_shape(int64_t m, int64_t n_tiles, int64_t k) {
-  const int64_t tiles = (m + kTM - 1) / kTM * n_tiles, steps = (k + BK - 1) / BK;
-  Shape s{(int)n_tiles, (int)tiles, 0, 1, (int)(steps * BK)};
-  const int64_t left = tiles % kCUs;
+Shape tile_shape(int tile, int64_t m, int64_t n, int64_t k) {
+  const bool big = tile == 256;
+  const int64_t tn = (n + tile - 1) / tile, tiles = (m + tile - 1) / tile * tn, steps = (k + BK - 1) / BK;
+  const int64_t slots = big ? kCUs : 2 * kCUs;
+  const double start = big ? 8.0 : 5.0;
+  const auto step = [&](int64_t wgs) { return big ? 1.8 : wgs > kCUs ? 1.2 : 0.7; };
+  const int64_t whole = tiles / slots * slots, left = tiles - whole;
+  Shape s{tile, (int)tn, (int)tiles, 0, 1, (int)(steps * BK), 0.0};
+  const double rounds = whole / slots * (steps * step(slots) + start);
+  s.cost = rounds + (left ? steps * step(left) + start : 0.0);
   if (left == 0) return s;
-  double best = 1.8 * steps;
-  for (int64_t sp = 2; sp <= steps / 2 && left * sp <= 4 * kCUs; ++sp) {
-    const int64_t per = (steps + sp - 1) / sp, real = (steps + per - 1) / per;
-    if (real != sp) continue;
-    const double cost = 1.8 * per * ((left * sp + kCUs - 1) / kCUs) + 8 + 0.12 * left * sp;
-    if (cost < best) {
-      best = cost;
-      s = {(int)n_tiles, (int)(tiles - left), (int)left, (int)sp, (int)(per * BK)};
-    }
+  for (int64_t sp = 2; sp <= steps / 2 && left * sp <= 4 * slots; ++sp) {
+    const int64_t per = (steps + sp - 1) / sp;
+    if ((steps + per - 1) / per != sp) continue;
+    const double cost = rounds + (step(left * sp) * per + start) * ((left * sp + slots - 1) / slots) + 8 +
+                        left * sp * tile * tile * 8 / 4.5e6;
+    if (cost < s.cost) s = {tile, (int)tn, (int)whole, (int)left, (int)sp, (int)(per * BK), cost};
   }
   return s;
 }
-size_t part_bytes(const Shape& s) { return (size_t)s.tail * s.splits * kTM * kTN * 4; }
-int64_t n_tiles(int64_t n) { return (n + kTN - 1) / kTN; }
-int64_t glu_tiles(int64_t hidden) { return (hidden + kTN / 2 - 1) / (kTN / 2); }
+// n: columns of the tiles' B operand (EPI_GLU: gate and up)
+Shape gemm_shape(int64_t m, int64_t n, int64_t k) {
+  const Shape a = tile_shape(256, m, n, k), b = tile_shape(128, m, n, k);
+  return a.cost <= b.cost ? a : b;
+}
+size_t part_bytes(const Shape& s) { return (size_t)s.tail * s.splits * s.tile * s.tile * 4; }
+int64_t glu_columns(int64_t hidden) { return (hidden + 31) / 32 * 64; }  // (blocks of 32 gate and 32 up columns)
 
+template <int EK, bool XA, bool XB, int EPI, int T>
+int launch_tiles(const GemmP& p, hipStream_t s) {
+  constexpr int WM = T / 64, WN = 2;
+  const int groups = p.full + p.tail * p.splits;
+  launch_kernel(gemm_kernel<EK, XA, XB, T, T, WM, WN, EPI>, dim3((unsigned)groups), dim3(WM * WN * 64), 0u, s, p);
+  if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
+  if (p.tail) {
+    constexpr int blocks = T / WM / 32 * (T / WN / 32) / (EPI == EPI_GLU ? 2 : 1);
+    launch_kernel(gemm_finish_kernel<EK, T, T, WM, WN, EPI>, dim3((unsigned)(p.tail * blocks)), dim3(WM * WN * 64), 0u, s, p);
+    if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
+  }
+  return LIK_OK;
+}
 template <int EK, bool XA, bool XB, int EPI>
 int launch_gemm(GemmP p, float* part, hipStream_t s) {
   if constexpr (!XA && !XB)
-    if (p.m <= kFewRows) return launch_few_rows<EK, EPI>(p, s);
-  const Shape sh = gemm_shape(p.m, EPI == EPI_GLU ? glu_tiles(p.hidden) : n_tiles(p.n), p.k);
+    if (few_rows(p.m, EPI == EPI_GLU ? 2ll * p.hidden : p.n, p.k)) return launch_few_rows<EK, EPI>(p, s);
+  const Shape sh = gemm_shape(p.m, EPI == EPI_GLU ? glu_columns(p.hidden) : p.n, p.k);
   p.tiles_n = sh.tiles_n;
   p.full = sh.full;
   p.tail = sh.tail;
   p.splits = sh.splits;
   p.k_per = sh.k_per;
   p.part = part;
-  launch_kernel(gemm_kernel<EK, XA, XB, kTM, kTN, 4, 2, EPI>, dim3((unsigned)(sh.full + sh.tail * sh.splits)), dim3(512),
-                0u, s, p);
-  if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
-  if (sh.tail) {
-    constexpr int blocks = kTM / 4 / 32 * (kTN / 2 / 32) / (EPI == EPI_GLU ? 2 : 1);
-    launch_kernel(gemm_finish_kernel<EK, kTM, kTN, 4, 2, EPI>, dim3((unsigned)(sh.tail * blocks)), dim3(512), 0u, s, p);
-    if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
-  }
-  return LIK_OK;
+  return sh.tile == 256 ? launch_tiles<EK, XA, XB, EPI, 256>(p, s) : launch_tiles<EK, XA, XB, EPI, 128>(p, s);
 }
 
 size_t most(size_t a, size_t b) { return a > b ? a : b; }
 size_t ffn_ws(int64_t rows, int d, int f) {
-  return most(part_bytes(gemm_shape(rows, glu_tiles(f), d)), part_bytes(gemm_shape(rows, n_tiles(d), f))) + 256;
+  return most(part_bytes(gemm_shape(rows, glu_columns(f), d)), part_bytes(gemm_shape(rows, d, f))) + 256;
 }
 
 struct FfnBwdWs {
@@ -628,8 +643,8 @@ FfnBwdWs ffn_bwd_ws(int64_t rows, int d, int f) {
   w.dgu = 0;
   w.part = align256((size_t)rows * 2 * f * 2);
   w.total = w.part + 256 +
-            most(most(part_bytes(gemm_shape(rows, n_tiles(f), d)), part_bytes(gemm_shape(rows, n_tiles(d), 2 * f))),
-                 most(part_bytes(gemm_shape(2 * f, n_tiles(d), rows)), part_bytes(gemm_shape(d, n_tiles(f), rows))));
+            most(most(part_bytes(gemm_shape(rows, f, d)), part_bytes(gemm_shape(rows, d, 2 * f))),
+                 most(part_bytes(gemm_shape(2 * f, d, rows)), part_bytes(gemm_shape(d, f, rows))));
   return w;
 }
 
@@ -639,7 +654,7 @@ int ffn_check(int32_t dtype, int64_t rows, int32_t d, int32_t f, int32_t act) {
   // 16-byte chunks of k; rows of weights and tokens within a 32-bit tile offset
   if (d % 8 || f % 8 || d > (1 << 20) || f > (1 << 20) || rows > 0x7fffff00) return LIK_ERR_UNSUPPORTED;
   const int64_t most_n = (2ll * f > d ? 2ll * f : d) / 128 + 1;  // workgroups of a launch, in 31 bits
-  if ((rows / 256 + 1) * most_n > (1 << 30)) return LIK_ERR_UNSUPPORTED;
+  if ((rows / 128 + 1) * most_n > (1 << 30)) return LIK_ERR_UNSUPPORTED;
   return LIK_OK;
 }
 // 16-byte rows; a tile of 256, and `more` rows before it, within a lane's 32-bit offset
