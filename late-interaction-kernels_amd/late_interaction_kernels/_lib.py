@@ -547,6 +547,15 @@ def prepare_tokens(x: torch.Tensor) -> torch.Tensor:
     return x
 
 
+def rows16(x: torch.Tensor) -> torch.Tensor:
+    """:func:`prepare_tokens` of a 16-bit tensor, without its steps where there is nothing to do."""
+    bits = x.data_ptr() | (x.shape[-1] << 1)
+    *outer, last = x.stride()
+    for s in outer:
+        bits |= s << 1
+    return prepare_tokens(x) if bits & 15 or last != 1 else x
+
+
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor | None:
     if nbytes <= 0:
         return None

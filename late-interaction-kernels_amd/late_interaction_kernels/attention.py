@@ -17,29 +17,25 @@ import torch
 
 from . import _lib
 from ._core import _i32, _mask_i8, assert_max_seqlens_cover, seqlen_max
-from .autograd import _needs_grad
 
 
 def _args(q, k, v, meta, qm, km, cu_q, cu_k):
     """The C struct of a call on prepared ``[n, L, H, d]`` (packed: ``[T, H, d]``) tensors."""
     left, right, scale, max_q, max_k = meta
-    packed = cu_q is not None
-    s = _lib.LikAttention()
-    s.q, s.k, s.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    s.dtype, s.heads, s.kv_heads, s.dim = _lib.DTYPE_CODE[q.dtype], q.shape[-2], k.shape[-2], q.shape[-1]
-    s.n = cu_q.numel() - 1 if packed else q.shape[0]
-    s.q_len, s.k_len = (max_q, max_k) if packed else (q.shape[1], k.shape[1])
-    s.q_stride_n, s.q_stride_l, s.q_stride_h = (0 if packed else q.stride(0)), q.stride(-3), q.stride(-2)
-    s.k_stride_n, s.k_stride_l, s.k_stride_h = (0 if packed else k.stride(0)), k.stride(-3), k.stride(-2)
-    s.v_stride_n, s.v_stride_l, s.v_stride_h = (0 if packed else v.stride(0)), v.stride(-3), v.stride(-2)
-    s.left, s.right, s.scale = left, right, scale
-    if packed:
-        s.cu_q, s.cu_k, s.q_rows, s.k_rows = cu_q.data_ptr(), cu_k.data_ptr(), q.shape[0], k.shape[0]
-    if qm is not None:
-        s.q_mask, s.q_mask_stride_n, s.q_mask_stride_l = qm.data_ptr(), qm.stride(0), qm.stride(1)
-    if km is not None:
-        s.k_mask, s.k_mask_stride_n, s.k_mask_stride_l = km.data_ptr(), km.stride(0), km.stride(1)
-    return s
+    code = _lib.DTYPE_CODE[q.dtype]
+    if cu_q is not None:
+        (qr, h, d), (kr, hk, _) = q.shape, k.shape
+        (ql, qh, _), (kl, kh, _), (vl, vh, _) = q.stride(), k.stride(), v.stride()
+        return _lib.LikAttention(q.data_ptr(), k.data_ptr(), v.data_ptr(), code, h, hk, d, cu_q.numel() - 1, max_q,
+                                 max_k, 0, ql, qh, 0, kl, kh, 0, vl, vh, cu_q.data_ptr(), cu_k.data_ptr(), qr, kr,
+                                 None, 0, 0, None, 0, 0, left, right, scale)
+    (n, lq, h, d), (_, lk, hk, _) = q.shape, k.shape
+    (qn, ql, qh, _), (kn, kl, kh, _), (vn, vl, vh, _) = q.stride(), k.stride(), v.stride()
+    qmn, qml = (0, 0) if qm is None else qm.stride()
+    kmn, kml = (0, 0) if km is None else km.stride()
+    return _lib.LikAttention(q.data_ptr(), k.data_ptr(), v.data_ptr(), code, h, hk, d, n, lq, lk, qn, ql, qh, kn, kl, kh,
+                             vn, vl, vh, None, None, 0, 0, _lib.ptr(qm), qmn, qml, _lib.ptr(km), kmn, kml, left, right,
+                             scale)
 
 
 def _forward(q, k, v, meta, qm, km, cu_q, cu_k, train):
@@ -65,7 +61,7 @@ def _forward(q, k, v, meta, qm, km, cu_q, cu_k, train):
 class _AttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, meta, qm, km, cu_q, cu_k):
-        q, k, v = (_lib.prepare_tokens(t) for t in (q, k, v))
+        q, k, v = _lib.rows16(q), _lib.rows16(k), _lib.rows16(v)
         out, lse, low = _forward(q, k, v, meta, qm, km, cu_q, cu_k, True)
         ctx.save_for_backward(q, k, v, out, lse, low, qm, km, cu_q, cu_k)
         ctx.meta = meta
@@ -83,7 +79,7 @@ class _AttentionFn(torch.autograd.Function):
         if need_k or need_v:
             gk, gv = (make(t.shape, dtype=t.dtype, device=t.device) for t in (k, v))
         if not none and (gq is not None or gk is not None):
-            g = _lib.prepare_tokens(grad)
+            g = _lib.rows16(grad)
             lib = _lib.load()
             nbytes = lib.lik_attention_backward_workspace_size(ctypes.byref(a))
             ws = _lib.workspace(nbytes, q.device)
@@ -124,13 +120,13 @@ def _check(q, k, v, causal, window, scale):
 
 def _run(q, k, v, meta, qm, km, cu_q, cu_k):
     d = q.shape[-1]
-    if _needs_grad(q, k, v):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         pad = -d % 8  # zero columns change no product; padded here so that autograd cuts the gradients
         if pad:
             q, k, v = (torch.nn.functional.pad(t, (0, pad)) for t in (q, k, v))
         out = _AttentionFn.apply(q, k, v, meta, qm, km, cu_q, cu_k)
     else:
-        q, k, v = (_lib.prepare_tokens(t) for t in (q, k, v))
+        q, k, v = _lib.rows16(q), _lib.rows16(k), _lib.rows16(v)
         out, _, _ = _forward(q, k, v, meta, qm, km, cu_q, cu_k, False)
     return out[..., :d] if d % 8 else out
 

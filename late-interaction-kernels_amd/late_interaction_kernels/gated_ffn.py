@@ -13,7 +13,6 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
-from .autograd import _needs_grad
 
 # what the forward keeps both projections in: more bits than the gradients' rounding (bf16's are scaled into fp16)
 _KEPT = {torch.bfloat16: torch.float16, torch.float16: torch.float32}
@@ -46,8 +45,8 @@ class _GatedFfnFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x2, w_in, w_out, r2, act):
-        x2, w_in, w_out = (_lib.prepare_tokens(t) for t in (x2, w_in, w_out))
-        out, h, gu = _forward(x2, w_in, w_out, None if r2 is None else _lib.prepare_tokens(r2), act, True)
+        x2, w_in, w_out = _lib.rows16(x2), _lib.rows16(w_in), _lib.rows16(w_out)
+        out, h, gu = _forward(x2, w_in, w_out, None if r2 is None else _lib.rows16(r2), act, True)
         ctx.save_for_backward(x2, w_in, w_out, h, gu)
         ctx.act = act
         return out
@@ -65,7 +64,7 @@ class _GatedFfnFn(torch.autograd.Function):
                 if t is not None:
                     t.zero_()
         elif need_x or need_in or need_out:
-            g = _lib.prepare_tokens(grad)
+            g = _lib.rows16(grad)
             lib, code = _lib.load(), _lib.DTYPE_CODE[x2.dtype]
             nbytes = lib.lik_gated_ffn_backward_workspace_size(code, rows, d, f)
             ws = _lib.workspace(nbytes, x2.device)
@@ -105,7 +104,7 @@ def gated_ffn(
         raise ValueError(f"x must be [..., d], w_in [2 hidden, d], w_out [d, hidden]; got {tuple(x.shape)}, "
                          f"{tuple(w_in.shape)}, {tuple(w_out.shape)}")
     d, f = x.shape[-1], w_out.shape[1]
-    if d < 1 or f < 1 or tuple(w_in.shape) != (2 * f, d) or w_out.shape[0] != d:
+    if d < 1 or f < 1 or w_in.shape != (2 * f, d) or w_out.shape[0] != d:
         raise ValueError(f"w_in must be [2 hidden, d={d}] and w_out [d={d}, hidden]; got {tuple(w_in.shape)} and "
                          f"{tuple(w_out.shape)}")
     if x.dtype not in (torch.bfloat16, torch.float16):
@@ -115,24 +114,29 @@ def gated_ffn(
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError(f"residual must match x ({tuple(x.shape)}, {x.dtype}); got {tuple(residual.shape)}, "
                          f"{residual.dtype}")
-    if any(t is not None and t.device != x.device for t in (w_in, w_out, residual)):
+    if w_in.device != x.device or w_out.device != x.device or (residual is not None and residual.device != x.device):
         raise ValueError("x, w_in, w_out and residual must be on the same device.")
     _lib.require_gpu(x)
     act = ACTIVATIONS[activation]
-    x2 = x.reshape(-1, d)
-    r2 = None if residual is None else residual.reshape(-1, d)
+    x2, r2 = x, residual
+    if x.dim() != 2:
+        x2 = x.reshape(-1, d)
+        r2 = None if residual is None else residual.reshape(-1, d)
     pd, pf = -d % 8, -f % 8
     if pd or pf:  # zero rows and columns add nothing to any product
         x2 = F.pad(x2, (0, pd))
         r2 = None if r2 is None else F.pad(r2, (0, pd))
         w_in = F.pad(w_in.unflatten(0, (2, f)), (0, pd, 0, pf)).reshape(2 * (f + pf), d + pd)
         w_out = F.pad(w_out, (0, pf, 0, pd))
-    if _needs_grad(*(t for t in (x, w_in, w_out, residual) if t is not None)):
+    if torch.is_grad_enabled() and (x.requires_grad or w_in.requires_grad or w_out.requires_grad
+                                    or (residual is not None and residual.requires_grad)):
         out = _GatedFfnFn.apply(x2, w_in, w_out, r2, act)
     else:
-        out, _, _ = _forward(*(_lib.prepare_tokens(t) for t in (x2, w_in, w_out)),
-                             None if r2 is None else _lib.prepare_tokens(r2), act, False)
-    return (out[:, :d] if pd else out).reshape(x.shape)
+        out, _, _ = _forward(_lib.rows16(x2), _lib.rows16(w_in), _lib.rows16(w_out),
+                             None if r2 is None else _lib.rows16(r2), act, False)
+    if pd:
+        out = out[:, :d]
+    return out if x.dim() == 2 else out.reshape(x.shape)
 
 
 __all__ = ["gated_ffn"]

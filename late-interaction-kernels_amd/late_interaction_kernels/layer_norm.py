@@ -10,17 +10,18 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .autograd import _needs_grad
 
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def _rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     """``x`` as ``[rows, d]`` with a contiguous last dim (a view where its strides allow one) and the row stride."""
-    x2 = x.reshape(-1, x.shape[-1])
-    if x2.stride(-1) != 1 and x2.shape[-1] > 1:
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    rs, cs = x2.stride()
+    if cs != 1 and x2.shape[1] > 1:
         x2 = x2.contiguous()
-    return x2, x2.stride(0)
+        rs = x2.stride(0)
+    return x2, rs
 
 
 def _forward(x, weight, bias, residual, eps, want_stats):
@@ -113,19 +114,22 @@ def layer_norm(
         raise TypeError(f"layer_norm takes fp16 / bf16 / fp32; got {x.dtype}")
     if d > 8192:
         raise ValueError(f"layer_norm takes rows of at most 8192 elements; got {d}")
-    if tuple(weight.shape) != (d,):
+    if weight.shape != (d,):
         raise ValueError(f"weight must be [{d}]; got {tuple(weight.shape)}")
     if weight.dtype not in (x.dtype, torch.float32):
         raise TypeError(f"weight must have the type of x ({x.dtype}) or be fp32; got {weight.dtype}")
-    if bias is not None and (tuple(bias.shape) != (d,) or bias.dtype != weight.dtype):
+    if bias is not None and (bias.shape != (d,) or bias.dtype != weight.dtype):
         raise ValueError(f"bias must be [{d}] of the weight's type; got {tuple(bias.shape)} {bias.dtype}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError(f"residual must match x ({tuple(x.shape)}, {x.dtype}); got {tuple(residual.shape)}, "
                          f"{residual.dtype}")
-    if any(t is not None and t.device != x.device for t in (weight, bias, residual)):
+    device = x.device
+    if (weight.device != device or (bias is not None and bias.device != device)
+            or (residual is not None and residual.device != device)):
         raise ValueError("x, weight, bias and residual must be on the same device.")
     _lib.require_gpu(x)
-    if _needs_grad(*(t for t in (x, weight, bias, residual) if t is not None)):
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
         return _LayerNormFn.apply(x, weight, bias, residual, float(eps))
     y, total, _ = _forward(x, weight.contiguous(), None if bias is None else bias.contiguous(), residual, float(eps),
                            False)
