@@ -113,12 +113,28 @@ __device__ __forceinline__ void store_row(char* row, int lane, int d, const floa
   each_chunk<NV>([&](int j, auto last) { store_chunk<EK, decltype(last)::value>(row, j * LPR + lane, d, v[j]); });
 }
 
-// Sum of a over the LPR lanes of a row, on every lane. LPR = 256: the four
-// wavefronts meet in LDS (s_red has 2 slots of 8 floats, used in turn).
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float a) {
+  const int x = __builtin_bit_cast(int, a);
+  return a + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(x, x, CTRL, 0xf, 0xf, false));
+}
+// Sum of a over the LPR lanes of a row, on every lane: within 16 lanes by data-parallel moves (each lane adds the
+// one opposite it), across them by the row and half swaps. LPR = 256: the four wavefronts meet in LDS (s_red has
+// 2 slots of 4 floats, used in turn).
 template <int LPR>
 __device__ __forceinline__ float row_sum(float a, float* s_red, int slot) {
-#pragma unroll
-  for (int o = 1; o < (LPR < 64 ? LPR : 64); o <<= 1) a += __shfl_xor(a, o);
+  a = dpp_add<0xb1>(a);   // lanes 1, 0, 3, 2 of each four
+  a = dpp_add<0x4e>(a);   // lanes 2, 3, 0, 1
+  a = dpp_add<0x141>(a);  // mirrored in eight
+  a = dpp_add<0x140>(a);  // mirrored in sixteen
+  if constexpr (LPR >= 32) {
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(a), false, false);
+    a = __uint_as_float((uint32_t)s[0]) + __uint_as_float((uint32_t)s[1]);
+  }
+  if constexpr (LPR >= 64) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(a), false, false);
+    a = __uint_as_float((uint32_t)s[0]) + __uint_as_float((uint32_t)s[1]);
+  }
   if constexpr (LPR == 256) {
     const int wv = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0) s_red[slot * 4 + wv] = a;
@@ -183,8 +199,12 @@ __global__ void __launch_bounds__(256) layer_norm_kernel(const NormP p) {
   }
 }
 
+// Workgroups of the backward a CU: what the registers of NV chunks of V values allow.
+template <int EK, int NV>
+constexpr int kBwdWgs = NV * El<EK>::V <= 24 ? 3 : 2;
+
 template <int EK, int LPR, int NV>
-__global__ void __launch_bounds__(256) layer_norm_bwd_kernel(const NormP p) {
+__global__ void __launch_bounds__(256, (kBwdWgs<EK, NV>)) layer_norm_bwd_kernel(const NormP p) {
   constexpr int V = El<EK>::V, RPW = 256 / LPR;
   __shared__ float s_red[8];
   extern __shared__ float s_col[];  // [2][LPR * NV * V] column sums of the workgroup (LPR < 256)
@@ -292,11 +312,19 @@ __global__ void __launch_bounds__(1024) norm_grads_kernel(const float* part, int
 }
 
 constexpr int kNormMaxDim = 8192;  // 256 lanes x 32 values in registers
-constexpr int kNormBwdWgs = 1024;  // four workgroups per CU
+constexpr int kNormBwdMost = 3 * 256;  // workgroups of the backward: one round of the CUs
 
+// slices: the workgroups whose partial sums a backward leaves.
 template <int EK, bool BWD, int LPR, int NV>
-int launch_norm_one(const NormP& p, int64_t wgs, hipStream_t s) {
+int launch_norm_one(const NormP& p, hipStream_t s, int& slices) {
+  const int64_t rpw = 256 / LPR, need = (p.rows + rpw - 1) / rpw;  // steps of the whole call
+  int64_t wgs = need < (1 << 20) ? need : (1 << 20);
   if constexpr (BWD) {
+    // one round of the CUs, the steps dealt out evenly (a partial round of workgroups or steps leaves CUs idle:
+    // 38400 x 768 bf16 58 us against 73 with 768 workgroups of 6 or 7 steps)
+    const int64_t most = 256 * kBwdWgs<EK, NV>, each = (need + most - 1) / most;
+    wgs = (need + each - 1) / each;
+    slices = (int)wgs;
     const uint32_t lds = LPR == 256 ? 0u : (uint32_t)(2 * LPR * NV * El<EK>::V * 4);
     launch_kernel(layer_norm_bwd_kernel<EK, LPR, NV>, dim3((unsigned)wgs), dim3(256), lds, s, p);
   } else {
@@ -312,31 +340,23 @@ int launch_norm_one(const NormP& p, int64_t wgs, hipStream_t s) {
 int norm_lanes(int chunks, int v) {
   return chunks <= 64 ? 16 : chunks <= 128 ? 32 : chunks <= 64 * 32 / v ? 64 : 256;
 }
-int64_t norm_bwd_wgs(int64_t rows, int64_t d, int v) {
-  const int64_t rpw = 256 / norm_lanes((int)((d + v - 1) / v), v);
-  const int64_t need = (rows + rpw - 1) / rpw;
-  return need < kNormBwdWgs ? need : kNormBwdWgs;
-}
-
 template <int EK, bool BWD, int LPR, int LO, int HI>
-int launch_norm_nv(const NormP& p, int nv, int64_t wgs, hipStream_t s) {
+int launch_norm_nv(const NormP& p, int nv, hipStream_t s, int& slices) {
   if constexpr (LO < HI) {
-    if (nv > LO) return launch_norm_nv<EK, BWD, LPR, LO + 1, HI>(p, nv, wgs, s);
+    if (nv > LO) return launch_norm_nv<EK, BWD, LPR, LO + 1, HI>(p, nv, s, slices);
   }
-  return launch_norm_one<EK, BWD, LPR, LO>(p, wgs, s);
+  return launch_norm_one<EK, BWD, LPR, LO>(p, s, slices);
 }
 
 template <int EK, bool BWD>
-int launch_norm(const NormP& p, hipStream_t s) {
+int launch_norm(const NormP& p, hipStream_t s, int& slices) {
   constexpr int V = El<EK>::V, MOST = 32 / V;
   const int chunks = (p.d + V - 1) / V;
   const int lpr = norm_lanes(chunks, V), nv = (chunks + lpr - 1) / lpr;
-  const int64_t rpw = 256 / lpr, need = (p.rows + rpw - 1) / rpw;
-  const int64_t wgs = BWD ? norm_bwd_wgs(p.rows, p.d, V) : (need < (1 << 20) ? need : (1 << 20));
-  if (lpr == 16) return launch_norm_nv<EK, BWD, 16, 1, 4>(p, nv, wgs, s);
-  if (lpr == 32) return launch_norm_nv<EK, BWD, 32, 3, 4>(p, nv, wgs, s);
-  if (lpr == 64) return launch_norm_nv<EK, BWD, 64, 3, MOST>(p, nv, wgs, s);
-  return launch_norm_nv<EK, BWD, 256, MOST / 4 + 1, MOST>(p, nv, wgs, s);
+  if (lpr == 16) return launch_norm_nv<EK, BWD, 16, 1, 4>(p, nv, s, slices);
+  if (lpr == 32) return launch_norm_nv<EK, BWD, 32, 3, 4>(p, nv, s, slices);
+  if (lpr == 64) return launch_norm_nv<EK, BWD, 64, 3, MOST>(p, nv, s, slices);
+  return launch_norm_nv<EK, BWD, 256, MOST / 4 + 1, MOST>(p, nv, s, slices);
 }
 
 // row base and stride on an element, d and the types in range
@@ -348,10 +368,10 @@ int norm_check(int32_t dtype, int32_t wdtype, int64_t rows, int64_t d) {
 }
 
 template <bool BWD>
-int norm_run(const NormP& p, int32_t dtype, hipStream_t s) {
-  if (dtype == LIK_BF16) return launch_norm<EK_BF16, BWD>(p, s);
-  if (dtype == LIK_F16) return launch_norm<EK_F16, BWD>(p, s);
-  return launch_norm<EK_F32, BWD>(p, s);
+int norm_run(const NormP& p, int32_t dtype, hipStream_t s, int& slices) {
+  if (dtype == LIK_BF16) return launch_norm<EK_BF16, BWD>(p, s, slices);
+  if (dtype == LIK_F16) return launch_norm<EK_F16, BWD>(p, s, slices);
+  return launch_norm<EK_F32, BWD>(p, s, slices);
 }
 
 }  // namespace
@@ -384,12 +404,14 @@ int lik_layer_norm(const void* x, int64_t x_stride, const void* residual, int64_
   p.y = (char*)y;
   p.s = (char*)sum;
   p.stat = stats;
-  return norm_run<false>(p, dtype, (hipStream_t)stream);
+  int none = 0;
+  return norm_run<false>(p, dtype, (hipStream_t)stream, none);
 }
 
 size_t lik_layer_norm_backward_workspace_size(int32_t dtype, int64_t rows, int32_t dim) {
   if (norm_check(dtype, dtype, rows, dim) != LIK_OK || rows == 0) return 0;
-  return (size_t)norm_bwd_wgs(rows, dim, dtype == LIK_F32 ? 4 : 8) * 2 * (size_t)dim * 4 + 256;
+  const int64_t wgs = rows < kNormBwdMost ? rows : kNormBwdMost;  // (at least a row each)
+  return (size_t)wgs * 2 * (size_t)dim * 4 + 256;
 }
 
 int lik_layer_norm_backward(const void* grad_y, int64_t grad_y_stride, const void* grad_sum, int64_t grad_sum_stride,
@@ -417,9 +439,9 @@ int lik_layer_norm_backward(const void* grad_y, int64_t grad_y_stride, const voi
   p.gx = (char*)grad_x;
   p.part = (float*)align256(workspace);
   const hipStream_t s = (hipStream_t)stream;
-  if (const int rc = norm_run<true>(p, dtype, s)) return rc;
+  int slices = 0;
+  if (const int rc = norm_run<true>(p, dtype, s, slices)) return rc;
   if (grad_weight || grad_bias) {
-    const int slices = (int)norm_bwd_wgs(rows, dim, dtype == LIK_F32 ? 4 : 8);
     const dim3 grid((unsigned)((2 * dim + 63) / 64)), block(1024);
     if (dtype == LIK_BF16)
       launch_kernel(norm_grads_kernel<EK_BF16>, grid, block, 0u, s, p.part, slices, dim, p.wf32, grad_weight, grad_bias);
