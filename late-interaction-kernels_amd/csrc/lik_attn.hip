@@ -1,5 +1,10 @@
 // Attention, forward. One pass over the keys with the running maximum and sum of
 // the softmax; the layout of the products is described in lik_attn.h.
+//
+// Bounds, measured with 256 sequences of 12 heads of 64: up to 128 tokens the rows' reads and writes (41 us, 4.9 TB/s),
+// at 1024 the softmax's vector instructions beside the MFMAs (1005 us, 820 TFLOP/s; per 32 x 64 scores 512 clocks of
+// MFMA and about 1000 of vector work, four wavefronts a SIMD). Between them tiles that a sequence does not fill:
+// 50 to 300 tokens 107 us (63 at the copy rate).
 #include "lik_attn.h"
 
 namespace lik {
@@ -219,7 +224,9 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 4 : 2) attention_kernel(const A
 // Few queries over long keys: bound by reading K and V once, so every key head's queries (all heads of the
 // group, up to 32 QB rows) are one wavefront's MFMA columns, and every wavefront has keys of its own: 32 at a
 // time through two private LDS buffers, no barrier, 4 to 8 KB in flight for each of K and V. A wavefront's keys
-// are a split; attention_join_kernel adds them.
+// are a split; attention_join_kernel adds them. 4 sequences of 5000 to 8192 keys, one query, 16 heads over 4 of 128,
+// fp16: 16 + 6 us (54 MB, 10.5 us at the copy rate; 47 + 7 us by attention_kernel, a wavefront of four at work and every
+// query head reading the keys).
 template <int EK, int DC, int QB>
 __global__ void __launch_bounds__(256, DC <= 2 ? 2 : 1) attention_rows_kernel(const AttP p) {
   using D = Dim<DC>;

@@ -16,7 +16,9 @@ are differentiable: an argmax-saving forward plus a deterministic HIP backward.
 Submodules mirror the reference: ``forward``, ``score_pairs``, ``padded``,
 ``plaid``, ``fp8``, ``varlen``, ``topk``, ``retrieve``, ``fused_head``,
 ``plaid_index``, and ``reference`` (eager PyTorch ground truth for callers'
-own comparisons; no op here uses it).
+own comparisons; no op here uses it). ``encoder`` adds the operators of the
+transformer encoder that makes the token vectors: ``attention``,
+``attention_varlen``, ``layer_norm`` and ``gated_ffn``, differentiable.
 """
 
 from importlib.metadata import PackageNotFoundError
