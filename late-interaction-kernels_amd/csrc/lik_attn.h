@@ -83,8 +83,8 @@ __device__ __forceinline__ Span span_of(const int32_t* cu, int64_t rows, int64_t
   return {a, (int)l};
 }
 
-// Keep bits of a mask row (len tokens) into LDS, 32 tokens a word; returns the
-// last kept token + 1 and whether every token before it is kept. All 256 threads.
+// Keep bits of a mask row (len tokens) into LDS, 32 tokens a word, by all 256 threads; returns the
+// last kept token + 1 and whether a token before it is dropped.
 struct Kept {
   int extent;
   bool holes;

@@ -66,12 +66,68 @@ __device__ __forceinline__ void store_part(const AttP& p, int split, int64_t row
     }
 }
 
-// A workgroup of four wavefronts owns 128 QB queries of one head, a wavefront 32 QB
-// of them as MFMA columns, and walks the keys that any of them keeps, 64 at a
-// time, in two LDS buffers: the next tile is loaded while this one is used.
+// What a wavefront does with 64 keys: K rows at kl and V rows at vl in LDS, its 32 queries in qf.
 //   scores  S^T[key][query] = K Q^T   (K rows from LDS, Q in registers)
 //   output  O^T[d][query]  += V^T P^T (V by transposing LDS reads, P as it lies)
-template <int EK, int DC, int QB>
+// whole: every pair is kept; else the arguments of mask_scores.
+template <int EK, int DC>
+__device__ __forceinline__ void attend_tile(const Frags<DC>& frags, uint32_t kl, uint32_t vl,
+                                            const u32x4 (&qf)[Dim<DC>::KS], f32x16 (&o)[DC], float& top, float& sum,
+                                            float c, bool whole, int kt, int klen, const uint32_t* bits, bool window,
+                                            int first, uint32_t reach, int lane) {
+  f32x16 s[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    s[u] = f32x16{};
+#pragma unroll
+    for (int k = 0; k < Dim<DC>::KS; ++k) s[u] = mfma16<EK>(s[u], frags.row(kl, u * 32, k), qf[k]);
+  }
+  if (!whole) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) mask_scores(s[u], kt + u * 32, klen, bits, window, first + u * 32, reach, lane);
+  }
+  u32x4 pf[4];
+  softmax_step<EK, DC, 2>(s, o, top, sum, c, pf);
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int d = 0; d < DC; ++d) o[d] = mfma16<EK>(o[d], frags.col(vl, k * 16, d), pf[k]);
+}
+
+// A wavefront's finished queries to memory. on: the lane's row exists, q_on: its mask keeps it.
+template <int EK, int DC>
+__device__ __forceinline__ void store_rows(const AttP& p, int split, int64_t row, int head, f32x16 (&o)[DC], float top,
+                                           float sum, bool on, bool q_on, int lane) {
+  const float total = sum + swap_half(sum);
+  const bool kept = q_on && total != 0.f;
+  const float inv = kept ? 1.0f / total : 0.f;
+  const float lse = kept ? fmaf(top, p.c, __builtin_amdgcn_logf(total)) : INFINITY;
+  if (p.splits > 1) {
+    if (on) store_part<DC>(p, split, row, head, o, inv, kept ? lse : -INFINITY, lane);
+    return;
+  }
+  if (p.lse && on && lane < 32) p.lse[(int64_t)head * p.q_total + row] = lse;
+  if (!kept)
+#pragma unroll
+    for (int d = 0; d < DC; ++d) o[d] = f32x16{};
+  store_cols<EK, DC>(p.out + (row * p.heads + head) * p.dim * 2, o, inv, p.dim, lane, on);
+  if (p.low) store_low<EK, DC>(p.low + (row * p.heads + head) * p.dim, o, inv, p.dim, lane, on);
+}
+
+// The window as one unsigned test: a key is kept where 0 <= key - query + back <= reach.
+struct Window {
+  bool on;
+  int back;
+  uint32_t reach;
+  __device__ __forceinline__ explicit Window(const AttP& p)
+      : on(p.left != kNone || p.right != kNone), back(p.left == kNone ? 0x3fffffff : p.left),
+        reach((uint32_t)back + (p.right == kNone ? 0x3fffffffu : (uint32_t)p.right)) {}
+};
+
+// A workgroup of four wavefronts owns 128 queries of one head, a wavefront 32 of them as MFMA columns, and
+// walks the keys that any of them keeps, 64 at a time, in two LDS buffers: the next tile is loaded while this one
+// is used.
+template <int EK, int DC>
 __global__ void __launch_bounds__(256, DC <= 2 ? 4 : 2) attention_kernel(const AttP p) {
   using D = Dim<DC>;
   __shared__ __attribute__((aligned(1024))) char s_tile[2][2 * D::TILE];
@@ -89,7 +145,7 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 4 : 2) attention_kernel(const A
   const int head = (int)(t % (uint32_t)p.heads), seq = (int)(t / (uint32_t)p.heads);
   const int kvh = head / p.group;
   const Span qs = span_of(p.cu_q, p.q_rows, p.q_len, seq), ks = span_of(p.cu_k, p.k_rows, p.k_len, seq);
-  const int q0 = tile * 128 * QB;
+  const int q0 = tile * 128;
   if (q0 >= qs.len) return;  // (all threads)
 
   const char* kbase = p.k.data + (p.cu_k ? ks.row * p.k.sl : seq * p.k.sn) + kvh * p.k.sh;
@@ -107,7 +163,7 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 4 : 2) attention_kernel(const A
 
   // The first tile's loads start before the keep bits are known (and again without the masked rows, if there
   // are any): a short sequence's time is a chain of such latencies.
-  const int q_end = (q0 + 128 * QB < qs.len ? q0 + 128 * QB : qs.len) - 1;  // last query of the workgroup
+  const int q_end = (q0 + 128 < qs.len ? q0 + 128 : qs.len) - 1;  // last query of the workgroup
   int kb = p.left == kNone || q0 - p.left < 0 ? 0 : (q0 - p.left) & ~63;
   int ke = p.right == kNone || (int64_t)q_end + p.right + 1 >= klen ? klen : q_end + p.right + 1;
   if (p.splits > 1) {  // this split's share
@@ -116,21 +172,12 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 4 : 2) attention_kernel(const A
     ke = kb + per * 64 < ke ? kb + per * 64 : ke;
   }
   if (kb < ke) issue(lds[0], kb);
-  // the lane's queries: column l32 of each of the wavefront's QB blocks
-  int qpos[QB];
-  bool qon[QB];
-  u32x4 qf[QB][D::KS];
+  const int qpos = q0 + wv * 32 + l32;  // the lane's query
+  const bool qon = qpos < qs.len && (!p.qm || p.qm[seq * p.qm_sn + qpos * p.qm_sl] != 0);
+  u32x4 qf[D::KS];
   const char* qbase = p.q.data + (p.cu_q ? qs.row * p.q.sl : seq * p.q.sn) + head * p.q.sh;
-#pragma unroll
-  for (int b = 0; b < QB; ++b) {
-    qpos[b] = q0 + (wv * QB + b) * 32 + l32;
-    qon[b] = qpos[b] < qs.len && (!p.qm || p.qm[seq * p.qm_sn + qpos[b] * p.qm_sl] != 0);
-    load_cols<DC>(qf[b], qon[b] ? qbase + qpos[b] * p.q.sl : nullptr, p.dim, lane);
-  }
-  bool any = qon[0];
-#pragma unroll
-  for (int b = 1; b < QB; ++b) any |= qon[b];
-  any = __ballot(any) != 0;  // this wavefront has a query
+  load_cols<DC>(qf, qon ? qbase + qpos * p.q.sl : nullptr, p.dim, lane);
+  const bool any = __ballot(qon) != 0;  // this wavefront has a query
 
   if (p.km) {
     const Kept kept = scan_mask(s_bits, p.km + seq * p.km_sn, p.km_sl, klen, s_kept);
@@ -144,20 +191,12 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 4 : 2) attention_kernel(const A
   }
   if (__syncthreads_or(any) == 0) ke = kb;  // no query of this tile is kept
 
-  const bool window = p.left != kNone || p.right != kNone;
-  // a key is kept where 0 <= key - query + back <= reach
-  const int back = p.left == kNone ? 0x3fffffff : p.left;
-  const uint32_t reach = (uint32_t)back + (p.right == kNone ? 0x3fffffffu : (uint32_t)p.right);
-  f32x16 o[QB][DC];
-  float top[QB], sum[QB];
+  const Window win(p);
+  f32x16 o[DC];
+  float top = -INFINITY, sum = 0.f;
 #pragma unroll
-  for (int b = 0; b < QB; ++b) {
-    top[b] = -INFINITY;
-    sum[b] = 0.f;
-#pragma unroll
-    for (int d = 0; d < DC; ++d) o[b][d] = f32x16{};
-  }
-  const int wq0 = q0 + wv * QB * 32, wq1 = wq0 + QB * 32 - 1;  // the wavefront's queries
+  for (int d = 0; d < DC; ++d) o[d] = f32x16{};
+  const int wq0 = q0 + wv * 32, wq1 = wq0 + 31;  // the wavefront's queries
   int buf = 0;
   for (int kt = kb; kt < ke; kt += 64, buf ^= 1) {
     // this tile is complete, and every wavefront is done with the other buffer
@@ -167,58 +206,11 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 4 : 2) attention_kernel(const A
     const uint32_t at = buf ? lds[1] : lds[0];
     const bool whole = kt + 64 <= klen && !holes && (p.right == kNone || kt + 63 <= wq0 + p.right) &&
                        (p.left == kNone || kt >= wq1 - p.left);
-    f32x16 s[QB][2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-#pragma unroll
-      for (int b = 0; b < QB; ++b) s[b][u] = f32x16{};
-#pragma unroll
-      for (int k = 0; k < D::KS; ++k) {
-        const u32x4 kf = frags.row(at, u * 32, k);
-#pragma unroll
-        for (int b = 0; b < QB; ++b) s[b][u] = mfma16<EK>(s[b][u], kf, qf[b][k]);
-      }
-    }
-    if (!whole) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int b = 0; b < QB; ++b)
-          mask_scores(s[b][u], kt + u * 32, klen, holes ? s_bits : nullptr, window,
-                      kt + u * 32 + 4 * (lane >> 5) - qpos[b] + back, reach, lane);
-    }
-    u32x4 pf[QB][4];
-#pragma unroll
-    for (int b = 0; b < QB; ++b) softmax_step<EK, DC, 2>(s[b], o[b], top[b], sum[b], p.c, pf[b]);
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-#pragma unroll
-      for (int d = 0; d < DC; ++d) {
-        const u32x4 vf = frags.col(at + D::TILE, k * 16, d);
-#pragma unroll
-        for (int b = 0; b < QB; ++b) o[b][d] = mfma16<EK>(o[b][d], vf, pf[b][k]);
-      }
+    attend_tile<EK, DC>(frags, at, at + D::TILE, qf, o, top, sum, p.c, whole, kt, klen, holes ? s_bits : nullptr, win.on,
+                        kt + 4 * (lane >> 5) - qpos + win.back, win.reach, lane);
   }
-
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load is in flight to LDS when the workgroup ends
-#pragma unroll
-  for (int b = 0; b < QB; ++b) {
-    const float total = sum[b] + swap_half(sum[b]);
-    const bool on = qpos[b] < qs.len, kept = qon[b] && total != 0.f;
-    const float inv = kept ? 1.0f / total : 0.f;
-    const float lse = kept ? fmaf(top[b], p.c, __builtin_amdgcn_logf(total)) : INFINITY;
-    const int64_t row = qs.row + qpos[b];
-    if (p.splits > 1) {
-      if (on) store_part<DC>(p, split, row, head, o[b], inv, kept ? lse : -INFINITY, lane);
-    } else {
-      if (p.lse && on && lane < 32) p.lse[(int64_t)head * p.q_total + row] = lse;
-      if (!kept)
-#pragma unroll
-        for (int d = 0; d < DC; ++d) o[b][d] = f32x16{};
-      store_cols<EK, DC>(p.out + (row * p.heads + head) * p.dim * 2, o[b], inv, p.dim, lane, on);
-      if (p.low) store_low<EK, DC>(p.low + (row * p.heads + head) * p.dim, o[b], inv, p.dim, lane, on);
-    }
-  }
+  store_rows<EK, DC>(p, split, qs.row + qpos, head, o, top, sum, qpos < qs.len, qon, lane);
 }
 
 // Few queries over long keys: bound by reading K and V once, so every key head's queries (all heads of the
@@ -432,7 +424,7 @@ int launch_forward(AttP p, hipStream_t s) {
     const int64_t per = (int64_t)p.tiles * p.splits;
     const unsigned grid = work_grid(p, per * p.n * p.heads, per * p.group);
     if (!grid) return LIK_ERR_UNSUPPORTED;
-    launch_kernel(attention_kernel<EK, DC, 1>, dim3(grid), dim3(256), bits, s, p);
+    launch_kernel(attention_kernel<EK, DC>, dim3(grid), dim3(256), bits, s, p);
   }
   if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
   if (p.splits > 1) {
