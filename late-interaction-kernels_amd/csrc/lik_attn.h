@@ -285,6 +285,16 @@ __device__ __forceinline__ void store_low(int8_t* row, const f32x16* acc, float 
     }
 }
 
+// The window as one unsigned test: a key is kept where 0 <= key - query + back <= reach.
+struct Window {
+  bool on;
+  int back;
+  uint32_t reach;
+  __device__ __forceinline__ explicit Window(const AttP& p)
+      : on(p.left != kNone || p.right != kNone), back(p.left == kNone ? 0x3fffffff : p.left),
+        reach((uint32_t)back + (p.right == kNone ? 0x3fffffffu : (uint32_t)p.right)) {}
+};
+
 // 16-byte rows; 64 of them within a lane's 32-bit offset
 inline bool att_rows_ok(const void* d, int64_t sn, int64_t sl, int64_t sh) {
   return (uintptr_t)d % 16 == 0 && sn % 8 == 0 && sl % 8 == 0 && sh % 8 == 0 && sl >= 0 && sl < (1 << 24);  // (64 rows of up to 2^25 bytes)

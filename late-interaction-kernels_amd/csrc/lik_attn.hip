@@ -114,16 +114,6 @@ __device__ __forceinline__ void store_rows(const AttP& p, int split, int64_t row
   if (p.low) store_low<EK, DC>(p.low + (row * p.heads + head) * p.dim, o, inv, p.dim, lane, on);
 }
 
-// The window as one unsigned test: a key is kept where 0 <= key - query + back <= reach.
-struct Window {
-  bool on;
-  int back;
-  uint32_t reach;
-  __device__ __forceinline__ explicit Window(const AttP& p)
-      : on(p.left != kNone || p.right != kNone), back(p.left == kNone ? 0x3fffffff : p.left),
-        reach((uint32_t)back + (p.right == kNone ? 0x3fffffffu : (uint32_t)p.right)) {}
-};
-
 // A workgroup of four wavefronts owns 128 queries of one head, a wavefront 32 of them as MFMA columns, and
 // walks the keys that any of them keeps, 64 at a time, in two LDS buffers: the next tile is loaded while this one
 // is used.

@@ -31,7 +31,7 @@ __device__ __forceinline__ float scale_for(float big) {
 // Gradient of q: the forward's walk over the keys (K rows also by transposing
 // reads, V rows in LDS), dq^T[d][query] += K^T ds^T. Its queries' delta, which the other kernel reads, comes
 // from the same registers.
-template <int EK, int DC, int QB>
+template <int EK, int DC>
 __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p) {
   using D = Dim<DC>;
   __shared__ __attribute__((aligned(1024))) char s_tile[2][2 * D::TILE];
@@ -48,51 +48,44 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p) {
   const int head = (int)(t % (uint32_t)p.heads), seq = (int)(t / (uint32_t)p.heads);
   const int kvh = head / p.group;
   const Span qs = span_of(p.cu_q, p.q_rows, p.q_len, seq), ks = span_of(p.cu_k, p.k_rows, p.k_len, seq);
-  const int q0 = tile * 128 * QB;
+  const int q0 = tile * 128;
   float* gmax = EK == EK_F16 ? p.gmax + ((int64_t)seq * p.heads + head) * p.q_tiles + tile : nullptr;
   if (q0 >= qs.len) {
     if (EK == EK_F16 && tid == 0) *gmax = 0.f;
     return;
   }
 
-  int qpos[QB];
-  float lse[QB], delta[QB];
-  u32x4 qf[QB][D::KS], gf[QB][D::KS];
+  u32x4 qf[D::KS], gf[D::KS];
   const char* qbase = p.q.data + (p.cu_q ? qs.row * p.q.sl : seq * p.q.sn) + head * p.q.sh;
   const char* gbase = p.g.data + (p.cu_q ? qs.row * p.g.sl : seq * p.g.sn) + head * p.g.sh;
-  bool any = false;
   float big = 0.f;
+  const int qpos = q0 + wv * 32 + l32;  // the lane's query
+  const int64_t at = (int64_t)head * p.q_total + qs.row + qpos;
+  const float lse = qpos < qs.len ? p.lse[at] : INFINITY;
+  const bool on = lse != INFINITY;  // +inf: past the end, masked, or without a key
+  load_cols<DC>(qf, on ? qbase + qpos * p.q.sl : nullptr, p.dim, lane);
+  load_cols<DC>(gf, on ? gbase + qpos * p.g.sl : nullptr, p.dim, lane);
+  const int64_t row = ((qs.row + qpos) * p.heads + head) * p.dim;
+  u32x4 of[D::KS];
+  load_cols<DC>(of, on ? p.out + row * 2 : nullptr, p.dim, lane);
+  float d = 0.f;
 #pragma unroll
-  for (int b = 0; b < QB; ++b) {
-    qpos[b] = q0 + (wv * QB + b) * 32 + l32;
-    const int64_t at = (int64_t)head * p.q_total + qs.row + qpos[b];
-    lse[b] = qpos[b] < qs.len ? p.lse[at] : INFINITY;
-    const bool on = lse[b] != INFINITY;  // +inf: past the end, masked, or without a key
-    load_cols<DC>(qf[b], on ? qbase + qpos[b] * p.q.sl : nullptr, p.dim, lane);
-    load_cols<DC>(gf[b], on ? gbase + qpos[b] * p.g.sl : nullptr, p.dim, lane);
-    const int64_t row = ((qs.row + qpos[b]) * p.heads + head) * p.dim;
-    u32x4 of[D::KS];
-    load_cols<DC>(of, on ? p.out + row * 2 : nullptr, p.dim, lane);
-    float d = 0.f;
+  for (int k = 0; k < D::KS; ++k) {
+    const int e = k * 16 + 8 * (lane >> 5);
+    u32x2 low = {0u, 0u};
+    if (on && e < p.dim) low = *(const u32x2*)(p.low + row + e);
 #pragma unroll
-    for (int k = 0; k < D::KS; ++k) {
-      const int e = k * 16 + 8 * (lane >> 5);
-      u32x2 low = {0u, 0u};
-      if (on && e < p.dim) low = *(const u32x2*)(p.low + row + e);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float g[2], o[2];
-        unpack2<EK>(gf[b][k][i / 2], g[0], g[1]);
-        unpack2<EK>(of[k][i / 2], o[0], o[1]);
-        d = fmaf(g[i % 2], with_low<EK>(o[i % 2], low[i / 4], i % 4), d);
-        if constexpr (EK == EK_F16) big = fmaxf(big, fabsf(g[i % 2]));
-      }
+    for (int i = 0; i < 8; ++i) {
+      float g[2], o[2];
+      unpack2<EK>(gf[k][i / 2], g[0], g[1]);
+      unpack2<EK>(of[k][i / 2], o[0], o[1]);
+      d = fmaf(g[i % 2], with_low<EK>(o[i % 2], low[i / 4], i % 4), d);
+      if constexpr (EK == EK_F16) big = fmaxf(big, fabsf(g[i % 2]));
     }
-    delta[b] = d + swap_half(d);
-    if (qpos[b] < qs.len && lane < 32) p.delta[at] = delta[b];
-    any |= on;
   }
-  any = __ballot(any) != 0;
+  const float delta = d + swap_half(d);
+  if (qpos < qs.len && lane < 32) p.delta[at] = delta;
+  const bool any = __ballot(on) != 0;  // this wavefront has a query
   float gs = 1.0f;  // of this wavefront's queries
   if constexpr (EK == EK_F16) {
 #pragma unroll
@@ -110,7 +103,7 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p) {
     klen = kept.extent;
     holes = kept.holes;
   }
-  const int q_end = (q0 + 128 * QB < qs.len ? q0 + 128 * QB : qs.len) - 1;
+  const int q_end = (q0 + 128 < qs.len ? q0 + 128 : qs.len) - 1;
   const int kb = p.left == kNone || q0 - p.left < 0 ? 0 : (q0 - p.left) & ~63;
   int ke = p.right == kNone || (int64_t)q_end + p.right + 1 >= klen ? klen : q_end + p.right + 1;
   if (__syncthreads_or(any) == 0 || !p.gq) ke = kb;
@@ -126,15 +119,11 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p) {
     vrows.issue(at + D::TILE, vbase + kt * p.v.sl, klen - kt, bits, wv, lane);
   };
 
-  const bool window = p.left != kNone || p.right != kNone;
-  const int back = p.left == kNone ? 0x3fffffff : p.left;
-  const uint32_t reach = (uint32_t)back + (p.right == kNone ? 0x3fffffffu : (uint32_t)p.right);
-  f32x16 acc[QB][DC];
+  const Window win(p);
+  f32x16 acc[DC];
 #pragma unroll
-  for (int b = 0; b < QB; ++b)
-#pragma unroll
-    for (int d = 0; d < DC; ++d) acc[b][d] = f32x16{};
-  const int wq0 = q0 + wv * QB * 32, wq1 = wq0 + QB * 32 - 1;
+  for (int d = 0; d < DC; ++d) acc[d] = f32x16{};
+  const int wq0 = q0 + wv * 32, wq1 = wq0 + 31;  // the wavefront's queries
   if (kb < ke) issue(lds[0], kb);
   int buf = 0;
   for (int kt = kb; kt < ke; kt += 64, buf ^= 1) {
@@ -146,65 +135,50 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p) {
                        (p.left == kNone || kt >= wq1 - p.left);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      f32x16 s[QB], dp[QB];
-#pragma unroll
-      for (int b = 0; b < QB; ++b) s[b] = dp[b] = f32x16{};
+      f32x16 s = {}, dp = {};
 #pragma unroll
       for (int k = 0; k < D::KS; ++k) {
         const u32x4 kf = frags.row(at, u * 32, k);
         const u32x4 vf = frags.row(at + D::TILE, u * 32, k);
-#pragma unroll
-        for (int b = 0; b < QB; ++b) {
-          s[b] = mfma16<EK>(s[b], kf, qf[b][k]);
-          dp[b] = mfma16<EK>(dp[b], vf, gf[b][k]);
-        }
+        s = mfma16<EK>(s, kf, qf[k]);
+        dp = mfma16<EK>(dp, vf, gf[k]);
       }
-      if (!whole) {
+      if (!whole)
+        mask_scores(s, kt + u * 32, klen, holes ? s_bits : nullptr, win.on,
+                    kt + u * 32 + 4 * (lane >> 5) - qpos + win.back, win.reach, lane);
+      u32x4 df[2];
 #pragma unroll
-        for (int b = 0; b < QB; ++b)
-          mask_scores(s[b], kt + u * 32, klen, holes ? s_bits : nullptr, window,
-                      kt + u * 32 + 4 * (lane >> 5) - qpos[b] + back, reach, lane);
+      for (int i = 0; i < 16; ++i) {
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[i], p.c, -lse));
+        s[i] = e * (EK == EK_F16 ? (dp[i] - delta) * gs : dp[i] - delta);
       }
-      u32x4 df[QB][2];
 #pragma unroll
-      for (int b = 0; b < QB; ++b) {
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float e = __builtin_amdgcn_exp2f(fmaf(s[b][i], p.c, -lse[b]));
-          s[b][i] = e * (EK == EK_F16 ? (dp[b][i] - delta[b]) * gs : dp[b][i] - delta[b]);
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) df[b][k][e] = pack2<EK>(s[b][k * 8 + 2 * e], s[b][k * 8 + 2 * e + 1]);
-      }
+        for (int e = 0; e < 4; ++e) df[k][e] = pack2<EK>(s[k * 8 + 2 * e], s[k * 8 + 2 * e + 1]);
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int d = 0; d < DC; ++d) {
           const u32x4 kf = frags.col(at, u * 32 + k * 16, d);
-#pragma unroll
-          for (int b = 0; b < QB; ++b) acc[b][d] = mfma16<EK>(acc[b][d], kf, df[b][k]);
+          acc[d] = mfma16<EK>(acc[d], kf, df[k]);
         }
     }
   }
   if (!p.gq) return;
-#pragma unroll
-  for (int b = 0; b < QB; ++b)
-    store_cols<EK, DC>(p.gq + ((qs.row + qpos[b]) * p.heads + head) * p.dim * 2, acc[b], p.scale / gs, p.dim, lane,
-                       qpos[b] < qs.len);
+  store_cols<EK, DC>(p.gq + ((qs.row + qpos) * p.heads + head) * p.dim * 2, acc, p.scale / gs, p.dim, lane,
+                     qpos < qs.len);
 }
 
-// Gradients of k and v: a wavefront owns 32 KB keys as MFMA columns and walks the queries of the group's
+// Gradients of k and v: a wavefront owns 32 keys as MFMA columns and walks the queries of the group's
 // heads, QT at a time. K and V are in registers; for head dims over 64 V's rows stay in LDS instead and the
 // steps are 32 queries (two wavefronts a SIMD then fit: 455 -> 258 us for 16 x 1030 causal rows, 16 / 4 heads).
 //   P[query][key] from S = Q K^T;  dv^T[d][key] += G^T P;  dp = G V^T;  dk^T[d][key] += Q^T ds
-template <int EK, int DC, int KB>
+template <int EK, int DC>
 __global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p) {
   using D = Dim<DC>;
   constexpr bool VL = DC > 2;  // V in LDS
   constexpr int QT = VL ? 32 : 64, TILE = D::PITCH * QT;
-  static_assert(!VL || KB == 1, "");
   __shared__ __attribute__((aligned(1024))) char s_tile[2][2 * TILE];
   __shared__ __attribute__((aligned(1024))) char s_v[VL ? 2 * D::TILE : 16];
   __shared__ __attribute__((aligned(16))) float s_stat[2][2][QT];
@@ -221,7 +195,7 @@ __global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p) {
   const int kv_heads = p.heads / p.group;
   const int kvh = (int)(t % (uint32_t)kv_heads), seq = (int)(t / (uint32_t)kv_heads);
   const Span qs = span_of(p.cu_q, p.q_rows, p.q_len, seq), ks = span_of(p.cu_k, p.k_rows, p.k_len, seq);
-  const int k0 = tile * 128 * KB;
+  const int k0 = tile * 128;
   if (k0 >= ks.len) return;
   float gs = 1.0f;
   if constexpr (EK == EK_F16) {
@@ -235,21 +209,14 @@ __global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p) {
     gs = scale_for(fmaxf(fmaxf(s_big[0], s_big[1]), fmaxf(s_big[2], s_big[3])));
   }
 
-  int kpos[KB];
-  bool kon[KB];
-  u32x4 kf[KB][D::KS], vf[KB][VL ? 1 : D::KS];
+  u32x4 kf[D::KS], vf[VL ? 1 : D::KS];
   const char* kbase = p.k.data + (p.cu_k ? ks.row * p.k.sl : seq * p.k.sn) + kvh * p.k.sh;
   const char* vbase = p.v.data + (p.cu_k ? ks.row * p.v.sl : seq * p.v.sn) + kvh * p.v.sh;
-  bool any = false;
-#pragma unroll
-  for (int b = 0; b < KB; ++b) {
-    kpos[b] = k0 + (wv * KB + b) * 32 + l32;
-    kon[b] = kpos[b] < ks.len && (!p.km || p.km[seq * p.km_sn + kpos[b] * p.km_sl] != 0);
-    load_cols<DC>(kf[b], kon[b] ? kbase + kpos[b] * p.k.sl : nullptr, p.dim, lane);
-    if constexpr (!VL) load_cols<DC>(vf[b], kon[b] ? vbase + kpos[b] * p.v.sl : nullptr, p.dim, lane);
-    any |= kon[b];
-  }
-  any = __ballot(any) != 0;
+  const int kpos = k0 + wv * 32 + l32;  // the lane's key
+  const bool kon = kpos < ks.len && (!p.km || p.km[seq * p.km_sn + kpos * p.km_sl] != 0);
+  load_cols<DC>(kf, kon ? kbase + kpos * p.k.sl : nullptr, p.dim, lane);
+  if constexpr (!VL) load_cols<DC>(vf, kon ? vbase + kpos * p.v.sl : nullptr, p.dim, lane);
+  const bool any = __ballot(kon) != 0;
   if constexpr (VL) {  // (what masked rows hold stays in their own columns)
     const Rows<DC> vrows(p.v.sl, p.dim, wv, lane);
 #pragma unroll
@@ -265,7 +232,7 @@ __global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p) {
     holes = kept.holes;
   }
   // queries that keep one of these keys: key - right <= query <= key + left
-  const int k_end = (k0 + 128 * KB < ks.len ? k0 + 128 * KB : ks.len) - 1;
+  const int k_end = (k0 + 128 < ks.len ? k0 + 128 : ks.len) - 1;
   const int qb = p.right == kNone || k0 - p.right < 0 ? 0 : (k0 - p.right) & ~63;
   int qe = p.left == kNone || (int64_t)k_end + p.left + 1 >= qlen ? qlen : k_end + p.left + 1;
   if (__syncthreads_or(any) == 0) qe = qb;
@@ -295,12 +262,10 @@ __global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p) {
   // a query keeps a key where 0 <= query - key + ahead <= reach
   const int ahead = p.right == kNone ? 0x3fffffff : p.right;
   const uint32_t reach = (uint32_t)ahead + (p.left == kNone ? 0x3fffffffu : (uint32_t)p.left);
-  f32x16 dk[KB][DC], dv[KB][DC];
+  f32x16 dk[DC], dv[DC];
 #pragma unroll
-  for (int b = 0; b < KB; ++b)
-#pragma unroll
-    for (int d = 0; d < DC; ++d) dk[b][d] = dv[b][d] = f32x16{};
-  const int wk0 = k0 + wv * KB * 32, wk1 = wk0 + KB * 32 - 1;  // the wavefront's keys
+  for (int d = 0; d < DC; ++d) dk[d] = dv[d] = f32x16{};
+  const int wk0 = k0 + wv * 32, wk1 = wk0 + 31;  // the wavefront's keys
   const int total = steps * p.group;
   int head = kvh * p.group, qt = qb;
   if (total) {
@@ -329,43 +294,32 @@ __global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p) {
           (p.left == kNone || now + QT - 1 <= wk0 + p.left) && (p.right == kNone || now >= wk1 - p.right);
 #pragma unroll
       for (int u = 0; u < QT / 32; ++u) {
-        f32x16 s[KB], dp[KB];
-#pragma unroll
-        for (int b = 0; b < KB; ++b) s[b] = dp[b] = f32x16{};
+        f32x16 s = {}, dp = {};
 #pragma unroll
         for (int k = 0; k < D::KS; ++k) {
           const u32x4 qf = frags.row(at, u * 32, k);
           const u32x4 gf = frags.row(at + TILE, u * 32, k);
-#pragma unroll
-          for (int b = 0; b < KB; ++b) {
-            s[b] = mfma16<EK>(s[b], qf, kf[b][k]);
-            dp[b] = mfma16<EK>(dp[b], gf, VL ? frags.row(lds_addr(s_v), wv * 32, k) : vf[b][VL ? 0 : k]);
-          }
+          s = mfma16<EK>(s, qf, kf[k]);
+          dp = mfma16<EK>(dp, gf, VL ? frags.row(lds_addr(s_v), wv * 32, k) : vf[VL ? 0 : k]);
         }
-        if (!whole) {
-#pragma unroll
-          for (int b = 0; b < KB; ++b)
-            mask_scores(s[b], 0, 64, nullptr, true, now + u * 32 + 4 * (lane >> 5) - kpos[b] + ahead, reach, lane);
-        }
-        u32x4 pf[KB][2], df[KB][2];
+        if (!whole)
+          mask_scores(s, 0, 64, nullptr, true, now + u * 32 + 4 * (lane >> 5) - kpos + ahead, reach, lane);
+        u32x4 pf[2], df[2];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const f32x4 ls = *(const f32x4*)&s_stat[buf][0][u * 32 + 8 * q + 4 * (lane >> 5)];
           const f32x4 dl = *(const f32x4*)&s_stat[buf][1][u * 32 + 8 * q + 4 * (lane >> 5)];
+          float e[4], ds[4];
 #pragma unroll
-          for (int b = 0; b < KB; ++b) {
-            float e[4], ds[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              e[i] = __builtin_amdgcn_exp2f(fmaf(s[b][q * 4 + i], p.c, -ls[i]));
-              const float x = dp[b][q * 4 + i] - dl[i];
-              ds[i] = e[i] * (EK == EK_F16 ? x * gs : x);
-            }
-            pf[b][q / 2][(q % 2) * 2] = pack2<EK>(e[0], e[1]);
-            pf[b][q / 2][(q % 2) * 2 + 1] = pack2<EK>(e[2], e[3]);
-            df[b][q / 2][(q % 2) * 2] = pack2<EK>(ds[0], ds[1]);
-            df[b][q / 2][(q % 2) * 2 + 1] = pack2<EK>(ds[2], ds[3]);
+          for (int i = 0; i < 4; ++i) {
+            e[i] = __builtin_amdgcn_exp2f(fmaf(s[q * 4 + i], p.c, -ls[i]));
+            const float x = dp[q * 4 + i] - dl[i];
+            ds[i] = e[i] * (EK == EK_F16 ? x * gs : x);
           }
+          pf[q / 2][(q % 2) * 2] = pack2<EK>(e[0], e[1]);
+          pf[q / 2][(q % 2) * 2 + 1] = pack2<EK>(e[2], e[3]);
+          df[q / 2][(q % 2) * 2] = pack2<EK>(ds[0], ds[1]);
+          df[q / 2][(q % 2) * 2 + 1] = pack2<EK>(ds[2], ds[3]);
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k)
@@ -373,26 +327,20 @@ __global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p) {
           for (int d = 0; d < DC; ++d) {
             const u32x4 gc = frags.col(at + TILE, u * 32 + k * 16, d);
             const u32x4 qc = frags.col(at, u * 32 + k * 16, d);
-#pragma unroll
-            for (int b = 0; b < KB; ++b) {
-              dv[b][d] = mfma16<EK>(dv[b][d], gc, pf[b][k]);
-              dk[b][d] = mfma16<EK>(dk[b][d], qc, df[b][k]);
-            }
+            dv[d] = mfma16<EK>(dv[d], gc, pf[k]);
+            dk[d] = mfma16<EK>(dk[d], qc, df[k]);
           }
       }
     }
     if (it + 1 < total && tid < 2 * QT) s_stat[buf ^ 1][tid / QT][tid % QT] = next;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // V's loads where there was no step
+  if (!kon)  // masked keys have no gradient (their lanes ran on zero rows)
 #pragma unroll
-  for (int b = 0; b < KB; ++b) {
-    if (!kon[b])  // masked keys have no gradient (their lanes ran on zero rows)
-#pragma unroll
-      for (int d = 0; d < DC; ++d) dk[b][d] = dv[b][d] = f32x16{};
-    const int64_t at = ((ks.row + kpos[b]) * kv_heads + kvh) * p.dim * 2;
-    store_cols<EK, DC>(p.gk + at, dk[b], p.scale / gs, p.dim, lane, kpos[b] < ks.len);
-    store_cols<EK, DC>(p.gv + at, dv[b], 1.0f, p.dim, lane, kpos[b] < ks.len);
-  }
+    for (int d = 0; d < DC; ++d) dk[d] = dv[d] = f32x16{};
+  const int64_t at = ((ks.row + kpos) * kv_heads + kvh) * p.dim * 2;
+  store_cols<EK, DC>(p.gk + at, dk, p.scale / gs, p.dim, lane, kpos < ks.len);
+  store_cols<EK, DC>(p.gv + at, dv, 1.0f, p.dim, lane, kpos < ks.len);
 }
 
 template <int EK, int DC>
@@ -400,14 +348,14 @@ int launch_backward(AttP p, hipStream_t s) {
   p.tiles = p.q_tiles;
   unsigned grid = work_grid(p, (int64_t)p.tiles * p.n * p.heads, (int64_t)p.tiles * p.group);
   if (!grid) return LIK_ERR_UNSUPPORTED;
-  launch_kernel(attention_dq_kernel<EK, DC, 1>, dim3(grid), dim3(256), p.km ? mask_words(p.k_len) * 4 : 0u, s, p);
+  launch_kernel(attention_dq_kernel<EK, DC>, dim3(grid), dim3(256), p.km ? mask_words(p.k_len) * 4 : 0u, s, p);
   if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
   p.tiles = (int)((p.k_len + 127) / 128);
   const int64_t wgs = (int64_t)p.n * (p.heads / p.group) * p.tiles;
   if (!p.gk || !wgs) return LIK_OK;
   grid = work_grid(p, wgs, p.tiles);
   if (!grid) return LIK_ERR_UNSUPPORTED;
-  launch_kernel(attention_dkv_kernel<EK, DC, 1>, dim3(grid), dim3(256), p.qm ? mask_words(p.q_len) * 4 : 0u, s, p);
+  launch_kernel(attention_dkv_kernel<EK, DC>, dim3(grid), dim3(256), p.qm ? mask_words(p.q_len) * 4 : 0u, s, p);
   return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;
 }
 
