@@ -171,14 +171,15 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p) {
 }
 
 // Gradients of k and v: a wavefront owns 32 keys as MFMA columns and walks the queries of the group's
-// heads, QT at a time. K and V are in registers; for head dims over 64 V's rows stay in LDS instead and the
-// steps are 32 queries (two wavefronts a SIMD then fit: 455 -> 258 us for 16 x 1030 causal rows, 16 / 4 heads).
+// heads, QT at a time, K in registers. For head dims over 32 V's rows stay in LDS, which leaves room for three
+// wavefronts a SIMD up to 64 (262 -> 252 us for the training step on 128 passages) and for two above, where a
+// step is 32 queries (455 -> 258 us of this kernel for 16 x 1030 causal rows, 16 / 4 heads of 128).
 //   P[query][key] from S = Q K^T;  dv^T[d][key] += G^T P;  dp = G V^T;  dk^T[d][key] += Q^T ds
 template <int EK, int DC>
-__global__ void __launch_bounds__(256, 2) attention_dkv_kernel(const AttP p) {
+__global__ void __launch_bounds__(256, DC <= 2 ? 3 : 2) attention_dkv_kernel(const AttP p) {
   using D = Dim<DC>;
-  constexpr bool VL = DC > 2;  // V in LDS
-  constexpr int QT = VL ? 32 : 64, TILE = D::PITCH * QT;
+  constexpr bool VL = DC > 1;  // V in LDS
+  constexpr int QT = DC > 2 ? 32 : 64, TILE = D::PITCH * QT;
   __shared__ __attribute__((aligned(1024))) char s_tile[2][2 * TILE];
   __shared__ __attribute__((aligned(1024))) char s_v[VL ? 2 * D::TILE : 16];
   __shared__ __attribute__((aligned(16))) float s_stat[2][2][QT];
