@@ -384,7 +384,9 @@ void forward_shape(AttP& p) {
     const int64_t most = (p.k_len + 255) / 256;
     if (s > most) s = most;
     if (s > 16) s = 16;
-    p.splits = 4 * (int)(s < 1 ? 1 : s);
+    if (s < 1) s = 1;
+    if (s < 2 && p.k_len > 1 << 17) s = 2;  // (a workgroup's keep bits, beside 128 KB of tiles)
+    p.splits = 4 * (int)s;
     return;
   }
   const int64_t wgs = (int64_t)p.n * p.heads * p.tiles;
@@ -401,9 +403,9 @@ size_t forward_ws(const AttP& p) {
 
 template <int EK, int DC>
 int launch_forward(AttP p, hipStream_t s) {
-  const uint32_t bits = p.km ? mask_words(p.k_len) * 4 : 0u;
   if (p.few) {
-    const int64_t per = p.splits / 4;
+    const int64_t per = p.splits / 4, steps = ((p.k_len + 31) / 32 + p.splits - 1) / p.splits;
+    const uint32_t bits = p.km ? mask_words(4 * 32 * steps) * 4 : 0u;  // a workgroup's keys
     const unsigned grid = work_grid(p, per * p.n * (p.heads / p.group), per);
     if (!grid) return LIK_ERR_UNSUPPORTED;
     if (p.q_len * p.group <= 32)
@@ -414,7 +416,7 @@ int launch_forward(AttP p, hipStream_t s) {
     const int64_t per = (int64_t)p.tiles * p.splits;
     const unsigned grid = work_grid(p, per * p.n * p.heads, per * p.group);
     if (!grid) return LIK_ERR_UNSUPPORTED;
-    launch_kernel(attention_kernel<EK, DC>, dim3(grid), dim3(256), bits, s, p);
+    launch_kernel(attention_kernel<EK, DC>, dim3(grid), dim3(256), p.km ? mask_words(p.k_len) * 4 : 0u, s, p);
   }
   if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
   if (p.splits > 1) {

@@ -326,6 +326,25 @@ def test_long_masked_keys():
     assert off(got[0], want) <= 1.25 * ROUNDOFF[BF]
 
 
+@pytest.mark.parametrize("lk", [1 << 17, (1 << 17) + 33, 1 << 18])
+@pytest.mark.parametrize("d", [64, 128])
+def test_longest_masks_with_many_heads(lk, d):
+    """As many keys as a mask may have, read by so many heads that a workgroup takes large shares of them: few rows
+    and a tile of rows. The heads' keys are one tensor."""
+    _case(lk, d)
+    h = 300
+    g = torch.Generator().manual_seed(11)
+    k, v = (torch.randn(1, lk, 1, d, generator=g).to(BF) for _ in range(2))
+    km = torch.zeros(1, lk, dtype=torch.bool)
+    km[0, :70] = km[0, lk // 2 - 9:lk // 2 + 50:2] = km[0, -40:] = True
+    at = km[0].nonzero()[:, 0]
+    for lq in (1, 66):
+        q = (torch.randn(1, lq, h, d, generator=g) * 1.5).to(BF)
+        got = attention(q.cuda(), *(t.cuda().expand(-1, -1, h, -1) for t in (k, v)), None, km.cuda()).cpu()
+        want = attention64(q[0].double(), k[0, at].double(), v[0, at].double(), torch.ones(lq, len(at)).bool(), d**-0.5)
+        assert off(got[0], want) <= 1.25 * ROUNDOFF[BF]
+
+
 def test_side_stream():
     q, k, v, gy = (t.cuda() for t in _make(2, 300, 300, 2, 2, 64, BF))
     want = attention(q, k, v)
