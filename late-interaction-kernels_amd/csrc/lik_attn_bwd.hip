@@ -8,8 +8,8 @@
 // same bits every time) and no fp32 gradient of q to clear, add to and convert.
 // 16 causal sequences of 1030 rows, 16 heads over 4 of 128, bf16: 197 us (530 TFLOP/s of its three products) and
 // 255 us (545, four), two wavefronts a SIMD at 238 and 256 registers, bound by the chain from scores to
-// probabilities to products inside a wavefront; 128 passages of 50 to 300 rows, 12 heads of 64: 87 and 106 us (50 each
-// at the copy rate), half of it tiles that a passage does not fill.
+// probabilities to products inside a wavefront. Sequences of 129 to 320 keys have one kernel for all three: 128 passages of 50 to 300
+// rows, 12 heads of 64: 160 us, the two 88 and 93.
 // p and ds are rounded once to the 16-bit type, as the products' operands have to be.
 // fp16 would lose small gradients there: g is scaled by the power of two that
 // brings its largest element to 1/2 .. 1 (of a wavefront's queries; of a key head's), and the sums are scaled
@@ -26,6 +26,30 @@ __device__ __forceinline__ float scale_for(float big) {
   int e;
   frexpf(big, &e);  // big = m 2^e, m in 1/2 .. 1
   return ldexpf(1.0f, -e);
+}
+
+// delta of the lane's query, whose g is in columns (on: it has one; else 0), and the largest |g| for fp16. row: its first
+// element in the output.
+template <int EK, int DC>
+__device__ __forceinline__ float row_delta(const AttP& p, const u32x4* gf, int64_t row, bool on, float& big, int lane) {
+  u32x4 of[Dim<DC>::KS];
+  load_cols<DC>(of, on ? p.out + row * 2 : nullptr, p.dim, lane);
+  float d = 0.f;
+#pragma unroll
+  for (int k = 0; k < Dim<DC>::KS; ++k) {
+    const int e = k * 16 + 8 * (lane >> 5);
+    u32x2 low = {0u, 0u};
+    if (on && e < p.dim) low = *(const u32x2*)(p.low + row + e);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float g[2], o[2];
+      unpack2<EK>(gf[k][i / 2], g[0], g[1]);
+      unpack2<EK>(of[k][i / 2], o[0], o[1]);
+      d = fmaf(g[i % 2], with_low<EK>(o[i % 2], low[i / 4], i % 4), d);
+      if constexpr (EK == EK_F16) big = fmaxf(big, fabsf(g[i % 2]));
+    }
+  }
+  return d + swap_half(d);
 }
 
 // Gradient of q: the forward's walk over the keys (K rows also by transposing
@@ -66,24 +90,7 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p) {
   load_cols<DC>(qf, on ? qbase + qpos * p.q.sl : nullptr, p.dim, lane);
   load_cols<DC>(gf, on ? gbase + qpos * p.g.sl : nullptr, p.dim, lane);
   const int64_t row = ((qs.row + qpos) * p.heads + head) * p.dim;
-  u32x4 of[D::KS];
-  load_cols<DC>(of, on ? p.out + row * 2 : nullptr, p.dim, lane);
-  float d = 0.f;
-#pragma unroll
-  for (int k = 0; k < D::KS; ++k) {
-    const int e = k * 16 + 8 * (lane >> 5);
-    u32x2 low = {0u, 0u};
-    if (on && e < p.dim) low = *(const u32x2*)(p.low + row + e);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float g[2], o[2];
-      unpack2<EK>(gf[k][i / 2], g[0], g[1]);
-      unpack2<EK>(of[k][i / 2], o[0], o[1]);
-      d = fmaf(g[i % 2], with_low<EK>(o[i % 2], low[i / 4], i % 4), d);
-      if constexpr (EK == EK_F16) big = fmaxf(big, fabsf(g[i % 2]));
-    }
-  }
-  const float delta = d + swap_half(d);
+  const float delta = row_delta<EK, DC>(p, gf, row, on, big, lane);
   if (qpos < qs.len && lane < 32) p.delta[at] = delta;
   const bool any = __ballot(on) != 0;  // this wavefront has a query
   float gs = 1.0f;  // of this wavefront's queries
@@ -344,8 +351,240 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 3 : 2) attention_dkv_kernel(con
   store_cols<EK, DC>(p.gv + at, dv, 1.0f, p.dim, lane, kpos < ks.len);
 }
 
+// All gradients of sequences of up to 32 KW keys in one pass: five products and one read of the rows, no sum in memory. A
+// workgroup has a key head. KW wavefronts own 32 keys each, as above (K and V in registers), and walk the queries 32 at a time; their
+// ds goes through LDS to DC more wavefronts with a block of 32 head dims each: dq^T[d][query] = K^T ds^T of the step before, over all
+// keys at once. The queries' statistics come first, by all wavefronts (one wait for memory, and the rows are in L2 for the walk):
+// up to kShortRows of them, all heads of the group together.
+// 128 passages of 50 to 300 rows padded to 300, 12 heads of 64, bf16: 160 us, 80 of them the reads and writes around the walk (65 at the copy
+// rate; a workgroup of 12 wavefronts at 168 registers fills a CU, so its walk overlaps no other's loads), 70 the steps.
+constexpr int kShortRows = 2048;
+template <int EK, int DC, int KW>
+__global__ void __launch_bounds__((KW + DC) * 64, (KW + DC + 3) / 4) attention_grads_kernel(const AttP p) {
+  using D = Dim<DC>;
+  constexpr int T = (KW + DC) * 64, TILE = 32 * D::PITCH, DS = 32 * 64;
+  __shared__ __attribute__((aligned(1024))) char s_k[KW * TILE];
+  __shared__ __attribute__((aligned(1024))) char s_tile[3][2 * TILE];
+  __shared__ __attribute__((aligned(1024))) char s_ds[2][KW * DS];  // [key][query], 16-byte chunks exchanged by (key / 4) % 4
+  __shared__ __attribute__((aligned(16))) float s_lse[kShortRows], s_delta[kShortRows];  // 32 a step
+  __shared__ float s_big[KW + DC];
+  __shared__ int s_blocks, s_last;
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int item = work_item(p);
+  if (item < 0) return;
+  const int kv_heads = p.heads / p.group;
+  const int kvh = item % kv_heads, seq = item / kv_heads;
+  const Span qs = span_of(p.cu_q, p.q_rows, p.q_len, seq), ks = span_of(p.cu_k, p.k_rows, p.k_len, seq);
+  if (tid == 0) s_blocks = s_last = 0;
+  __syncthreads();
+
+  const int head0 = kvh * p.group, most = (qs.len + 31) / 32;
+  const char* const q0 = p.q.data + (p.cu_q ? qs.row * p.q.sl : seq * p.q.sn);
+  const char* const g0 = p.g.data + (p.cu_q ? qs.row * p.g.sl : seq * p.g.sn);
+  // +inf: past the end, masked, or without a key
+  auto lse_of = [&](int head, int pos) {
+    return pos < qs.len ? p.lse[(int64_t)head * p.q_total + qs.row + pos] : INFINITY;
+  };
+  // the wavefront's keys; rows that are none or masked are zeros
+  const bool keys = wv < KW;
+  const int kpos = wv * 32 + l32;
+  // (what the first loads wait for, at once)
+  const bool kon = keys && kpos < ks.len && (!p.km || p.km[seq * p.km_sn + kpos * p.km_sl] != 0);
+  float lse = wv < most * p.group ? lse_of(head0 + wv / most, wv % most * 32 + l32) : INFINITY;
+  const float lse0 = wv < 4 ? lse_of(head0, wv * 8 + lane / 8) : INFINITY;
+
+  // Q and G of 32 queries, by four wavefronts; rows without a statistic are not read
+  const bool loads = wv < 4;
+  const Rows<DC, 32, 4> qrows(p.q.sl, p.dim, wv & 3, lane), grows(p.g.sl, p.dim, wv & 3, lane);
+  auto issue = [&](int buf, int head, int qt, float lse) {
+    const bool on = lse != INFINITY;
+    const uint32_t at = lds_addr(s_tile[buf]) + wv * 1024;
+    dma16(at, on ? qrows.off[0] : kOob, raw_desc(q0 + head * p.q.sh + qt * p.q.sl, 0xffffff00u));
+    dma16(at + TILE, on ? grows.off[0] : kOob, raw_desc(g0 + head * p.g.sh + qt * p.g.sl, 0xffffff00u));
+  };
+  if (loads) issue(0, head0, 0, lse0);
+  const char* kbase = p.k.data + (p.cu_k ? ks.row * p.k.sl : seq * p.k.sn) + kvh * p.k.sh;
+  const char* vbase = p.v.data + (p.cu_k ? ks.row * p.v.sl : seq * p.v.sn) + kvh * p.v.sh;
+  u32x4 kf[D::KS], vf[D::KS];
+  load_cols<DC>(kf, kon ? kbase + kpos * p.k.sl : nullptr, p.dim, lane);
+  load_cols<DC>(vf, kon ? vbase + kpos * p.v.sl : nullptr, p.dim, lane);
+  const bool any = __ballot(kon) != 0;
+  if (any && lane == 0) atomicMax(&s_blocks, wv + 1);
+
+  float gs = 1.0f, big = 0.f;
+  for (int it = wv; it < most * p.group;) {
+    const int head = head0 + it / most, qt = it % most * 32, pos = qt + l32;
+    const bool on = lse != INFINITY;
+    const int64_t row = ((qs.row + pos) * p.heads + head) * p.dim;
+    u32x4 gf[D::KS];
+    load_cols<DC>(gf, on ? g0 + head * p.g.sh + pos * p.g.sl : nullptr, p.dim, lane);
+    const float d = row_delta<EK, DC>(p, gf, row, on, big, lane);
+    if (lane < 32) {
+      s_lse[it * 32 + l32] = lse;
+      s_delta[it * 32 + l32] = d;
+    }
+    if (__ballot(on) && lane == 0) atomicMax(&s_last, qt + 32);
+    it += KW + DC;
+    if (it < most * p.group) lse = lse_of(head0 + it / most, it % most * 32 + l32);
+  }
+  if constexpr (EK == EK_F16) {
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) big = fmaxf(big, __shfl_xor(big, s));
+    if (lane == 0) s_big[wv] = big;
+  }
+  if (keys)
+#pragma unroll
+    for (int k = 0; k < D::KS; ++k)
+      *(u32x4*)(s_k + kpos * D::PITCH + (((2 * k + h) ^ D::swz(l32)) << 4)) = kf[k];
+  __syncthreads();
+  const int blocks = (s_blocks + 1) & ~1;  // of 32 keys, read in pairs
+  int qe = s_last < qs.len ? s_last : qs.len;  // queries to walk: a window ends before the last one
+  if (p.left != kNone && (int64_t)ks.len + p.left < qe) qe = ks.len + p.left;
+  if (!blocks) qe = 0;
+  const int steps = (qe + 31) / 32, total = steps * p.group;
+  if constexpr (EK == EK_F16) {
+    big = 0.f;
+#pragma unroll
+    for (int w = 0; w < KW + DC; ++w) big = fmaxf(big, s_big[w]);
+    gs = scale_for(big);
+  }
+
+  struct Pos {
+    int head, qt;
+  };
+  auto after = [&](Pos a) { return a.qt + 32 < qe ? Pos{a.head, a.qt + 32} : Pos{a.head + 1, 0}; };
+  const Frags<DC> frags(lane);
+  if (keys) {
+    // a query keeps a key where 0 <= query - key + ahead <= reach
+    const int ahead = p.right == kNone ? 0x3fffffff : p.right;
+    const uint32_t reach = (uint32_t)ahead + (p.left == kNone ? 0x3fffffffu : (uint32_t)p.left);
+    const int wk0 = wv * 32, wk1 = wk0 + 31;
+    const uint32_t kept = kon ? 0xffffffffu : 0u;
+    f32x16 dk[DC], dv[DC];
+#pragma unroll
+    for (int d = 0; d < DC; ++d) dk[d] = dv[d] = f32x16{};
+    auto issue_step = [&](int buf, Pos a) {
+      issue(buf, a.head, a.qt, s_lse[(a.head - head0) * most * 32 + a.qt + wv * 8 + lane / 8]);
+    };
+    Pos now = {head0, 0}, ahead2 = after(now);
+    if (loads && total > 1) issue_step(1, ahead2);
+    int buf = 0;
+    for (int it = 0; it < total; ++it, buf = buf == 2 ? 0 : buf + 1) {
+      if (it + 1 < total) asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      ahead2 = after(ahead2);
+      if (loads && it + 2 < total) issue_step(buf ? buf - 1 : 2, ahead2);
+      const int qt = now.qt, stat = (now.head - head0) * most * 32 + qt;
+      now = after(now);
+      if (wv >= blocks) continue;
+      char* const ds_row = s_ds[it & 1] + kpos * 64 + 8 * h;
+      u32x4 pf[2], df[2] = {};
+      if (any && (p.left == kNone || qt <= wk1 + p.left) && (p.right == kNone || qt + 31 >= wk0 - p.right)) {
+        const uint32_t at = lds_addr(s_tile[buf]);
+        f32x16 s = {}, dp = {};
+#pragma unroll
+        for (int k = 0; k < D::KS; ++k) {
+          s = mfma16<EK>(s, frags.row(at, 0, k), kf[k]);
+          dp = mfma16<EK>(dp, frags.row(at + TILE, 0, k), vf[k]);
+        }
+        if ((p.left != kNone && qt + 31 > wk0 + p.left) || (p.right != kNone && qt < wk1 - p.right))
+          mask_scores(s, 0, 64, nullptr, true, qt + 4 * h - kpos + ahead, reach, lane);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 ls = *(const f32x4*)&s_lse[stat + 8 * q + 4 * h];
+          const f32x4 dl = *(const f32x4*)&s_delta[stat + 8 * q + 4 * h];
+          float e[4], ds[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            e[i] = __builtin_amdgcn_exp2f(fmaf(s[q * 4 + i], p.c, -ls[i]));
+            const float x = dp[q * 4 + i] - dl[i];
+            ds[i] = e[i] * (EK == EK_F16 ? x * gs : x);
+          }
+          pf[q / 2][(q % 2) * 2] = pack2<EK>(e[0], e[1]);
+          pf[q / 2][(q % 2) * 2 + 1] = pack2<EK>(e[2], e[3]);
+          df[q / 2][(q % 2) * 2] = pack2<EK>(ds[0], ds[1]) & kept;
+          df[q / 2][(q % 2) * 2 + 1] = pack2<EK>(ds[2], ds[3]) & kept;
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int d = 0; d < DC; ++d) {
+            dv[d] = mfma16<EK>(dv[d], frags.col(at + TILE, k * 16, d), pf[k]);
+            dk[d] = mfma16<EK>(dk[d], frags.col(at, k * 16, d), df[k]);
+          }
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *(u32x2*)(ds_row + ((q ^ ((l32 >> 2) & 3)) << 4)) = u32x2{df[q / 2][(q % 2) * 2], df[q / 2][(q % 2) * 2 + 1]};
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (!kon)  // as above
+#pragma unroll
+      for (int d = 0; d < DC; ++d) dk[d] = dv[d] = f32x16{};
+    const int64_t at = ((ks.row + kpos) * kv_heads + kvh) * p.dim * 2;
+    store_cols<EK, DC>(p.gk + at, dk, p.scale / gs, p.dim, lane, kpos < ks.len);
+    store_cols<EK, DC>(p.gv + at, dv, 1.0f, p.dim, lane, kpos < ks.len);
+  } else {
+    const int block = wv - KW;  // of 32 head dims
+    // transposing reads of ds: lane l has query l % 32 of keys row0 + 4 (l / 32) + {0..3, 8..11}, as Frags::col
+    const int i16 = lane & 15, col = (lane & 16) + 4 * (i16 & 3), c0 = 4 * h + (i16 >> 2);
+    const uint32_t lo = c0 * 64 + (((col >> 3) ^ ((c0 >> 2) & 3)) << 4) + ((col & 4) << 1);
+    const uint32_t hi = (c0 + 8) * 64 + (((col >> 3) ^ (((c0 + 8) >> 2) & 3)) << 4) + ((col & 4) << 1);
+    Pos before = {head0, 0};
+    for (int it = 0; it <= total; ++it) {
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (it && p.gq) {
+        const uint32_t at = lds_addr(s_ds[(it - 1) & 1]), kt = lds_addr(s_k);
+        f32x16 acc = {};
+        for (int b = 0; b < blocks; b += 2)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t d = at + b * DS + k * 1024;
+            const u32x2 x = lds_tr(d + lo), y = lds_tr(d + hi);
+            acc = mfma16<EK>(acc, frags.col(kt + b * TILE, k * 16, block), u32x4{x[0], x[1], y[0], y[1]});
+          }
+        const int pos = before.qt + l32;
+        store_cols<EK, 1>(p.gq + (((qs.row + pos) * p.heads + before.head) * p.dim + block * 32) * 2, &acc, p.scale / gs,
+                          p.dim - block * 32, lane, pos < qs.len);
+        before = after(before);
+      }
+    }
+  }
+  if (p.gq) {  // queries after the last step have none of the keys
+    const int chunks = p.group * p.dim / 8;
+    for (int i = tid; i < (qs.len - steps * 32) * chunks; i += T) {
+      const int64_t row = (qs.row + steps * 32 + i / chunks) * p.heads + head0;
+      *(u32x4*)(p.gq + row * p.dim * 2 + i % chunks * 16) = u32x4{0u, 0u, 0u, 0u};
+    }
+  }
+}
+
+// One kernel for all gradients: 129 to 320 keys (up to 128 the two kernels have more workgroups a CU: 128 passages of 128 rows 160 us, one
+// kernel 171; a key head more than one of these is one tile of theirs), if a workgroup's walk is short or there are enough
+// of them (4 key heads of 63 steps: 111 us, two kernels 71; 192 of 32: 82 and 101; 256 of 64: 178 and 232). Where k and v need no
+// gradient the first of the two kernels alone is faster.
+bool one_pass(const AttP& p) {
+  const int64_t steps = (p.q_len + 31) / 32 * p.group;
+  return p.gk && p.k_len > 128 && p.k_len <= 320 && steps * 32 <= kShortRows &&
+         (steps <= 32 || (int64_t)p.n * (p.heads / p.group) >= 192);
+}
+template <int EK, int DC, int KW>
+int launch_grads(AttP p, hipStream_t s) {
+  const unsigned grid = work_grid(p, (int64_t)p.n * (p.heads / p.group), 1);
+  if (!grid) return LIK_ERR_UNSUPPORTED;
+  launch_kernel(attention_grads_kernel<EK, DC, KW>, dim3(grid), dim3((KW + DC) * 64), 0u, s, p);
+  return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;
+}
+
 template <int EK, int DC>
 int launch_backward(AttP p, hipStream_t s) {
+  if constexpr (DC <= 2) {
+    if (one_pass(p)) {
+      if (p.k_len <= 192) return launch_grads<EK, DC, 6>(p, s);
+      return launch_grads<EK, DC, 10>(p, s);
+    }
+  }
   p.tiles = p.q_tiles;
   unsigned grid = work_grid(p, (int64_t)p.tiles * p.n * p.heads, (int64_t)p.tiles * p.group);
   if (!grid) return LIK_ERR_UNSUPPORTED;
