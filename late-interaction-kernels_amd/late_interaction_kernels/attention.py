@@ -14,6 +14,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._core import _i32, _mask_i8, assert_max_seqlens_cover, seqlen_max
@@ -68,6 +69,7 @@ class _AttentionFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         q, k, v, out, lse, low, qm, km, cu_q, cu_k = ctx.saved_tensors
         need_q, need_k, need_v = ctx.needs_input_grad[:3]

@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -52,6 +53,7 @@ class _GatedFfnFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         x2, w_in, w_out, h, gu = ctx.saved_tensors
         (rows, d), f = x2.shape, w_out.shape[1]

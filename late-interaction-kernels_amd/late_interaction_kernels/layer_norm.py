@@ -8,6 +8,7 @@ is normalised. The row's mean, variance and the gradients' sums are fp32.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -56,6 +57,7 @@ class _LayerNormFn(torch.autograd.Function):
         return y if total is None else (y, total)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, gy, gs=None):
         s, w, stats = ctx.saved_tensors
         need_x = ctx.needs_input_grad[0] or ctx.needs_input_grad[3]
