@@ -496,13 +496,14 @@ __global__ void __launch_bounds__(512) few_rows_kernel(const GemmP p) {
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n0 = (int)blockIdx.x * (EPI == EPI_GLU ? 16 : 32);
   const int n = EPI == EPI_GLU ? n0 + (l32 & 15) : n0 + l32;
-  const int row = EPI == EPI_GLU && l32 >= 16 ? p.hidden + n : n;
+  // rows from n0 on, whose address is 64 bits wide: all rows together can pass a lane's 32-bit offset
+  const int row = EPI == EPI_GLU && l32 >= 16 ? p.hidden + (l32 & 15) : l32;
   const uint32_t boff = n < (EPI == EPI_GLU ? p.hidden : p.n) ? (uint32_t)(row * p.b_ld) : kOob;
   uint32_t aoff[MB];
 #pragma unroll
   for (int j = 0; j < MB; ++j) aoff[j] = j * 32 + l32 < p.m ? (uint32_t)((j * 32 + l32) * p.a_ld) : kOob;
   const __amdgpu_buffer_rsrc_t rb =
-      __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p.b), (short)0, (int)0xffffff00u, 0x00020000);
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p.b + n0 * p.b_ld), (short)0, (int)0xffffff00u, 0x00020000);
   const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<char*>(p.a), (short)0, (int)0xffffff00u, 0x00020000);
   f32x16 acc[MB];
