@@ -512,7 +512,8 @@ int lik_gated_ffn_backward(const void* grad, int64_t grad_stride, const void* x,
  *   bound the longest sequence.
  * Query i keeps key j of its sequence where i - left <= j <= i + right (-1:
  * unbounded; positions count from the sequence's start) and the masks keep both. A
- * query that keeps no key gives zeros. scale > 0.
+ * query that keeps no key gives zeros. scale > 0. A call without queries or sequences (n, q_len or q_rows 0) succeeds: what
+ * it writes are zeros.
  */
 typedef struct {
   const void* q;

@@ -299,8 +299,11 @@ struct Window {
 inline bool att_rows_ok(const void* d, int64_t sn, int64_t sl, int64_t sh) {
   return (uintptr_t)d % 16 == 0 && sn % 8 == 0 && sl % 8 == 0 && sh % 8 == 0 && sl >= 0 && sl < (1 << 24);  // (64 rows of up to 2^25 bytes)
 }
-// Checks the arguments that both directions share and fills the parameters; false: nothing to do, or rc is an error.
+// Checks the arguments that both directions share and fills the parameters; false: there is no query (rc is LIK_OK: what
+// the call writes are zeros), or rc is an error.
 bool attention_shape(const lik_attention_t* a, AttP& p, int& rc);
+// Zeros in the rows of an output or gradient (null: not wanted).
+int clear_rows(void* data, int64_t rows, int heads, int dim, hipStream_t s);
 
 }  // namespace enc
 }  // namespace lik

@@ -435,10 +435,21 @@ int run_forward(const AttP& p, hipStream_t s) {
   return launch_forward<EK, 4>(p, s);
 }
 
+__global__ void __launch_bounds__(256) clear_kernel(u32x4* at, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+    at[i] = u32x4{0u, 0u, 0u, 0u};
+}
+
 }  // namespace
 
-// Checks the arguments that both directions share and fills the parameters;
-// false: nothing to do, or rc is an error.
+int clear_rows(void* data, int64_t rows, int heads, int dim, hipStream_t s) {
+  const int64_t n = rows * heads * dim / 8;
+  if (!data || n <= 0) return LIK_OK;
+  const int64_t wgs = (n + 255) / 256;
+  launch_kernel(clear_kernel, dim3((unsigned)(wgs < 4096 ? wgs : 4096)), dim3(256), 0u, s, (u32x4*)data, n);
+  return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;
+}
+
 bool attention_shape(const lik_attention_t* a, AttP& p, int& rc) {
   rc = LIK_ERR_INVALID;
   if (!a || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads || a->dim < 1 || a->n < 0 || a->q_len < 0 ||
@@ -452,7 +463,7 @@ bool attention_shape(const lik_attention_t* a, AttP& p, int& rc) {
   if ((a->k_mask && a->k_len > kMaskMost) || (a->q_mask && a->q_len > kMaskMost)) return false;
   p.q_total = a->cu_q ? a->q_rows : a->n * a->q_len;
   rc = LIK_OK;
-  if (a->n == 0 || p.q_total == 0) return false;
+  if (a->n == 0 || p.q_total == 0 || a->q_len == 0) return false;
   const bool keys = (a->cu_k ? a->k_rows : a->n * a->k_len) > 0;
   if (!a->q || (keys && (!a->k || !a->v))) {
     rc = LIK_ERR_INVALID;
@@ -510,9 +521,11 @@ int lik_attention(const lik_attention_t* a, void* out, float* lse, int8_t* out_l
                   lik_stream_t stream) {
   AttP p{};
   int rc;
-  if (!attention_shape(a, p, rc)) return rc;
-  if (!out) return LIK_ERR_INVALID;
+  const bool queries = attention_shape(a, p, rc);
+  if (rc != LIK_OK) return rc;
+  if (!out && p.q_total > 0) return LIK_ERR_INVALID;
   if ((uintptr_t)out % 16 || (uintptr_t)out_low % 16) return LIK_ERR_UNSUPPORTED;
+  if (!queries) return clear_rows(out, p.q_total, a->heads, a->dim, (hipStream_t)stream);
   forward_shape(p);
   if (p.splits > 1) {
     if (!workspace || workspace_bytes < forward_ws(p)) return LIK_ERR_WORKSPACE;

@@ -592,7 +592,7 @@ int launch_backward(AttP p, hipStream_t s) {
   if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
   p.tiles = (int)((p.k_len + 127) / 128);
   const int64_t wgs = (int64_t)p.n * (p.heads / p.group) * p.tiles;
-  if (!p.gk || !wgs) return LIK_OK;
+  if (!p.gk) return LIK_OK;
   grid = work_grid(p, wgs, p.tiles);
   if (!grid) return LIK_ERR_UNSUPPORTED;
   launch_kernel(attention_dkv_kernel<EK, DC>, dim3(grid), dim3(256), p.qm ? mask_words(p.q_len) * 4 : 0u, s, p);
@@ -633,10 +633,20 @@ int lik_attention_backward(const lik_attention_t* a, const void* out, const floa
                            void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes, lik_stream_t stream) {
   AttP p{};
   int rc;
-  if (!attention_shape(a, p, rc)) return rc != LIK_OK ? rc : LIK_ERR_INVALID;  // no query: nothing writes grad_k
-  if (!out || !lse || !out_low || !grad || !grad_k != !grad_v) return LIK_ERR_INVALID;
-  if (!att_rows_ok(grad, grad_stride_n, grad_stride_l, grad_stride_h) || (uintptr_t)out % 16 || (uintptr_t)out_low % 16 ||
-      (uintptr_t)grad_q % 16 || (uintptr_t)grad_k % 16 || (uintptr_t)grad_v % 16)
+  const bool queries = attention_shape(a, p, rc);
+  if (rc != LIK_OK) return rc;
+  const hipStream_t s = (hipStream_t)stream;
+  if (!grad_k != !grad_v) return LIK_ERR_INVALID;
+  if ((uintptr_t)grad_q % 16 || (uintptr_t)grad_k % 16 || (uintptr_t)grad_v % 16) return LIK_ERR_UNSUPPORTED;
+  if (!queries || a->k_len == 0) {  // no kernel comes by the keys
+    const int64_t keys = a->cu_k ? a->k_rows : a->n * a->k_len;
+    rc = clear_rows(grad_k, keys, a->kv_heads, a->dim, s);
+    if (rc == LIK_OK) rc = clear_rows(grad_v, keys, a->kv_heads, a->dim, s);
+    if (rc == LIK_OK) rc = clear_rows(grad_q, p.q_total, a->heads, a->dim, s);
+    return rc;
+  }
+  if (!out || !lse || !out_low || !grad) return LIK_ERR_INVALID;
+  if (!att_rows_ok(grad, grad_stride_n, grad_stride_l, grad_stride_h) || (uintptr_t)out % 16 || (uintptr_t)out_low % 16)
     return LIK_ERR_UNSUPPORTED;
   if (!workspace || workspace_bytes < backward_ws(p)) return LIK_ERR_WORKSPACE;
   char* ws = align256(workspace);
@@ -650,8 +660,7 @@ int lik_attention_backward(const lik_attention_t* a, const void* out, const floa
   p.gq = (char*)grad_q;
   p.gk = (char*)grad_k;
   p.gv = (char*)grad_v;
-  return a->dtype == LIK_BF16 ? run_backward<EK_BF16>(p, (hipStream_t)stream)
-                              : run_backward<EK_F16>(p, (hipStream_t)stream);
+  return a->dtype == LIK_BF16 ? run_backward<EK_BF16>(p, s) : run_backward<EK_F16>(p, s);
 }
 
 }  // extern "C"
