@@ -556,7 +556,7 @@ typedef struct {
  * rows' softmax statistics for the backward pass (log2 of the sum of 2^(scale
  * log2(e) q k); +inf for a query that keeps no key). out_low (optional, out's shape):
  * what the rounding took off out, for the backward pass. Packed rows that belong
- * to no sequence are left as they are.
+ * to no sequence come out as zeros (the gradients' too).
  */
 size_t lik_attention_workspace_size(const lik_attention_t* a);
 int lik_attention(const lik_attention_t* a, void* out, float* lse, int8_t* out_low, void* workspace,

@@ -83,6 +83,20 @@ __device__ __forceinline__ Span span_of(const int32_t* cu, int64_t rows, int64_t
   return {a, (int)l};
 }
 
+// Zeros in the packed rows of `out` ([rows][16-byte chunks of a row]) that belong to no sequence, a share by each work item's
+// workgroup. (Called beside span_of: the offsets arrive together.)
+__device__ __forceinline__ void clear_uncovered(const AttP& p, int item, const int32_t* cu, int64_t rows, int row_chunks,
+                                                char* out) {
+  if (!cu) return;
+  int64_t first = cu[0], end = cu[p.n];
+  first = first < 0 ? 0 : first > rows ? rows : first;
+  end = end < first ? first : end > rows ? rows : end;
+  const int64_t front = first * row_chunks, chunks = front + (rows - end) * row_chunks;
+  if (chunks == 0) return;
+  for (int64_t i = (int64_t)item * blockDim.x + threadIdx.x; i < chunks; i += (int64_t)p.wgs * blockDim.x)
+    *(u32x4*)(out + (i < front ? i : end * row_chunks + i - front) * 16) = u32x4{0u, 0u, 0u, 0u};
+}
+
 // Keep bits of a mask row (len tokens) into LDS, 32 tokens a word, by all 256 threads; returns the
 // last kept token + 1 and whether a token before it is dropped.
 struct Kept {

@@ -136,6 +136,7 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 4 : 2) attention_kernel(const A
   const int kvh = head / p.group;
   const Span qs = span_of(p.cu_q, p.q_rows, p.q_len, seq), ks = span_of(p.cu_k, p.k_rows, p.k_len, seq);
   const int q0 = tile * 128;
+  if (p.splits == 1) clear_uncovered(p, item, p.cu_q, p.q_rows, p.heads * p.dim / 8, p.out);
   if (q0 >= qs.len) return;  // (all threads)
 
   const char* kbase = p.k.data + (p.cu_k ? ks.row * p.k.sl : seq * p.k.sn) + kvh * p.k.sh;
@@ -333,9 +334,11 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttP p) {
   const int64_t rh = (int64_t)blockIdx.x * 4 + wv;
   const int64_t row = rh / p.heads;
   const int head = (int)(rh % p.heads);
-  bool on = row < p.q_total;
-  if (on && p.cu_q) on = row >= p.cu_q[0] && row < p.cu_q[p.n];  // else in no sequence
-  if (!on) return;
+  if (row >= p.q_total) return;
+  if (p.cu_q && (row < p.cu_q[0] || row >= p.cu_q[p.n])) {  // in no sequence
+    if (lane * 8 < p.dim) *(u32x4*)(p.out + (rh * p.dim + lane * 8) * 2) = u32x4{0u, 0u, 0u, 0u};
+    return;
+  }
   // (at most 64 splits)
   const float l = lane < p.splits ? p.part_lse[((int64_t)lane * p.heads + head) * p.q_total + row] : -INFINITY;
   float top = l;

@@ -73,6 +73,7 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p) {
   const int kvh = head / p.group;
   const Span qs = span_of(p.cu_q, p.q_rows, p.q_len, seq), ks = span_of(p.cu_k, p.k_rows, p.k_len, seq);
   const int q0 = tile * 128;
+  if (p.gq) clear_uncovered(p, item, p.cu_q, p.q_rows, p.heads * p.dim / 8, p.gq);
   float* gmax = EK == EK_F16 ? p.gmax + ((int64_t)seq * p.heads + head) * p.q_tiles + tile : nullptr;
   if (q0 >= qs.len) {
     if (EK == EK_F16 && tid == 0) *gmax = 0.f;
@@ -195,15 +196,17 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 3 : 2) attention_dkv_kernel(con
   extern __shared__ uint32_t s_bits[];
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kv_heads = p.heads / p.group;
   const int item = work_item(p);
   if (item < 0) return;
   uint32_t t = (uint32_t)item;
   const int tile = (int)(t % (uint32_t)p.tiles);
   t /= (uint32_t)p.tiles;
-  const int kv_heads = p.heads / p.group;
   const int kvh = (int)(t % (uint32_t)kv_heads), seq = (int)(t / (uint32_t)kv_heads);
   const Span qs = span_of(p.cu_q, p.q_rows, p.q_len, seq), ks = span_of(p.cu_k, p.k_rows, p.k_len, seq);
   const int k0 = tile * 128;
+  clear_uncovered(p, item, p.cu_k, p.k_rows, kv_heads * p.dim / 8, p.gk);
+  clear_uncovered(p, item, p.cu_k, p.k_rows, kv_heads * p.dim / 8, p.gv);
   if (k0 >= ks.len) return;
   float gs = 1.0f;
   if constexpr (EK == EK_F16) {
@@ -371,11 +374,14 @@ __global__ void __launch_bounds__((KW + DC) * 64, (KW + DC + 3) / 4) attention_g
   __shared__ int s_blocks, s_last;
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kv_heads = p.heads / p.group;
   const int item = work_item(p);
   if (item < 0) return;
-  const int kv_heads = p.heads / p.group;
   const int kvh = item % kv_heads, seq = item / kv_heads;
   const Span qs = span_of(p.cu_q, p.q_rows, p.q_len, seq), ks = span_of(p.cu_k, p.k_rows, p.k_len, seq);
+  if (p.gq) clear_uncovered(p, item, p.cu_q, p.q_rows, p.heads * p.dim / 8, p.gq);
+  clear_uncovered(p, item, p.cu_k, p.k_rows, kv_heads * p.dim / 8, p.gk);
+  clear_uncovered(p, item, p.cu_k, p.k_rows, kv_heads * p.dim / 8, p.gv);
   if (tid == 0) s_blocks = s_last = 0;
   __syncthreads();
 

@@ -197,7 +197,8 @@ def attention_varlen(
 
     Args:
         q: ``[sum(Lq_i), H, d]`` fp16 / bf16; k, v: ``[sum(Lk_i), Hk, d]``.
-        cu_seqlens_q, cu_seqlens_k: ``[n + 1]`` int32 cumulative offsets that cover every row.
+        cu_seqlens_q, cu_seqlens_k: ``[n + 1]`` int32 cumulative offsets. Rows outside
+            ``cu[0] .. cu[-1]`` are in no sequence: zeros, and no gradient.
         max_seqlen_q, max_seqlen_k: hard bounds on the lengths; inferred with one
             device->host sync each if omitted, otherwise checked by an on-device assert.
         causal, window, scale: as in :func:`attention`; positions count from each sequence's start.
