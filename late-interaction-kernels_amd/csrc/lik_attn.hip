@@ -102,14 +102,14 @@ __device__ __forceinline__ void store_rows(const AttP& p, int split, int64_t row
   const bool kept = q_on && total != 0.f;
   const float inv = kept ? 1.0f / total : 0.f;
   const float lse = kept ? fmaf(top, p.c, __builtin_amdgcn_logf(total)) : INFINITY;
+  if (!kept)  // a masked row's sums hold what the values hold: not zero times that
+#pragma unroll
+    for (int d = 0; d < DC; ++d) o[d] = f32x16{};
   if (p.splits > 1) {
     if (on) store_part<DC>(p, split, row, head, o, inv, kept ? lse : -INFINITY, lane);
     return;
   }
   if (p.lse && on && lane < 32) p.lse[(int64_t)head * p.q_total + row] = lse;
-  if (!kept)
-#pragma unroll
-    for (int d = 0; d < DC; ++d) o[d] = f32x16{};
   store_cols<EK, DC>(p.out + (row * p.heads + head) * p.dim * 2, o, inv, p.dim, lane, on);
   if (p.low) store_low<EK, DC>(p.low + (row * p.heads + head) * p.dim, o, inv, p.dim, lane, on);
 }
@@ -319,6 +319,9 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 2 : 1) attention_rows_kernel(co
   for (int b = 0; b < QB; ++b) {
     const float total = sum[b] + swap_half(sum[b]);
     const bool kept = row[b] >= 0 && total != 0.f;
+    if (!kept)  // (as in store_rows)
+#pragma unroll
+      for (int d = 0; d < DC; ++d) o[b][d] = f32x16{};
     if (on[b])
       store_part<DC>(p, split, qs.row + (row[b] < 0 ? -1 - row[b] : row[b]), head[b], o[b], kept ? 1.0f / total : 0.f,
                      kept ? fmaf(top[b], p.c, __builtin_amdgcn_logf(total)) : -INFINITY, lane);
