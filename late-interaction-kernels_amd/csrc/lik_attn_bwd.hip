@@ -52,6 +52,32 @@ __device__ __forceinline__ float row_delta(const AttP& p, const u32x4* gf, int64
   return d + swap_half(d);
 }
 
+// Whether the lane's key, whose sums dk and dv are, has a gradient: it is kept, and so is a query that sees it. Pairs that
+// are not kept add p = 0 times what the rows hold, which is no zero where a kept key or its value is not finite; then
+// (and only then) the queries' statistics are asked.
+template <int DC>
+__device__ __forceinline__ bool key_seen(const AttP& p, const f32x16* dk, const f32x16* dv, bool kon, int kpos,
+                                         const float* lse, int qlen) {
+  float zero[8] = {};  // NaN where an element is not finite
+#pragma unroll
+  for (int d = 0; d < DC; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      zero[i % 4] = fmaf(dk[d][i], 0.f, zero[i % 4]);
+      zero[4 + i % 4] = fmaf(dv[d][i], 0.f, zero[4 + i % 4]);
+    }
+  float sum = ((zero[0] + zero[1]) + (zero[2] + zero[3])) + ((zero[4] + zero[5]) + (zero[6] + zero[7]));
+  sum += swap_half(sum);
+  const bool odd = kon && !(sum == 0.f);
+  if (__ballot(odd) == 0) return kon;
+  bool seen = !odd;
+  for (int h = 0; h < p.group; ++h)
+    for (int q = 0; q < qlen && __ballot(!seen) != 0; ++q)
+      seen = seen || (lse[(int64_t)h * p.q_total + q] != INFINITY && (p.left == kNone || q <= kpos + p.left) &&
+                      (p.right == kNone || q >= kpos - p.right));
+  return kon && seen;
+}
+
 // Gradient of q: the forward's walk over the keys (K rows also by transposing
 // reads, V rows in LDS), dq^T[d][query] += K^T ds^T. Its queries' delta, which the other kernel reads, comes
 // from the same registers.
@@ -174,6 +200,9 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p) {
     }
   }
   if (!p.gq) return;
+  if (!on)  // no gradient, whatever the keys and values hold (their lanes ran on zero rows)
+#pragma unroll
+    for (int d = 0; d < DC; ++d) acc[d] = f32x16{};
   store_cols<EK, DC>(p.gq + ((qs.row + qpos) * p.heads + head) * p.dim * 2, acc, p.scale / gs, p.dim, lane,
                      qpos < qs.len);
 }
@@ -346,7 +375,7 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 3 : 2) attention_dkv_kernel(con
     if (it + 1 < total && tid < 2 * QT) s_stat[buf ^ 1][tid / QT][tid % QT] = next;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // V's loads where there was no step
-  if (!kon)  // masked keys have no gradient (their lanes ran on zero rows)
+  if (!key_seen<DC>(p, dk, dv, kon, kpos, p.lse + (int64_t)kvh * p.group * p.q_total + qs.row, qs.len))
 #pragma unroll
     for (int d = 0; d < DC; ++d) dk[d] = dv[d] = f32x16{};
   const int64_t at = ((ks.row + kpos) * kv_heads + kvh) * p.dim * 2;
@@ -525,7 +554,7 @@ __global__ void __launch_bounds__((KW + DC) * 64, (KW + DC + 3) / 4) attention_g
         *(u32x2*)(ds_row + ((q ^ ((l32 >> 2) & 3)) << 4)) = u32x2{df[q / 2][(q % 2) * 2], df[q / 2][(q % 2) * 2 + 1]};
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (!kon)  // as above
+    if (!key_seen<DC>(p, dk, dv, kon, kpos, p.lse + (int64_t)kvh * p.group * p.q_total + qs.row, qs.len))
 #pragma unroll
       for (int d = 0; d < DC; ++d) dk[d] = dv[d] = f32x16{};
     const int64_t at = ((ks.row + kpos) * kv_heads + kvh) * p.dim * 2;
@@ -551,6 +580,8 @@ __global__ void __launch_bounds__((KW + DC) * 64, (KW + DC + 3) / 4) attention_g
             acc = mfma16<EK>(acc, frags.col(kt + b * TILE, k * 16, block), u32x4{x[0], x[1], y[0], y[1]});
           }
         const int pos = before.qt + l32;
+        // queries without a statistic: no gradient, whatever the keys hold
+        if (s_lse[(before.head - head0) * most * 32 + pos] == INFINITY) acc = f32x16{};
         store_cols<EK, 1>(p.gq + (((qs.row + pos) * p.heads + before.head) * p.dim + block * 32) * 2, &acc, p.scale / gs,
                           p.dim - block * 32, lane, pos < qs.len);
         before = after(before);
