@@ -97,20 +97,21 @@ __device__ __forceinline__ void clear_uncovered(const AttP& p, int item, const i
     *(u32x4*)(out + (i < front ? i : end * row_chunks + i - front) * 16) = u32x4{0u, 0u, 0u, 0u};
 }
 
-// Keep bits of a mask row (len tokens) into LDS, 32 tokens a word, by all 256 threads; returns the
+// Keep bits of len tokens (kept(t): whether token t is) into LDS, 32 tokens a word, by all 256 threads; returns the
 // last kept token + 1 and whether a token before it is dropped.
 struct Kept {
   int extent;
   bool holes;
 };
-__device__ __forceinline__ Kept scan_mask(uint32_t* bits, const int8_t* mask, int64_t stride, int len, int* s_kept) {
+template <typename F>
+__device__ __forceinline__ Kept scan_kept(uint32_t* bits, int len, int* s_kept, F kept) {
   const int tid = threadIdx.x;
   if (tid < 2) s_kept[tid] = 0;
   __syncthreads();
   int last = 0, count = 0;
   for (int t0 = 0; t0 < len; t0 += 256) {
     const int t = t0 + tid;
-    const bool on = t < len && mask[t * stride] != 0;
+    const bool on = t < len && kept(t);
     const uint64_t b = __ballot(on);
     if ((tid & 63) == 0) {
       bits[t >> 5] = (uint32_t)b;
@@ -126,7 +127,10 @@ __device__ __forceinline__ Kept scan_mask(uint32_t* bits, const int8_t* mask, in
   __syncthreads();
   return {s_kept[0], s_kept[1] != s_kept[0]};
 }
-// words of keep bits that scan_mask writes for len tokens
+__device__ __forceinline__ Kept scan_mask(uint32_t* bits, const int8_t* mask, int64_t stride, int len, int* s_kept) {
+  return scan_kept(bits, len, s_kept, [=](int t) { return mask[t * stride] != 0; });
+}
+// words of keep bits that are written for len tokens
 inline uint32_t mask_words(int64_t len) { return (uint32_t)((len + 255) / 256 * 8); }
 constexpr int64_t kMaskMost = 1 << 18;  // tokens whose keep bits fit LDS beside the tiles
 

@@ -207,6 +207,12 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p) {
                      qpos < qs.len);
 }
 
+// Masked keys under a causal order or a window leave single queries without a key: their statistics say which. (Without
+// either, a mask leaves all queries without one or none. Longer sequences' bits do not fit LDS: there the rows are read.)
+__host__ __device__ __forceinline__ bool by_statistic(const AttP& p) {
+  return p.km && (p.left != kNone || p.right != kNone) && p.q_len <= kMaskMost;
+}
+
 // Gradients of k and v: a wavefront owns 32 keys as MFMA columns and walks the queries of the group's
 // heads, QT at a time, K in registers. For head dims over 32 V's rows stay in LDS, which leaves room for three
 // wavefronts a SIMD up to 64 (262 -> 252 us for the training step on 128 passages) and for two above, where a
@@ -264,10 +270,21 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 3 : 2) attention_dkv_kernel(con
       vrows.issue(lds_addr(s_v) + i * D::TILE, vbase + (k0 + 64 * i) * p.v.sl, ks.len - k0 - 64 * i, nullptr, wv, lane);
   }
 
+  // Queries that keep no key are not read: what their rows of q and g hold would meet p = 0 in the products, which is no
+  // zero for infinities and NaN.
   int qlen = qs.len;
+  if (p.left != kNone && (int64_t)ks.len + p.left < qlen) qlen = ks.len + p.left;  // (the window ends before the last ones)
   bool holes = false;
-  if (p.qm) {
-    const Kept kept = scan_mask(s_bits, p.qm + seq * p.qm_sn, p.qm_sl, qlen, s_kept);
+  if (p.qm || by_statistic(p)) {
+    const float* lse = p.lse + (int64_t)kvh * p.group * p.q_total + qs.row;
+    const Kept kept = by_statistic(p) ? scan_kept(s_bits, qlen, s_kept,
+                                                  [&](int t) {
+                                                    bool on = false;
+                                                    for (int h = 0; h < p.group; ++h)
+                                                      on = on || lse[h * p.q_total + t] != INFINITY;
+                                                    return on;
+                                                  })
+                                      : scan_mask(s_bits, p.qm + seq * p.qm_sn, p.qm_sl, qlen, s_kept);
     qlen = kept.extent;
     holes = kept.holes;
   }
@@ -632,7 +649,8 @@ int launch_backward(AttP p, hipStream_t s) {
   if (!p.gk) return LIK_OK;
   grid = work_grid(p, wgs, p.tiles);
   if (!grid) return LIK_ERR_UNSUPPORTED;
-  launch_kernel(attention_dkv_kernel<EK, DC>, dim3(grid), dim3(256), p.qm ? mask_words(p.q_len) * 4 : 0u, s, p);
+  launch_kernel(attention_dkv_kernel<EK, DC>, dim3(grid), dim3(256),
+                p.qm || by_statistic(p) ? mask_words(p.q_len) * 4 : 0u, s, p);
   return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;
 }
 
