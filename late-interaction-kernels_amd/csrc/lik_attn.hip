@@ -12,7 +12,10 @@ namespace enc {
 namespace {
 
 // One step of the softmax on 32 NU scores of a lane's column: s to probabilities, packed as MFMA operands in pf;
-// top, sum and the output so far follow the running maximum.
+// top, sum and the output so far follow the running maximum. The sum is that of the rounded probabilities, which are the
+// output's weights: whatever the values have in common comes out exact. (With the sum before the rounding the output was off
+// by the weights' missing share of it, and delta = g o against g v with it: gradients of q and k over values of 16 +- 1 were
+// 2 roundoffs off.)
 template <int EK, int DC, int NU>
 __device__ __forceinline__ void softmax_step(f32x16 (&s)[NU], f32x16 (&o)[DC], float& top, float& sum, float c,
                                              u32x4 (&pf)[2 * NU]) {
@@ -33,20 +36,19 @@ __device__ __forceinline__ void softmax_step(f32x16 (&s)[NU], f32x16 (&o)[DC], f
     for (int d = 0; d < DC; ++d) o[d] *= alpha;
   }
   const float mc = top == -INFINITY ? 0.f : top * c;
-  float add = 0.f;
 #pragma unroll
   for (int u = 0; u < NU; ++u)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float e = __builtin_amdgcn_exp2f(fmaf(s[u][i], c, -mc));
-      s[u][i] = e;
-      add += e;
-    }
-  sum += add;
+    for (int i = 0; i < 16; ++i) s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], c, -mc));
+  float add[2] = {};
 #pragma unroll
   for (int k = 0; k < 2 * NU; ++k)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) pf[k][e] = pack2<EK>(s[k / 2][(k % 2) * 8 + 2 * e], s[k / 2][(k % 2) * 8 + 2 * e + 1]);
+    for (int e = 0; e < 4; ++e) {
+      pf[k][e] = pack2<EK>(s[k / 2][(k % 2) * 8 + 2 * e], s[k / 2][(k % 2) * 8 + 2 * e + 1]);
+      add[e % 2] = add2<EK>(pf[k][e], add[e % 2]);
+    }
+  sum += add[0] + add[1];
 }
 
 // One split's share of a row's output: its mean of the values in fp32, and its statistic.
