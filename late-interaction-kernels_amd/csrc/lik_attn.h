@@ -40,7 +40,8 @@ struct AttP {
   float* delta;                   // [heads][q_total]: sum_d g o
   char *gq, *gk, *gv;             // contiguous gradients
   float* gmax;                    // fp16: [sequence][head][q tile]: largest |g|
-  int q_tiles;                    // backward: q tiles of a sequence
+  float* vmax;                    // fp16: [sequence][key head][k tile]: largest |v|
+  int q_tiles, k_tiles;           // backward: tiles of 128 rows of a sequence
   float* part_o;                  // forward split over keys: [split][q_total][heads][dim] fp32
   float* part_lse;                // [split][heads][q_total]
   int splits, tiles;              // q tiles (k tiles) of a sequence

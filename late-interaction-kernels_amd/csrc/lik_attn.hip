@@ -11,6 +11,15 @@ namespace lik {
 namespace enc {
 namespace {
 
+// The reference maximum only moves when a score passes it by more than 2^kRise, and probabilities are 2^kLift
+// times those to that reference. bf16: up to 256 instead of 1, which no rounding sees, and the output is rescaled less often. fp16: up
+// to 2^15; what is 2^-26 of a row's largest is still a normal number (2^-14) and what is 2^-36 is not dropped, so the
+// weights of many such keys are not lost (a lift of 0 dropped them under 2^-25).
+template <int EK>
+constexpr float kRise = EK == EK_F16 ? 3.0f : 8.0f;
+template <int EK>
+constexpr float kLift = EK == EK_F16 ? 12.0f : 0.0f;
+
 // One step of the softmax on 32 NU scores of a lane's column: s to probabilities, packed as MFMA operands in pf;
 // top, sum and the output so far follow the running maximum. The sum is that of the rounded probabilities, which are the
 // output's weights: whatever the values have in common comes out exact. (With the sum before the rounding the output was off
@@ -25,9 +34,7 @@ __device__ __forceinline__ void softmax_step(f32x16 (&s)[NU], f32x16 (&o)[DC], f
 #pragma unroll
     for (int i = 0; i < 16; ++i) m = fmaxf(m, s[u][i]);
   m = fmaxf(m, swap_half(m));
-  // The reference maximum only moves when a score passes it by more than 2^8: until then the probabilities
-  // are up to 256 instead of 1, which no type's relative rounding sees, and the output needs no rescaling.
-  if (__ballot(fmaf(m, c, -8.0f) > top * c) != 0) {
+  if (__ballot(fmaf(m, c, -kRise<EK>) > top * c) != 0) {
     const float up = fmaxf(m, top);
     const float alpha = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((top - up) * c);
     top = up;
@@ -35,7 +42,7 @@ __device__ __forceinline__ void softmax_step(f32x16 (&s)[NU], f32x16 (&o)[DC], f
 #pragma unroll
     for (int d = 0; d < DC; ++d) o[d] *= alpha;
   }
-  const float mc = top == -INFINITY ? 0.f : top * c;
+  const float mc = top == -INFINITY ? 0.f : fmaf(top, c, -kLift<EK>);
 #pragma unroll
   for (int u = 0; u < NU; ++u)
 #pragma unroll
@@ -103,7 +110,7 @@ __device__ __forceinline__ void store_rows(const AttP& p, int split, int64_t row
   const float total = sum + swap_half(sum);
   const bool kept = q_on && total != 0.f;
   const float inv = kept ? 1.0f / total : 0.f;
-  const float lse = kept ? fmaf(top, p.c, __builtin_amdgcn_logf(total)) : INFINITY;
+  const float lse = kept ? fmaf(top, p.c, __builtin_amdgcn_logf(total) - kLift<EK>) : INFINITY;
   if (!kept)  // a masked row's sums hold what the values hold: not zero times that
 #pragma unroll
     for (int d = 0; d < DC; ++d) o[d] = f32x16{};
@@ -326,7 +333,7 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 2 : 1) attention_rows_kernel(co
       for (int d = 0; d < DC; ++d) o[b][d] = f32x16{};
     if (on[b])
       store_part<DC>(p, split, qs.row + (row[b] < 0 ? -1 - row[b] : row[b]), head[b], o[b], kept ? 1.0f / total : 0.f,
-                     kept ? fmaf(top[b], p.c, __builtin_amdgcn_logf(total)) : -INFINITY, lane);
+                     kept ? fmaf(top[b], p.c, __builtin_amdgcn_logf(total) - kLift<EK>) : -INFINITY, lane);
   }
 }
 

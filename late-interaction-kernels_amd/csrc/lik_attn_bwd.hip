@@ -10,22 +10,84 @@
 // 255 us (545, four), two wavefronts a SIMD at 238 and 256 registers, bound by the chain from scores to
 // probabilities to products inside a wavefront. Sequences of 129 to 320 keys have one kernel for all three: 128 passages of 50 to 300
 // rows, 12 heads of 64: 160 us, the two 88 and 93.
-// p and ds are rounded once to the 16-bit type, as the products' operands have to be.
-// fp16 would lose small gradients there: g is scaled by the power of two that
-// brings its largest element to 1/2 .. 1 (of a wavefront's queries; of a key head's), and the sums are scaled
-// back.
+// p and ds are rounded once to the 16-bit type, as the products' operands have to be. fp16 has no range for either: p is
+// held 2^14 times (2^-28 is still a normal number), and ds 2^14 gs times, gs the power of two that brings the bound
+// |g v - delta| <= 2 dim max|g| max|v| to 1 .. 2 (of a wavefront's queries; of a key head's): nothing passes 2^15, and the
+// largest elements, some 2^6 under the bound, keep 20 powers of two below them. The sums are scaled back.
 #include "lik_attn.h"
 
 namespace lik {
 namespace enc {
 namespace {
 
-// The power of two that brings a largest |g| of `big` to 1/2 .. 1 (1 for zeros, infinities and NaN).
-__device__ __forceinline__ float scale_for(float big) {
-  if (!(big > 0.f) || !(big < INFINITY)) return 1.0f;
+// log2 of what p is held times
+template <int EK>
+constexpr float kLiftP = EK == EK_F16 ? 14.0f : 0.0f;
+template <int EK>
+constexpr float kUnliftP = EK == EK_F16 ? 1.0f / 16384 : 1.0f;
+// gs from the largest |g| and |v| (1 where one is zero)
+__device__ __forceinline__ float scale_for(float g, float v, int dim) {
+  const float bound = 2.0f * (float)dim * g * v;
+  if (!(bound > 0.f)) return 1.0f;
   int e;
-  frexpf(big, &e);  // big = m 2^e, m in 1/2 .. 1
-  return ldexpf(1.0f, -e);
+  frexpf(bound, &e);  // bound = m 2^e, m in 1/2 .. 1
+  return ldexpf(2.0f, -e);
+}
+// The largest finite |x| of N chunks of fp16 elements: rows that are not finite are NaN in the end, at any scale.
+template <int N>
+__device__ __forceinline__ float max_finite(const u32x4* x) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 m = {0, 0};
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x[k][i] & 0x7fff7fffu));
+  uint32_t top = m[0] > m[1] ? m[0] : m[1];
+  if (__ballot(top >= 0x7c00u) != 0) {  // infinities or NaN: one by one
+    top = 0;
+    for (int k = 0; k < N; ++k)
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t a = (x[k][i / 2] >> (16 * (i % 2))) & 0x7fffu;
+        if (a < 0x7c00u && a > top) top = a;
+      }
+  }
+  return f16_to_f32((uint16_t)top);
+}
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) x = fmaxf(x, __shfl_xor(x, s));
+  return x;
+}
+
+// fp16: the largest |v| of 128 keys of a key head.
+__global__ void __launch_bounds__(256) attention_vmax_kernel(const AttP p) {
+  __shared__ float s_big[4];
+  const int tid = threadIdx.x, kv_heads = p.heads / p.group;
+  const int tile = (int)(blockIdx.x % (unsigned)p.k_tiles);
+  const unsigned t = blockIdx.x / (unsigned)p.k_tiles;
+  const int kvh = (int)(t % (unsigned)kv_heads), seq = (int)(t / (unsigned)kv_heads);
+  const Span ks = span_of(p.cu_k, p.k_rows, p.k_len, seq);
+  const char* base = p.v.data + (p.cu_k ? ks.row * p.v.sl : seq * p.v.sn) + kvh * p.v.sh;
+  const int chunks = p.dim / 8;
+  u32x4 x[8];  // (at most 16 chunks a row)
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int i = j * 256 + tid, pos = tile * 128 + i / chunks;
+    x[j] = u32x4{0u, 0u, 0u, 0u};
+    if (i < 128 * chunks && pos < ks.len && (!p.km || p.km[seq * p.km_sn + pos * p.km_sl] != 0))
+      x[j] = *(const u32x4*)(base + pos * p.v.sl + i % chunks * 16);
+  }
+  const float big = wave_max(max_finite<8>(x));
+  if ((tid & 63) == 0) s_big[tid >> 6] = big;
+  __syncthreads();
+  if (tid == 0) p.vmax[blockIdx.x] = fmaxf(fmaxf(s_big[0], s_big[1]), fmaxf(s_big[2], s_big[3]));
+}
+// A key head's largest |v| (all lanes of a wavefront).
+__device__ __forceinline__ float head_vmax(const AttP& p, int seq, int kvh, int lane) {
+  const float* at = p.vmax + ((int64_t)seq * (p.heads / p.group) + kvh) * p.k_tiles;
+  float big = 0.f;
+  for (int i = lane; i < p.k_tiles; i += 64) big = fmaxf(big, at[i]);
+  return wave_max(big);
 }
 
 // delta of the lane's query, whose g is in columns (on: it has one; else 0), and the largest |g| for fp16. row: its first
@@ -46,9 +108,9 @@ __device__ __forceinline__ float row_delta(const AttP& p, const u32x4* gf, int64
       unpack2<EK>(gf[k][i / 2], g[0], g[1]);
       unpack2<EK>(of[k][i / 2], o[0], o[1]);
       d = fmaf(g[i % 2], with_low<EK>(o[i % 2], low[i / 4], i % 4), d);
-      if constexpr (EK == EK_F16) big = fmaxf(big, fabsf(g[i % 2]));
     }
   }
+  if constexpr (EK == EK_F16) big = fmaxf(big, max_finite<Dim<DC>::KS>(gf));
   return d + swap_half(d);
 }
 
@@ -122,10 +184,9 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p) {
   const bool any = __ballot(on) != 0;  // this wavefront has a query
   float gs = 1.0f;  // of this wavefront's queries
   if constexpr (EK == EK_F16) {
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) big = fmaxf(big, __shfl_xor(big, s));
+    big = wave_max(big);
     if (lane == 0) s_big[wv] = big;
-    gs = scale_for(big);
+    gs = scale_for(big, head_vmax(p, seq, kvh, lane), p.dim);
     __syncthreads();
     if (tid == 0) *gmax = fmaxf(fmaxf(s_big[0], s_big[1]), fmaxf(s_big[2], s_big[3]));
   }
@@ -154,6 +215,7 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p) {
   };
 
   const Window win(p);
+  const float lift = kLiftP<EK> - lse;
   f32x16 acc[DC];
 #pragma unroll
   for (int d = 0; d < DC; ++d) acc[d] = f32x16{};
@@ -183,7 +245,7 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p) {
       u32x4 df[2];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(s[i], p.c, -lse));
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[i], p.c, lift));
         s[i] = e * (EK == EK_F16 ? (dp[i] - delta) * gs : dp[i] - delta);
       }
 #pragma unroll
@@ -203,7 +265,7 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p) {
   if (!on)  // no gradient, whatever the keys and values hold (their lanes ran on zero rows)
 #pragma unroll
     for (int d = 0; d < DC; ++d) acc[d] = f32x16{};
-  store_cols<EK, DC>(p.gq + ((qs.row + qpos) * p.heads + head) * p.dim * 2, acc, p.scale / gs, p.dim, lane,
+  store_cols<EK, DC>(p.gq + ((qs.row + qpos) * p.heads + head) * p.dim * 2, acc, p.scale * kUnliftP<EK> / gs, p.dim, lane,
                      qpos < qs.len);
 }
 
@@ -248,11 +310,10 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 3 : 2) attention_dkv_kernel(con
     const float* gm = p.gmax + ((int64_t)seq * p.heads + kvh * p.group) * p.q_tiles;
     float big = 0.f;
     for (int i = tid; i < p.group * p.q_tiles; i += 256) big = fmaxf(big, gm[i]);
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) big = fmaxf(big, __shfl_xor(big, s));
+    big = wave_max(big);
     if (lane == 0) s_big[wv] = big;
     __syncthreads();
-    gs = scale_for(fmaxf(fmaxf(s_big[0], s_big[1]), fmaxf(s_big[2], s_big[3])));
+    gs = scale_for(fmaxf(fmaxf(s_big[0], s_big[1]), fmaxf(s_big[2], s_big[3])), head_vmax(p, seq, kvh, lane), p.dim);
   }
 
   u32x4 kf[D::KS], vf[VL ? 1 : D::KS];
@@ -305,7 +366,7 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 3 : 2) attention_dkv_kernel(con
     qrows.issue(at, q0 + head * p.q.sh + qt * p.q.sl, qlen - qt, bits, wv, lane);
     grows.issue(at + TILE, g0 + head * p.g.sh + qt * p.g.sl, qlen - qt, bits, wv, lane);
   };
-  // threads 0..QT - 1: a query's statistic (+inf past the end: p = 0), QT..2 QT - 1: its delta
+  // threads 0..QT - 1: a query's statistic (+inf past the end: p = 0), QT..2 QT - 1: its delta; in LDS less p's lift
   auto stat = [&](int head, int qt) {
     float x = 0.f;
     if (tid < 2 * QT) {
@@ -314,6 +375,9 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 3 : 2) attention_dkv_kernel(con
       x = pos < qlen ? (tid < QT ? p.lse[at] : p.delta[at]) : tid < QT ? INFINITY : 0.f;
     }
     return x;
+  };
+  auto put_stat = [&](int buf, float x) {
+    if (tid < 2 * QT) s_stat[buf][tid / QT][tid % QT] = EK == EK_F16 && tid < QT ? x - kLiftP<EK> : x;
   };
 
   // a query keeps a key where 0 <= query - key + ahead <= reach
@@ -328,7 +392,7 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 3 : 2) attention_dkv_kernel(con
   if (total) {
     const float x = stat(head, qt);
     issue(lds[0], head, qt);
-    if (tid < 2 * QT) s_stat[0][tid / QT][tid % QT] = x;
+    put_stat(0, x);
   }
   int buf = 0;
   for (int it = 0; it < total; ++it, buf ^= 1) {
@@ -389,15 +453,15 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 3 : 2) attention_dkv_kernel(con
           }
       }
     }
-    if (it + 1 < total && tid < 2 * QT) s_stat[buf ^ 1][tid / QT][tid % QT] = next;
+    if (it + 1 < total) put_stat(buf ^ 1, next);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // V's loads where there was no step
   if (!key_seen<DC>(p, dk, dv, kon, kpos, p.lse + (int64_t)kvh * p.group * p.q_total + qs.row, qs.len))
 #pragma unroll
     for (int d = 0; d < DC; ++d) dk[d] = dv[d] = f32x16{};
   const int64_t at = ((ks.row + kpos) * kv_heads + kvh) * p.dim * 2;
-  store_cols<EK, DC>(p.gk + at, dk, p.scale / gs, p.dim, lane, kpos < ks.len);
-  store_cols<EK, DC>(p.gv + at, dv, 1.0f, p.dim, lane, kpos < ks.len);
+  store_cols<EK, DC>(p.gk + at, dk, p.scale * kUnliftP<EK> / gs, p.dim, lane, kpos < ks.len);
+  store_cols<EK, DC>(p.gv + at, dv, kUnliftP<EK>, p.dim, lane, kpos < ks.len);
 }
 
 // All gradients of sequences of up to 32 KW keys in one pass: five products and one read of the rows, no sum in memory. A
@@ -416,7 +480,7 @@ __global__ void __launch_bounds__((KW + DC) * 64, (KW + DC + 3) / 4) attention_g
   __shared__ __attribute__((aligned(1024))) char s_tile[3][2 * TILE];
   __shared__ __attribute__((aligned(1024))) char s_ds[2][KW * DS];  // [key][query], 16-byte chunks exchanged by (key / 4) % 4
   __shared__ __attribute__((aligned(16))) float s_lse[kShortRows], s_delta[kShortRows];  // 32 a step
-  __shared__ float s_big[KW + DC];
+  __shared__ float s_big[2][KW + DC];  // |g|, |v|
   __shared__ int s_blocks, s_last;
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -473,7 +537,7 @@ __global__ void __launch_bounds__((KW + DC) * 64, (KW + DC + 3) / 4) attention_g
     load_cols<DC>(gf, on ? g0 + head * p.g.sh + pos * p.g.sl : nullptr, p.dim, lane);
     const float d = row_delta<EK, DC>(p, gf, row, on, big, lane);
     if (lane < 32) {
-      s_lse[it * 32 + l32] = lse;
+      s_lse[it * 32 + l32] = lse - kLiftP<EK>;
       s_delta[it * 32 + l32] = d;
     }
     if (__ballot(on) && lane == 0) atomicMax(&s_last, qt + 32);
@@ -481,9 +545,12 @@ __global__ void __launch_bounds__((KW + DC) * 64, (KW + DC + 3) / 4) attention_g
     if (it < most * p.group) lse = lse_of(head0 + it / most, it % most * 32 + l32);
   }
   if constexpr (EK == EK_F16) {
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) big = fmaxf(big, __shfl_xor(big, s));
-    if (lane == 0) s_big[wv] = big;
+    const float vbig = wave_max(max_finite<D::KS>(vf));
+    big = wave_max(big);
+    if (lane == 0) {
+      s_big[0][wv] = big;
+      s_big[1][wv] = vbig;
+    }
   }
   if (keys)
 #pragma unroll
@@ -496,10 +563,13 @@ __global__ void __launch_bounds__((KW + DC) * 64, (KW + DC + 3) / 4) attention_g
   if (!blocks) qe = 0;
   const int steps = (qe + 31) / 32, total = steps * p.group;
   if constexpr (EK == EK_F16) {
-    big = 0.f;
+    float vbig = big = 0.f;
 #pragma unroll
-    for (int w = 0; w < KW + DC; ++w) big = fmaxf(big, s_big[w]);
-    gs = scale_for(big);
+    for (int w = 0; w < KW + DC; ++w) {
+      big = fmaxf(big, s_big[0][w]);
+      vbig = fmaxf(vbig, s_big[1][w]);
+    }
+    gs = scale_for(big, vbig, p.dim);
   }
 
   struct Pos {
@@ -575,8 +645,8 @@ __global__ void __launch_bounds__((KW + DC) * 64, (KW + DC + 3) / 4) attention_g
 #pragma unroll
       for (int d = 0; d < DC; ++d) dk[d] = dv[d] = f32x16{};
     const int64_t at = ((ks.row + kpos) * kv_heads + kvh) * p.dim * 2;
-    store_cols<EK, DC>(p.gk + at, dk, p.scale / gs, p.dim, lane, kpos < ks.len);
-    store_cols<EK, DC>(p.gv + at, dv, 1.0f, p.dim, lane, kpos < ks.len);
+    store_cols<EK, DC>(p.gk + at, dk, p.scale * kUnliftP<EK> / gs, p.dim, lane, kpos < ks.len);
+    store_cols<EK, DC>(p.gv + at, dv, kUnliftP<EK>, p.dim, lane, kpos < ks.len);
   } else {
     const int block = wv - KW;  // of 32 head dims
     // transposing reads of ds: lane l has query l % 32 of keys row0 + 4 (l / 32) + {0..3, 8..11}, as Frags::col
@@ -599,8 +669,8 @@ __global__ void __launch_bounds__((KW + DC) * 64, (KW + DC + 3) / 4) attention_g
         const int pos = before.qt + l32;
         // queries without a statistic: no gradient, whatever the keys hold
         if (s_lse[(before.head - head0) * most * 32 + pos] == INFINITY) acc = f32x16{};
-        store_cols<EK, 1>(p.gq + (((qs.row + pos) * p.heads + before.head) * p.dim + block * 32) * 2, &acc, p.scale / gs,
-                          p.dim - block * 32, lane, pos < qs.len);
+        store_cols<EK, 1>(p.gq + (((qs.row + pos) * p.heads + before.head) * p.dim + block * 32) * 2, &acc,
+                          p.scale * kUnliftP<EK> / gs, p.dim - block * 32, lane, pos < qs.len);
         before = after(before);
       }
     }
@@ -639,12 +709,18 @@ int launch_backward(AttP p, hipStream_t s) {
       return launch_grads<EK, DC, 10>(p, s);
     }
   }
+  if constexpr (EK == EK_F16) {
+    const int64_t tiles = (int64_t)p.n * (p.heads / p.group) * p.k_tiles;
+    if (tiles > 0x3fffffff) return LIK_ERR_UNSUPPORTED;
+    launch_kernel(attention_vmax_kernel, dim3((unsigned)tiles), dim3(256), 0u, s, p);
+    if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
+  }
   p.tiles = p.q_tiles;
   unsigned grid = work_grid(p, (int64_t)p.tiles * p.n * p.heads, (int64_t)p.tiles * p.group);
   if (!grid) return LIK_ERR_UNSUPPORTED;
   launch_kernel(attention_dq_kernel<EK, DC>, dim3(grid), dim3(256), p.km ? mask_words(p.k_len) * 4 : 0u, s, p);
   if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
-  p.tiles = (int)((p.k_len + 127) / 128);
+  p.tiles = p.k_tiles;
   const int64_t wgs = (int64_t)p.n * (p.heads / p.group) * p.tiles;
   if (!p.gk) return LIK_OK;
   grid = work_grid(p, wgs, p.tiles);
@@ -662,9 +738,11 @@ int run_backward(const AttP& p, hipStream_t s) {
   return launch_backward<EK, 4>(p, s);
 }
 
-int q_tiles(const AttP& p) { return (int)((p.q_len + 127) / 128); }
+int tiles128(int64_t len) { return (int)((len + 127) / 128); }
+size_t gmax_bytes(const AttP& p) { return align256((size_t)p.n * p.heads * tiles128(p.q_len) * 4); }
 size_t backward_ws(const AttP& p) {
-  return align256((size_t)p.q_total * p.heads * 4) + (size_t)p.n * p.heads * q_tiles(p) * 4 + 256;
+  return align256((size_t)p.q_total * p.heads * 4) + gmax_bytes(p) +
+         (size_t)p.n * (p.heads / p.group) * tiles128(p.k_len) * 4 + 256;
 }
 
 }  // namespace
@@ -710,7 +788,9 @@ int lik_attention_backward(const lik_attention_t* a, const void* out, const floa
   p.out = (char*)const_cast<void*>(out);
   p.lse = const_cast<float*>(lse);
   p.low = const_cast<int8_t*>(out_low);
-  p.q_tiles = q_tiles(p);
+  p.vmax = (float*)((char*)p.gmax + gmax_bytes(p));
+  p.q_tiles = tiles128(p.q_len);
+  p.k_tiles = tiles128(p.k_len);
   p.g = {(const char*)grad, grad_stride_n * 2, grad_stride_l * 2, grad_stride_h * 2};
   p.gq = (char*)grad_q;
   p.gk = (char*)grad_k;
