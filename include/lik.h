@@ -480,11 +480,11 @@ int lik_layer_norm_backward(const void* grad_y, int64_t grad_y_stride, const voi
  * w_in [2 hidden, dim]: Wg, then Wu; w_out [dim, hidden]; activation 0: gelu
  * (erf), 1: gelu by tanh, 2: silu; bf16 / fp16. dim and hidden are multiples of 8,
  * every row starts on 16 bytes. out [rows, dim] and hidden_act [rows, hidden]
- * (act * up, always written) are contiguous; gate_up (optional, [rows, 2 hidden]
- * values of 2 bytes for bf16 and 4 for fp16) keeps both projections for the backward
- * pass.
+ * (act * up, always written) are contiguous; gate_up (optional, 16-byte aligned, lik_gated_ffn_kept_size bytes) keeps
+ * both projections for the backward pass.
  */
 size_t lik_gated_ffn_workspace_size(int32_t dtype, int64_t rows, int32_t dim, int32_t hidden);
+size_t lik_gated_ffn_kept_size(int32_t dtype, int64_t rows, int32_t dim, int32_t hidden);
 int lik_gated_ffn(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int32_t dim, int32_t hidden,
                   const void* w_in, int64_t w_in_stride, const void* w_out, int64_t w_out_stride, const void* residual,
                   int64_t residual_stride, int32_t activation, void* out, void* hidden_act, void* gate_up,

@@ -11,8 +11,8 @@
 //             dw_in = [dg du]^T x, dw_out = gy^T h   A and B across k, k = rows
 // Sums over k are fp32 (MFMA accumulators, fp32 partial sums where k is split). h, dg and du are rounded
 // once to the 16-bit type, as the next product's operands have to be. g and u are kept for the backward so
-// that dg and du carry next to no other rounding: of bf16 calls in fp16 (11 bits against the 8 of dg and
-// du) divided by 16, which holds up to 1.0e6, of fp16 calls in fp32.
+// that dg and du carry next to no other rounding, at any size: of bf16 calls the upper 20 bits of the fp32 value
+// (12 significant bits against the 8 of dg and du), of fp16 calls fp32.
 #include "lik_enc.h"
 
 namespace lik {
@@ -35,7 +35,7 @@ struct GemmP {
   int64_t out_ld;
   const char* res;     // EPI_STORE: added before the rounding; null: none
   int64_t res_ld;
-  char* gu;            // EPI_GLU: [m][2 hidden] kept g and u (null: not kept); EPI_GLU_BWD: read
+  char* gu;            // EPI_GLU: kept g and u (null: not kept), KeptBlock; EPI_GLU_BWD: read
   int hidden;
   int act;
 };
@@ -48,10 +48,10 @@ __device__ __forceinline__ float act_of(float x, float& slope) {
     if (SLOPE) slope = s * (1.0f + x * (1.0f - s));
     return x * s;
   } else if constexpr (ACT == ACT_GELU_TANH) {
-    // (1 + tanh u) / 2 = sigmoid(2 u), u = sqrt(2 / pi) (x + 0.044715 x^3)
-    const float x2 = x * x;
-    const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-1.5957691216f * x * fmaf(0.044715f, x2, 1.0f)));
-    if (SLOPE) slope = s * (1.0f + x * (1.0f - s) * 1.5957691216f * fmaf(0.134145f, x2, 1.0f));
+    // (1 + tanh u) / 2 = sigmoid(2 u), u = sqrt(2 / pi) (x + 0.044715 x^3); 0 or 1 past |x| = 64, whose powers stay finite
+    const float z = __builtin_amdgcn_fmed3f(x, -64.0f, 64.0f), z2 = z * z;
+    const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-1.5957691216f * z * fmaf(0.044715f, z2, 1.0f)));
+    if (SLOPE) slope = s * (1.0f + z * (1.0f - s) * 1.5957691216f * fmaf(0.134145f, z2, 1.0f));
     return x * s;
   } else {
     // cdf(-|x|) = erfc(|x| / sqrt 2) / 2 = poly(s) exp(-x^2 / 2), s = 1 / (1 + p |x| / sqrt 2): Abramowitz and
@@ -174,17 +174,28 @@ __device__ __forceinline__ void unpack8(const u32x4& x, float* v) {
   for (int i = 0; i < 4; ++i) unpack2<EK>(x[i], v[2 * i], v[2 * i + 1]);
 }
 
-// The kept g and u: bytes of a value, and eight of them (n + 8 h + 0..7 of quads 2 j, 2 j + 1).
+// The kept g and u: blocks of 32 rows by 32 hidden columns [rows / 32][hidden / 32], each as the accumulators lie, so that a
+// wavefront writes and reads whole KB. bf16: of g, then of u, two KB of 16-bit pieces (quads 0 and 1, 2 and 3 of a lane), then one KB
+// with the last 4 bits of both in a byte. fp16: the four quads of g, then of u.
 template <int EK>
-struct Kept {
-  static constexpr int B = EK == EK_BF16 ? 2 : 4;
-  static constexpr float DOWN = 0.0625f, UP = 16.0f;
-};
+constexpr int kKeptBlock = EK == EK_BF16 ? 5120 : 8192;
+// A lane's 16 bytes in the first KB of the block of row m and column n (multiples of 32 but for the lane's part of m).
+template <int EK>
+__device__ __forceinline__ char* kept_at(const GemmP& p, int m, int n, int h) {
+  const int64_t block = (int64_t)(m >> 5) * ((p.hidden + 31) >> 5) + (n >> 5);
+  return p.gu + block * kKeptBlock<EK> + ((m & 31) + 32 * h) * 16;
+}
+// The upper 20 bits of an fp32 value (rounded to nearest): 16 of them, and 4 in a nibble of the byte that g and u share.
+__device__ __forceinline__ uint32_t round20(float x) { return __float_as_uint(x) + 0x800u; }
+__device__ __forceinline__ uint32_t pack_upper(uint32_t a, uint32_t b) {  // upper halves of a and b
+  return __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+__device__ __forceinline__ uint32_t low_byte(uint32_t g, uint32_t u) { return ((g >> 12) & 0xfu) | ((u >> 8) & 0xf0u); }
 
 // What the epilogue of a 32 x 32 block reads: the residual, or g and u.
 template <int EK, int EPI>
 struct Extra {
-  u32x4 x[EPI == EPI_GLU_BWD ? (EK == EK_BF16 ? 4 : 8) : 2];
+  u32x4 x[EPI == EPI_GLU_BWD ? (EK == EK_BF16 ? 5 : 8) : 2];
 };
 // Lane (l32, h) of a block's accumulators holds m = l32 and n = 8 q + 4 h + e of quad q, element e. The block
 // starts at column n (a hidden column for both GLU epilogues); columns come in groups of 8.
@@ -197,27 +208,15 @@ __device__ __forceinline__ void load_extra(const GemmP& p, Extra<EK, EPI>& ex, i
       const int c = n + 16 * j + 8 * h;
       if (p.res && m < p.m && c < p.n) ex.x[j] = *(const u32x4*)(p.res + m * p.res_ld + c * 2);
     }
-  } else if constexpr (EPI == EPI_GLU_BWD && EK == EK_BF16) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      ex.x[2 * j] = ex.x[2 * j + 1] = u32x4{0u, 0u, 0u, 0u};
-      const int c = n + 16 * j + 8 * h;
-      if (m < p.m && c < p.hidden) {
-        const char* at = p.gu + ((int64_t)m * 2 * p.hidden + c) * 2;
-        ex.x[2 * j] = *(const u32x4*)at;
-        ex.x[2 * j + 1] = *(const u32x4*)(at + (int64_t)p.hidden * 2);
-      }
-    }
   } else if constexpr (EPI == EPI_GLU_BWD) {
+    constexpr int N = EK == EK_BF16 ? 5 : 8;
+    if (m - (m & 31) < p.m && n < p.hidden) {
+      const char* at = kept_at<EK>(p, m, n, h);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      ex.x[2 * q] = ex.x[2 * q + 1] = u32x4{0u, 0u, 0u, 0u};
-      const int c = n + 8 * q + 4 * h;
-      if (m < p.m && n + 8 * q < p.hidden) {
-        const char* at = p.gu + ((int64_t)m * 2 * p.hidden + c) * 4;
-        ex.x[2 * q] = *(const u32x4*)at;
-        ex.x[2 * q + 1] = *(const u32x4*)(at + (int64_t)p.hidden * 4);
-      }
+      for (int i = 0; i < N; ++i) ex.x[i] = *(const u32x4*)(at + i * 1024);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) ex.x[i] = u32x4{0u, 0u, 0u, 0u};
     }
   }
 }
@@ -248,47 +247,46 @@ __device__ __forceinline__ void finish_block(const GemmP& p, const f32x16& c0, c
       const u32x4 o =
           join_halves(pack2<EK>(v[0], v[1]), pack2<EK>(v[2], v[3]), pack2<EK>(v[4], v[5]), pack2<EK>(v[6], v[7]));
       if (on) *(u32x4*)(p.out + m * p.out_ld + c * 2) = o;
-      if (p.gu) {
+      if (p.gu && m - (m & 31) < p.m && n < p.hidden) {
+        const int part = NJ == 1 ? (n >> 4) & 1 : j;  // (blocks of 16 columns are halves)
+        char* at = kept_at<EK>(p, m, n, h);
         if constexpr (EK == EK_BF16) {
-          constexpr float d = Kept<EK>::DOWN;
-          u32x4 g, u;
+          u32x4 kg, ku;
+          u32x2 low = {0u, 0u};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            g[e] = pack2<EK_F16>(c0[8 * j + 2 * e] * d, c0[8 * j + 2 * e + 1] * d);
-            u[e] = pack2<EK_F16>(c1[8 * j + 2 * e] * d, c1[8 * j + 2 * e + 1] * d);
+          for (int e = 0; e < 8; e += 2) {
+            const uint32_t g0 = round20(c0[8 * j + e]), g1 = round20(c0[8 * j + e + 1]);
+            const uint32_t u0 = round20(c1[8 * j + e]), u1 = round20(c1[8 * j + e + 1]);
+            kg[e / 2] = pack_upper(g0, g1);
+            ku[e / 2] = pack_upper(u0, u1);
+            low[e / 4] |= (low_byte(g0, u0) | low_byte(g1, u1) << 8) << (e % 4 * 8);
           }
-          g = join_halves(g[0], g[1], g[2], g[3]);
-          u = join_halves(u[0], u[1], u[2], u[3]);
-          char* at = p.gu + ((int64_t)m * 2 * p.hidden + c) * 2;
-          if (on) {
-            *(u32x4*)at = g;
-            *(u32x4*)(at + (int64_t)p.hidden * 2) = u;
-          }
+          *(u32x4*)(at + part * 1024) = kg;
+          *(u32x4*)(at + 2048 + part * 1024) = ku;
+          *(u32x2*)(at + 4096 + part * 8) = low;
         } else {
 #pragma unroll
-          for (int q = 2 * j; q < 2 * j + 2; ++q)
-            if (m < p.m && n + 8 * q < p.hidden) {
-              char* at = p.gu + ((int64_t)m * 2 * p.hidden + n + 8 * q + 4 * h) * 4;
-              *(f32x4*)at = f32x4{c0[4 * q], c0[4 * q + 1], c0[4 * q + 2], c0[4 * q + 3]};
-              *(f32x4*)(at + (int64_t)p.hidden * 4) = f32x4{c1[4 * q], c1[4 * q + 1], c1[4 * q + 2], c1[4 * q + 3]};
-            }
+          for (int q = 0; q < 2; ++q) {
+            const int e = 8 * j + 4 * q;
+            *(f32x4*)(at + (2 * part + q) * 1024) = f32x4{c0[e], c0[e + 1], c0[e + 2], c0[e + 3]};
+            *(f32x4*)(at + 4096 + (2 * part + q) * 1024) = f32x4{c1[e], c1[e + 1], c1[e + 2], c1[e + 3]};
+          }
         }
       }
     } else {
       float g[8], u[8], dg[8], du[8];
       if constexpr (EK == EK_BF16) {
-        unpack8<EK_F16>(split_halves(ex.x[2 * j]), g);
-        unpack8<EK_F16>(split_halves(ex.x[2 * j + 1]), u);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          g[e] *= Kept<EK>::UP;
-          u[e] *= Kept<EK>::UP;
+          const uint32_t kg = ex.x[j][e / 2], ku = ex.x[2 + j][e / 2], low = ex.x[4][2 * j + e / 4] >> (e % 4 * 8);
+          g[e] = __uint_as_float((e % 2 ? kg & 0xffff0000u : kg << 16) | (low & 0xfu) << 12);
+          u[e] = __uint_as_float((e % 2 ? ku & 0xffff0000u : ku << 16) | (low & 0xf0u) << 8);
         }
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          g[e] = __uint_as_float(ex.x[4 * j + 2 * (e / 4)][e % 4]);
-          u[e] = __uint_as_float(ex.x[4 * j + 2 * (e / 4) + 1][e % 4]);
+          g[e] = __uint_as_float(ex.x[2 * j + e / 4][e % 4]);
+          u[e] = __uint_as_float(ex.x[4 + 2 * j + e / 4][e % 4]);
         }
       }
       float a[8], slope[8];
@@ -773,6 +771,11 @@ extern "C" {
 size_t lik_gated_ffn_workspace_size(int32_t dtype, int64_t rows, int32_t dim, int32_t hidden) {
   if (ffn_check(dtype, rows, dim, hidden, ACT_GELU) != LIK_OK || rows == 0) return 0;
   return ffn_ws(rows, dim, hidden);
+}
+
+size_t lik_gated_ffn_kept_size(int32_t dtype, int64_t rows, int32_t dim, int32_t hidden) {
+  if (ffn_check(dtype, rows, dim, hidden, ACT_GELU) != LIK_OK) return 0;
+  return (size_t)((rows + 31) / 32) * ((hidden + 31) / 32) * (dtype == LIK_BF16 ? kKeptBlock<EK_BF16> : kKeptBlock<EK_F16>);
 }
 
 int lik_gated_ffn(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int32_t dim, int32_t hidden,

@@ -85,6 +85,7 @@ EXPORTED_SYMBOLS = (
     "lik_layer_norm_backward_workspace_size",
     "lik_gated_ffn",
     "lik_gated_ffn_workspace_size",
+    "lik_gated_ffn_kept_size",
     "lik_gated_ffn_backward",
     "lik_gated_ffn_backward_workspace_size",
     "lik_attention",
@@ -301,6 +302,8 @@ def load() -> ctypes.CDLL:
     lib.lik_layer_norm_backward.restype = ctypes.c_int
     lib.lik_gated_ffn_workspace_size.argtypes = [_i32, _i64, _i32, _i32]
     lib.lik_gated_ffn_workspace_size.restype = ctypes.c_size_t
+    lib.lik_gated_ffn_kept_size.argtypes = [_i32, _i64, _i32, _i32]
+    lib.lik_gated_ffn_kept_size.restype = ctypes.c_size_t
     lib.lik_gated_ffn.argtypes = [_p, _i64, _i32, _i64, _i32, _i32, _p, _i64, _p, _i64, _p, _i64, _i32, _p, _p, _p, _p,
                                   ctypes.c_size_t, _p]
     lib.lik_gated_ffn.restype = ctypes.c_int

@@ -15,8 +15,6 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 
-# what the forward keeps both projections in: more bits than the gradients' rounding (bf16's are scaled into fp16)
-_KEPT = {torch.bfloat16: torch.float16, torch.float16: torch.float32}
 ACTIVATIONS = {"gelu": 0, "gelu_tanh": 1, "silu": 2}
 
 
@@ -26,10 +24,10 @@ def _forward(x2, w_in, w_out, r2, act, want_kept):
     out = torch.empty(rows, d, dtype=x2.dtype, device=x2.device)
     h = torch.empty(rows, f, dtype=x2.dtype, device=x2.device)
     gu = None
-    if want_kept:
-        gu = torch.empty(rows, 2 * f, dtype=_KEPT[x2.dtype], device=x2.device)
     if rows:
         lib, code = _lib.load(), _lib.DTYPE_CODE[x2.dtype]
+        if want_kept:
+            gu = torch.empty(lib.lik_gated_ffn_kept_size(code, rows, d, f), dtype=torch.uint8, device=x2.device)
         nbytes = lib.lik_gated_ffn_workspace_size(code, rows, d, f)
         ws = _lib.workspace(nbytes, x2.device)
         with _lib.on_device(x2.device):
