@@ -13,6 +13,10 @@
 // once to the 16-bit type, as the next product's operands have to be. g and u are kept for the backward so
 // that dg and du carry next to no other rounding, at any size: of bf16 calls the upper 20 bits of the fp32 value
 // (12 significant bits against the 8 of dg and du), of fp16 calls fp32.
+// fp16 has no range for dg and du of any gy (nor for large inputs): they are held s times, s the power of two that brings a
+// bound of theirs to 2^14 .. 2^15, d max|gy| max|Wo| max(|u| max|act'|, |act(g)|), and dx and dw_in are scaled back. The last factor
+// comes from the forward, a value a kept block; a kernel finds the others. The bound is some 2^7 to 2^12 above the largest
+// elements, which leaves 17 powers of two of normal numbers below those.
 #include "lik_enc.h"
 
 namespace lik {
@@ -38,6 +42,8 @@ struct GemmP {
   char* gu;            // EPI_GLU: kept g and u (null: not kept), KeptBlock; EPI_GLU_BWD: read
   int hidden;
   int act;
+  float* bound;        // fp16, EPI_GLU with gu: [blocks][2] largest factors of dg and du (blocks of 16 columns: one each)
+  const float* scale;  // fp16, null: 1. EPI_GLU_BWD: dg and du are held as many times; EPI_STORE: the sums are multiplied by it
 };
 
 // act(x) and its derivative
@@ -185,6 +191,17 @@ __device__ __forceinline__ char* kept_at(const GemmP& p, int m, int n, int h) {
   const int64_t block = (int64_t)(m >> 5) * ((p.hidden + 31) >> 5) + (n >> 5);
   return p.gu + block * kKeptBlock<EK> + ((m & 31) + 32 * h) * 16;
 }
+// Bound of |act'|: gelu 1.13, silu 1.10.
+constexpr float kSlopeMost = 1.25f;
+__device__ __forceinline__ float max_finite(float big, float x) {  // (rows that are not finite are NaN at any scale)
+  const float a = fabsf(x);
+  return a < INFINITY ? fmaxf(big, a) : big;
+}
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) x = fmaxf(x, __shfl_xor(x, s));
+  return x;
+}
 // The upper 20 bits of an fp32 value (rounded to nearest): 16 of them, and 4 in a nibble of the byte that g and u share.
 __device__ __forceinline__ uint32_t round20(float x) { return __float_as_uint(x) + 0x800u; }
 __device__ __forceinline__ uint32_t pack_upper(uint32_t a, uint32_t b) {  // upper halves of a and b
@@ -225,6 +242,9 @@ __device__ __forceinline__ void load_extra(const GemmP& p, Extra<EK, EPI>& ex, i
 template <int EK, int EPI, int NJ = 2>
 __device__ __forceinline__ void finish_block(const GemmP& p, const f32x16& c0, const f32x16& c1,
                                              const Extra<EK, EPI>& ex, int m, int n, int h) {
+  float scale = 1.0f, bound = 0.f;
+  if constexpr (EK == EK_F16 && EPI != EPI_GLU)
+    if (p.scale) scale = *p.scale;
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {  // quads 2 j, 2 j + 1: 16 columns
     const int c = n + 16 * j + 8 * h;
@@ -233,7 +253,7 @@ __device__ __forceinline__ void finish_block(const GemmP& p, const f32x16& c0, c
       float v[8];
       unpack8<EK>(split_halves(ex.x[j]), v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += c0[8 * j + e];
+      for (int e = 0; e < 8; ++e) v[e] = EK == EK_F16 ? fmaf(c0[8 * j + e], scale, v[e]) : v[e] + c0[8 * j + e];
       const u32x4 o =
           join_halves(pack2<EK>(v[0], v[1]), pack2<EK>(v[2], v[3]), pack2<EK>(v[4], v[5]), pack2<EK>(v[6], v[7]));
       if (on) *(u32x4*)(p.out + m * p.out_ld + c * 2) = o;
@@ -242,6 +262,10 @@ __device__ __forceinline__ void finish_block(const GemmP& p, const f32x16& c0, c
 #pragma unroll
       for (int e = 0; e < 8; ++e) g[e] = c0[8 * j + e];
       act8<false>(p.act, g, v, nullptr);
+      if constexpr (EK == EK_F16)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          bound = max_finite(max_finite(bound, v[e]), kSlopeMost * c1[8 * j + e]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] *= c1[8 * j + e];
       const u32x4 o =
@@ -293,7 +317,7 @@ __device__ __forceinline__ void finish_block(const GemmP& p, const f32x16& c0, c
       act8<true>(p.act, g, a, slope);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float dh = c0[8 * j + e];
+        const float dh = EK == EK_F16 ? c0[8 * j + e] * scale : c0[8 * j + e];
         du[e] = dh * a[e];
         dg[e] = dh * u[e] * slope[e];
       }
@@ -307,6 +331,83 @@ __device__ __forceinline__ void finish_block(const GemmP& p, const f32x16& c0, c
         *(u32x4*)(o + (int64_t)p.hidden * 2) = ou;
       }
     }
+  }
+  if constexpr (EK == EK_F16 && EPI == EPI_GLU)
+    if (p.gu && m - (m & 31) < p.m && n < p.hidden) {
+      bound = wave_max(bound);
+      const int64_t block = (int64_t)(m >> 5) * ((p.hidden + 31) >> 5) + (n >> 5);
+      if ((m & 31) + h == 0) {
+        if (NJ == 1) p.bound[2 * block + ((n >> 4) & 1)] = bound;
+        else *(f32x2*)(p.bound + 2 * block) = f32x2{bound, 0.f};
+      }
+    }
+}
+
+// fp16: the largest finite |gy|, |Wo| and forward's factor, a workgroup's share: part[3][gridDim.x]. Bound by reading
+// them once, with too little in flight: 40 MB of 16480 rows (1024, 2816) 16 us with 1024 workgroups, 28 with 256.
+struct BoundP {
+  const char *g, *w;  // [rows][d], [d][f]
+  int64_t g_ld, w_ld, rows;
+  int d, f;
+  const float* factor;  // [blocks][2]
+  int64_t blocks;
+  float* part;
+  float* scale;  // s, 1 / s
+};
+__device__ __forceinline__ float rows_max(const char* at, int64_t ld, int64_t rows, int d) {
+  typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+  const int chunks = d / 8;
+  int lpr = 1;  // lanes of a row
+  while (lpr < chunks && lpr < 64) lpr *= 2;
+  const int c0 = (int)threadIdx.x % lpr, step = 256 / lpr;
+  i16x2 top = {0, 0};
+  for (int64_t r = (int64_t)blockIdx.x * step + threadIdx.x / lpr; r < rows; r += (int64_t)gridDim.x * step)
+#pragma unroll 4
+    for (int c = c0; c < chunks; c += lpr) {
+      const u32x4 x = *(const u32x4*)(at + r * ld + c * 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const i16x2 a = __builtin_bit_cast(i16x2, x[i] & 0x7fff7fffu);
+        const i16x2 finite = (a - i16x2{0x7c00, 0x7c00}) >> 15;  // -1; infinities and NaN: 0
+        top = __builtin_elementwise_max(top, a & finite);
+      }
+    }
+  return f16_to_f32((uint16_t)(top[0] > top[1] ? top[0] : top[1]));
+}
+__global__ void __launch_bounds__(256) bound_kernel(const BoundP p) {
+  __shared__ float s_big[3][4];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, cols = (p.f + 31) / 32;
+  float big[3] = {rows_max(p.g, p.g_ld, p.rows, p.d), rows_max(p.w, p.w_ld, p.d, p.f), 0.f};
+  for (int64_t b = (int64_t)blockIdx.x * 256 + tid; b < p.blocks; b += (int64_t)gridDim.x * 256) {
+    const f32x2 x = *(const f32x2*)(p.factor + 2 * b);
+    big[2] = fmaxf(big[2], x[0]);
+    if ((int)(b % cols) * 32 + 16 < p.f) big[2] = fmaxf(big[2], x[1]);
+  }
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    big[i] = wave_max(big[i]);
+    if (lane == 0) s_big[i][wv] = big[i];
+  }
+  __syncthreads();
+  if (tid < 3)
+    p.part[tid * gridDim.x + blockIdx.x] = fmaxf(fmaxf(s_big[tid][0], s_big[tid][1]), fmaxf(s_big[tid][2], s_big[tid][3]));
+}
+constexpr int kBoundWgs = 1024;
+__global__ void __launch_bounds__(64) scale_kernel(const BoundP p) {
+  float bound = (float)p.d;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    float x = 0.f;
+#pragma unroll
+    for (int k = 0; k < kBoundWgs / 64; ++k) x = fmaxf(x, p.part[i * kBoundWgs + k * 64 + threadIdx.x]);
+    bound *= wave_max(x);
+  }
+  int e = 15;  // where nothing is: s = 1
+  if (bound > 0.f) frexpf(bound, &e);  // bound < 2^e
+  const int up = e < -85 ? 100 : 15 - e;
+  if (threadIdx.x == 0) {
+    p.scale[0] = ldexpf(1.0f, up);
+    p.scale[1] = ldexpf(1.0f, -up);
   }
 }
 
@@ -640,18 +741,22 @@ size_t ffn_ws(int64_t rows, int d, int f) {
   return most(part_bytes(gemm_shape(rows, glu_columns(f), d)), part_bytes(gemm_shape(rows, d, f))) + 256;
 }
 
-struct FfnBwdWs {
-  size_t dgu, part, total;
+struct FfnBwdWs {  // dg and du come first
+  size_t bound, part, total;
 };
 FfnBwdWs ffn_bwd_ws(int64_t rows, int d, int f) {
   FfnBwdWs w;
-  w.dgu = 0;
-  w.part = align256((size_t)rows * 2 * f * 2);
+  w.bound = align256((size_t)rows * 2 * f * 2);
+  w.part = w.bound + align256((3 * kBoundWgs + 2) * 4);
   w.total = w.part + 256 +
             most(most(part_bytes(gemm_shape(rows, f, d)), part_bytes(gemm_shape(rows, d, 2 * f))),
                  most(part_bytes(gemm_shape(2 * f, d, rows)), part_bytes(gemm_shape(d, f, rows))));
   return w;
 }
+
+int64_t kept_blocks(int64_t rows, int f) { return ((rows + 31) / 32) * ((f + 31) / 32); }
+// (fp16: the forward's factors after the blocks)
+float* kept_bound(void* gu, int64_t rows, int f) { return (float*)((char*)gu + kept_blocks(rows, f) * kKeptBlock<EK_F16>); }
 
 int ffn_check(int32_t dtype, int64_t rows, int32_t d, int32_t f, int32_t act) {
   if (dtype != LIK_BF16 && dtype != LIK_F16) return LIK_ERR_UNSUPPORTED;
@@ -685,6 +790,7 @@ int ffn_forward(const void* x, int64_t x_ld, int64_t rows, int d, int f, const v
   p.out = (char*)h;
   p.out_ld = (int64_t)f * 2;
   p.gu = (char*)gu;
+  if (EK == EK_F16 && gu) p.bound = kept_bound(gu, rows, f);
   if (const int rc = launch_gemm<EK, false, false, EPI_GLU>(p, part, s)) return rc;
   p.a = (const char*)h;
   p.a_ld = (int64_t)f * 2;
@@ -704,7 +810,7 @@ int ffn_backward(const void* g, int64_t g_ld, const void* x, int64_t x_ld, int64
                  const void* w_in, int64_t wi_ld, const void* w_out, int64_t wo_ld, const void* h, const void* gu,
                  int act, void* gx, void* gw_in, void* gw_out, char* ws, hipStream_t s) {
   const FfnBwdWs w = ffn_bwd_ws(rows, d, f);
-  char* dgu = ws + w.dgu;
+  char* dgu = ws;
   float* part = (float*)(ws + w.part);
   GemmP p{};
   p.act = act;
@@ -720,7 +826,18 @@ int ffn_backward(const void* g, int64_t g_ld, const void* x, int64_t x_ld, int64
     p.out = dgu;
     p.out_ld = (int64_t)f * 4;
     p.gu = (char*)const_cast<void*>(gu);
+    if (EK == EK_F16) {
+      float* at = (float*)(ws + w.bound);
+      const BoundP b{(const char*)g, (const char*)w_out, g_ld * 2, wo_ld * 2, rows, d, f, kept_bound(p.gu, rows, f),
+                     kept_blocks(rows, f), at, at + 3 * kBoundWgs};
+      launch_kernel(bound_kernel, dim3(kBoundWgs), dim3(256), 0u, s, b);
+      if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
+      launch_kernel(scale_kernel, dim3(1), dim3(64), 0u, s, b);
+      if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
+      p.scale = b.scale;
+    }
     if (const int rc = launch_gemm<EK, false, true, EPI_GLU_BWD>(p, part, s)) return rc;
+    if (p.scale) ++p.scale;  // 1 / s
   }
   if (gx) {
     p.a = dgu;
@@ -746,6 +863,7 @@ int ffn_backward(const void* g, int64_t g_ld, const void* x, int64_t x_ld, int64
     if (const int rc = launch_gemm<EK, true, true, EPI_STORE>(p, part, s)) return rc;
   }
   if (gw_out) {
+    p.scale = nullptr;
     p.m = d;
     p.n = f;
     p.a = (const char*)g;
@@ -775,7 +893,7 @@ size_t lik_gated_ffn_workspace_size(int32_t dtype, int64_t rows, int32_t dim, in
 
 size_t lik_gated_ffn_kept_size(int32_t dtype, int64_t rows, int32_t dim, int32_t hidden) {
   if (ffn_check(dtype, rows, dim, hidden, ACT_GELU) != LIK_OK) return 0;
-  return (size_t)((rows + 31) / 32) * ((hidden + 31) / 32) * (dtype == LIK_BF16 ? kKeptBlock<EK_BF16> : kKeptBlock<EK_F16>);
+  return (size_t)kept_blocks(rows, hidden) * (dtype == LIK_BF16 ? kKeptBlock<EK_BF16> : kKeptBlock<EK_F16> + 8);
 }
 
 int lik_gated_ffn(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int32_t dim, int32_t hidden,
