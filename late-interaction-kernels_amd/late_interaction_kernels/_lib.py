@@ -360,6 +360,17 @@ def plain_op(*tensors: torch.Tensor) -> bool:
         return False
 
 
+def differentiates(*tensors: torch.Tensor | None) -> bool:
+    """Whether a call on these tensors goes through its autograd function: one wants a
+    gradient, or forward-mode differentiation is active, whose tangents only
+    the function can see (it has no rule for them and refuses)."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return getattr(torch.autograd.forward_ad, "_current_level", 0) >= 0
+
+
 # the current stream's handle and the current device, without a Stream object or a
 # device switch where torch has these
 _raw_stream = (getattr(torch._C, "_cuda_getCurrentRawStream", None)

@@ -122,7 +122,7 @@ def _check(q, k, v, causal, window, scale):
 
 def _run(q, k, v, meta, qm, km, cu_q, cu_k):
     d = q.shape[-1]
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _lib.differentiates(q, k, v):
         pad = -d % 8  # zero columns change no product; padded here so that autograd cuts the gradients
         if pad:
             q, k, v = (torch.nn.functional.pad(t, (0, pad)) for t in (q, k, v))

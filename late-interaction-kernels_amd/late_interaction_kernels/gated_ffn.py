@@ -128,8 +128,7 @@ def gated_ffn(
         r2 = None if r2 is None else F.pad(r2, (0, pd))
         w_in = F.pad(w_in.unflatten(0, (2, f)), (0, pd, 0, pf)).reshape(2 * (f + pf), d + pd)
         w_out = F.pad(w_out, (0, pf, 0, pd))
-    if torch.is_grad_enabled() and (x.requires_grad or w_in.requires_grad or w_out.requires_grad
-                                    or (residual is not None and residual.requires_grad)):
+    if _lib.differentiates(x, w_in, w_out, residual):
         out = _GatedFfnFn.apply(x2, w_in, w_out, r2, act)
     else:
         out, _, _ = _forward(_lib.rows16(x2), _lib.rows16(w_in), _lib.rows16(w_out),

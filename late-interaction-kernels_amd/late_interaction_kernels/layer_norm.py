@@ -130,8 +130,7 @@ def layer_norm(
             or (residual is not None and residual.device != device)):
         raise ValueError("x, weight, bias and residual must be on the same device.")
     _lib.require_gpu(x)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
+    if _lib.differentiates(x, weight, bias, residual):
         return _LayerNormFn.apply(x, weight, bias, residual, float(eps))
     y, total, _ = _forward(x, weight.contiguous(), None if bias is None else bias.contiguous(), residual, float(eps),
                            False)
