@@ -457,7 +457,7 @@ int lik_quantize_fp8(const void* x, int32_t dtype, int64_t rows, int32_t dim, ui
  *   y = (s - mean(s)) / sqrt(var(s) + eps) * weight + bias
  * dtype bf16 / fp16 / fp32; weight and bias (null: none) in it or in fp32.
  * y is contiguous. stats (optional) [rows, 2]: mean and 1 / sqrt(var + eps) for the
- * backward pass. dim <= 8192 (LIK_ERR_UNSUPPORTED above).
+ * backward pass. dim <= 8192, every array on one of its elements (else LIK_ERR_UNSUPPORTED).
  */
 int lik_layer_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, int32_t dtype,
                    int64_t rows, int32_t dim, const void* weight, const void* bias, int32_t weight_dtype, float eps,
@@ -465,7 +465,7 @@ int lik_layer_norm(const void* x, int64_t x_stride, const void* residual, int64_
 /*
  * Its gradients: grad_x [rows, dim] (contiguous; of x and of the residual alike)
  * = the norm's from grad_y, plus grad_sum (null: none); grad_weight and grad_bias
- * [dim] in weight_dtype (null: not wanted). sum is what was normalised. Sums
+ * [dim] in weight_dtype (null: not wanted; else rows >= 1). sum is what was normalised. Sums
  * over rows are taken in a fixed order.
  */
 size_t lik_layer_norm_backward_workspace_size(int32_t dtype, int64_t rows, int32_t dim);

@@ -361,12 +361,18 @@ int launch_norm(const NormP& p, hipStream_t s, int& slices) {
   return launch_norm_nv<EK, BWD, 256, MOST / 4 + 1, MOST>(p, nv, s, slices);
 }
 
-// row base and stride on an element, d and the types in range
+// d and the types in range
 int norm_check(int32_t dtype, int32_t wdtype, int64_t rows, int64_t d) {
   if (dtype != LIK_BF16 && dtype != LIK_F16 && dtype != LIK_F32) return LIK_ERR_UNSUPPORTED;
   if (wdtype != dtype && wdtype != LIK_F32) return LIK_ERR_UNSUPPORTED;
   if (rows < 0 || d < 1) return LIK_ERR_INVALID;
   return d <= kNormMaxDim ? LIK_OK : LIK_ERR_UNSUPPORTED;
+}
+
+// every array (null: not there) starts on one of its elements
+template <typename... P>
+bool on_element(int64_t size, P... p) {
+  return (... && ((uintptr_t)p % (uintptr_t)size == 0));
 }
 
 template <bool BWD>
@@ -391,7 +397,9 @@ int lik_layer_norm(const void* x, int64_t x_stride, const void* residual, int64_
   if (const int rc = norm_check(dtype, weight_dtype, rows, dim)) return rc;
   if (rows == 0) return LIK_OK;
   if (!x || !weight || !y || (residual && !sum)) return LIK_ERR_INVALID;
-  const int64_t e = dtype == LIK_F32 ? 4 : 2;
+  const int64_t e = dtype == LIK_F32 ? 4 : 2, we = weight_dtype == LIK_F32 ? 4 : 2;
+  if (!on_element(e, x, residual, y, sum) || !on_element(we, weight, bias) || !on_element(4, stats))
+    return LIK_ERR_UNSUPPORTED;
   NormP p{};
   p.x = (const char*)x;
   p.x_sr = x_stride * e;
@@ -421,11 +429,14 @@ int lik_layer_norm_backward(const void* grad_y, int64_t grad_y_stride, const voi
                             int32_t dim, const void* weight, int32_t weight_dtype, void* grad_x, void* grad_weight,
                             void* grad_bias, void* workspace, size_t workspace_bytes, lik_stream_t stream) {
   if (const int rc = norm_check(dtype, weight_dtype, rows, dim)) return rc;
-  if (rows == 0) return LIK_OK;
+  if (rows == 0) return grad_weight || grad_bias ? LIK_ERR_INVALID : LIK_OK;  // the weights' would stay unwritten
   if (!grad_y || !sum || !stats || !weight || !grad_x) return LIK_ERR_INVALID;
   if (!workspace || workspace_bytes < lik_layer_norm_backward_workspace_size(dtype, rows, dim))
     return LIK_ERR_WORKSPACE;
-  const int64_t e = dtype == LIK_F32 ? 4 : 2;
+  const int64_t e = dtype == LIK_F32 ? 4 : 2, we = weight_dtype == LIK_F32 ? 4 : 2;
+  if (!on_element(e, grad_y, grad_sum, sum, grad_x) || !on_element(we, weight, grad_weight, grad_bias) ||
+      !on_element(4, stats))
+    return LIK_ERR_UNSUPPORTED;
   NormP p{};
   p.x = (const char*)sum;
   p.x_sr = sum_stride * e;
