@@ -561,13 +561,23 @@ def prepare_tokens(x: torch.Tensor) -> torch.Tensor:
     return x
 
 
-def rows16(x: torch.Tensor) -> torch.Tensor:
-    """:func:`prepare_tokens` of a 16-bit tensor, without its steps where there is nothing to do."""
+def rows16(x: torch.Tensor, dim: int, far: int) -> torch.Tensor:
+    """:func:`prepare_tokens` of a 16-bit tensor, without its steps where there is nothing to do, and with a stride of
+    ``dim`` that is less than ``far`` (a copy where it is not)."""
+    strides = x.stride()
+    *outer, last = strides
     bits = x.data_ptr() | (x.shape[-1] << 1)
-    *outer, last = x.stride()
     for s in outer:
         bits |= s << 1
-    return prepare_tokens(x) if bits & 15 or last != 1 else x
+    if not bits & 15 and last == 1 and strides[dim] < far:
+        return x
+    x = prepare_tokens(x)
+    if x.stride(dim) >= far:
+        return x.clone(memory_format=torch.contiguous_format)
+    # a dim of one element keeps the stride it had, which nothing steps by
+    if any(n == 1 and s & 7 for n, s in zip(x.shape, x.stride())):
+        x = x.as_strided(x.shape, [0 if n == 1 else s for n, s in zip(x.shape, x.stride())])
+    return x
 
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor | None:

@@ -20,6 +20,9 @@ from . import _lib
 from ._core import _i32, _mask_i8, assert_max_seqlens_cover, seqlen_max
 
 
+_FAR = 1 << 24  # elements from token to token: the kernels reach 64 tokens by 32-bit offsets
+
+
 def _args(q, k, v, meta, qm, km, cu_q, cu_k):
     """The C struct of a call on prepared ``[n, L, H, d]`` (packed: ``[T, H, d]``) tensors."""
     left, right, scale, max_q, max_k = meta
@@ -62,7 +65,7 @@ def _forward(q, k, v, meta, qm, km, cu_q, cu_k, train):
 class _AttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, meta, qm, km, cu_q, cu_k):
-        q, k, v = _lib.rows16(q), _lib.rows16(k), _lib.rows16(v)
+        q, k, v = _lib.rows16(q, -3, _FAR), _lib.rows16(k, -3, _FAR), _lib.rows16(v, -3, _FAR)
         out, lse, low = _forward(q, k, v, meta, qm, km, cu_q, cu_k, True)
         ctx.save_for_backward(q, k, v, out, lse, low, qm, km, cu_q, cu_k)
         ctx.meta = meta
@@ -81,7 +84,7 @@ class _AttentionFn(torch.autograd.Function):
         if need_k or need_v:
             gk, gv = (make(t.shape, dtype=t.dtype, device=t.device) for t in (k, v))
         if not none and (gq is not None or gk is not None):
-            g = _lib.rows16(grad)
+            g = _lib.rows16(grad, -3, _FAR)
             lib = _lib.load()
             nbytes = lib.lik_attention_backward_workspace_size(ctypes.byref(a))
             ws = _lib.workspace(nbytes, q.device)
@@ -128,7 +131,7 @@ def _run(q, k, v, meta, qm, km, cu_q, cu_k):
             q, k, v = (torch.nn.functional.pad(t, (0, pad)) for t in (q, k, v))
         out = _AttentionFn.apply(q, k, v, meta, qm, km, cu_q, cu_k)
     else:
-        q, k, v = _lib.rows16(q), _lib.rows16(k), _lib.rows16(v)
+        q, k, v = _lib.rows16(q, -3, _FAR), _lib.rows16(k, -3, _FAR), _lib.rows16(v, -3, _FAR)
         out, _, _ = _forward(q, k, v, meta, qm, km, cu_q, cu_k, False)
     return out[..., :d] if d % 8 else out
 

@@ -18,6 +18,15 @@ from . import _lib
 ACTIVATIONS = {"gelu": 0, "gelu_tanh": 1, "silu": 2}
 
 
+_FAR = (1 << 21) + 1  # elements from row to row: the kernels reach 256 rows by 32-bit offsets
+
+
+def _near(x2, w_in, w_out, r2):
+    f = w_out.shape[1]  # w_in's up rows are that many rows away
+    return (_lib.rows16(x2, 0, _FAR), _lib.rows16(w_in, 0, _FAR if f < 768 else min(_FAR, 0x7FF80000 // (f + 256))),
+            _lib.rows16(w_out, 0, _FAR), None if r2 is None else _lib.rows16(r2, 0, _FAR))
+
+
 def _forward(x2, w_in, w_out, r2, act, want_kept):
     rows, d = x2.shape
     f = w_out.shape[1]
@@ -44,8 +53,8 @@ class _GatedFfnFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x2, w_in, w_out, r2, act):
-        x2, w_in, w_out = _lib.rows16(x2), _lib.rows16(w_in), _lib.rows16(w_out)
-        out, h, gu = _forward(x2, w_in, w_out, None if r2 is None else _lib.rows16(r2), act, True)
+        x2, w_in, w_out, r2 = _near(x2, w_in, w_out, r2)
+        out, h, gu = _forward(x2, w_in, w_out, r2, act, True)
         ctx.save_for_backward(x2, w_in, w_out, h, gu)
         ctx.act = act
         return out
@@ -64,7 +73,7 @@ class _GatedFfnFn(torch.autograd.Function):
                 if t is not None:
                     t.zero_()
         elif need_x or need_in or need_out:
-            g = _lib.rows16(grad)
+            g = _lib.rows16(grad, 0, _FAR)
             lib, code = _lib.load(), _lib.DTYPE_CODE[x2.dtype]
             nbytes = lib.lik_gated_ffn_backward_workspace_size(code, rows, d, f)
             ws = _lib.workspace(nbytes, x2.device)
@@ -131,8 +140,7 @@ def gated_ffn(
     if _lib.differentiates(x, w_in, w_out, residual):
         out = _GatedFfnFn.apply(x2, w_in, w_out, r2, act)
     else:
-        out, _, _ = _forward(_lib.rows16(x2), _lib.rows16(w_in), _lib.rows16(w_out),
-                             None if r2 is None else _lib.rows16(r2), act, False)
+        out, _, _ = _forward(*_near(x2, w_in, w_out, r2), act, False)
     if pd:
         out = out[:, :d]
     return out if x.dim() == 2 else out.reshape(x.shape)
