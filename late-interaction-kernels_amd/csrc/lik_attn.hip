@@ -385,17 +385,23 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttP p) {
   }
 }
 
-// Splits of the keys. Up to 64 rows a key head and no window: attention_rows_kernel, whose workgroups fill the
-// CUs once (LDS: two a CU up to head dim 64, else one), a wavefront 64 keys at least. More rows: where the tiles
-// of queries do not fill the 256 CUs and the keys are long, down to 256 keys a split.
+// Splits of the keys. Up to 64 rows a key head and no window: attention_rows_kernel may take the call, whose
+// workgroups fill the CUs once (LDS: two a CU up to head dim 64, else one), a wavefront 64 keys at least. It writes at
+// least four fp32 shares of each row and reads them again, for reading the keys once: shared heads, where the shares are at
+// most a third of the keys' and values' bytes (12 k_len each row); heads of their own, only where the key heads alone do not
+// fill the CUs and rows are few for the keys. us of both kernels, this one first: 16 / 4 heads of 128, 300 keys, 512
+// sequences, 1 query 90 and 203, 16 queries 219 and 210 (1000 keys 365 and 554); 12 heads of 64, 1000 keys, 1 query, 24
+// sequences 21 and 25, 48 sequences 34 and 27; 512 sequences of 64 queries and 300 keys 375 and 122, without 1.6 GB of shares.
+// More rows: where the tiles of queries do not fill the 256 CUs and the keys are long, down to 256 keys a split.
 void forward_shape(AttP& p) {
   p.tiles = (int)((p.q_len + 127) / 128);
   const bool window = p.left != kNone || p.right != kNone;
-  p.few = !window && p.q_len * p.group <= 64 && p.k_len >= 256;
+  const int64_t rows = p.q_len * p.group, units = (int64_t)p.n * (p.heads / p.group), slots = p.dim <= 64 ? 512 : 256;
+  p.few = !window && rows <= 64 && p.k_len >= 256 &&
+          (p.group > 1 ? 12 * rows <= p.k_len : units <= slots && p.k_len >= 512 && 48 * rows <= p.k_len);
   int64_t s;
   if (p.few) {
-    const int64_t units = (int64_t)p.n * (p.heads / p.group);
-    s = (p.dim <= 64 ? 512 : 256) / units;
+    s = slots / units;
     const int64_t most = (p.k_len + 255) / 256;
     if (s > most) s = most;
     if (s > 16) s = 16;
