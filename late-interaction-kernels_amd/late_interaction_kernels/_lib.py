@@ -360,6 +360,9 @@ def plain_op(*tensors: torch.Tensor) -> bool:
         return False
 
 
+_forward_ad = torch.autograd.forward_ad
+
+
 def differentiates(*tensors: torch.Tensor | None) -> bool:
     """Whether a call on these tensors goes through its autograd function: one wants a
     gradient, or forward-mode differentiation is active, whose tangents only
@@ -368,7 +371,7 @@ def differentiates(*tensors: torch.Tensor | None) -> bool:
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
-    return getattr(torch.autograd.forward_ad, "_current_level", 0) >= 0
+    return getattr(_forward_ad, "_current_level", 0) >= 0
 
 
 # the current stream's handle and the current device, without a Stream object or a
