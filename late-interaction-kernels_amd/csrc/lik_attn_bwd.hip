@@ -133,10 +133,14 @@ __device__ __forceinline__ bool key_seen(const AttP& p, const f32x16* dk, const 
   const bool odd = kon && !(sum == 0.f);
   if (__ballot(odd) == 0) return kon;
   bool seen = !odd;
+  const int lane = threadIdx.x & 63;
   for (int h = 0; h < p.group; ++h)
-    for (int q = 0; q < qlen && __ballot(!seen) != 0; ++q)
-      seen = seen || (lse[(int64_t)h * p.q_total + q] != INFINITY && (p.left == kNone || q <= kpos + p.left) &&
-                      (p.right == kNone || q >= kpos - p.right));
+    for (int q0 = 0; q0 < qlen && __ballot(!seen) != 0; q0 += 64) {  // a lane a query, then a lane a key
+      const uint64_t have = __ballot(q0 + lane < qlen && lse[(int64_t)h * p.q_total + q0 + lane] != INFINITY);
+      const int lo = p.right == kNone || kpos - p.right < q0 ? 0 : kpos - p.right - q0;
+      const int hi = p.left == kNone || kpos + p.left > q0 + 63 ? 63 : kpos + p.left - q0;
+      if (lo <= 63 && hi >= 0) seen = seen || (have & (~0ull << lo) & (~0ull >> (63 - hi))) != 0;
+    }
   return kon && seen;
 }
 
