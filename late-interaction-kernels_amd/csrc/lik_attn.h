@@ -266,13 +266,6 @@ __device__ __forceinline__ float with_low(float r, uint32_t low, int k) {
   return __uint_as_float(__float_as_uint(r) + (uint32_t)(byte << kLow<EK>));
 }
 
-// Four consecutive elements of accumulator quads 2 j and 2 j + 1 as 16-bit pairs
-// to eight consecutive ones a lane: half h then holds elements 16 j + 8 h + 0..7.
-__device__ __forceinline__ u32x4 join_halves(uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1) {
-  const auto s0 = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
-  const auto s1 = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
-  return u32x4{(uint32_t)s0[0], (uint32_t)s1[0], (uint32_t)s0[1], (uint32_t)s1[1]};
-}
 // One column's DB x 32 elements times f to its row in memory (dim elements).
 template <int EK, int DC>
 __device__ __forceinline__ void store_cols(char* row, const f32x16* acc, float f, int dim, int lane, bool on) {

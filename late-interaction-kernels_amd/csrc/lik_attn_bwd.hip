@@ -53,11 +53,6 @@ __device__ __forceinline__ float max_finite(const u32x4* x) {
   }
   return f16_to_f32((uint16_t)top);
 }
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) x = fmaxf(x, __shfl_xor(x, s));
-  return x;
-}
 
 // fp16: the largest |v| of 128 keys of a key head.
 __global__ void __launch_bounds__(256) attention_vmax_kernel(const AttP p) {

@@ -107,6 +107,20 @@ __device__ __forceinline__ f32x16 mfma16(const f32x16& c, const u32x4& a, const 
   return mfma32<EK>(c, &a, &b);
 }
 
+// Four consecutive elements of accumulator quads 2 j and 2 j + 1, as 16-bit pairs, to eight consecutive ones a lane
+// (the wavefront's halves exchange): half h then holds elements 16 j + 8 h + 0..7.
+__device__ __forceinline__ u32x4 join_halves(uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1) {
+  const auto s0 = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
+  const auto s1 = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
+  return u32x4{(uint32_t)s0[0], (uint32_t)s1[0], (uint32_t)s0[1], (uint32_t)s1[1]};
+}
+// On every lane.
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) x = fmaxf(x, __shfl_xor(x, s));
+  return x;
+}
+
 // The workgroups of one XCD (round-robin by block index) get a contiguous range of tiles.
 __device__ __forceinline__ uint32_t xcd_tile(uint32_t id, uint32_t n) {
   const uint32_t x = id & 7u, per = n >> 3, extra = n & 7u;

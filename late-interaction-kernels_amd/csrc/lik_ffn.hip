@@ -161,14 +161,7 @@ struct Stage {
   }
 };
 
-// Four consecutive n of accumulator quads 2 j and 2 j + 1, as 16-bit pairs, to
-// eight consecutive n per lane (the wavefront's halves exchange): lane half h
-// then holds n = 16 j + 8 h + 0..7 of its m. split_halves is the inverse.
-__device__ __forceinline__ u32x4 join_halves(uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1) {
-  const auto s0 = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
-  const auto s1 = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
-  return u32x4{(uint32_t)s0[0], (uint32_t)s1[0], (uint32_t)s0[1], (uint32_t)s1[1]};
-}
+// The inverse of join_halves.
 __device__ __forceinline__ u32x4 split_halves(const u32x4& x) {
   const auto s0 = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false);
   const auto s1 = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
@@ -196,11 +189,6 @@ constexpr float kSlopeMost = 1.25f;
 __device__ __forceinline__ float max_finite(float big, float x) {  // (rows that are not finite are NaN at any scale)
   const float a = fabsf(x);
   return a < INFINITY ? fmaxf(big, a) : big;
-}
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) x = fmaxf(x, __shfl_xor(x, s));
-  return x;
 }
 // The upper 20 bits of an fp32 value (rounded to nearest): 16 of them, and 4 in a nibble of the byte that g and u share.
 __device__ __forceinline__ uint32_t round20(float x) { return __float_as_uint(x) + 0x800u; }
