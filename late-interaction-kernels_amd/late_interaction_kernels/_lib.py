@@ -575,6 +575,8 @@ def rows16(x: torch.Tensor, dim: int, far: int) -> torch.Tensor:
     if not bits & 15 and last == 1 and strides[dim] < far:
         return x
     x = prepare_tokens(x)
+    if x.numel() == 0:  # (with whatever strides)
+        return x.new_empty(x.shape)
     if x.stride(dim) >= far:
         return x.clone(memory_format=torch.contiguous_format)
     # a dim of one element keeps the stride it had, which nothing steps by

@@ -84,3 +84,21 @@ def test_one_row_inside_odd_ones():
     res = [(y, *torch.autograd.grad(y, ls, gy)) for ls in (ts, us) for y in (attention(*ls),)]
     assert all(torch.equal(a, b) for a, b in zip(*res))
     assert torch.equal(attention(q, k, v), res[0][0])
+
+
+def test_no_rows_inside_odd_ones():
+    """Keys of no rows, in a tensor whose rows are no multiple of 16 bytes apart, are no keys."""
+    from late_interaction_kernels.encoder import attention_varlen
+
+    q = torch.randn(5, 2, 64, device="cuda", dtype=BF, requires_grad=True)
+    k = torch.randn(0, 2, 67, device="cuda", dtype=BF)[..., 3:].requires_grad_()
+    cu_q, cu_k = (torch.tensor([0, n], dtype=torch.int32, device="cuda") for n in (5, 0))
+    out = attention_varlen(q, k, k, cu_q, cu_k, 5, 9)
+    gq, gk = torch.autograd.grad(out, (q, k), torch.ones_like(out))
+    assert torch.equal(out, torch.zeros_like(out)) and torch.equal(gq, torch.zeros_like(gq)) and gk.shape == k.shape
+    y = attention(q[None].detach(), k[None].detach(), k[None].detach())
+    assert torch.equal(y, torch.zeros_like(y))
+    x = torch.randn(0, 67, device="cuda", dtype=BF)[:, 3:].requires_grad_()
+    wi, wo = torch.ones(96, 64, device="cuda", dtype=BF), torch.ones(64, 48, device="cuda", dtype=BF)
+    (gx,) = torch.autograd.grad(gated_ffn(x, wi, wo, x).sum(), x)
+    assert gx.shape == x.shape
