@@ -266,20 +266,27 @@ __device__ __forceinline__ float with_low(float r, uint32_t low, int k) {
   return __uint_as_float(__float_as_uint(r) + (uint32_t)(byte << kLow<EK>));
 }
 
-// One column's DB x 32 elements times f to its row in memory (dim elements).
+// One column's DB x 32 elements times f to its row in memory (dim elements). Returns 0, or NaN if one of the lane's is
+// not finite.
 template <int EK, int DC>
-__device__ __forceinline__ void store_cols(char* row, const f32x16* acc, float f, int dim, int lane, bool on) {
+__device__ __forceinline__ float store_cols(char* row, const f32x16* acc, float f, int dim, int lane, bool on) {
+  float odd[2] = {};
 #pragma unroll
   for (int db = 0; db < DC; ++db)
 #pragma unroll
     for (int q = 0; q < 4; q += 2) {
       const f32x16& a = acc[db];
-      const u32x4 o = join_halves(pack2<EK>(a[q * 4] * f, a[q * 4 + 1] * f), pack2<EK>(a[q * 4 + 2] * f, a[q * 4 + 3] * f),
-                                  pack2<EK>(a[q * 4 + 4] * f, a[q * 4 + 5] * f),
-                                  pack2<EK>(a[q * 4 + 6] * f, a[q * 4 + 7] * f));
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] = pack2<EK>(a[q * 4 + 2 * i] * f, a[q * 4 + 2 * i + 1] * f);
+        odd[i % 2] = add2<EK>(w[i], odd[i % 2], 0.f);
+      }
+      const u32x4 o = join_halves(w[0], w[1], w[2], w[3]);
       const int e = db * 32 + 8 * q + 8 * (lane >> 5);
       if (on && e < dim) *(u32x4*)(row + e * 2) = o;
     }
+  return odd[0] + odd[1];
 }
 // The same elements' bytes.
 template <int EK, int DC>

@@ -109,26 +109,21 @@ __device__ __forceinline__ float row_delta(const AttP& p, const u32x4* gf, int64
   return d + swap_half(d);
 }
 
-// Whether the lane's key, whose sums dk and dv are, has a gradient: it is kept, and so is a query that sees it. Pairs that
-// are not kept add p = 0 times what the rows hold, which is no zero where a kept key or its value is not finite; then
-// (and only then) the queries' statistics are asked.
-template <int DC>
-__device__ __forceinline__ bool key_seen(const AttP& p, const f32x16* dk, const f32x16* dv, bool kon, int kpos,
-                                         const float* lse, int qlen) {
-  float zero[8] = {};  // NaN where an element is not finite
+// Gradients of the lane's key (kon: it is kept) to memory, from their sums; those of a key that no kept query sees are zeros.
+// Its pairs added p = 0 times what the rows hold, which is no zero where a kept key or its value is not finite: then (and only
+// then) the queries' statistics (`lse`, [heads of the group][q_total], the sequence's first row) are asked. at: the row's byte in
+// both; kpos < klen: it exists.
+template <int EK, int DC>
+__device__ __forceinline__ void store_key(const AttP& p, f32x16* dk, f32x16* dv, float fk, int64_t at, bool kon, int kpos,
+                                          int klen, const float* lse, int qlen, int lane) {
+  if (!kon)  // (their lanes ran on zero rows)
 #pragma unroll
-  for (int d = 0; d < DC; ++d)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      zero[i % 4] = fmaf(dk[d][i], 0.f, zero[i % 4]);
-      zero[4 + i % 4] = fmaf(dv[d][i], 0.f, zero[4 + i % 4]);
-    }
-  float sum = ((zero[0] + zero[1]) + (zero[2] + zero[3])) + ((zero[4] + zero[5]) + (zero[6] + zero[7]));
-  sum += swap_half(sum);
-  const bool odd = kon && !(sum == 0.f);
-  if (__ballot(odd) == 0) return kon;
-  bool seen = !odd;
-  const int lane = threadIdx.x & 63;
+    for (int d = 0; d < DC; ++d) dk[d] = dv[d] = f32x16{};
+  float odd = store_cols<EK, DC>(p.gk + at, dk, fk, p.dim, lane, kpos < klen) +
+              store_cols<EK, DC>(p.gv + at, dv, kUnliftP<EK>, p.dim, lane, kpos < klen);
+  odd += swap_half(odd);
+  bool seen = odd == 0.f;
+  if (__ballot(!seen) == 0) return;
   for (int h = 0; h < p.group; ++h)
     for (int q0 = 0; q0 < qlen && __ballot(!seen) != 0; q0 += 64) {  // a lane a query, then a lane a key
       const uint64_t have = __ballot(q0 + lane < qlen && lse[(int64_t)h * p.q_total + q0 + lane] != INFINITY);
@@ -136,7 +131,12 @@ __device__ __forceinline__ bool key_seen(const AttP& p, const f32x16* dk, const 
       const int hi = p.left == kNone || kpos + p.left > q0 + 63 ? 63 : kpos + p.left - q0;
       if (lo <= 63 && hi >= 0) seen = seen || (have & (~0ull << lo) & (~0ull >> (63 - hi))) != 0;
     }
-  return kon && seen;
+  const int e = 8 * (lane >> 5);  // (the lane's own 16 bytes, written above)
+  for (int d = e; d < p.dim; d += 16)
+    if (!seen && kpos < klen) {
+      *(u32x4*)(p.gk + at + d * 2) = u32x4{0u, 0u, 0u, 0u};
+      *(u32x4*)(p.gv + at + d * 2) = u32x4{0u, 0u, 0u, 0u};
+    }
 }
 
 // Gradient of q: the forward's walk over the keys (K rows also by transposing
@@ -455,12 +455,9 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 3 : 2) attention_dkv_kernel(con
     if (it + 1 < total) put_stat(buf ^ 1, next);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // V's loads where there was no step
-  if (!key_seen<DC>(p, dk, dv, kon, kpos, p.lse + (int64_t)kvh * p.group * p.q_total + qs.row, qs.len))
-#pragma unroll
-    for (int d = 0; d < DC; ++d) dk[d] = dv[d] = f32x16{};
   const int64_t at = ((ks.row + kpos) * kv_heads + kvh) * p.dim * 2;
-  store_cols<EK, DC>(p.gk + at, dk, p.scale * kUnliftP<EK> / gs, p.dim, lane, kpos < ks.len);
-  store_cols<EK, DC>(p.gv + at, dv, kUnliftP<EK>, p.dim, lane, kpos < ks.len);
+  store_key<EK, DC>(p, dk, dv, p.scale * kUnliftP<EK> / gs, at, kon, kpos, ks.len,
+                    p.lse + (int64_t)kvh * p.group * p.q_total + qs.row, qs.len, lane);
 }
 
 // All gradients of sequences of up to 32 KW keys in one pass: five products and one read of the rows, no sum in memory. A
@@ -640,12 +637,9 @@ __global__ void __launch_bounds__((KW + DC) * 64, (KW + DC + 3) / 4) attention_g
         *(u32x2*)(ds_row + ((q ^ ((l32 >> 2) & 3)) << 4)) = u32x2{df[q / 2][(q % 2) * 2], df[q / 2][(q % 2) * 2 + 1]};
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (!key_seen<DC>(p, dk, dv, kon, kpos, p.lse + (int64_t)kvh * p.group * p.q_total + qs.row, qs.len))
-#pragma unroll
-      for (int d = 0; d < DC; ++d) dk[d] = dv[d] = f32x16{};
     const int64_t at = ((ks.row + kpos) * kv_heads + kvh) * p.dim * 2;
-    store_cols<EK, DC>(p.gk + at, dk, p.scale * kUnliftP<EK> / gs, p.dim, lane, kpos < ks.len);
-    store_cols<EK, DC>(p.gv + at, dv, kUnliftP<EK>, p.dim, lane, kpos < ks.len);
+    store_key<EK, DC>(p, dk, dv, p.scale * kUnliftP<EK> / gs, at, kon, kpos, ks.len,
+                      p.lse + (int64_t)head0 * p.q_total + qs.row, qs.len, lane);
   } else {
     const int block = wv - KW;  // of 32 head dims
     // transposing reads of ds: lane l has query l % 32 of keys row0 + 4 (l / 32) + {0..3, 8..11}, as Frags::col

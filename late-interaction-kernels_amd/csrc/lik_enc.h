@@ -48,13 +48,13 @@ __device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b) {
   }
 }
 
-// c plus the two packed elements, in fp32 (one instruction, rounded once; subnormals are kept)
+// c plus f times the two packed elements, in fp32 (one instruction, rounded once; subnormals are kept)
 template <int EK>
-__device__ __forceinline__ float add2(uint32_t w, float c) {
+__device__ __forceinline__ float add2(uint32_t w, float c, float f = 1.0f) {
   if constexpr (EK == EK_F16)
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), f16x2{(_Float16)1.0f, (_Float16)1.0f}, c, false);
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), f16x2{(_Float16)f, (_Float16)f}, c, false);
   else
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), bf16x2{(__bf16)1.0f, (__bf16)1.0f}, c, false);
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), bf16x2{(__bf16)f, (__bf16)f}, c, false);
 }
 
 constexpr uint32_t kOob = 0xfffffff0u;  // a lane offset outside every buffer: the load returns (or writes to LDS) zeros
