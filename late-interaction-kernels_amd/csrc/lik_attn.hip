@@ -1,10 +1,10 @@
 // Attention, forward. One pass over the keys with the running maximum and sum of
 // the softmax; the layout of the products is described in lik_attn.h.
 //
-// Bounds, measured with 256 sequences of 12 heads of 64: up to 128 tokens the rows' reads and writes (41 us, 4.9 TB/s),
-// at 1024 the softmax's vector instructions beside the MFMAs (1005 us, 820 TFLOP/s; per 32 x 64 scores 512 clocks of
-// MFMA and about 1000 of vector work, four wavefronts a SIMD). Between them tiles that a sequence does not fill:
-// 50 to 300 tokens 107 us (63 at the copy rate).
+// Bounds, measured with 256 padded sequences of 12 heads of 64 (a call among others): up to 128 tokens the rows' reads and
+// writes (50 us, 4.0 TB/s), at 1024 the softmax's vector instructions beside the MFMAs (1042 us, 790 TFLOP/s; per 32 x 64 scores
+// 512 clocks of MFMA and about 1000 of vector work, four wavefronts a SIMD). Between them tiles that a sequence does not fill:
+// 50 to 300 tokens 105 us (63 at the copy rate).
 #include "lik_attn.h"
 
 namespace lik {

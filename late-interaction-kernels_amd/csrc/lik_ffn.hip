@@ -402,9 +402,9 @@ __global__ void __launch_bounds__(64) scale_kernel(const BoundP p) {
 // Measured at 256 x 256: a step of 64 k takes 1.7 to 1.8 us with all CUs busy, 1.2 PFLOP/s (a library product of
 // 8192^3 reaches 1.25 to 1.3: the chip's power bounds both; LDS reads have no bank conflicts and L2 serves the
 // loads at 24 bytes a clock and CU). A round's first loads and its epilogue, about 8 us, run under nothing, since a
-// tile takes a whole CU: that is a third of a round at 768 k. 16480 rows (1024, 2816) bf16: gate and up 244 us with the
-// activation and 279 MB written, dh 197 us with 372 MB read and written, dx 170 + 12 us, dw_in and dw_out 288 + 24 us,
-// the output projection 106 + 12 us.
+// tile takes a whole CU: that is a third of a round at 768 k. 16480 rows (1024, 2816) bf16: gate and up 220 us with the
+// activation and 325 MB written, dh 184 us with 418 MB read and written, dx 161 + 12 us, dw_in and dw_out 273 + 24 us,
+// the output projection 100 + 12 us.
 // A workgroup of WM x WN wavefronts owns a TM x TN tile and walks k in steps of 64 (whole 128-byte lines of
 // either layout), four k steps of 16 each; the operands of one are read from LDS while the one before is
 // multiplied. A has three LDS buffers and B two (all 160 KB at 256 x 256): before a step's last k step its

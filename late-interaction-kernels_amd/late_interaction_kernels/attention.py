@@ -151,7 +151,8 @@ def attention(
 
     Args:
         q: ``[n, Lq, H, d]`` fp16 / bf16, ``d`` at most 128 (a multiple of 8 in the
-            kernels; other sizes are padded in a copy). Any strides.
+            kernels; other sizes are padded in a copy). Any strides (rows off 16 bytes, or
+            tokens 2^24 elements apart, are copied).
         k, v: ``[n, Lk, Hk, d]``; ``H`` a multiple of ``Hk``.
         q_mask: ``[n, Lq]``, True = keep. Rows that it drops come out as zeros and
             give no gradient; whatever they hold is not used.

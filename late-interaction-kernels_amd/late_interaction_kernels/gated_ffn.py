@@ -105,7 +105,9 @@ def gated_ffn(
 
     Returns:
         ``[..., d]`` of the type of ``x``. ``d`` and ``hidden`` are multiples of 8 in the
-        kernels; other sizes are padded with zeros (a copy of the inputs per call).
+        kernels; other sizes are padded with zeros (a copy of the inputs per call). The
+        product of both projections is held in the type of ``x``: in fp16 it is infinite past
+        65504.
     """
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}; got {activation!r}")
