@@ -42,7 +42,16 @@ __device__ __forceinline__ void softmax_step(f32x16 (&s)[NU], f32x16 (&o)[DC], f
 #pragma unroll
     for (int d = 0; d < DC; ++d) o[d] *= alpha;
   }
-  const float mc = top == -INFINITY ? 0.f : fmaf(top, c, -kLift<EK>);
+  float mc = top == -INFINITY ? 0.f : fmaf(top, c, -kLift<EK>);
+  // A reference this large is spaced too widely to be taken off inside the exponent (by 2^5 at 3e9): off the scores first.
+  if (__ballot(fabsf(mc) > 1048576.0f) != 0) {
+    const float off = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[u][i] -= off;
+    mc = -kLift<EK>;
+  }
 #pragma unroll
   for (int u = 0; u < NU; ++u)
 #pragma unroll
