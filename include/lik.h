@@ -553,8 +553,8 @@ typedef struct {
 /*
  * out [n, q_len, heads, dim] (packed: [q_rows, heads, dim]), contiguous, in the
  * inputs' type. lse (optional) fp32 [heads, n * q_len] (packed: [heads, q_rows]): the
- * rows' softmax statistics for the backward pass (log2 of the sum of 2^(scale
- * log2(e) q k); +inf for a query that keeps no key). out_low (optional, out's shape):
+ * rows' softmax statistics for the backward pass (log of the sum of exp(scale
+ * q k), over scale; +inf for a query that keeps no key). out_low (optional, out's shape):
  * what the rounding took off out, for the backward pass. Packed rows that belong
  * to no sequence come out as zeros (the gradients' too).
  */

@@ -33,17 +33,17 @@ struct AttP {
   int64_t q_len, k_len, q_total;  // q_total: rows of the output per head
   int n, heads, group, dim;       // group: query heads of one key head
   int left, right;                // INT32_MAX: unbounded
-  float scale, c;                 // c = scale log2 e
+  float scale, c, inv_c;          // c = scale log2 e
   char* out;                      // [q_total][heads][dim]
   int8_t* low;                    // what the output's rounding took off, by element (below); null: not kept
-  float* lse;                     // [heads][q_total]: log2 of the sum of 2^(c q k); +inf where nothing is kept
+  float* lse;                     // [heads][q_total]: L with p = 2^(c (q k - L)), log2(sum 2^(c q k)) / c; +inf where nothing is kept
   float* delta;                   // [heads][q_total]: sum_d g o
   char *gq, *gk, *gv;             // contiguous gradients
   float* gmax;                    // fp16: [sequence][head][q tile]: largest |g|
   float* vmax;                    // fp16: [sequence][key head][k tile]: largest |v|
   int q_tiles, k_tiles;           // backward: tiles of 128 rows of a sequence
   float* part_o;                  // forward split over keys: [split][q_total][heads][dim] fp32
-  float* part_lse;                // [split][heads][q_total]
+  float* part_lse;                // [split][heads][q_total]: L of a split's keys; -inf where none is kept
   int splits, tiles;              // q tiles (k tiles) of a sequence
   bool few;                       // forward: attention_rows_kernel
   int chunk, wgs;                 // workgroups: `chunk` in a row go to one XCD; wgs of them have work

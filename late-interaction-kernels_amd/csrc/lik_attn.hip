@@ -24,9 +24,9 @@ constexpr float kLift = EK == EK_F16 ? 12.0f : 0.0f;
 // top, sum and the output so far follow the running maximum. The sum is that of the rounded probabilities, which are the
 // output's weights: whatever the values have in common comes out exact. (With the sum before the rounding the output was off
 // by the weights' missing share of it, and delta = g o against g v with it: gradients of q and k over values of 16 +- 1 were
-// 2 roundoffs off.)
-template <int EK, int DC, int NU>
-__device__ __forceinline__ void softmax_step(f32x16 (&s)[NU], f32x16 (&o)[DC], float& top, float& sum, float c,
+// 2 roundoffs off.) STAT: `whole` is the sum before the rounding, for the statistic that the gradients' probabilities come from.
+template <int EK, int DC, int NU, bool STAT>
+__device__ __forceinline__ void softmax_step(f32x16 (&s)[NU], f32x16 (&o)[DC], float& top, float& sum, float& whole, float c,
                                              u32x4 (&pf)[2 * NU]) {
   float m = s[0][0];
 #pragma unroll
@@ -39,12 +39,14 @@ __device__ __forceinline__ void softmax_step(f32x16 (&s)[NU], f32x16 (&o)[DC], f
     const float alpha = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((top - up) * c);
     top = up;
     sum *= alpha;
+    if constexpr (STAT) whole *= alpha;
 #pragma unroll
     for (int d = 0; d < DC; ++d) o[d] *= alpha;
   }
   float mc = top == -INFINITY ? 0.f : fmaf(top, c, -kLift<EK>);
-  // A reference this large is spaced too widely to be taken off inside the exponent (by 2^5 at 3e9): off the scores first.
-  if (__ballot(fabsf(mc) > 1048576.0f) != 0) {
+  // A large reference is spaced too widely to be taken off inside the exponent (2^11: by 2^-12; 3e9: by 2^8): off the
+  // scores first.
+  if (__ballot(fabsf(mc) > 2048.0f) != 0) {
     const float off = top == -INFINITY ? 0.f : top;
 #pragma unroll
     for (int u = 0; u < NU; ++u)
@@ -56,6 +58,14 @@ __device__ __forceinline__ void softmax_step(f32x16 (&s)[NU], f32x16 (&o)[DC], f
   for (int u = 0; u < NU; ++u)
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], c, -mc));
+  if constexpr (STAT) {
+    float add[2] = {};
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) add[i % 2] += s[u][i];
+    whole += add[0] + add[1];
+  }
   float add[2] = {};
 #pragma unroll
   for (int k = 0; k < 2 * NU; ++k)
@@ -88,10 +98,10 @@ __device__ __forceinline__ void store_part(const AttP& p, int split, int64_t row
 //   scores  S^T[key][query] = K Q^T   (K rows from LDS, Q in registers)
 //   output  O^T[d][query]  += V^T P^T (V by transposing LDS reads, P as it lies)
 // whole: every pair is kept; else the arguments of mask_scores.
-template <int EK, int DC>
+template <int EK, int DC, bool STAT>
 __device__ __forceinline__ void attend_tile(const Frags<DC>& frags, uint32_t kl, uint32_t vl,
                                             const u32x4 (&qf)[Dim<DC>::KS], f32x16 (&o)[DC], float& top, float& sum,
-                                            float c, bool whole, int kt, int klen, const uint32_t* bits, bool window,
+                                            float& stat, float c, bool whole, int kt, int klen, const uint32_t* bits, bool window,
                                             int first, uint32_t reach, int lane) {
   f32x16 s[2];
 #pragma unroll
@@ -105,7 +115,7 @@ __device__ __forceinline__ void attend_tile(const Frags<DC>& frags, uint32_t kl,
     for (int u = 0; u < 2; ++u) mask_scores(s[u], kt + u * 32, klen, bits, window, first + u * 32, reach, lane);
   }
   u32x4 pf[4];
-  softmax_step<EK, DC, 2>(s, o, top, sum, c, pf);
+  softmax_step<EK, DC, 2, STAT>(s, o, top, sum, stat, c, pf);
 #pragma unroll
   for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -113,13 +123,14 @@ __device__ __forceinline__ void attend_tile(const Frags<DC>& frags, uint32_t kl,
 }
 
 // A wavefront's finished queries to memory. on: the lane's row exists, q_on: its mask keeps it.
+// whole: the sum of the probabilities before their rounding (or sum again).
 template <int EK, int DC>
 __device__ __forceinline__ void store_rows(const AttP& p, int split, int64_t row, int head, f32x16 (&o)[DC], float top,
-                                           float sum, bool on, bool q_on, int lane) {
-  const float total = sum + swap_half(sum);
+                                           float sum, float whole, bool on, bool q_on, int lane) {
+  const float total = sum + swap_half(sum), stat = whole + swap_half(whole);
   const bool kept = q_on && total != 0.f;
   const float inv = kept ? 1.0f / total : 0.f;
-  const float lse = kept ? fmaf(top, p.c, __builtin_amdgcn_logf(total) - kLift<EK>) : INFINITY;
+  const float lse = kept ? fmaf(__builtin_amdgcn_logf(stat) - kLift<EK>, p.inv_c, top) : INFINITY;
   if (!kept)  // a masked row's sums hold what the values hold: not zero times that
 #pragma unroll
     for (int d = 0; d < DC; ++d) o[d] = f32x16{};
@@ -135,7 +146,7 @@ __device__ __forceinline__ void store_rows(const AttP& p, int split, int64_t row
 // A workgroup of four wavefronts owns 128 queries of one head, a wavefront 32 of them as MFMA columns, and
 // walks the keys that any of them keeps, 64 at a time, in two LDS buffers: the next tile is loaded while this one
 // is used.
-template <int EK, int DC>
+template <int EK, int DC, bool STAT>
 __global__ void __launch_bounds__(256, DC <= 2 ? 4 : 2) attention_kernel(const AttP p) {
   using D = Dim<DC>;
   __shared__ __attribute__((aligned(1024))) char s_tile[2][2 * D::TILE];
@@ -202,7 +213,7 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 4 : 2) attention_kernel(const A
 
   const Window win(p);
   f32x16 o[DC];
-  float top = -INFINITY, sum = 0.f;
+  float top = -INFINITY, sum = 0.f, stat = 0.f;
 #pragma unroll
   for (int d = 0; d < DC; ++d) o[d] = f32x16{};
   const int wq0 = q0 + wv * 32, wq1 = wq0 + 31;  // the wavefront's queries
@@ -215,11 +226,11 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 4 : 2) attention_kernel(const A
     const uint32_t at = buf ? lds[1] : lds[0];
     const bool whole = kt + 64 <= klen && !holes && (p.right == kNone || kt + 63 <= wq0 + p.right) &&
                        (p.left == kNone || kt >= wq1 - p.left);
-    attend_tile<EK, DC>(frags, at, at + D::TILE, qf, o, top, sum, p.c, whole, kt, klen, holes ? s_bits : nullptr, win.on,
+    attend_tile<EK, DC, STAT>(frags, at, at + D::TILE, qf, o, top, sum, stat, p.c, whole, kt, klen, holes ? s_bits : nullptr, win.on,
                         kt + 4 * (lane >> 5) - qpos + win.back, win.reach, lane);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load is in flight to LDS when the workgroup ends
-  store_rows<EK, DC>(p, split, qs.row + qpos, head, o, top, sum, qpos < qs.len, qon, lane);
+  store_rows<EK, DC>(p, split, qs.row + qpos, head, o, top, sum, STAT ? stat : sum, qpos < qs.len, qon, lane);
 }
 
 // Few queries over long keys: bound by reading K and V once, so every key head's queries (all heads of the
@@ -290,11 +301,11 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 2 : 1) attention_rows_kernel(co
   }
 
   f32x16 o[QB][DC];
-  float top[QB], sum[QB];
+  float top[QB], sum[QB], stat[QB];
 #pragma unroll
   for (int b = 0; b < QB; ++b) {
     top[b] = -INFINITY;
-    sum[b] = 0.f;
+    sum[b] = stat[b] = 0.f;
 #pragma unroll
     for (int d = 0; d < DC; ++d) o[b][d] = f32x16{};
   }
@@ -318,7 +329,7 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 2 : 1) attention_rows_kernel(co
     for (int b = 0; b < QB; ++b) {
       if (holes || kt + 32 > ke)
         mask_scores(s[b][0], kt - first, ke - first, holes ? s_bits : nullptr, false, 0, 0u, lane);
-      softmax_step<EK, DC, 1>(s[b], o[b], top[b], sum[b], p.c, pf[b]);
+      softmax_step<EK, DC, 1, true>(s[b], o[b], top[b], sum[b], stat[b], p.c, pf[b]);
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k)
@@ -335,18 +346,18 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 2 : 1) attention_rows_kernel(co
   }
 #pragma unroll
   for (int b = 0; b < QB; ++b) {
-    const float total = sum[b] + swap_half(sum[b]);
+    const float total = sum[b] + swap_half(sum[b]), whole = stat[b] + swap_half(stat[b]);
     const bool kept = row[b] >= 0 && total != 0.f;
     if (!kept)  // (as in store_rows)
 #pragma unroll
       for (int d = 0; d < DC; ++d) o[b][d] = f32x16{};
     if (on[b])
       store_part<DC>(p, split, qs.row + (row[b] < 0 ? -1 - row[b] : row[b]), head[b], o[b], kept ? 1.0f / total : 0.f,
-                     kept ? fmaf(top[b], p.c, __builtin_amdgcn_logf(total) - kLift<EK>) : -INFINITY, lane);
+                     kept ? fmaf(__builtin_amdgcn_logf(whole) - kLift<EK>, p.inv_c, top[b]) : -INFINITY, lane);
   }
 }
 
-// Joins the splits of a row: sum_s 2^(lse_s - lse) o_s. A wavefront a row and head: its lanes take the splits'
+// Joins the splits of a row: sum_s 2^(c (L_s - L)) o_s. A wavefront a row and head: its lanes take the splits'
 // statistics, then two elements each.
 template <int EK>
 __global__ void __launch_bounds__(256) attention_join_kernel(const AttP p) {
@@ -365,13 +376,13 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttP p) {
   float top = l;
 #pragma unroll
   for (int s = 1; s < 64; s <<= 1) top = max_nan(top, __shfl_xor(top, s));
-  const float w = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(l - top);
+  const float w = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((l - top) * p.c);
   float total = w;
 #pragma unroll
   for (int s = 1; s < 64; s <<= 1) total += __shfl_xor(total, s);
   const float inv = top == -INFINITY ? 0.f : 1.0f / total;
   if (p.lse && lane == 0)
-    p.lse[(int64_t)head * p.q_total + row] = top == -INFINITY ? INFINITY : top + __builtin_amdgcn_logf(total);
+    p.lse[(int64_t)head * p.q_total + row] = top == -INFINITY ? INFINITY : fmaf(__builtin_amdgcn_logf(total), p.inv_c, top);
   s_w[wv][lane] = w * inv;  // (a wavefront reads only what it wrote itself)
   __builtin_amdgcn_wave_barrier();
   const int e = 4 * (lane & 31);
@@ -446,7 +457,8 @@ int launch_forward(AttP p, hipStream_t s) {
     const int64_t per = (int64_t)p.tiles * p.splits;
     const unsigned grid = work_grid(p, per * p.n * p.heads, per * p.group);
     if (!grid) return LIK_ERR_UNSUPPORTED;
-    launch_kernel(attention_kernel<EK, DC>, dim3(grid), dim3(256), p.km ? mask_words(p.k_len) * 4 : 0u, s, p);
+    const auto kernel = p.lse || p.splits > 1 ? attention_kernel<EK, DC, true> : attention_kernel<EK, DC, false>;
+    launch_kernel(kernel, dim3(grid), dim3(256), p.km ? mask_words(p.k_len) * 4 : 0u, s, p);
   }
   if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
   if (p.splits > 1) {
@@ -528,6 +540,7 @@ bool attention_shape(const lik_attention_t* a, AttP& p, int& rc) {
   p.right = a->right < 0 || a->right >= (1 << 30) ? kNone : a->right;
   p.scale = a->scale;
   p.c = a->scale * 1.4426950408889634f;
+  p.inv_c = 1.0f / p.c;
   return true;
 }
 

@@ -25,6 +25,13 @@ template <int EK>
 constexpr float kLiftP = EK == EK_F16 ? 14.0f : 0.0f;
 template <int EK>
 constexpr float kUnliftP = EK == EK_F16 ? 1.0f / 16384 : 1.0f;
+// A pair's probability from its score and the query's L, 2^kLiftP times. L is taken off the score first, not inside the
+// exponent: c L past 2^11 or so is spaced too widely for that (scores of 1e5 gave gradients 1% off), and one more
+// instruction costs less than asking for it.
+template <int EK>
+__device__ __forceinline__ float pair_p(const AttP& p, float s, float l) {
+  return __builtin_amdgcn_exp2f(EK == EK_F16 ? fmaf(s - l, p.c, kLiftP<EK>) : (s - l) * p.c);
+}
 // gs from the largest |g| and |v| (1 where one is zero)
 __device__ __forceinline__ float scale_for(float g, float v, int dim) {
   const float bound = 2.0f * (float)dim * g * v;
@@ -214,7 +221,6 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p) {
   };
 
   const Window win(p);
-  const float lift = kLiftP<EK> - lse;
   f32x16 acc[DC];
 #pragma unroll
   for (int d = 0; d < DC; ++d) acc[d] = f32x16{};
@@ -244,7 +250,7 @@ __global__ void __launch_bounds__(256, 2) attention_dq_kernel(const AttP p) {
       u32x4 df[2];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(s[i], p.c, lift));
+        const float e = pair_p<EK>(p, s[i], lse);
         s[i] = e * (EK == EK_F16 ? (dp[i] - delta) * gs : dp[i] - delta);
       }
 #pragma unroll
@@ -286,7 +292,7 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 3 : 2) attention_dkv_kernel(con
   constexpr int QT = DC > 2 ? 32 : 64, TILE = D::PITCH * QT;
   __shared__ __attribute__((aligned(1024))) char s_tile[2][2 * TILE];
   __shared__ __attribute__((aligned(1024))) char s_v[VL ? 2 * D::TILE : 16];
-  __shared__ __attribute__((aligned(16))) float s_stat[2][2][QT];
+  __shared__ __attribute__((aligned(16))) float s_stat[2][2][QT];  // L and delta
   __shared__ int s_kept[2];
   __shared__ float s_big[4];
   extern __shared__ uint32_t s_bits[];
@@ -365,7 +371,7 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 3 : 2) attention_dkv_kernel(con
     qrows.issue(at, q0 + head * p.q.sh + qt * p.q.sl, qlen - qt, bits, wv, lane);
     grows.issue(at + TILE, g0 + head * p.g.sh + qt * p.g.sl, qlen - qt, bits, wv, lane);
   };
-  // threads 0..QT - 1: a query's statistic (+inf past the end: p = 0), QT..2 QT - 1: its delta; in LDS less p's lift
+  // threads 0..QT - 1: a query's L (+inf past the end: p = 0), QT..2 QT - 1: its delta
   auto stat = [&](int head, int qt) {
     float x = 0.f;
     if (tid < 2 * QT) {
@@ -374,9 +380,6 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 3 : 2) attention_dkv_kernel(con
       x = pos < qlen ? (tid < QT ? p.lse[at] : p.delta[at]) : tid < QT ? INFINITY : 0.f;
     }
     return x;
-  };
-  auto put_stat = [&](int buf, float x) {
-    if (tid < 2 * QT) s_stat[buf][tid / QT][tid % QT] = EK == EK_F16 && tid < QT ? x - kLiftP<EK> : x;
   };
 
   // a query keeps a key where 0 <= query - key + ahead <= reach
@@ -391,7 +394,7 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 3 : 2) attention_dkv_kernel(con
   if (total) {
     const float x = stat(head, qt);
     issue(lds[0], head, qt);
-    put_stat(0, x);
+    if (tid < 2 * QT) s_stat[0][tid / QT][tid % QT] = x;
   }
   int buf = 0;
   for (int it = 0; it < total; ++it, buf ^= 1) {
@@ -432,7 +435,7 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 3 : 2) attention_dkv_kernel(con
           float e[4], ds[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            e[i] = __builtin_amdgcn_exp2f(fmaf(s[q * 4 + i], p.c, -ls[i]));
+            e[i] = pair_p<EK>(p, s[q * 4 + i], ls[i]);
             const float x = dp[q * 4 + i] - dl[i];
             ds[i] = e[i] * (EK == EK_F16 ? x * gs : x);
           }
@@ -452,7 +455,7 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 3 : 2) attention_dkv_kernel(con
           }
       }
     }
-    if (it + 1 < total) put_stat(buf ^ 1, next);
+    if (it + 1 < total && tid < 2 * QT) s_stat[buf ^ 1][tid / QT][tid % QT] = next;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // V's loads where there was no step
   const int64_t at = ((ks.row + kpos) * kv_heads + kvh) * p.dim * 2;
@@ -475,7 +478,7 @@ __global__ void __launch_bounds__((KW + DC) * 64, (KW + DC + 3) / 4) attention_g
   __shared__ __attribute__((aligned(1024))) char s_k[KW * TILE];
   __shared__ __attribute__((aligned(1024))) char s_tile[3][2 * TILE];
   __shared__ __attribute__((aligned(1024))) char s_ds[2][KW * DS];  // [key][query], 16-byte chunks exchanged by (key / 4) % 4
-  __shared__ __attribute__((aligned(16))) float s_lse[kShortRows], s_delta[kShortRows];  // 32 a step
+  __shared__ __attribute__((aligned(16))) float s_lse[kShortRows], s_delta[kShortRows];  // L and delta, 32 a step
   __shared__ float s_big[2][KW + DC];  // |g|, |v|
   __shared__ int s_blocks, s_last;
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
@@ -533,7 +536,7 @@ __global__ void __launch_bounds__((KW + DC) * 64, (KW + DC + 3) / 4) attention_g
     load_cols<DC>(gf, on ? g0 + head * p.g.sh + pos * p.g.sl : nullptr, p.dim, lane);
     const float d = row_delta<EK, DC>(p, gf, row, on, big, lane);
     if (lane < 32) {
-      s_lse[it * 32 + l32] = lse - kLiftP<EK>;
+      s_lse[it * 32 + l32] = lse;
       s_delta[it * 32 + l32] = d;
     }
     if (__ballot(on) && lane == 0) atomicMax(&s_last, qt + 32);
@@ -615,7 +618,7 @@ __global__ void __launch_bounds__((KW + DC) * 64, (KW + DC + 3) / 4) attention_g
           float e[4], ds[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            e[i] = __builtin_amdgcn_exp2f(fmaf(s[q * 4 + i], p.c, -ls[i]));
+            e[i] = pair_p<EK>(p, s[q * 4 + i], ls[i]);
             const float x = dp[q * 4 + i] - dl[i];
             ds[i] = e[i] * (EK == EK_F16 ? x * gs : x);
           }
