@@ -6,10 +6,10 @@
 // those of k and v. Both compute the scores and g v again: seven products where
 // one kernel with the gradient of q in memory would take five, but no atomics (the
 // same bits every time) and no fp32 gradient of q to clear, add to and convert.
-// 16 causal sequences of 1030 rows, 16 heads over 4 of 128, bf16: 181 us (577 TFLOP/s of its three products) and
-// 233 us (597, four), two wavefronts a SIMD at 226 and 250 registers, bound by the chain from scores to
+// 16 causal sequences of 1030 rows, 16 heads over 4 of 128, bf16: 184 us (567 TFLOP/s of its three products) and
+// 237 us (587, four), two wavefronts a SIMD at 226 and 250 registers, bound by the chain from scores to
 // probabilities to products inside a wavefront. Sequences of 129 to 320 keys have one kernel for all three: 128 passages of 50 to 300
-// rows, 12 heads of 64: 154 us, the two 88 and 93.
+// rows, 12 heads of 64: 155 us, the two 88 and 93.
 // p and ds are rounded once to the 16-bit type, as the products' operands have to be. fp16 has no range for either: p is
 // held 2^14 times (2^-28 is still a normal number), and ds 2^14 gs times, gs the power of two that brings the bound
 // |g v - delta| <= 2 dim max|g| max|v| to 1 .. 2 (of a wavefront's queries; of a key head's): nothing passes 2^15, and the
@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(256, DC <= 2 ? 3 : 2) attention_dkv_kernel(con
 // ds goes through LDS to DC more wavefronts with a block of 32 head dims each: dq^T[d][query] = K^T ds^T of the step before, over all
 // keys at once. The queries' statistics come first, by all wavefronts (one wait for memory, and the rows are in L2 for the walk):
 // up to kShortRows of them, all heads of the group together.
-// 128 passages of 50 to 300 rows padded to 300, 12 heads of 64, bf16: 154 us, about 80 of them the reads and writes around the walk (65
+// 128 passages of 50 to 300 rows padded to 300, 12 heads of 64, bf16: 155 us, about 80 of them the reads and writes around the walk (65
 // at the copy rate; a workgroup of 12 wavefronts at 162 registers fills a CU, so its walk overlaps no other's loads), the rest the steps.
 constexpr int kShortRows = 2048;
 template <int EK, int DC, int KW>
