@@ -574,6 +574,63 @@ int lik_attention_backward(const lik_attention_t* a, const void* out, const floa
                            void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes, lik_stream_t stream);
 
 /*
+ * Rotary positions of q [.., heads, dim] and k [.., kv_heads, dim] (either null: not
+ * wanted), bf16 / fp16 / fp32, dim up to 1024. Of each head's first 2 * pairs elements
+ * the pairs (i, i + pairs), or (2 i, 2 i + 1) where interleaved is set, become
+ *   amplitude (a cos t - b sin t, b cos t + a sin t),  t = position * frequencies[i],
+ * with -t where inverse is set (the gradients); the other elements are copied.
+ * padded: row l of sequence i and head h at data + i*stride_n + l*stride_l + h*stride_h;
+ * packed (cu_seqlens [n + 1]): row l at l*stride_l, len rows; rows outside
+ *   cu_seqlens[0] .. cu_seqlens[n] come out as zeros.
+ * positions (32- or 64-bit integers, with strides; not with cu_seqlens): null counts from
+ * offset at each sequence's start. frequencies [pairs] are 32- or 64-bit floats; the angle
+ * is computed and reduced in 64 bits. q_out and k_out are contiguous.
+ */
+typedef struct {
+  const void* q;
+  const void* k;
+  int32_t dtype;
+  int32_t heads;
+  int32_t kv_heads;
+  int32_t dim;
+  int64_t n;
+  int64_t len;
+  int64_t q_stride_n;
+  int64_t q_stride_l;
+  int64_t q_stride_h;
+  int64_t k_stride_n;
+  int64_t k_stride_l;
+  int64_t k_stride_h;
+  const int32_t* cu_seqlens;
+  const void* positions;
+  int64_t position_stride_n;
+  int64_t position_stride_l;
+  int64_t offset;
+  const void* frequencies;
+  int32_t position_bits;
+  int32_t frequency_bits;
+  int32_t pairs;
+  int32_t interleaved;
+  int32_t inverse;
+  float amplitude;
+} lik_rotary_t;
+
+int lik_rotary(const lik_rotary_t* a, void* q_out, void* k_out, lik_stream_t stream);
+
+/*
+ * Rows of x [rows, dim] (bf16 / fp16 / fp32) as 8-bit integers with a scale each:
+ *   scale = max(fp32(max|x| / 127), 2^-126),  out = x / scale to the nearest integer, ties to even
+ * (the rounding is that of the exact quotient). A row that holds an infinity or a NaN has the
+ * scale NaN and zeros. out rows are out_stride bytes apart; bytes from dim to the next
+ * multiple of 16 are written as zeros as far as out_stride has them.
+ */
+int lik_quantize_int8(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int32_t dim, int8_t* out,
+                      int64_t out_stride, float* scale, lik_stream_t stream);
+/* And back: out [rows, dim], contiguous, of dtype = x * scale, rounded once. */
+int lik_dequantize_int8(const int8_t* x, int64_t x_stride, const float* scale, int32_t dtype, int64_t rows, int32_t dim,
+                        void* out, lik_stream_t stream);
+
+/*
  * Allocation-free scoring. No counterpart in the reference: this entry point
  * is for callers that cannot allocate device memory (code under HIP graph
  * capture, tight serving loops, harnesses that forbid hipMalloc). It scores

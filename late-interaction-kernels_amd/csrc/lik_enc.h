@@ -48,6 +48,58 @@ __device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b) {
   }
 }
 
+// A 16-byte chunk of V elements from element e of a row; those past `end` are not touched (and load as zeros).
+// Rows may start on any element: the 16-byte access is left to the hardware.
+template <int EK>
+__device__ __forceinline__ void chunk_load(const char* row, int e, int end, u32x4& w) {
+  constexpr int V = El<EK>::V, B = El<EK>::B;
+  typedef u32x4 __attribute__((aligned(2))) u32x4_u;
+  if (e + V <= end) {
+    w = *(const u32x4_u*)(row + (int64_t)e * B);
+    return;
+  }
+  w = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (e + i < end) {
+      if constexpr (EK == EK_F32) w[i] = ((const uint32_t*)row)[e + i];
+      else w[i / 2] |= (uint32_t)((const uint16_t*)row)[e + i] << (i % 2 * 16);
+    }
+}
+template <int EK>
+__device__ __forceinline__ void chunk_store(char* row, int e, int end, const u32x4& w) {
+  constexpr int V = El<EK>::V, B = El<EK>::B;
+  typedef u32x4 __attribute__((aligned(2))) u32x4_u;
+  if (e + V <= end) {
+    *(u32x4_u*)(row + (int64_t)e * B) = w;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (e + i < end) {
+      if constexpr (EK == EK_F32) ((uint32_t*)row)[e + i] = w[i];
+      else ((uint16_t*)row)[e + i] = (uint16_t)(w[i / 2] >> (i % 2 * 16));
+    }
+}
+template <int EK>
+__device__ __forceinline__ void chunk_widen(const u32x4& w, float* v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (EK == EK_F32) v[i] = __uint_as_float(w[i]);
+    else unpack2<EK>(w[i], v[2 * i], v[2 * i + 1]);
+  }
+}
+template <int EK>
+__device__ __forceinline__ u32x4 chunk_narrow(const float* v) {
+  u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (EK == EK_F32) w[i] = __float_as_uint(v[i]);
+    else w[i] = pack2<EK>(v[2 * i], v[2 * i + 1]);
+  }
+  return w;
+}
+
 // c plus f times the two packed elements, in fp32 (one instruction, rounded once; subnormals are kept)
 template <int EK>
 __device__ __forceinline__ float add2(uint32_t w, float c, float f = 1.0f) {

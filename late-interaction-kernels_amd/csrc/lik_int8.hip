@@ -1,0 +1,219 @@
+// Token vectors as 8-bit integers with a scale each, and back (the definition: lik_int8.h).
+//
+// Bound by HBM: a row stays in the registers of its lanes between the maximum and the conversion, so each
+// element is read once and one byte written; rows past 4096 elements (fp32: 2048) are read twice, the second
+// time from L2.
+#include "lik_int8.h"
+
+namespace lik {
+namespace enc {
+namespace {
+
+struct QuantP {
+  const char* x;
+  int64_t x_ld;  // bytes
+  int64_t rows;
+  int dim, end;  // end: bytes of a row that are written
+  int8_t* out;
+  int64_t out_ld;
+  float* scale;
+};
+
+template <int V>
+__device__ __forceinline__ void store_int8(int8_t* row, int e, int end, const uint32_t* w) {
+  typedef uint32_t __attribute__((aligned(1))) u32_u;
+  typedef u32x2 __attribute__((aligned(1))) u32x2_u;
+  if (e + V <= end) {
+    if constexpr (V == 8) *(u32x2_u*)(row + e) = u32x2{w[0], w[1]};
+    else *(u32_u*)(row + e) = w[0];
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (e + i < end) row[e + i] = (int8_t)(w[i / 4] >> (i % 4 * 8));
+}
+
+// LPR lanes a row with NV chunks each in registers, U rows at once.
+template <int EK, int LPR, int NV, int U>
+__global__ void __launch_bounds__(256) quantize_kernel(const QuantP p) {
+  constexpr int V = El<EK>::V, RPW = 64 / LPR;
+  const int lane = threadIdx.x % LPR, g = threadIdx.x % 64 / LPR;
+  const int64_t first = (threadIdx.x / 64) * (RPW * U) + g, step = (int64_t)gridDim.x * (4 * RPW * U);
+  for (int64_t b = (int64_t)blockIdx.x * (4 * RPW * U); b < p.rows; b += step) {
+    const int64_t r0 = b + first;
+    u32x4 w[U][NV];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        w[u][j] = u32x4{0u, 0u, 0u, 0u};
+        if (r0 + u * RPW < p.rows) chunk_load<EK>(p.x + (r0 + u * RPW) * p.x_ld, (j * LPR + lane) * V, p.dim, w[u][j]);
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) m = absmax_bits<EK>(w[u][j], m);
+#pragma unroll
+      for (int o = LPR / 2; o >= 1; o >>= 1) m = absmax_join<EK>(m, (uint32_t)__shfl_xor((int)m, o));
+      float s, inv;
+      row_scale<EK>(m, s, inv);
+      const int64_t r = r0 + u * RPW;
+      if (r >= p.rows) continue;
+      if (lane == 0) p.scale[r] = s;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        uint32_t q[V / 4];
+        chunk_to_int8<EK>(w[u][j], s, inv, q);
+        store_int8<V>(p.out + r * p.out_ld, (j * LPR + lane) * V, p.end, q);
+      }
+    }
+  }
+}
+
+// Wider rows: a workgroup each, read twice.
+template <int EK>
+__global__ void __launch_bounds__(256) quantize_wide_kernel(const QuantP p) {
+  constexpr int V = El<EK>::V;
+  __shared__ uint32_t s_m[4];
+  for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+    const char* row = p.x + r * p.x_ld;
+    u32x4 w;
+    uint32_t m = 0;
+    for (int e = threadIdx.x * V; e < p.dim; e += 256 * V) {
+      chunk_load<EK>(row, e, p.dim, w);
+      m = absmax_bits<EK>(w, m);
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) m = absmax_join<EK>(m, (uint32_t)__shfl_xor((int)m, o));
+    if (threadIdx.x % 64 == 0) s_m[threadIdx.x / 64] = m;
+    __syncthreads();
+    m = absmax_join<EK>(absmax_join<EK>(s_m[0], s_m[1]), absmax_join<EK>(s_m[2], s_m[3]));
+    float s, inv;
+    row_scale<EK>(m, s, inv);
+    if (threadIdx.x == 0) p.scale[r] = s;
+    for (int e = threadIdx.x * V; e < p.end; e += 256 * V) {
+      uint32_t q[V / 4];
+      chunk_load<EK>(row, e, p.dim, w);
+      chunk_to_int8<EK>(w, s, inv, q);
+      store_int8<V>(p.out + r * p.out_ld, e, p.end, q);
+    }
+    __syncthreads();  // (s_m is the next row's)
+  }
+}
+
+// (a launch has less than 2^32 threads)
+unsigned groups(int64_t want) { return (unsigned)(want < (1 << 22) ? want : 1 << 22); }
+template <int EK, int LPR, int NV, int U>
+void launch_rows(const QuantP& p, hipStream_t s) {
+  const int64_t per = 4 * (64 / LPR) * U;
+  launch_kernel(quantize_kernel<EK, LPR, NV, U>, dim3(groups((p.rows + per - 1) / per)), dim3(256), 0u, s, p);
+}
+template <int EK>
+int launch_quantize(const QuantP& p, hipStream_t s) {
+  const int ch = (p.end + El<EK>::V - 1) / El<EK>::V;
+  if (ch <= 16) launch_rows<EK, 16, 1, 4>(p, s);
+  else if (ch <= 32) launch_rows<EK, 16, 2, 2>(p, s);
+  else if (ch <= 64) launch_rows<EK, 16, 4, 1>(p, s);
+  else if (ch <= 128) launch_rows<EK, 64, 2, 2>(p, s);
+  else if (ch <= 192) launch_rows<EK, 64, 3, 1>(p, s);
+  else if (ch <= 256) launch_rows<EK, 64, 4, 1>(p, s);
+  else if (ch <= 384) launch_rows<EK, 64, 6, 1>(p, s);
+  else if (ch <= 512) launch_rows<EK, 64, 8, 1>(p, s);
+  else launch_kernel(quantize_wide_kernel<EK>, dim3(groups(p.rows)), dim3(256), 0u, s, p);
+  return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;
+}
+
+struct DequantP {
+  const int8_t* x;
+  int64_t x_ld, rows;
+  const float* scale;
+  int dim;
+  char* out;
+};
+
+// A thread takes 16 elements of a row.
+template <int EK>
+__global__ void __launch_bounds__(256) dequantize_kernel(const DequantP p) {
+  constexpr int B = El<EK>::B, V = El<EK>::V;
+  typedef u32x4 __attribute__((aligned(1))) u32x4_u;
+  const int chunks = (p.dim + 15) / 16;
+  const int64_t all = p.rows * chunks, step = (int64_t)gridDim.x * 256;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += step) {
+    const int64_t r = i / chunks;
+    const int e = (int)(i - r * chunks) * 16;
+    const int8_t* in = p.x + r * p.x_ld;
+    const float s = p.scale[r];
+    u32x4 w = {0u, 0u, 0u, 0u};
+    if (e + 16 <= p.dim) w = *(const u32x4_u*)(in + e);
+    else
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        if (e + k < p.dim) w[k / 4] |= (uint32_t)(uint8_t)in[e + k] << (k % 4 * 8);
+    char* out = p.out + r * ((int64_t)p.dim * B);
+#pragma unroll
+    for (int c = 0; c < 16 / V; ++c) {
+      float v[V];
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k] = s * (float)(int8_t)(w[(c * V + k) / 4] >> ((c * V + k) % 4 * 8));
+      if (e + c * V < p.dim) chunk_store<EK>(out, e + c * V, p.dim, chunk_narrow<EK>(v));
+    }
+  }
+}
+template <int EK>
+int launch_dequantize(const DequantP& p, hipStream_t s) {
+  const int64_t all = p.rows * ((p.dim + 15) / 16);
+  launch_kernel(dequantize_kernel<EK>, dim3(groups((all + 255) / 256)), dim3(256), 0u, s, p);
+  return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;
+}
+
+int rows_check(int32_t dtype, int64_t rows, int32_t dim) {
+  if (dtype != LIK_BF16 && dtype != LIK_F16 && dtype != LIK_F32) return LIK_ERR_UNSUPPORTED;
+  if (rows < 0 || dim < 1) return LIK_ERR_INVALID;
+  if (dim > (1 << 24) || rows > (1ll << 40)) return LIK_ERR_UNSUPPORTED;
+  return LIK_OK;
+}
+
+}  // namespace
+}  // namespace enc
+}  // namespace lik
+
+using namespace lik;
+using namespace lik::enc;
+
+extern "C" {
+
+int lik_quantize_int8(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int32_t dim, int8_t* out,
+                      int64_t out_stride, float* scale, lik_stream_t stream) {
+  if (const int rc = rows_check(dtype, rows, dim)) return rc;
+  if (rows == 0) return LIK_OK;
+  if (!x || !out || !scale || out_stride < dim) return LIK_ERR_INVALID;
+  const int eb = dtype == LIK_F32 ? 4 : 2;
+  if ((uintptr_t)x % eb || (uintptr_t)scale % 4) return LIK_ERR_UNSUPPORTED;
+  const int64_t end = (dim + 15) / 16 * 16;
+  const QuantP p{(const char*)x, x_stride * eb, rows, dim, (int)(end < out_stride ? end : out_stride), out, out_stride,
+                 scale};
+  hipStream_t s = (hipStream_t)stream;
+  switch (dtype) {
+    case LIK_BF16: return launch_quantize<EK_BF16>(p, s);
+    case LIK_F16: return launch_quantize<EK_F16>(p, s);
+    default: return launch_quantize<EK_F32>(p, s);
+  }
+}
+
+int lik_dequantize_int8(const int8_t* x, int64_t x_stride, const float* scale, int32_t dtype, int64_t rows, int32_t dim,
+                        void* out, lik_stream_t stream) {
+  if (const int rc = rows_check(dtype, rows, dim)) return rc;
+  if (rows == 0) return LIK_OK;
+  if (!x || !out || !scale) return LIK_ERR_INVALID;
+  if ((uintptr_t)out % (dtype == LIK_F32 ? 4 : 2) || (uintptr_t)scale % 4) return LIK_ERR_UNSUPPORTED;
+  const DequantP p{x, x_stride, rows, scale, dim, (char*)out};
+  hipStream_t s = (hipStream_t)stream;
+  switch (dtype) {
+    case LIK_BF16: return launch_dequantize<EK_BF16>(p, s);
+    case LIK_F16: return launch_dequantize<EK_F16>(p, s);
+    default: return launch_dequantize<EK_F32>(p, s);
+  }
+}
+
+}  // extern "C"

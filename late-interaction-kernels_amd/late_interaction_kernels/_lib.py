@@ -92,6 +92,9 @@ EXPORTED_SYMBOLS = (
     "lik_attention_workspace_size",
     "lik_attention_backward",
     "lik_attention_backward_workspace_size",
+    "lik_rotary",
+    "lik_quantize_int8",
+    "lik_dequantize_int8",
 )
 
 _p = ctypes.c_void_p
@@ -180,6 +183,39 @@ class LikAttention(ctypes.Structure):
         ("left", _i32),
         ("right", _i32),
         ("scale", ctypes.c_float),
+    ]
+
+
+class LikRotary(ctypes.Structure):
+    """Mirror of ``lik_rotary_t``."""
+
+    _fields_ = [
+        ("q", _p),
+        ("k", _p),
+        ("dtype", _i32),
+        ("heads", _i32),
+        ("kv_heads", _i32),
+        ("dim", _i32),
+        ("n", _i64),
+        ("len", _i64),
+        ("q_stride_n", _i64),
+        ("q_stride_l", _i64),
+        ("q_stride_h", _i64),
+        ("k_stride_n", _i64),
+        ("k_stride_l", _i64),
+        ("k_stride_h", _i64),
+        ("cu_seqlens", _p),
+        ("positions", _p),
+        ("position_stride_n", _i64),
+        ("position_stride_l", _i64),
+        ("offset", _i64),
+        ("frequencies", _p),
+        ("position_bits", _i32),
+        ("frequency_bits", _i32),
+        ("pairs", _i32),
+        ("interleaved", _i32),
+        ("inverse", _i32),
+        ("amplitude", ctypes.c_float),
     ]
 
 
@@ -321,6 +357,12 @@ def load() -> ctypes.CDLL:
     lib.lik_attention_backward.argtypes = [P(LikAttention), _p, _p, _p, _p, _i64, _i64, _i64, _p, _p, _p, _p,
                                            ctypes.c_size_t, _p]
     lib.lik_attention_backward.restype = ctypes.c_int
+    lib.lik_rotary.argtypes = [P(LikRotary), _p, _p, _p]
+    lib.lik_rotary.restype = ctypes.c_int
+    lib.lik_quantize_int8.argtypes = [_p, _i64, _i32, _i64, _i32, _p, _i64, _p, _p]
+    lib.lik_quantize_int8.restype = ctypes.c_int
+    lib.lik_dequantize_int8.argtypes = [_p, _i64, _p, _i32, _i64, _i32, _p, _p]
+    lib.lik_dequantize_int8.restype = ctypes.c_int
     _lib = lib
     return lib
 

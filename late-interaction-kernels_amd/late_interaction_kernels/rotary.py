@@ -1,0 +1,231 @@
+"""``rotary``: rotary positions of queries and keys, padded, packed or at given
+positions, differentiable; ``rotary_frequencies``: the frequencies it takes.
+
+Pair i of a head is turned by ``position * frequencies[i]``. The angle is computed
+and reduced in 64 bits (far positions keep their phase), the rotation is fp32 and
+rounded once. The gradient is the rotation the other way; being linear it can be
+differentiated again.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from ._core import _i32
+
+_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def rotary_frequencies(
+    dim: int,
+    base: float = 10000.0,
+    *,
+    scaling: str | None = None,
+    factor: float = 1.0,
+    original_length: int | None = None,
+    low: float | None = None,
+    high: float | None = None,
+    device: torch.device | str | None = None,
+) -> tuple[torch.Tensor, float]:
+    """Frequencies of ``dim`` rotated elements and the amplitude that goes with them.
+
+    ``f_i = base ** (-2 i / dim)``, in radians a position, ``i < dim / 2``. ``scaling``
+    adapts them to contexts ``factor`` times as long as the ``original_length`` a model was trained on:
+
+    - ``"linear"``: ``f_i / factor``.
+    - ``"ntk"``: the base times ``factor ** (dim / (dim - 2))``, so that the lowest frequency
+      is divided by ``factor`` and the highest is kept.
+    - ``"bands"``: by the turns ``original_length * f_i / (2 pi)`` of a pair over the original
+      length: at most ``low`` (default 1) turns ``f_i / factor``, at least ``high`` (default 4) ``f_i``, between
+      them a blend that is linear in the turns.
+    - ``"yarn"`` (Peng et al., "YaRN: Efficient context window extension of large language
+      models", 2023): the blend is linear in the pair's index, between the pairs that turn
+      ``high`` (default 32, rounded down) and ``low`` (default 1, rounded up) times; the amplitude is
+      ``0.1 ln factor + 1``.
+
+    Returns:
+        ``(frequencies, amplitude)``: fp64 ``[dim / 2]`` on ``device``, and 1.0 except for "yarn".
+    """
+    if dim < 2 or dim % 2:
+        raise ValueError(f"dim must be even and at least 2; got {dim}")
+    if not (base > 0 and math.isfinite(base)):
+        raise ValueError(f"base must be positive and finite; got {base}")
+    if not (factor >= 1 and math.isfinite(factor)):
+        raise ValueError(f"factor must be finite and at least 1; got {factor}")
+    if scaling not in (None, "linear", "ntk", "bands", "yarn"):
+        raise ValueError(f"scaling must be None, 'linear', 'ntk', 'bands' or 'yarn'; got {scaling!r}")
+    if scaling is None and factor != 1:
+        raise ValueError("factor needs a scaling")
+    i = torch.arange(dim // 2, dtype=torch.float64)
+    amplitude = 1.0
+    if scaling == "ntk":
+        if dim < 4:
+            raise ValueError("'ntk' needs a dim of at least 4")
+        base = base * factor ** (dim / (dim - 2))
+    f = base ** (-2.0 * i / dim)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling in ("bands", "yarn"):
+        if original_length is None or original_length < 1:
+            raise ValueError(f"{scaling!r} needs the original_length; got {original_length}")
+        low = 1.0 if low is None else float(low)
+        high = (4.0 if scaling == "bands" else 32.0) if high is None else float(high)
+        if not 0 < low < high:
+            raise ValueError(f"low and high must be 0 < low < high; got {low} and {high}")
+        if scaling == "bands":
+            keep = ((original_length * f / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+        else:
+            if base <= 1:
+                raise ValueError(f"'yarn' needs a base above 1; got {base}")
+
+            def pair(turns):  # the (fractional) pair that turns so many times over the original length
+                return dim * math.log(original_length / (2 * math.pi * turns)) / (2 * math.log(base))
+
+            first, last = max(math.floor(pair(high)), 0), min(math.ceil(pair(low)), dim - 1)
+            keep = 1 - ((i - first) / max(last - first, 0.001)).clamp(0, 1)
+            amplitude = 0.1 * math.log(factor) + 1
+        f = f * keep + f / factor * (1 - keep)
+    return f.to(device), amplitude
+
+
+def _launch(q, k, frequencies, positions, cu, meta):
+    """``(q', k')`` of the tensors that are not None."""
+    offset, interleaved, amplitude, inverse = meta
+    x = q if q is not None else k
+    outs = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
+    if x.numel() == 0 and (k is None or k.numel() == 0):
+        return tuple(outs)
+
+    def strides(t):
+        if t is None:
+            return 0, 0, 0
+        s = t.stride()
+        return (0, s[0], s[1]) if t.dim() == 3 else s[:3]
+
+    if x.dim() == 3:
+        n, length = (1, x.shape[0]) if cu is None else (cu.numel() - 1, x.shape[0])
+    else:
+        n, length = x.shape[:2]
+    pn = pl = 0
+    if positions is not None:
+        pn, pl = positions.stride() if positions.dim() == 2 else (0, positions.stride(0))
+    a = _lib.LikRotary(
+        _lib.ptr(q), _lib.ptr(k), _lib.DTYPE_CODE[x.dtype], 0 if q is None else q.shape[-2],
+        0 if k is None else k.shape[-2], x.shape[-1], n, length, *strides(q), *strides(k), _lib.ptr(cu),
+        _lib.ptr(positions), pn, pl, offset, frequencies.data_ptr(),
+        0 if positions is None else 8 * positions.element_size(), 8 * frequencies.element_size(), frequencies.numel(),
+        int(interleaved), int(inverse), amplitude)
+    with _lib.on_device(x.device):
+        rc = _lib.load().lik_rotary(ctypes.byref(a), _lib.ptr(outs[0]), _lib.ptr(outs[1]), _lib.stream_of(x))
+    _lib.check(rc, "lik_rotary")
+    return tuple(outs)
+
+
+def _unit(t):
+    """``t`` with a contiguous last dim."""
+    return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+class _RotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, frequencies, positions, cu, meta):
+        ctx.save_for_backward(frequencies, positions, cu)
+        ctx.meta = meta
+        ctx.set_materialize_grads(False)
+        return _launch(_unit(q), _unit(k), frequencies, positions, cu, meta)
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        offset, interleaved, amplitude, inverse = ctx.meta
+        gq, gk = (g if need else None for g, need in zip((gq, gk), ctx.needs_input_grad))
+        if gq is not None or gk is not None:
+            gq, gk = _RotaryFn.apply(gq, gk, *ctx.saved_tensors, (offset, interleaved, amplitude, not inverse))
+        return gq, gk, None, None, None, None
+
+
+def rotary(
+    q: torch.Tensor,
+    k: torch.Tensor | None = None,
+    *,
+    frequencies: torch.Tensor,
+    positions: torch.Tensor | None = None,
+    cu_seqlens: torch.Tensor | None = None,
+    offset: int = 0,
+    interleaved: bool = False,
+    amplitude: float = 1.0,
+) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """Rotary positions of ``q`` and (in the same launch) ``k``, in front of :func:`attention.attention`.
+
+    Args:
+        q: ``[n, L, H, d]`` or packed ``[T, H, d]``, fp16 / bf16 / fp32, ``d`` at most 1024, any strides.
+        k: the same with heads of its own number, or None.
+        frequencies: ``[r / 2]`` fp32 / fp64, radians a position (:func:`rotary_frequencies`);
+            the first ``r`` elements of each head are turned, the others are copied.
+        positions: int32 / int64 ``[n, L]`` or ``[L]`` (packed: ``[T]``); None counts from
+            ``offset`` at the start of each sequence.
+        cu_seqlens: ``[s + 1]`` int32 cumulative offsets of packed sequences, where positions are
+            counted. Rows outside ``cu[0] .. cu[-1]`` come out as zeros and get no gradient.
+        interleaved: pairs are elements ``(2 i, 2 i + 1)`` instead of ``(i, i + r / 2)``.
+        amplitude: of the turned elements.
+
+    Returns:
+        ``q'`` of the shape and type of ``q``, or ``(q', k')``; contiguous.
+    """
+    if q.dim() not in (3, 4):
+        raise ValueError(f"q must be [n, L, heads, d] or packed [tokens, heads, d]; got {tuple(q.shape)}")
+    if q.dtype not in _DTYPES:
+        raise TypeError(f"rotary takes fp16 / bf16 / fp32; got {q.dtype}")
+    d = q.shape[-1]
+    if k is not None:
+        if k.dtype != q.dtype:
+            raise TypeError(f"q and k must have one type; got {q.dtype} and {k.dtype}")
+        if k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != d:
+            raise ValueError(f"k must match q ({tuple(q.shape)}) but in its heads; got {tuple(k.shape)}")
+    if not 2 <= d <= 1024:
+        raise ValueError(f"rotary takes head dims of 2 to 1024; got {d}")
+    if frequencies.dim() != 1 or not 1 <= frequencies.numel() <= d // 2:
+        raise ValueError(f"frequencies must be [r / 2] with 2 <= r <= {d}; got {tuple(frequencies.shape)}")
+    if frequencies.dtype not in (torch.float32, torch.float64):
+        raise TypeError(f"frequencies must be fp32 or fp64; got {frequencies.dtype}")
+    if frequencies.requires_grad and torch.is_grad_enabled():
+        raise ValueError("rotary gives no gradient to its frequencies; pass frequencies.detach()")
+    if max(q.shape[-2], 0 if k is None else k.shape[-2]) > 65536:
+        raise ValueError("rotary takes at most 65536 heads")
+    if positions is not None:
+        if cu_seqlens is not None or offset != 0:
+            raise ValueError("positions say everything: give them without cu_seqlens and offset")
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"positions must be int32 or int64; got {positions.dtype}")
+        if tuple(positions.shape) not in ({q.shape[:1]} if q.dim() == 3 else {q.shape[:2], q.shape[1:2]}):
+            raise ValueError(f"positions must be {list(q.shape[:-2])}{' or [L]' if q.dim() == 4 else ''}; got "
+                             f"{tuple(positions.shape)}")
+    if cu_seqlens is not None:
+        if q.dim() != 3:
+            raise ValueError("cu_seqlens go with packed [tokens, heads, d]")
+        if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"cu_seqlens must be [s + 1] cumulative offsets; got {tuple(cu_seqlens.shape)} "
+                             f"{cu_seqlens.dtype}")
+    elif q.dim() == 3 and positions is None:
+        raise ValueError("packed rows need cu_seqlens or positions")
+    if not isinstance(offset, int) or isinstance(offset, bool) or abs(offset) > 2**31:
+        raise ValueError(f"offset must be an int of at most 2^31; got {offset!r}")
+    amplitude = float(amplitude)
+    if not math.isfinite(amplitude):
+        raise ValueError(f"amplitude must be finite; got {amplitude}")
+    if any(t is not None and t.device != q.device for t in (k, frequencies, positions, cu_seqlens)):
+        raise ValueError("q, k, frequencies, positions and cu_seqlens must be on the same device.")
+    _lib.require_gpu(q)
+    frequencies, cu = frequencies.detach().contiguous(), _i32(cu_seqlens)
+    meta = (offset, bool(interleaved), amplitude, False)
+    if _lib.differentiates(q, k):
+        out = _RotaryFn.apply(q, k, frequencies, positions, cu, meta)
+    else:
+        out = _launch(_unit(q), _unit(k), frequencies, positions, cu, meta)
+    return out[0] if k is None else out
+
+
+__all__ = ["rotary", "rotary_frequencies"]
