@@ -631,6 +631,42 @@ int lik_dequantize_int8(const int8_t* x, int64_t x_stride, const float* scale, i
                         void* out, lik_stream_t stream);
 
 /*
+ * Linear layer on 8-bit integers, with v = x_scale weight_scale (x weight^T) + bias:
+ *   out [rows, out_features] = act(v) + residual, or where gated is set act(v_gate) v_up + residual
+ * x [rows, in]: of bf16 / fp16 / fp32, quantised within the call as lik_quantize_int8 does, or (LIK_INT8)
+ * integers with x_scale [rows], in a multiple of 16 and every row on 16 bytes. weight
+ * [out_features, in] (gated: [2 out_features, in], the gate's rows, then the up rows) with
+ * weight_scale and bias (null: none; of out_dtype or fp32) of as many elements; its rows start on 16 bytes and
+ * are readable to the next multiple of 16 (what is there does not matter). activation -1: none,
+ * else as in lik_gated_ffn. residual (null: none) is of out_dtype. Sums are exact
+ * integers (in <= 131071); out is contiguous, of bf16 / fp16 / fp32, rounded once.
+ */
+#define LIK_INT8 4
+typedef struct {
+  const void* x;
+  const float* x_scale;
+  const int8_t* weight;
+  const float* weight_scale;
+  const void* bias;
+  const void* residual;
+  int64_t x_stride;
+  int64_t weight_stride;
+  int64_t residual_stride;
+  int64_t rows;
+  int32_t in;
+  int32_t out_features;
+  int32_t x_dtype;
+  int32_t out_dtype;
+  int32_t bias_dtype;
+  int32_t activation;
+  int32_t gated;
+} lik_linear_int8_t;
+
+size_t lik_linear_int8_workspace_size(const lik_linear_int8_t* a);
+int lik_linear_int8(const lik_linear_int8_t* a, void* out, void* workspace, size_t workspace_bytes,
+                    lik_stream_t stream);
+
+/*
  * Allocation-free scoring. No counterpart in the reference: this entry point
  * is for callers that cannot allocate device memory (code under HIP graph
  * capture, tight serving loops, harnesses that forbid hipMalloc). It scores

@@ -95,6 +95,8 @@ EXPORTED_SYMBOLS = (
     "lik_rotary",
     "lik_quantize_int8",
     "lik_dequantize_int8",
+    "lik_linear_int8",
+    "lik_linear_int8_workspace_size",
 )
 
 _p = ctypes.c_void_p
@@ -216,6 +218,30 @@ class LikRotary(ctypes.Structure):
         ("interleaved", _i32),
         ("inverse", _i32),
         ("amplitude", ctypes.c_float),
+    ]
+
+
+class LikLinearInt8(ctypes.Structure):
+    """Mirror of ``lik_linear_int8_t``."""
+
+    _fields_ = [
+        ("x", _p),
+        ("x_scale", _p),
+        ("weight", _p),
+        ("weight_scale", _p),
+        ("bias", _p),
+        ("residual", _p),
+        ("x_stride", _i64),
+        ("weight_stride", _i64),
+        ("residual_stride", _i64),
+        ("rows", _i64),
+        ("in_features", _i32),
+        ("out_features", _i32),
+        ("x_dtype", _i32),
+        ("out_dtype", _i32),
+        ("bias_dtype", _i32),
+        ("activation", _i32),
+        ("gated", _i32),
     ]
 
 
@@ -363,6 +389,10 @@ def load() -> ctypes.CDLL:
     lib.lik_quantize_int8.restype = ctypes.c_int
     lib.lik_dequantize_int8.argtypes = [_p, _i64, _p, _i32, _i64, _i32, _p, _p]
     lib.lik_dequantize_int8.restype = ctypes.c_int
+    lib.lik_linear_int8_workspace_size.argtypes = [P(LikLinearInt8)]
+    lib.lik_linear_int8_workspace_size.restype = ctypes.c_size_t
+    lib.lik_linear_int8.argtypes = [P(LikLinearInt8), _p, _p, ctypes.c_size_t, _p]
+    lib.lik_linear_int8.restype = ctypes.c_int
     _lib = lib
     return lib
 

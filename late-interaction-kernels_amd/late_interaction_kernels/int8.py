@@ -7,9 +7,12 @@ and a weight quantised the same way (a scale per output channel). Inference only
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
+from .gated_ffn import ACTIVATIONS
 from .layer_norm import _rows
 
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -80,4 +83,109 @@ def dequantize_int8_per_token(
     return out
 
 
-__all__ = ["dequantize_int8_per_token", "quantize_int8_per_token"]
+_LIK_INT8 = 4
+_FAR = 1 << 23  # bytes from row to row of integers: the kernels reach 256 rows by 32-bit offsets
+
+
+def _integer_rows(x: torch.Tensor, zeros: bool, far: int = _FAR) -> torch.Tensor:
+    """``x`` with rows that start on 16 bytes and go on to a multiple of 16 (with zeros there, or with whatever the
+    storage holds): a copy where they do not."""
+    n, k = x.shape
+    rs, cs = x.stride()
+    room = x.storage_offset() + (n - 1) * rs + (k + 15) // 16 * 16 <= x.untyped_storage().nbytes()
+    if (cs == 1 or k == 1) and rs % 16 == 0 and rs < far and x.data_ptr() % 16 == 0 and (k % 16 == 0 or
+                                                                                        (room and not zeros)):
+        return x
+    y = torch.nn.functional.pad(x, (0, -k % 16)) if k % 16 else x.clone(memory_format=torch.contiguous_format)
+    return y if y.data_ptr() % 16 == 0 and y.stride() == (y.shape[1], 1) else y.clone(memory_format=torch.contiguous_format)
+
+
+def linear_int8(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    weight_scale: torch.Tensor,
+    bias: torch.Tensor | None = None,
+    residual: torch.Tensor | None = None,
+    *,
+    x_scale: torch.Tensor | None = None,
+    activation: str | None = None,
+    gated: bool = False,
+    out_dtype: torch.dtype | None = None,
+) -> torch.Tensor:
+    """``act(x W^T + bias) + residual`` with both factors as 8-bit integers; ``gated``:
+    ``act(x Wg^T + bg) * (x Wu^T + bu) + residual``.
+
+    Args:
+        x: ``[..., in]`` fp16 / bf16 / fp32, quantised per token within the call (as by
+            :func:`quantize_int8_per_token`), or int8 with its ``x_scale``. ``in`` at most 131071: sums are exact.
+        weight: int8 ``[out, in]`` (gated: ``[2 out, in]``, the gate's rows, then the up rows).
+        weight_scale: fp32, one for each of its rows.
+        bias: as many, of the output's type or fp32, or None.
+        residual: ``[..., out]`` of the output's type, or None; added after the activation.
+        x_scale: fp32 ``x.shape[:-1]``, for int8 ``x`` only.
+        activation: None, "gelu" (erf), "gelu_tanh" or "silu".
+        out_dtype: fp16 / bf16 / fp32; default the type of ``x`` (int8: bf16).
+
+    Returns:
+        ``[..., out]``, everything after the integer sums in fp32 and rounded once. ``in`` is a multiple
+        of 16 in the kernels; a weight of another width (int8 ``x`` too) is padded in a copy per
+        call, unless its rows lie a multiple of 16 bytes apart (a slice of a wider one).
+    """
+    if activation is not None and activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be None or one of {sorted(ACTIVATIONS)}; got {activation!r}")
+    if x.dim() < 1 or weight.dim() != 2:
+        raise ValueError(f"x must be [..., in] and weight [out, in]; got {tuple(x.shape)} and {tuple(weight.shape)}")
+    total, k = weight.shape
+    if x.shape[-1] != k or k < 1 or total < 1 or (gated and total % 2):
+        raise ValueError(f"weight must be [{'2 out' if gated else 'out'}, in={x.shape[-1]}]; got {tuple(weight.shape)}")
+    if k > 131071:
+        raise ValueError(f"linear_int8 takes at most 131071 input features; got {k}")
+    n = total // 2 if gated else total
+    if x.dtype != torch.int8 and x.dtype not in _DTYPES:
+        raise TypeError(f"linear_int8 takes fp16 / bf16 / fp32 / int8; got {x.dtype}")
+    if weight.dtype != torch.int8 or weight_scale.dtype != torch.float32:
+        raise TypeError(f"weight must be int8 and weight_scale fp32; got {weight.dtype} and {weight_scale.dtype}")
+    if weight_scale.shape != (total,):
+        raise ValueError(f"weight_scale must be [{total}]; got {tuple(weight_scale.shape)}")
+    if (x.dtype == torch.int8) != (x_scale is not None):
+        raise ValueError("x_scale goes with int8 x, and only with it")
+    if x_scale is not None and (x_scale.shape != x.shape[:-1] or x_scale.dtype != torch.float32):
+        raise ValueError(f"x_scale must be fp32 {list(x.shape[:-1])}; got {x_scale.dtype} {tuple(x_scale.shape)}")
+    out_dtype = out_dtype or (torch.bfloat16 if x.dtype == torch.int8 else x.dtype)
+    if out_dtype not in _DTYPES:
+        raise TypeError(f"linear_int8 gives fp16 / bf16 / fp32; got {out_dtype}")
+    if bias is not None and (bias.shape != (total,) or bias.dtype not in (out_dtype, torch.float32)):
+        raise ValueError(f"bias must be [{total}] of {out_dtype} or fp32; got {tuple(bias.shape)} {bias.dtype}")
+    if residual is not None and (residual.shape != (*x.shape[:-1], n) or residual.dtype != out_dtype):
+        raise ValueError(f"residual must be {[*x.shape[:-1], n]} of {out_dtype}; got {tuple(residual.shape)} "
+                         f"{residual.dtype}")
+    if any(t is not None and t.device != x.device for t in (weight, weight_scale, bias, residual, x_scale)):
+        raise ValueError("x, weight, their scales, bias and residual must be on the same device.")
+    _lib.require_gpu(x)
+    _no_gradient("linear_int8", x, weight_scale, bias, residual, x_scale)
+    out = torch.empty(*x.shape[:-1], n, dtype=out_dtype, device=x.device)
+    if out.numel() == 0:
+        return out
+    x2, xs = _rows(x)
+    if x.dtype == torch.int8:
+        x2 = _integer_rows(x2, True)
+        k, xs, x_scale = x2.shape[1], x2.stride(0), x_scale.contiguous()
+    w = _integer_rows(weight, False, _FAR if not gated else min(_FAR, 0xFFF00000 // (n + 256)))
+    r2, rs = (None, 0) if residual is None else _rows(residual)
+    weight_scale = weight_scale.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    a = _lib.LikLinearInt8(
+        x2.data_ptr(), _lib.ptr(x_scale), w.data_ptr(), weight_scale.data_ptr(), _lib.ptr(bias), _lib.ptr(r2), xs,
+        w.stride(0), rs, x2.shape[0], k, n, _LIK_INT8 if x.dtype == torch.int8 else _lib.DTYPE_CODE[x.dtype],
+        _lib.DTYPE_CODE[out_dtype], 0 if bias is None else _lib.DTYPE_CODE[bias.dtype],
+        -1 if activation is None else ACTIVATIONS[activation], int(gated))
+    lib = _lib.load()
+    nbytes = lib.lik_linear_int8_workspace_size(ctypes.byref(a))
+    ws = _lib.workspace(nbytes, x.device)
+    with _lib.on_device(x.device):
+        rc = lib.lik_linear_int8(ctypes.byref(a), out.data_ptr(), _lib.ptr(ws), nbytes, _lib.stream_of(x))
+    _lib.check(rc, "lik_linear_int8")
+    return out
+
+
+__all__ = ["dequantize_int8_per_token", "linear_int8", "quantize_int8_per_token"]
