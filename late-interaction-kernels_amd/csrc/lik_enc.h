@@ -49,12 +49,14 @@ __device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b) {
 }
 
 // A 16-byte chunk of V elements from element e of a row; those past `end` are not touched (and load as zeros).
-// Rows may start on any element: the 16-byte access is left to the hardware.
-template <int EK>
+// Rows may start on any element: the 16-byte access is left to the hardware. WHOLE: all of the chunk's elements are
+// there (a load that may be taken to pieces is waited for before the next one starts, so those without ends
+// are asked for as such).
+template <int EK, bool WHOLE = false>
 __device__ __forceinline__ void chunk_load(const char* row, int e, int end, u32x4& w) {
   constexpr int V = El<EK>::V, B = El<EK>::B;
   typedef u32x4 __attribute__((aligned(2))) u32x4_u;
-  if (e + V <= end) {
+  if (WHOLE || e + V <= end) {
     w = *(const u32x4_u*)(row + (int64_t)e * B);
     return;
   }
@@ -66,11 +68,11 @@ __device__ __forceinline__ void chunk_load(const char* row, int e, int end, u32x
       else w[i / 2] |= (uint32_t)((const uint16_t*)row)[e + i] << (i % 2 * 16);
     }
 }
-template <int EK>
+template <int EK, bool WHOLE = false>
 __device__ __forceinline__ void chunk_store(char* row, int e, int end, const u32x4& w) {
   constexpr int V = El<EK>::V, B = El<EK>::B;
   typedef u32x4 __attribute__((aligned(2))) u32x4_u;
-  if (e + V <= end) {
+  if (WHOLE || e + V <= end) {
     *(u32x4_u*)(row + (int64_t)e * B) = w;
     return;
   }

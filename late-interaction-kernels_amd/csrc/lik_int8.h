@@ -1,9 +1,9 @@
 // Rows as 8-bit integers with a scale each: the definition that the quantising kernels share.
 //   s = max(fp32(max|x| / 127), 2^-126),  q = x / s to the nearest integer, ties to even
-// q is that of the exact quotient: x * (1 / s) is off by at most 127 * 2^-22 = 3e-5, so only quotients that
-// close to a half-integer can be on its wrong side. For those the remainder x - q s decides: it is a whole
-// multiple of the smaller of both spacings and at most s, hence exact in one fma (x one binade under s = 2^k is
-// the exception, and there the product with 1 / s = 2^-k is exact).
+// q is that of the exact quotient: x * (1 / s) is off by at most 127 * 2^-22 = 3e-5 (the reciprocal by one unit), so its
+// nearest integer can be the wrong one of two where the quotient lies that close to the middle. The remainder x - q s tells:
+// it is a whole multiple of the smaller of both spacings and little over s / 2, hence exact in one fma (x one binade
+// under s = 2^k is the exception, and there the product with 1 / s = 2^-k is exact); under s / 2, q is right.
 #pragma once
 #include "lik_enc.h"
 
@@ -31,6 +31,28 @@ __device__ __forceinline__ uint32_t absmax_join(uint32_t a, uint32_t b) {
   typedef unsigned short us2 __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, a), __builtin_bit_cast(us2, b)));
 }
+template <int EK, int CTRL>
+__device__ __forceinline__ uint32_t absmax_dpp(uint32_t m) {
+  return absmax_join<EK>(m, (uint32_t)__builtin_amdgcn_update_dpp((int)m, (int)m, CTRL, 0xf, 0xf, false));
+}
+// Over the LPR (16 to 64) lanes of a row, on every lane: within 16 by data-parallel moves (the lane opposite in two, four,
+// eight, sixteen), across them by the row and half swaps.
+template <int EK, int LPR>
+__device__ __forceinline__ uint32_t absmax_lanes(uint32_t m) {
+  m = absmax_dpp<EK, 0xb1>(m);
+  m = absmax_dpp<EK, 0x4e>(m);
+  m = absmax_dpp<EK, 0x141>(m);
+  m = absmax_dpp<EK, 0x140>(m);
+  if constexpr (LPR >= 32) {
+    const auto s = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+    m = absmax_join<EK>((uint32_t)s[0], (uint32_t)s[1]);
+  }
+  if constexpr (LPR == 64) {
+    const auto s = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+    m = absmax_join<EK>((uint32_t)s[0], (uint32_t)s[1]);
+  }
+  return m;
+}
 // The row's scale (NaN where it holds an infinity or a NaN) and what its elements are multiplied by first.
 template <int EK>
 __device__ __forceinline__ void row_scale(uint32_t m, float& s, float& inv) {
@@ -38,8 +60,10 @@ __device__ __forceinline__ void row_scale(uint32_t m, float& s, float& inv) {
   if constexpr (EK == EK_F32) amax = __uint_as_float(m);
   else amax = el_to_f32<EK>(max(m & 0xffffu, m >> 16));
   const bool fine = amax < INFINITY;
-  s = fmaxf(amax / 127.0f, 1.1754943508e-38f);
-  inv = fine ? 1.0f / s : 0.f;
+  // the quotient's bits have a period of 7, so it keeps 2^-7 of a step away from the middle of two floats: rounding the
+  // 64-bit product is rounding the quotient
+  s = fmaxf((float)((double)amax * (1.0 / 127.0)), 1.1754943508e-38f);
+  inv = fine ? __builtin_amdgcn_rcpf(s) : 0.f;
   if (!fine) s = __uint_as_float(0x7fc00000u);
 }
 // The integers of a chunk's elements, 4 to a word; inv = 0: zeros.
@@ -47,22 +71,19 @@ template <int EK>
 __device__ __forceinline__ void chunk_to_int8(const u32x4& w, float s, float inv, uint32_t* out) {
   constexpr int V = El<EK>::V;
   constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: added, the sum's lowest bits are the nearest integer
-  float v[V], y[V], most = 0.f;
+  float v[V], y[V], rem[V], most = 0.f;
   chunk_widen<EK>(w, v);
+  const float half = 0.5f * s;
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    const float q = v[e] * inv;
-    y[e] = q + kRound;
-    most = fmaxf(most, fabsf(q - (y[e] - kRound)));
+    y[e] = fmaf(v[e], inv, kRound);
+    rem[e] = fmaf(kRound - y[e], s, v[e]);
+    most = fmaxf(most, fabsf(rem[e]));
   }
-  if (most > 0.4999f) {
-    const float half = 0.5f * s;
+  if (most >= half)  // (rare: a tie, or a product on the wrong side)
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float r = y[e] - kRound, rem = fmaf(-r, s, v[e]);
-      if (fabsf(rem) > half || (fabsf(rem) == half && (__float_as_uint(y[e]) & 1u))) y[e] += copysignf(1.0f, rem);
-    }
-  }
+    for (int e = 0; e < V; ++e)
+      if (fabsf(rem[e]) > half || (fabsf(rem[e]) == half && (__float_as_uint(y[e]) & 1u))) y[e] += copysignf(1.0f, rem[e]);
 #pragma unroll
   for (int g = 0; g < V / 4; ++g) {
     const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(y[4 * g + 1]), __float_as_uint(y[4 * g]), 0x0c0c0400u);

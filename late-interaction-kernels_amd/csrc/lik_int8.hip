@@ -33,29 +33,40 @@ __device__ __forceinline__ void store_int8(int8_t* row, int e, int end, const ui
     if (e + i < end) row[e + i] = (int8_t)(w[i / 4] >> (i % 4 * 8));
 }
 
-// LPR lanes a row with NV chunks each in registers, U rows at once.
+// LPR lanes a row with NV chunks each in registers, U rows at once. Only a lane's last chunk can reach past the row.
 template <int EK, int LPR, int NV, int U>
 __global__ void __launch_bounds__(256) quantize_kernel(const QuantP p) {
   constexpr int V = El<EK>::V, RPW = 64 / LPR;
   const int lane = threadIdx.x % LPR, g = threadIdx.x % 64 / LPR;
+  const int whole = p.dim / V;
   const int64_t first = (threadIdx.x / 64) * (RPW * U) + g, step = (int64_t)gridDim.x * (4 * RPW * U);
   for (int64_t b = (int64_t)blockIdx.x * (4 * RPW * U); b < p.rows; b += step) {
     const int64_t r0 = b + first;
     u32x4 w[U][NV];
+    // every lane loads: rows and chunks past the end name the last ones
+    if (whole)
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const int64_t r = r0 + u * RPW < p.rows ? r0 + u * RPW : p.rows - 1;
+          const int c = j * LPR + lane;
+          chunk_load<EK, true>(p.x + r * p.x_ld, (j < NV - 1 || c < whole ? c : whole - 1) * V, p.dim, w[u][j]);
+        }
 #pragma unroll
     for (int u = 0; u < U; ++u)
+      if ((NV - 1) * LPR + lane >= whole) w[u][NV - 1] = u32x4{0u, 0u, 0u, 0u};
+    if (p.dim % V && (NV - 1) * LPR + lane == whole) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        w[u][j] = u32x4{0u, 0u, 0u, 0u};
-        if (r0 + u * RPW < p.rows) chunk_load<EK>(p.x + (r0 + u * RPW) * p.x_ld, (j * LPR + lane) * V, p.dim, w[u][j]);
-      }
+      for (int u = 0; u < U; ++u)
+        if (r0 + u * RPW < p.rows) chunk_load<EK>(p.x + (r0 + u * RPW) * p.x_ld, whole * V, p.dim, w[u][NV - 1]);
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       uint32_t m = 0;
 #pragma unroll
       for (int j = 0; j < NV; ++j) m = absmax_bits<EK>(w[u][j], m);
-#pragma unroll
-      for (int o = LPR / 2; o >= 1; o >>= 1) m = absmax_join<EK>(m, (uint32_t)__shfl_xor((int)m, o));
+      m = absmax_lanes<EK, LPR>(m);
       float s, inv;
       row_scale<EK>(m, s, inv);
       const int64_t r = r0 + u * RPW;
@@ -84,8 +95,7 @@ __global__ void __launch_bounds__(256) quantize_wide_kernel(const QuantP p) {
       chunk_load<EK>(row, e, p.dim, w);
       m = absmax_bits<EK>(w, m);
     }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) m = absmax_join<EK>(m, (uint32_t)__shfl_xor((int)m, o));
+    m = absmax_lanes<EK, 64>(m);
     if (threadIdx.x % 64 == 0) s_m[threadIdx.x / 64] = m;
     __syncthreads();
     m = absmax_join<EK>(absmax_join<EK>(s_m[0], s_m[1]), absmax_join<EK>(s_m[2], s_m[3]));
@@ -112,13 +122,20 @@ void launch_rows(const QuantP& p, hipStream_t s) {
 template <int EK>
 int launch_quantize(const QuantP& p, hipStream_t s) {
   const int ch = (p.end + El<EK>::V - 1) / El<EK>::V;
-  if (ch <= 16) launch_rows<EK, 16, 1, 4>(p, s);
+  // the fewest chunks a lane: all but its last are whole. Few rows: a wavefront each (32 rows of 768 bf16: .. us)
+  if (p.rows <= 1024 && ch <= 64) launch_rows<EK, 64, 1, 1>(p, s);
+  else if (p.rows <= 1024 && ch <= 128) launch_rows<EK, 64, 2, 1>(p, s);
+  else if (ch <= 16) launch_rows<EK, 16, 1, 4>(p, s);
   else if (ch <= 32) launch_rows<EK, 16, 2, 2>(p, s);
+  else if (ch <= 48) launch_rows<EK, 16, 3, 1>(p, s);
   else if (ch <= 64) launch_rows<EK, 16, 4, 1>(p, s);
-  else if (ch <= 128) launch_rows<EK, 64, 2, 2>(p, s);
+  else if (ch <= 96) launch_rows<EK, 32, 3, 1>(p, s);
+  else if (ch <= 128) launch_rows<EK, 32, 4, 1>(p, s);
   else if (ch <= 192) launch_rows<EK, 64, 3, 1>(p, s);
   else if (ch <= 256) launch_rows<EK, 64, 4, 1>(p, s);
+  else if (ch <= 320) launch_rows<EK, 64, 5, 1>(p, s);
   else if (ch <= 384) launch_rows<EK, 64, 6, 1>(p, s);
+  else if (ch <= 448) launch_rows<EK, 64, 7, 1>(p, s);
   else if (ch <= 512) launch_rows<EK, 64, 8, 1>(p, s);
   else launch_kernel(quantize_wide_kernel<EK>, dim3(groups(p.rows)), dim3(256), 0u, s, p);
   return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;

@@ -5,6 +5,8 @@
 #include "lik_act.h"
 #include "lik_int8.h"
 
+#include <utility>
+
 namespace lik {
 namespace enc {
 namespace {
@@ -27,6 +29,7 @@ struct LinP {
   const char* res;     // of the output's type; null: none
   int64_t res_ld;
   char* out;           // [m][n]
+  bool rows16;         // whose rows start on 16 bytes
   int act;             // -1: none
 };
 
@@ -62,6 +65,25 @@ __device__ __forceinline__ f32x4 load4(const char* p, bool f32, int n, int end) 
   }
   return v;
 }
+template <int OK>
+__device__ __forceinline__ void store4(char* row, int n, int end, const float* v) {
+  typedef u32x4 __attribute__((aligned(4))) u32x4_u;
+  typedef u32x2 __attribute__((aligned(2))) u32x2_u;
+  if (n + 4 <= end) {
+    if constexpr (OK == EK_F32)
+      *(u32x4_u*)(row + (int64_t)n * 4) =
+          u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+    else
+      *(u32x2_u*)(row + (int64_t)n * 2) = u32x2{pack2<OK>(v[0], v[1]), pack2<OK>(v[2], v[3])};
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (n + e < end) {
+      if constexpr (OK == EK_F32) ((float*)row)[n + e] = v[e];
+      else ((uint16_t*)row)[n + e] = (uint16_t)f32_to_el<OK>(v[e]);
+    }
+}
 // n: the block's first column, `more`: rows of the weight before it (the up half: n hidden ones)
 template <int OK>
 __device__ __forceinline__ void load_cols(const LinP& p, Cols& c, int n, int more, int h) {
@@ -81,12 +103,17 @@ template <int OK>
 struct Res {
   u32x4 x[kResChunks<OK>];
 };
+// Column of chunk j of a lane, from the block's first.
+template <int OK>
+__device__ __forceinline__ int chunk_column(int j, int h) {
+  return OK == EK_F32 ? 8 * j + 4 * h : 16 * j + 8 * h;
+}
 template <int OK>
 __device__ __forceinline__ void load_res(const LinP& p, Res<OK>& r, int m, int n, int h) {
 #pragma unroll
   for (int j = 0; j < kResChunks<OK>; ++j) {
     r.x[j] = u32x4{0u, 0u, 0u, 0u};
-    const int c = OK == EK_F32 ? n + 8 * j + 4 * h : n + 16 * j + 8 * h;
+    const int c = n + chunk_column<OK>(j, h);
     if (p.res && m < p.m && c < p.n) chunk_load<OK>(p.res + m * p.res_ld, c, p.n, r.x[j]);
   }
 }
@@ -99,48 +126,58 @@ __device__ __forceinline__ void activate(int act, float* v) {
   for (int e = 0; e < 8; ++e) v[e] = y[e];
 }
 
-// Lane (m, h) of a block's sums: c0 (GLU: of the gate), c1 (GLU: of the up half); NJ: groups of 16 columns.
+// Weight scales and biases of a lane's columns in 16 of a block: two quads.
+struct Cols8 {
+  f32x4 s[2], b[2];
+};
+// Lane (m, h) of 16 columns' sums, c0 (GLU: of the gate) and c1 (GLU: of the up half), as it stores them: 16-byte
+// chunks, one or (fp32) two; r: the residual's.
+template <int OK, bool GLU>
+__device__ __forceinline__ void group_outputs(const LinP& p, const int* c0, const int* c1, const Cols8& w0,
+                                              const Cols8& w1, const u32x4* r, float sx, u32x4* out) {
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = fmaf((float)c0[e], sx * w0.s[e / 4][e % 4], w0.b[e / 4][e % 4]);
+  activate(p.act, v);
+  if constexpr (GLU)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= fmaf((float)c1[e], sx * w1.s[e / 4][e % 4], w1.b[e / 4][e % 4]);
+  if constexpr (OK == EK_F32) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) out[e / 4][e % 4] = __float_as_uint(v[e] + __uint_as_float(r[e / 4][e % 4]));
+  } else {
+    if (p.res) {  // in the accumulators' order
+      const auto s0 = __builtin_amdgcn_permlane32_swap(r[0][0], r[0][2], false, false);
+      const auto s1 = __builtin_amdgcn_permlane32_swap(r[0][1], r[0][3], false, false);
+      const u32x4 x = {(uint32_t)s0[0], (uint32_t)s1[0], (uint32_t)s0[1], (uint32_t)s1[1]};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float a, b;
+        unpack2<OK>(x[i], a, b);
+        v[2 * i] += a;
+        v[2 * i + 1] += b;
+      }
+    }
+    out[0] = join_halves(pack2<OK>(v[0], v[1]), pack2<OK>(v[2], v[3]), pack2<OK>(v[4], v[5]), pack2<OK>(v[6], v[7]));
+  }
+}
 template <int OK, bool GLU, int NJ = 2>
 __device__ __forceinline__ void finish_block(const LinP& p, const i32x16& c0, const i32x16& c1, const Cols& w0,
                                              const Cols& w1, const Res<OK>& r, float sx, int m, int n, int h) {
+  constexpr int C = kResChunks<OK> / 2;  // chunks of a group
   char* row = p.out + m * ((int64_t)p.n * El<OK>::B);
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    float v[8];
+  for (int g = 0; g < NJ; ++g) {
+    int a0[8], a1[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      v[e] = fmaf((float)c0[8 * j + e], sx * w0.s[2 * j + e / 4][e % 4], w0.b[2 * j + e / 4][e % 4]);
-    activate(p.act, v);
-    if constexpr (GLU)
+    for (int e = 0; e < 8; ++e) a0[e] = c0[8 * g + e], a1[e] = c1[8 * g + e];
+    u32x4 o[C];
+    group_outputs<OK, GLU>(p, a0, a1, Cols8{{w0.s[2 * g], w0.s[2 * g + 1]}, {w0.b[2 * g], w0.b[2 * g + 1]}},
+                           Cols8{{w1.s[2 * g], w1.s[2 * g + 1]}, {w1.b[2 * g], w1.b[2 * g + 1]}}, r.x + C * g, sx, o);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        v[e] *= fmaf((float)c1[8 * j + e], sx * w1.s[2 * j + e / 4][e % 4], w1.b[2 * j + e / 4][e % 4]);
-    if constexpr (OK == EK_F32) {
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int c = n + 16 * j + 8 * q + 4 * h;
-        u32x4 o;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = __float_as_uint(v[4 * q + e] + __uint_as_float(r.x[2 * j + q][e]));
-        if (m < p.m && c < p.n) chunk_store<OK>(row, c, p.n, o);
-      }
-    } else {
-      const int c = n + 16 * j + 8 * h;
-      if (p.res) {  // in the accumulators' order
-        const auto s0 = __builtin_amdgcn_permlane32_swap(r.x[j][0], r.x[j][2], false, false);
-        const auto s1 = __builtin_amdgcn_permlane32_swap(r.x[j][1], r.x[j][3], false, false);
-        const u32x4 x = {(uint32_t)s0[0], (uint32_t)s1[0], (uint32_t)s0[1], (uint32_t)s1[1]};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float a, b;
-          unpack2<OK>(x[i], a, b);
-          v[2 * i] += a;
-          v[2 * i + 1] += b;
-        }
-      }
-      const u32x4 o =
-          join_halves(pack2<OK>(v[0], v[1]), pack2<OK>(v[2], v[3]), pack2<OK>(v[4], v[5]), pack2<OK>(v[6], v[7]));
-      if (m < p.m && c < p.n) chunk_store<OK>(row, c, p.n, o);
+    for (int j = 0; j < C; ++j) {
+      const int c = n + chunk_column<OK>(C * g + j, h);
+      if (m < p.m && c < p.n) chunk_store<OK>(row, c, p.n, o[j]);
     }
   }
 }
@@ -150,28 +187,29 @@ __device__ __forceinline__ void finish_block(const LinP& p, const i32x16& c0, co
 constexpr int BK = 64;
 template <int T, int NW>
 struct Stage {
-  static constexpr int BYTES = T * BK;
-  static constexpr int NI = BYTES / 1024 / NW;  // 1 KB loads of a wavefront
-  static_assert(BYTES % (1024 * NW) == 0, "");
+  static constexpr int BYTES = T * BK, LOADS = BYTES / 1024;  // loads of 1 KB: a wavefront's are wv, wv + NW, ..
+  static constexpr int NI = (LOADS + NW - 1) / NW;
+  static_assert(BYTES % 1024 == 0, "");
   __device__ __forceinline__ static int swz(int r) { return (r >> 2) & 3; }
   // Lane offsets of the wavefront's loads from the tile's origin; glu: rows 32..63 of each 64 are up rows.
   __device__ __forceinline__ static void offsets(uint32_t* off, int wv, int lane, int64_t ld, int rows, bool glu,
                                                  int hidden) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int slot = (wv * NI + i) * 64 + lane, r = slot / 4, c = (slot % 4) ^ swz(r);
+      const int slot = (i * NW + wv) * 64 + lane, r = slot / 4, c = (slot % 4) ^ swz(r);
       const int at = glu ? (r / 64) * 32 + r % 32 : r;
-      off[i] = at < rows ? (uint32_t)((at + (glu && (r & 32) ? (int64_t)hidden : 0)) * ld + c * 16) : kOob;
+      off[i] = r < T && at < rows ? (uint32_t)((at + (glu && (r & 32) ? (int64_t)hidden : 0)) * ld + c * 16) : kOob;
     }
   }
+  // `spare`: 1 KB for a wavefront's load past the tile (all wavefronts count as many)
   __device__ __forceinline__ static void issue(uint32_t lds, const uint32_t* off, int i, int wv, int lane,
-                                               const u32x4& desc, int k_left) {
+                                               const u32x4& desc, int k_left, uint32_t spare) {
     uint32_t o = off[i];
     if (k_left < BK) {
-      const int slot = (wv * NI + i) * 64 + lane;
+      const int slot = (i * NW + wv) * 64 + lane;
       if (((slot % 4) ^ swz(slot / 4)) * 16 >= k_left) o = kOob;
     }
-    dma16(lds + (wv * NI + i) * 1024, o, desc);
+    dma16((i + 1) * NW <= LOADS || i * NW + wv < LOADS ? lds + (i * NW + wv) * 1024 : spare, o, desc);
   }
   // Lane addresses of MFMA operands: lane l has row row0 + l % 32, k = 32 ks + 16 (l / 32) + 0..15.
   __device__ __forceinline__ static void bases(uint32_t* a, int row0, int lane) {
@@ -225,8 +263,8 @@ linear8_kernel(const LinP p) {
     else fb[set][j - MB] = SB::frag(rb, lds + SA::BYTES, j - MB, ks);
   };
   auto issue = [&](int j, uint32_t lds, const u32x4& da, const u32x4& db, int left) {
-    if (j < SA::NI) SA::issue(lds, offa, j, wv, lane, da, left);
-    else SB::issue(lds + SA::BYTES, offb, j - SA::NI, wv, lane, db, left);
+    if (j < SA::NI) SA::issue(lds, offa, j, wv, lane, da, left, 0);
+    else SB::issue(lds + SA::BYTES, offb, j - SA::NI, wv, lane, db, left, 0);
   };
 
   i32x16 acc[NB][MB];
@@ -311,6 +349,277 @@ linear8_kernel(const LinP p) {
   }
 }
 
+constexpr int kNt = 2;  // a store's streaming hint
+// f(0), f(1), .. f(N - 1) as constants
+template <typename F, int... I>
+__device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F f) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F f) {
+  each_of(std::make_integer_sequence<int, N>{}, f);
+}
+
+// Many tiles: a workgroup per CU walks over its tiles of 256 x TN without a break. The loads run NS - 1 steps ahead,
+// over the tiles' ends; of a finished tile's outputs some are stored at once and DEF 16-byte stores a lane wait in
+// registers for the next tile's steps, so that the writes of all CUs do not come in bursts with nothing else to do.
+// The waits count: a step waits for its own loads only, with all younger loads and stores in flight. So every
+// store is issued whatever its lanes hold (a lane without an output names an offset out of range), and column
+// edges, which store element by element, wait for everything.
+template <int OK, bool GLU, int TN, int DEF>
+__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) linear8_stream_kernel(const LinP p) {
+  constexpr int TM = 256, NW = 8, WM = 4, WN = 2, NS = 4;
+  constexpr int MB = TM / WM / 32, NB = TN / WN / 32, PAIR = GLU ? 2 : 1;
+  constexpr int PER = OK == EK_F32 ? 4 : 2;           // stores of a block
+  constexpr int ALL = NB / PAIR * MB * PER, NOW = ALL - DEF;  // stores of a tile, and those at once
+  using SA = Stage<TM, NW>;
+  using SB = Stage<TN, NW>;
+  constexpr int SBYTES = SA::BYTES + SB::BYTES, NI = SA::NI + SB::NI;
+  constexpr bool SPARE = SB::LOADS % NW != 0;
+  __shared__ __attribute__((aligned(1024))) char s_tile[NS * SBYTES + (SPARE ? 1024 : 0)];
+  __shared__ float s_sx[2][TM];
+  __shared__ __attribute__((aligned(16))) float s_sw[2][TN], s_b[2][TN];
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wv % WM, wn = wv / WM;
+  const int steps = (p.k + BK - 1) / BK;
+  // tiles of this workgroup: t, t + stride, ..: its XCD's share, dealt round its workgroups
+  const uint32_t x = blockIdx.x & 7u, per = (uint32_t)p.full >> 3, extra = (uint32_t)p.full & 7u;
+  const int end = (int)(x * per + (x < extra ? x : extra) + per + (x < extra ? 1 : 0));
+  const int stride = ((int)gridDim.x - (int)x + 7) / 8;
+  int t = end - (int)(per + (x < extra ? 1 : 0)) + (int)(blockIdx.x >> 3);
+  if (t >= end) return;
+
+  const uint32_t lds0 = lds_addr(s_tile), spare = lds0 + NS * SBYTES;
+  uint32_t ra[2], rb[2];
+  SA::bases(ra, wm * (TM / WM), lane);
+  SB::bases(rb, wn * (TN / WN), lane);
+  // the loads' own place: tile lt, step ls of it
+  int lt = t, ls = 0;
+  uint32_t offa[SA::NI], offb[SB::NI], into = lds0;
+  const char *la, *lb;
+  auto seek = [&]() {
+    const int tm = lt / p.tiles_n, m0 = tm * TM, n0 = (lt - tm * p.tiles_n) * (TN / PAIR);
+    SA::offsets(offa, wv, lane, p.a_ld, p.m - m0, false, 0);
+    SB::offsets(offb, wv, lane, p.b_ld, p.n - n0, GLU, p.n);
+    la = p.a + (int64_t)m0 * p.a_ld;
+    lb = p.b + (int64_t)n0 * p.b_ld;
+  };
+  u32x4 da, db;
+  int left;
+  auto aim = [&]() {  // past the last tile nothing is loaded, but counted alike
+    const uint32_t size = lt < end ? 0xffffff00u : 0u;
+    da = raw_desc(la + ls * BK, size);
+    db = raw_desc(lb + ls * BK, size);
+    left = p.k - ls * BK;
+  };
+  auto issue = [&](int j) {
+    if (j < SA::NI) SA::issue(into, offa, j, wv, lane, da, left, spare);
+    else SB::issue(into + SA::BYTES, offb, j - SA::NI, wv, lane, db, left, spare);
+  };
+  auto advance = [&]() {
+    into = into == lds0 + (NS - 1) * SBYTES ? lds0 : into + SBYTES;
+    if (++ls == steps) {
+      ls = 0;
+      lt += stride;
+      if (lt < end) seek();
+    }
+  };
+  // weight scales, biases and token scales of a tile, one or two values a thread; as they come, since whatever is done
+  // with a loaded value waits for all that is in flight
+  float col0 = 0.f;
+  uint32_t col1 = 0;
+  auto load_tile_cols = [&](int tile) {
+    const int tm = tile / p.tiles_n, m0 = tm * TM, n0 = (tile - tm * p.tiles_n) * (TN / PAIR);
+    if (tid < TM) {
+      col0 = m0 + tid < p.m ? p.sx[m0 + tid] : 0.f;
+    } else if (tid - TM < TN) {
+      const int r = tid - TM, n = n0 + (GLU ? r / 64 * 32 + r % 32 : r);
+      const int at = GLU && (r & 32) ? n + p.n : n;
+      col0 = n < p.n ? p.sw[at] : 0.f;
+      col1 = 0;
+      if (p.bias && n < p.n) {
+        if (OK == EK_F32 || p.bias32) col1 = ((const uint32_t*)p.bias)[at];
+        else col1 = ((const uint16_t*)p.bias)[at];
+      }
+    }
+  };
+  auto keep_tile_cols = [&](int buf) {
+    if (tid < TM) s_sx[buf][tid] = col0;
+    else if (tid - TM < TN) {
+      s_sw[buf][tid - TM] = col0;
+      s_b[buf][tid - TM] = OK == EK_F32 || p.bias32 ? __uint_as_float(col1) : el_to_f32<OK>(col1);
+    }
+  };
+
+  u32x4 fa[2][MB], fb[2][NB];
+  auto read = [&](int set, uint32_t lds, int ks, int j) {
+    if (j < MB) fa[set][j] = SA::frag(ra, lds, j, ks);
+    else fb[set][j - MB] = SB::frag(rb, lds + SA::BYTES, j - MB, ks);
+  };
+  i32x16 acc[NB][MB];
+  auto k_step = [&](auto SET, uint32_t lds, int ks, auto EXTRA, auto extra_op) {
+    constexpr int set = decltype(SET)::value;
+    constexpr int S = NB * MB, R = MB + NB, OPS = R + decltype(EXTRA)::value;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      acc[s / MB][s % MB] = mfma_i8(acc[s / MB][s % MB], fb[set][s / MB], fa[set][s % MB]);
+#pragma unroll
+      for (int o = s * OPS / S; o < (s + 1) * OPS / S; ++o) {
+        if (o < R) read(set ^ 1, lds, ks, o);
+        else extra_op(o - R);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  using std::integral_constant;
+  constexpr integral_constant<int, 0> S0{}, NONE{};
+  constexpr integral_constant<int, 1> S1{};
+  constexpr integral_constant<int, NI> LOADS{};
+
+  u32x4 later[DEF ? DEF : 1];  // deferred outputs,
+  uint32_t out_off[MB][2];     // their rows' lane offsets
+  __amdgpu_buffer_rsrc_t out_desc = __builtin_amdgcn_make_buffer_rsrc(p.out, (short)0, 0, 0x00020000);
+#pragma unroll
+  for (int d = 0; d < (DEF ? DEF : 1); ++d) later[d] = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int j = 0; j < MB; ++j) out_off[j][0] = out_off[j][1] = kOob;
+  // Store O of a tile, of block (O / PER / MB, O / PER % MB): 16 rows (the block's first or last) of 64 bytes, so that the
+  // chunks of two lanes that are 16 apart have changed places.
+  auto put = [&](auto O, const u32x4& v) {
+    constexpr int o = decltype(O)::value, g = o % PER, j = o / PER % MB, i = o / PER / MB;
+    __builtin_amdgcn_raw_buffer_store_b128(v, out_desc, out_off[j][g & 1], i * 32 * El<OK>::B + g / 2 * 64, kNt);
+  };
+
+  load_tile_cols(t);
+  keep_tile_cols(0);
+  seek();
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i) {
+    aim();
+#pragma unroll
+    for (int j = 0; j < NI; ++j) issue(j);
+    advance();
+  }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+  for (int j = 0; j < MB + NB; ++j) read(0, lds0, 0, j);
+  uint32_t cur = lds0, next = lds0 + SBYTES;
+  // One step of 64 k; AT: which one of the tile, while its stores matter. Younger than the loads that it waits for
+  // (which started NS - 2 steps before) are the loads of NS - 2 steps, the deferred stores of those steps that are
+  // of this tile, and the stores at once of the tile before if they came in between.
+  auto step = [&](auto AT) {
+    constexpr int at = decltype(AT)::value, from = at > NS - 2 ? at - (NS - 2) : 0, to = at < DEF ? at : DEF;
+    constexpr int young = (NS - 2) * NI + (at < NS - 2 ? NOW : 0) + (to > from ? to - from : 0);
+    aim();
+    k_step(S0, cur, 1, LOADS, issue);
+    // the next step is complete in LDS, and every wavefront has read all of this one
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(young < 63 ? young : 63) : "memory");
+    k_step(S1, next, 0, NONE, [&](int) {});
+    if constexpr (at < DEF) put(integral_constant<int, NOW + at>{}, later[at]);
+    advance();
+    cur = next;
+    next = next == lds0 + (NS - 1) * SBYTES ? lds0 : next + SBYTES;
+  };
+  constexpr int HEAD = DEF + NS - 2;  // steps that know of stores
+
+  for (int buf = 0;; buf ^= 1) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int j = 0; j < MB; ++j) acc[i][j] = i32x16{};
+    const int after = t + stride;
+    if (after < end) load_tile_cols(after);
+    each<HEAD>([&](auto I) {
+      if (decltype(I)::value < steps) step(I);
+    });
+    for (int i = HEAD; i < steps; ++i) step(integral_constant<int, HEAD>{});
+    if (steps < DEF)
+      each<DEF>([&](auto I) {
+        if (decltype(I)::value >= steps) put(integral_constant<int, NOW + decltype(I)::value>{}, later[decltype(I)::value]);
+      });
+
+    const int tm = t / p.tiles_n, m0 = tm * TM, n0 = (t - tm * p.tiles_n) * (TN / PAIR);
+    const bool edge = !p.rows16 || n0 + TN / PAIR > p.n;
+    const int64_t out_ld = (int64_t)p.n * El<OK>::B;
+    out_desc = __builtin_amdgcn_make_buffer_rsrc(p.out + m0 * out_ld + n0 * El<OK>::B, (short)0, (int)0xffffff00u, 0x00020000);
+    float sx[MB];
+#pragma unroll
+    for (int j = 0; j < MB; ++j) {
+      const int r = wm * (TM / WM) + j * 32 + l32;
+      sx[j] = s_sx[buf][r];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const int ro = wm * (TM / WM) + j * 32 + g * 16 + (lane & 15);
+        out_off[j][g] = edge || m0 + ro >= p.m
+                            ? kOob
+                            : (uint32_t)(ro * out_ld + wn * (TN / WN / PAIR) * El<OK>::B + (lane & 16) * 2 + h * 16);
+      }
+    }
+    each<NB / PAIR>([&](auto I) {
+      constexpr int i = decltype(I)::value, C = PER / 2;
+      const int n = n0 + wn * (TN / WN / PAIR) + i * 32;
+      Res<OK> res[MB];
+#pragma unroll
+      for (int j = 0; j < MB; ++j) load_res<OK>(p, res[j], m0 + wm * (TM / WM) + j * 32 + l32, n, h);
+      u32x4 o[MB][PER];
+      each<2>([&](auto G) {
+        constexpr int g = decltype(G)::value;
+        Cols8 w0, w1;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int at = wn * (TN / WN) + i * PAIR * 32 + 16 * g + 8 * q + 4 * h;
+          w0.s[q] = *(const f32x4*)&s_sw[buf][at];
+          w0.b[q] = *(const f32x4*)&s_b[buf][at];
+          if (GLU) w1.s[q] = *(const f32x4*)&s_sw[buf][at + 32], w1.b[q] = *(const f32x4*)&s_b[buf][at + 32];
+        }
+        each<MB>([&](auto J) {
+          constexpr int j = decltype(J)::value;
+          int a0[8], a1[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) a0[e] = acc[i * PAIR][j][8 * g + e], a1[e] = acc[i * PAIR + PAIR - 1][j][8 * g + e];
+          group_outputs<OK, GLU>(p, a0, a1, w0, w1, res[j].x + C * g, sx[j], o[j] + C * g);
+          if (edge) {
+            const int m = m0 + wm * (TM / WM) + j * 32 + l32;
+#pragma unroll
+            for (int k = 0; k < C; ++k) {
+              const int c = n + chunk_column<OK>(g * C + k, h);
+              if (m < p.m && c < p.n) chunk_store<OK>(p.out + m * out_ld, c, p.n, o[j][g * C + k]);
+            }
+          }
+          // two chunks are whole: the block's last 16 rows of the first and its first 16 of the second change places
+          if constexpr (C == 2 || g == 1) {
+            constexpr int k0 = C == 2 ? 2 * g : 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const auto s2 = __builtin_amdgcn_permlane16_swap(o[j][k0][e], o[j][k0 + 1][e], false, false);
+              o[j][k0][e] = (uint32_t)s2[0];
+              o[j][k0 + 1][e] = (uint32_t)s2[1];
+            }
+            each<2>([&](auto K) {
+              constexpr int k = k0 + decltype(K)::value, at = (i * MB + j) * PER + k;
+              if constexpr (at < NOW) put(integral_constant<int, at>{}, o[j][k]);
+              else later[at - NOW] = o[j][k];
+            });
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        });
+      });
+    });
+    if (edge) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (after >= end) break;
+    keep_tile_cols(buf ^ 1);
+    t = after;
+#pragma unroll
+    for (int j = 0; j < MB + NB; ++j) read(0, cur, 0, j);  // (again: they need no registers meanwhile)
+  }
+  if (DEF)
+    each<DEF>([&](auto I) {
+      put(integral_constant<int, NOW + decltype(I)::value>{}, later[decltype(I)::value]);
+    });
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load is in flight to LDS when the workgroup ends
+}
+
 // The tail's epilogue: a workgroup adds the splits of one block of every wavefront.
 template <int OK, bool GLU, int TM, int TN, int WM, int WN>
 __global__ void __launch_bounds__(WM* WN * 64) linear8_finish_kernel(const LinP p) {
@@ -346,58 +655,84 @@ __global__ void __launch_bounds__(WM* WN * 64) linear8_finish_kernel(const LinP 
   finish_block<OK, GLU>(p, c[0], c[PAIR - 1], w0, w1, r, m < p.m ? p.sx[m] : 0.f, m, n, h);
 }
 
-// Few rows: the weight is read once for all of them. A workgroup owns 32 weight rows (GLU: 16 gate and the 16 up rows of
-// the same columns, which meet in one lane's accumulators) and all 32 MB rows of x, its eight wavefronts an eighth of k
-// each: operands go from memory to registers as they lie, the eight sums meet in LDS. Rows that are no integers yet
-// are quantised on the way, by every workgroup for itself: the wavefronts' maxima meet in LDS first. (XK: EK_FP8
-// stands for 8-bit integers.)
-constexpr int kInt8 = EK_FP8;
+// Few rows: the weight is read once for all of them. A workgroup owns 16 weight rows (GLU: 8 gate and the 8 up rows of
+// the same columns) and all of up to 16 MB rows of x, its eight wavefronts an eighth of k each: operands go from memory
+// to registers as they lie, the eight sums meet in LDS. Rows that are no integers yet are quantised on the way, by every
+// workgroup for itself: the wavefronts' maxima meet in LDS first.
+constexpr int kInt8 = EK_FP8;  // XK: 8-bit integers
 template <int XK, int OK, bool GLU, int MB>
 __global__ void __launch_bounds__(512) few_rows8_kernel(const LinP p) {
-  constexpr int NW = 8, U = XK == EK_F32 ? 2 : 4;
-  constexpr int XB = XK == kInt8 ? 1 : XK == EK_F32 ? 4 : 2;  // bytes of an element
-  constexpr int XC = XB;                                      // 16-byte chunks of 16 elements
-  __shared__ __attribute__((aligned(16))) int s_sum[NW][MB][4][64][4];
-  __shared__ uint32_t s_max[NW][MB * 32];
-  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+  constexpr int NW = 8, U = XK == kInt8 ? 4 : XK == EK_F32 ? 1 : 2;
+  constexpr int XC = XK == kInt8 ? 1 : XK == EK_F32 ? 4 : 2;  // 16-byte chunks of 16 elements of x
+  __shared__ __attribute__((aligned(16))) int s_sum[NW][MB][64][4];
+  __shared__ uint32_t s_max[NW][MB * 16];
+  const int lane = threadIdx.x & 63, l16 = lane & 15, quad = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n0 = (int)blockIdx.x * (GLU ? 16 : 32);
-  const int n = GLU ? n0 + (l32 & 15) : n0 + l32;
-  const char* wrow = p.b + (int64_t)(GLU && l32 >= 16 ? n + p.n : n) * p.b_ld;
+  const int n0 = (int)blockIdx.x * (GLU ? 8 : 16);
+  const int n = n0 + (GLU ? l16 & 7 : l16);
+  const char* wrow = p.b + (int64_t)(GLU && l16 >= 8 ? n + p.n : n) * p.b_ld;
   const bool won = n < p.n;
   const int k16 = (p.k + 15) / 16 * 16;
-  i32x16 acc[MB];
-#pragma unroll
-  for (int j = 0; j < MB; ++j) acc[j] = i32x16{};
-  const int all = (p.k + 31) / 32, per = (all + NW - 1) / NW, first = wv * per;
+  const int all = (p.k + 63) / 64, per = (all + NW - 1) / NW, first = wv * per;
   const int end = first + per < all ? first + per : all;
+  // what the epilogue reads comes meanwhile: four columns of one row a lane
+  const int m = wv * 16 + l16, c = n0 + 4 * quad;
+  const bool last = wv < MB && m < p.m && (!GLU || quad < 2) && c < p.n;
+  f32x4 s0 = {}, b0 = {}, s1 = {}, b1 = {}, res = {};
+  i32x4 acc[MB];
+#pragma unroll
+  for (int j = 0; j < MB; ++j) acc[j] = i32x4{0, 0, 0, 0};
   u32x4 fb[U], x[U][MB][XC];
+  auto load_w = [&](int ks) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int e = (ks + u) * 64 + 16 * quad;
+      fb[u] = u32x4{0u, 0u, 0u, 0u};
+      if (won && ks + u < end && e < k16) fb[u] = *(const u32x4*)(wrow + e);
+    }
+  };
   auto load_x = [&](int ks) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int j = 0; j < MB; ++j) {
-        const int e = (ks + u) * 32 + 16 * h, m = j * 32 + l32;
-        const bool on = ks + u < end && m < p.m;
+        const int e = (ks + u) * 64 + 16 * quad, row = j * 16 + l16;
+        const bool on = ks + u < end && row < p.m;
 #pragma unroll
-        for (int c = 0; c < XC; ++c) {
-          x[u][j][c] = u32x4{0u, 0u, 0u, 0u};
+        for (int i = 0; i < XC; ++i) {
+          x[u][j][i] = u32x4{0u, 0u, 0u, 0u};
           if constexpr (XK == kInt8) {
-            if (on && e < k16) x[u][j][c] = *(const u32x4*)(p.a + m * p.a_ld + e);
+            if (on && e < k16) x[u][j][i] = *(const u32x4*)(p.a + row * p.a_ld + e);
           } else {
-            const int at = e + c * El<XK>::V;
-            if (on && at < p.k) chunk_load<XK>(p.a + m * p.a_ld, at, p.k, x[u][j][c]);
+            constexpr int V = El<XK>::V;
+            if (on && e + (i + 1) * V <= p.k) chunk_load<XK, true>(p.a + row * p.a_ld, e + i * V, p.k, x[u][j][i]);
           }
         }
       }
-  };
-  auto load_w = [&](int ks) {
+    if constexpr (XK != kInt8) {  // the row's end: after all whole loads, since each of these is waited for
+      constexpr int V = El<XK>::V;
+      if (p.k % V != 0 && ks <= p.k / 64 && ks + U > p.k / 64)
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int e = (ks + u) * 32 + 16 * h;
-      fb[u] = u32x4{0u, 0u, 0u, 0u};
-      if (won && ks + u < end && e < k16) fb[u] = *(const u32x4*)(wrow + e);
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int j = 0; j < MB; ++j)
+#pragma unroll
+            for (int i = 0; i < XC; ++i) {
+              const int e = (ks + u) * 64 + 16 * quad + i * V, row = j * 16 + l16;
+              if (ks + u < end && row < p.m && e < p.k && e + V > p.k)
+                chunk_load<XK>(p.a + row * p.a_ld, e, p.k, x[u][j][i]);
+            }
     }
+  };
+  auto load_last = [&]() {
+    if (!last) return;
+    s0 = load4<EK_F32>((const char*)p.sw, true, c, p.n);
+    if (GLU) s1 = load4<EK_F32>((const char*)(p.sw + p.n), true, c, p.n);
+    if (p.bias) {
+      b0 = load4<OK>(p.bias, p.bias32, c, p.n);
+      if (GLU) b1 = load4<OK>(p.bias + (int64_t)p.n * (OK == EK_F32 || p.bias32 ? 4 : 2), p.bias32, c, p.n);
+    }
+    if (p.res) res = load4<OK>(p.res + m * p.res_ld, false, c, p.n);
   };
   float sx[MB], inv[MB];
   load_w(first);
@@ -408,29 +743,34 @@ __global__ void __launch_bounds__(512) few_rows8_kernel(const LinP p) {
     // from the last steps to the first, which stay in registers
     for (int ks = first + (per - 1) / U * U; ks >= first; ks -= U) {
       load_x(ks);
+      if (ks == first) load_last();
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int j = 0; j < MB; ++j)
 #pragma unroll
-          for (int c = 0; c < XC; ++c) top[j] = absmax_bits<XK>(x[u][j][c], top[j]);
+          for (int i = 0; i < XC; ++i) top[j] = absmax_bits<XK>(x[u][j][i], top[j]);
     }
 #pragma unroll
     for (int j = 0; j < MB; ++j) {
-      top[j] = absmax_join<XK>(top[j], (uint32_t)__shfl_xor((int)top[j], 32));
-      if (h == 0) s_max[wv][j * 32 + l32] = top[j];
+      const auto s16 = __builtin_amdgcn_permlane16_swap(top[j], top[j], false, false);
+      top[j] = absmax_join<XK>((uint32_t)s16[0], (uint32_t)s16[1]);
+      const auto s32 = __builtin_amdgcn_permlane32_swap(top[j], top[j], false, false);
+      top[j] = absmax_join<XK>((uint32_t)s32[0], (uint32_t)s32[1]);
+      if (quad == 0) s_max[wv][j * 16 + l16] = top[j];
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < MB; ++j) {
 #pragma unroll
-      for (int w = 0; w < NW; ++w) top[j] = absmax_join<XK>(top[j], s_max[w][j * 32 + l32]);
+      for (int w = 0; w < NW; ++w) top[j] = absmax_join<XK>(top[j], s_max[w][j * 16 + l16]);
       row_scale<XK>(top[j], sx[j], inv[j]);
     }
   } else {
     load_x(first);
+    load_last();
 #pragma unroll
-    for (int j = 0; j < MB; ++j) sx[j] = j * 32 + l32 < p.m ? p.sx[j * 32 + l32] : 0.f;
+    for (int j = 0; j < MB; ++j) sx[j] = j * 16 + l16 < p.m ? p.sx[j * 16 + l16] : 0.f;
   }
   for (int ks = first; ks < end; ks += U) {
     if (ks != first) {
@@ -447,67 +787,70 @@ __global__ void __launch_bounds__(512) few_rows8_kernel(const LinP p) {
         } else {
           constexpr int W = El<XK>::V / 4;  // words of a chunk's integers
 #pragma unroll
-          for (int c = 0; c < XC; ++c) {
+          for (int i = 0; i < XC; ++i) {
             uint32_t w[W];
-            chunk_to_int8<XK>(x[u][j][c], sx[j], inv[j], w);
+            chunk_to_int8<XK>(x[u][j][i], sx[j], inv[j], w);
 #pragma unroll
-            for (int i = 0; i < W; ++i) q[c * W + i] = w[i];
+            for (int e = 0; e < W; ++e) q[i * W + e] = w[e];
           }
         }
-        acc[j] = mfma_i8(acc[j], fb[u], q);
+        // lane l: weight row (x row) l % 16, k = 16 (l / 16) + 0..15; sums of x row l % 16, weight rows 4 (l / 16) + 0..3
+        acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, fb[u]), __builtin_bit_cast(i32x4, q),
+                                                       acc[j], 0, 0, 0);
       }
   }
 #pragma unroll
-  for (int j = 0; j < MB; ++j)
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      *(i32x4*)s_sum[wv][j][q][lane] = i32x4{acc[j][4 * q], acc[j][4 * q + 1], acc[j][4 * q + 2], acc[j][4 * q + 3]};
+  for (int j = 0; j < MB; ++j) *(i32x4*)s_sum[wv][j][lane] = acc[j];
   __syncthreads();
-  if (wv >= MB) return;
-  const int m = wv * 32 + l32;
+  if (!last) return;
   float s = sx[0];
 #pragma unroll
   for (int j = 1; j < MB; ++j) s = wv == j ? sx[j] : s;
-  Res<OK> r;
-  load_res<OK>(p, r, m, n0, h);
-  Cols w0, w1;
-  load_cols<OK>(p, w0, n0, 0, h);
-  if (GLU) load_cols<OK>(p, w1, n0, p.n, h);
-  i32x16 c = {};
+  i32x4 sum = {0, 0, 0, 0}, up = {0, 0, 0, 0};
 #pragma unroll
-  for (int w = 0; w < NW; ++w)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const i32x4 v = *(const i32x4*)s_sum[w][wv][q][lane];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) c[4 * q + e] += v[e];
-    }
-  if constexpr (GLU) {
-    i32x16 up = {};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) up[e] = c[8 + e];
-    finish_block<OK, GLU, 1>(p, c, up, w0, w1, r, s, m, n0, h);
-  } else {
-    finish_block<OK, GLU>(p, c, c, w0, w1, r, s, m, n0, h);
+  for (int w = 0; w < NW; ++w) {
+    sum += *(const i32x4*)s_sum[w][wv][lane];
+    if (GLU) up += *(const i32x4*)s_sum[w][wv][lane + 32];
   }
+  float v[8], y[8];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = v[e + 4] = fmaf((float)sum[e], s * s0[e], b0[e]);
+  if (p.act >= 0) {
+    act8<false>(p.act, v, y, nullptr);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = y[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (GLU) v[e] *= fmaf((float)up[e], s * s1[e], b1[e]);
+    v[e] += res[e];
+  }
+  store4<OK>(p.out + m * ((int64_t)p.n * El<OK>::B), c, p.n, v);
 }
 
 constexpr int kCUs = 256;
 bool few_rows(int64_t m) { return m <= 64; }
+// Whether few_rows8_kernel quantises its rows itself: each workgroup does it for all of them, which costs more than a
+// launch of its own where there is much (768 to 2304 features: 1 row 4.1 us, 32 rows 7.3 against 3.5 + 3.8 in two launches, 64
+// rows 10.3 against 3.6 + 4.8; 32 rows of 1152 10.2 against 3.5 + 4.2).
+bool quantise_within(int64_t m, int64_t k) { return (m <= 16 ? 16 : m <= 32 ? 32 : 64) * k <= 32 * 1024; }
 
 struct Shape {
-  bool large;
+  int tile;  // 256, 192: 256 x as many, walked; 1: 256 x 128; 0: small
   int tiles_n, full, tail, splits, k_per;
 };
 // n: rows of the weight's tiles
 Shape shape_of(int64_t m, int64_t n, int64_t k, bool glu) {
-  const bool large = (m + 255) / 256 * ((n + 127) / 128) >= kCUs;
-  const int64_t tm = large ? 256 : glu ? 64 : 128, tn = large || glu ? 128 : 64;
+  const int64_t rt = (m + 255) / 256;
+  const auto rounds = [&](int64_t tn) { return (rt * ((n + tn - 1) / tn) + kCUs - 1) / kCUs; };
+  int tile = rt * ((n + 127) / 128) >= kCUs ? 1 : 0;
+  if (rt * ((n + 255) / 256) >= kCUs) tile = glu || 4 * rounds(256) <= 3 * rounds(192) ? 256 : 192;
+  const int64_t tm = tile ? 256 : glu ? 64 : 128, tn = tile > 1 ? tile : tile || glu ? 128 : 64;
   const int64_t cols = (n + tn - 1) / tn;
-  return Shape{large, (int)cols, (int)((m + tm - 1) / tm * cols), 0, 1, (int)k};
+  return Shape{tile, (int)cols, (int)((m + tm - 1) / tm * cols), 0, 1, (int)k};
 }
 int64_t glu_rows(int64_t n) { return (n + 31) / 32 * 64; }  // (blocks of 32 gate and 32 up rows)
-size_t part_bytes(const Shape& s) { return (size_t)s.tail * s.splits * (s.large ? 256 * 128 : 128 * 64) * 4; }
+size_t part_bytes(const Shape& s) { return (size_t)s.tail * s.splits * (s.tile ? 256 * 128 : 128 * 64) * 4; }
 
 template <int OK, bool GLU, int TM, int TN, int NS, int OCC>
 int launch_tiles(const LinP& p, hipStream_t s) {
@@ -530,7 +873,16 @@ int launch_gemm(LinP p, int* part, hipStream_t s) {
   p.splits = sh.splits;
   p.k_per = sh.k_per;
   p.part = part;
-  if (sh.large) return launch_tiles<OK, GLU, 256, 128, 3, 2>(p, s);
+  if (sh.tile > 1) {
+    const unsigned groups = p.full < kCUs ? p.full : kCUs;
+    constexpr int DEF = OK == EK_F32 && !GLU ? 0 : 8;
+    if (GLU || sh.tile == 256)
+      launch_kernel(linear8_stream_kernel<OK, GLU, 256, DEF>, dim3(groups), dim3(512), 0u, s, p);
+    else if constexpr (!GLU)
+      launch_kernel(linear8_stream_kernel<OK, GLU, 192, OK == EK_F32 ? 0 : 8>, dim3(groups), dim3(512), 0u, s, p);
+    return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;
+  }
+  if (sh.tile) return launch_tiles<OK, GLU, 256, 128, 3, 2>(p, s);
   // (a wavefront has 32 columns of a 128 x 64 tile: gate and up blocks need 64)
   if constexpr (GLU) return launch_tiles<OK, GLU, 64, 128, 3, 3>(p, s);
   else return launch_tiles<OK, GLU, 128, 64, 3, 3>(p, s);
@@ -538,21 +890,23 @@ int launch_gemm(LinP p, int* part, hipStream_t s) {
 
 template <int XK, int OK, bool GLU>
 int launch_few(const LinP& p, hipStream_t s) {
-  const unsigned nb = GLU ? (p.n + 15) / 16 : (p.n + 31) / 32;
-  if (p.m <= 32)
+  const unsigned nb = GLU ? (p.n + 7) / 8 : (p.n + 15) / 16;
+  if (p.m <= 16)
     launch_kernel(few_rows8_kernel<XK, OK, GLU, 1>, dim3(nb), dim3(512), 0u, s, p);
-  else
+  else if (p.m <= 32)
     launch_kernel(few_rows8_kernel<XK, OK, GLU, 2>, dim3(nb), dim3(512), 0u, s, p);
+  else
+    launch_kernel(few_rows8_kernel<XK, OK, GLU, 4>, dim3(nb), dim3(512), 0u, s, p);
   return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;
 }
 
 template <int OK, bool GLU>
 int run(const lik_linear_int8_t* a, LinP p, char* ws, hipStream_t s) {
-  if (few_rows(a->rows)) switch (a->x_dtype) {
+  const bool few = few_rows(a->rows);
+  if (few && a->x_dtype != LIK_INT8 && quantise_within(a->rows, a->in)) switch (a->x_dtype) {
       case LIK_BF16: return launch_few<EK_BF16, OK, GLU>(p, s);
       case LIK_F16: return launch_few<EK_F16, OK, GLU>(p, s);
-      case LIK_F32: return launch_few<EK_F32, OK, GLU>(p, s);
-      default: return launch_few<kInt8, OK, GLU>(p, s);
+      default: return launch_few<EK_F32, OK, GLU>(p, s);
     }
   if (a->x_dtype != LIK_INT8) {
     const int64_t k16 = ((int64_t)p.k + 15) / 16 * 16;
@@ -566,7 +920,7 @@ int run(const lik_linear_int8_t* a, LinP p, char* ws, hipStream_t s) {
     p.a_ld = k16;
     p.sx = sx;
   }
-  return launch_gemm<OK, GLU>(p, (int*)ws, s);
+  return few ? launch_few<kInt8, OK, GLU>(p, s) : launch_gemm<OK, GLU>(p, (int*)ws, s);
 }
 
 constexpr int64_t kFar = 0xfff00000ll;  // bytes that a lane's 32-bit offset reaches
@@ -581,10 +935,10 @@ int linear_check(const lik_linear_int8_t* a) {
   return groups < (1 << 24) ? LIK_OK : LIK_ERR_UNSUPPORTED;  // (a launch has less than 2^32 threads)
 }
 size_t linear_ws(const lik_linear_int8_t* a) {
-  if (few_rows(a->rows)) return 0;
-  const Shape sh = shape_of(a->rows, a->gated ? glu_rows(a->out_features) : a->out_features, a->in, a->gated != 0);
-  size_t b = part_bytes(sh);
-  if (a->x_dtype != LIK_INT8)
+  const bool few = few_rows(a->rows);
+  size_t b = few ? 0
+                 : part_bytes(shape_of(a->rows, a->gated ? glu_rows(a->out_features) : a->out_features, a->in, a->gated != 0));
+  if (a->x_dtype != LIK_INT8 && !(few && quantise_within(a->rows, a->in)))
     b += align256((size_t)(a->rows * (((int64_t)a->in + 15) / 16 * 16))) + align256((size_t)a->rows * 4);
   return b ? b + 256 : 0;
 }
@@ -636,6 +990,7 @@ int lik_linear_int8(const lik_linear_int8_t* a, void* out, void* workspace, size
   p.res = (const char*)a->residual;
   p.res_ld = a->residual_stride * ob;
   p.out = (char*)out;
+  p.rows16 = (uintptr_t)out % 16 == 0 && (int64_t)p.n * ob % 16 == 0;
   p.act = a->activation;
   char* ws = workspace ? align256(workspace) : nullptr;
   hipStream_t s = (hipStream_t)stream;

@@ -29,13 +29,15 @@ struct RotP {
   const void* freq;
   bool pos64, freq64;
   int pairs, dim;
+  int rot, items;       // items of a head: of pairs, all
   int tokens;           // of a workgroup
   float amp, sign;
 };
 
 constexpr int kMostTokens = 32, kTable = 2048;  // tokens and cosines of a workgroup
 
-template <int EK, bool INTER>
+// WHOLE: no chunk is taken to pieces (there are V pairs at least, and no elements behind them or V at least).
+template <int EK, bool INTER, bool WHOLE>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotP p) {
   constexpr int V = El<EK>::V;
   __shared__ double s_pos[kMostTokens];
@@ -84,59 +86,72 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotP p) {
     }
     __syncthreads();
 
-    // a chunk: V pairs, or V of the elements behind them
-    const int rot = (p.pairs + V - 1) / V, rest = (p.dim - 2 * p.pairs + V - 1) / V;
-    const int chunks = rot + rest, heads = p.t[0].heads + p.t[1].heads;
-    for (int i = tid; i < tokens * heads * chunks; i += 256) {
-      const int t = i / (heads * chunks), r = i - t * (heads * chunks);
-      int head = r / chunks;
-      const int c = r - head * chunks;
-      const int which = head >= p.t[0].heads;
-      const RotP::Rows& x = p.t[which];
-      if (which) head -= p.t[0].heads;
-      const char* in = x.x + s_at[which][t] + head * x.sh;
-      char* out = x.y + ((row0 + t) * x.heads + head) * ((int64_t)p.dim * El<EK>::B);
-      u32x4 wa, wb;
-      if (c >= rot) {
-        const int e = 2 * p.pairs + (c - rot) * V;
-        chunk_load<EK>(in, e, p.dim, wa);
-        if (!s_on[t]) wa = u32x4{0u, 0u, 0u, 0u};
-        chunk_store<EK>(out, e, p.dim, wa);
-        continue;
+    // An item: two chunks, of V pairs or of the elements behind them (lanes of both kinds take the same way).
+    const int heads = p.t[0].heads + p.t[1].heads, items = tokens * heads * p.items;
+    for (int i = tid; i < items; i += 256) {
+      const int th = i / p.items, c = i - th * p.items, t = th / heads;
+      int head = th - t * heads;
+      const bool is_k = head >= p.t[0].heads;
+      if (is_k) head -= p.t[0].heads;
+      const char* in = is_k ? p.t[1].x + s_at[1][t] + head * p.t[1].sh : p.t[0].x + s_at[0][t] + head * p.t[0].sh;
+      char* out = (is_k ? p.t[1].y : p.t[0].y) +
+                  ((row0 + t) * (is_k ? p.t[1].heads : p.t[0].heads) + head) * ((int64_t)p.dim * El<EK>::B);
+      const bool turned = c < p.rot;
+      // the first pair. WHOLE: the last chunk of a kind ends where its elements do and shares some with the one before
+      const int j = WHOLE && turned && c * V > p.pairs - V ? p.pairs - V : c * V;
+      int ea = turned ? (INTER ? 2 * j : j) : 2 * p.pairs + (c - p.rot) * 2 * V;
+      int eb = turned && !INTER ? j + p.pairs : ea + V;
+      if (WHOLE && !turned) {
+        ea = ea < p.dim - V ? ea : p.dim - V;
+        eb = eb < p.dim - V ? eb : p.dim - V;
       }
-      const int j = c * V;
-      const int ea = INTER ? 2 * j : j, eb = INTER ? 2 * j + V : j + p.pairs;
-      const int enda = INTER ? 2 * p.pairs : p.pairs, endb = 2 * p.pairs;
-      chunk_load<EK>(in, ea, enda, wa);
-      chunk_load<EK>(in, eb, endb, wb);
+      const int enda = turned ? (INTER ? 2 * p.pairs : p.pairs) : p.dim, endb = turned ? 2 * p.pairs : p.dim;
+      u32x4 wa, wb = {0u, 0u, 0u, 0u};
+      chunk_load<EK, WHOLE>(in, ea, enda, wa);
+      if (WHOLE || eb < endb) chunk_load<EK, WHOLE>(in, eb, endb, wb);
       float v[2 * V], y[2 * V];
       chunk_widen<EK>(wa, v);
       chunk_widen<EK>(wb, v + V);
+      const int at = t * p.pairs + (turned ? j : 0);
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        const f32x2 cs = s_cs[t * p.pairs + (j + k < p.pairs ? j + k : 0)];
+        const f32x2 cs = s_cs[WHOLE || j + k < p.pairs ? at + k : at];
         const int ia = INTER ? 2 * k : k, ib = INTER ? 2 * k + 1 : V + k;
         y[ia] = fmaf(v[ia], cs[0], -v[ib] * cs[1]);
         y[ib] = fmaf(v[ib], cs[0], v[ia] * cs[1]);
       }
-      wa = chunk_narrow<EK>(y);
-      wb = chunk_narrow<EK>(y + V);
-      if (!s_on[t]) wa = wb = u32x4{0u, 0u, 0u, 0u};
-      chunk_store<EK>(out, ea, enda, wa);
-      chunk_store<EK>(out, eb, endb, wb);
+      const u32x4 ya = chunk_narrow<EK>(y), yb = chunk_narrow<EK>(y + V);
+      const bool on = s_on[t];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        wa[k] = !on ? 0u : turned ? ya[k] : wa[k];
+        wb[k] = !on ? 0u : turned ? yb[k] : wb[k];
+      }
+      chunk_store<EK, WHOLE>(out, ea, enda, wa);
+      if (WHOLE || eb < endb) chunk_store<EK, WHOLE>(out, eb, endb, wb);
     }
     __syncthreads();  // (the arrays are the next tokens')
   }
 }
 
-template <int EK>
-int launch_rotary(const RotP& p, bool inter, hipStream_t s) {
+template <int EK, bool INTER>
+int launch_rotary(RotP p, hipStream_t s) {
+  constexpr int V = El<EK>::V;
+  const int rest = p.dim - 2 * p.pairs;
+  p.rot = (p.pairs + V - 1) / V;
+  p.items = p.rot + (rest + 2 * V - 1) / (2 * V);
+  // Three items a thread: more tokens a workgroup leave some CUs a workgroup more than others (44928 tokens of 24 heads of
+  // 64, bf16: 8 tokens 55 us, 16 58 us, 32 61 us). Few rows: as many workgroups as there can be.
+  const int64_t per = (int64_t)(p.t[0].heads + p.t[1].heads) * p.items;
+  p.tokens = 1;
+  while (p.tokens < kMostTokens && p.tokens * per < 768 && 2 * p.tokens * p.pairs <= kTable && p.rows >= 2048 * p.tokens)
+    p.tokens *= 2;
   const int64_t want = (p.rows + p.tokens - 1) / p.tokens;
   const unsigned groups = (unsigned)(want < (1 << 22) ? want : 1 << 22);  // (a launch has less than 2^32 threads)
-  if (inter)
-    launch_kernel(rotary_kernel<EK, true>, dim3(groups), dim3(256), 0u, s, p);
+  if (p.pairs >= V && (rest == 0 || rest >= V))
+    launch_kernel(rotary_kernel<EK, INTER, true>, dim3(groups), dim3(256), 0u, s, p);
   else
-    launch_kernel(rotary_kernel<EK, false>, dim3(groups), dim3(256), 0u, s, p);
+    launch_kernel(rotary_kernel<EK, INTER, false>, dim3(groups), dim3(256), 0u, s, p);
   return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;
 }
 
@@ -185,12 +200,10 @@ extern "C" int lik_rotary(const lik_rotary_t* a, void* q_out, void* k_out, lik_s
   p.dim = a->dim;
   p.amp = a->amplitude;
   p.sign = a->inverse ? -1.0f : 1.0f;
-  p.tokens = kMostTokens;
-  while (p.tokens > 1 && (p.tokens * p.pairs > kTable || p.rows < 1024 * p.tokens)) p.tokens /= 2;
   hipStream_t s = (hipStream_t)stream;
   switch (a->dtype) {
-    case LIK_BF16: return launch_rotary<EK_BF16>(p, a->interleaved != 0, s);
-    case LIK_F16: return launch_rotary<EK_F16>(p, a->interleaved != 0, s);
-    default: return launch_rotary<EK_F32>(p, a->interleaved != 0, s);
+    case LIK_BF16: return a->interleaved ? launch_rotary<EK_BF16, true>(p, s) : launch_rotary<EK_BF16, false>(p, s);
+    case LIK_F16: return a->interleaved ? launch_rotary<EK_F16, true>(p, s) : launch_rotary<EK_F16, false>(p, s);
+    default: return a->interleaved ? launch_rotary<EK_F32, true>(p, s) : launch_rotary<EK_F32, false>(p, s);
   }
 }

@@ -12,6 +12,7 @@ import contextlib
 import contextvars
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 import torch
@@ -245,6 +246,16 @@ class LikLinearInt8(ctypes.Structure):
     ]
 
 
+def packer(cls: type[ctypes.Structure]):
+    """``pack(*fields) -> bytes`` of a struct of pointers, integers and floats: a quarter of the time that making the
+    ctypes object takes."""
+    return struct.Struct("@" + "".join({_p: "P", _i64: "q", _i32: "i", ctypes.c_float: "f"}[t] for _, t in cls._fields_)).pack
+
+
+pack_rotary = packer(LikRotary)
+pack_linear_int8 = packer(LikLinearInt8)
+
+
 class LikLaunchOpts(ctypes.Structure):
     """Mirror of ``lik_launch_opts_t``."""
 
@@ -383,15 +394,15 @@ def load() -> ctypes.CDLL:
     lib.lik_attention_backward.argtypes = [P(LikAttention), _p, _p, _p, _p, _i64, _i64, _i64, _p, _p, _p, _p,
                                            ctypes.c_size_t, _p]
     lib.lik_attention_backward.restype = ctypes.c_int
-    lib.lik_rotary.argtypes = [P(LikRotary), _p, _p, _p]
+    lib.lik_rotary.argtypes = [_p, _p, _p, _p]  # (packed, or a pointer to one)
     lib.lik_rotary.restype = ctypes.c_int
     lib.lik_quantize_int8.argtypes = [_p, _i64, _i32, _i64, _i32, _p, _i64, _p, _p]
     lib.lik_quantize_int8.restype = ctypes.c_int
     lib.lik_dequantize_int8.argtypes = [_p, _i64, _p, _i32, _i64, _i32, _p, _p]
     lib.lik_dequantize_int8.restype = ctypes.c_int
-    lib.lik_linear_int8_workspace_size.argtypes = [P(LikLinearInt8)]
+    lib.lik_linear_int8_workspace_size.argtypes = [_p]
     lib.lik_linear_int8_workspace_size.restype = ctypes.c_size_t
-    lib.lik_linear_int8.argtypes = [P(LikLinearInt8), _p, _p, ctypes.c_size_t, _p]
+    lib.lik_linear_int8.argtypes = [_p, _p, _p, ctypes.c_size_t, _p]
     lib.lik_linear_int8.restype = ctypes.c_int
     _lib = lib
     return lib

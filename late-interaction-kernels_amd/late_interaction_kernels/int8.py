@@ -7,8 +7,6 @@ and a weight quantised the same way (a scale per output channel). Inference only
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
@@ -44,14 +42,14 @@ def quantize_int8_per_token(X: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor
         raise TypeError(f"quantize_int8_per_token takes fp16 / bf16 / fp32; got {X.dtype}")
     _lib.require_gpu(X)
     _no_gradient("quantize_int8_per_token", X)
-    out = torch.empty(X.shape, dtype=torch.int8, device=X.device)
+    out = torch.empty_like(X, dtype=torch.int8, memory_format=torch.contiguous_format)
     scale = torch.empty(X.shape[:-1], dtype=torch.float32, device=X.device)
     if X.numel():
-        d = X.shape[-1]
         x2, xs = _rows(X)
+        rows, d = x2.shape
         with _lib.on_device(X.device):
-            rc = _lib.load().lik_quantize_int8(x2.data_ptr(), xs, _lib.DTYPE_CODE[X.dtype], x2.shape[0], d,
-                                               out.data_ptr(), d, scale.data_ptr(), _lib.stream_of(X))
+            rc = _lib.load().lik_quantize_int8(x2.data_ptr(), xs, _lib.DTYPE_CODE[X.dtype], rows, d, out.data_ptr(), d,
+                                               scale.data_ptr(), _lib.stream_of(X))
         _lib.check(rc, "lik_quantize_int8")
     return out, scale
 
@@ -73,7 +71,7 @@ def dequantize_int8_per_token(
         raise ValueError("X_int8 and scale must be on the same device.")
     _lib.require_gpu(X_int8)
     _no_gradient("dequantize_int8_per_token", scale)
-    out = torch.empty(X_int8.shape, dtype=dtype, device=X_int8.device)
+    out = torch.empty_like(X_int8, dtype=dtype, memory_format=torch.contiguous_format)
     if out.numel():
         (x2, xs), scale = _rows(X_int8), scale.contiguous()
         with _lib.on_device(out.device):
@@ -87,17 +85,18 @@ _LIK_INT8 = 4
 _FAR = 1 << 23  # bytes from row to row of integers: the kernels reach 256 rows by 32-bit offsets
 
 
-def _integer_rows(x: torch.Tensor, zeros: bool, far: int = _FAR) -> torch.Tensor:
+def _integer_rows(x: torch.Tensor, zeros: bool, far: int) -> torch.Tensor:
     """``x`` with rows that start on 16 bytes and go on to a multiple of 16 (with zeros there, or with whatever the
-    storage holds): a copy where they do not."""
+    storage holds), less than ``far`` apart: a copy where they do not."""
     n, k = x.shape
     rs, cs = x.stride()
-    room = x.storage_offset() + (n - 1) * rs + (k + 15) // 16 * 16 <= x.untyped_storage().nbytes()
-    if (cs == 1 or k == 1) and rs % 16 == 0 and rs < far and x.data_ptr() % 16 == 0 and (k % 16 == 0 or
-                                                                                        (room and not zeros)):
-        return x
+    if (cs == 1 or k == 1) and not (rs | x.data_ptr()) & 15 and rs < far:
+        if k % 16 == 0:
+            return x
+        if not zeros and x.storage_offset() + (n - 1) * rs + (k + 15) // 16 * 16 <= x.untyped_storage().nbytes():
+            return x
     y = torch.nn.functional.pad(x, (0, -k % 16)) if k % 16 else x.clone(memory_format=torch.contiguous_format)
-    return y if y.data_ptr() % 16 == 0 and y.stride() == (y.shape[1], 1) else y.clone(memory_format=torch.contiguous_format)
+    return y if y.is_contiguous() and y.data_ptr() % 16 == 0 else y.clone(memory_format=torch.contiguous_format)
 
 
 def linear_int8(
@@ -136,54 +135,78 @@ def linear_int8(
     if x.dim() < 1 or weight.dim() != 2:
         raise ValueError(f"x must be [..., in] and weight [out, in]; got {tuple(x.shape)} and {tuple(weight.shape)}")
     total, k = weight.shape
-    if x.shape[-1] != k or k < 1 or total < 1 or (gated and total % 2):
-        raise ValueError(f"weight must be [{'2 out' if gated else 'out'}, in={x.shape[-1]}]; got {tuple(weight.shape)}")
+    *lead, width = x.shape
+    dtype, device = x.dtype, x.device
+    if width != k or k < 1 or total < 1 or (gated and total % 2):
+        raise ValueError(f"weight must be [{'2 out' if gated else 'out'}, in={width}]; got {tuple(weight.shape)}")
     if k > 131071:
         raise ValueError(f"linear_int8 takes at most 131071 input features; got {k}")
     n = total // 2 if gated else total
-    if x.dtype != torch.int8 and x.dtype not in _DTYPES:
-        raise TypeError(f"linear_int8 takes fp16 / bf16 / fp32 / int8; got {x.dtype}")
+    int8 = dtype == torch.int8
+    if not int8 and dtype not in _DTYPES:
+        raise TypeError(f"linear_int8 takes fp16 / bf16 / fp32 / int8; got {dtype}")
     if weight.dtype != torch.int8 or weight_scale.dtype != torch.float32:
         raise TypeError(f"weight must be int8 and weight_scale fp32; got {weight.dtype} and {weight_scale.dtype}")
     if weight_scale.shape != (total,):
         raise ValueError(f"weight_scale must be [{total}]; got {tuple(weight_scale.shape)}")
-    if (x.dtype == torch.int8) != (x_scale is not None):
+    if int8 != (x_scale is not None):
         raise ValueError("x_scale goes with int8 x, and only with it")
-    if x_scale is not None and (x_scale.shape != x.shape[:-1] or x_scale.dtype != torch.float32):
-        raise ValueError(f"x_scale must be fp32 {list(x.shape[:-1])}; got {x_scale.dtype} {tuple(x_scale.shape)}")
-    out_dtype = out_dtype or (torch.bfloat16 if x.dtype == torch.int8 else x.dtype)
+    if int8:
+        if list(x_scale.shape) != lead or x_scale.dtype != torch.float32:
+            raise ValueError(f"x_scale must be fp32 {lead}; got {x_scale.dtype} {tuple(x_scale.shape)}")
+        if x_scale.device != device:
+            raise ValueError("x, weight, their scales, bias and residual must be on the same device.")
+    out_dtype = out_dtype or (torch.bfloat16 if int8 else dtype)
     if out_dtype not in _DTYPES:
         raise TypeError(f"linear_int8 gives fp16 / bf16 / fp32; got {out_dtype}")
-    if bias is not None and (bias.shape != (total,) or bias.dtype not in (out_dtype, torch.float32)):
-        raise ValueError(f"bias must be [{total}] of {out_dtype} or fp32; got {tuple(bias.shape)} {bias.dtype}")
-    if residual is not None and (residual.shape != (*x.shape[:-1], n) or residual.dtype != out_dtype):
-        raise ValueError(f"residual must be {[*x.shape[:-1], n]} of {out_dtype}; got {tuple(residual.shape)} "
-                         f"{residual.dtype}")
-    if any(t is not None and t.device != x.device for t in (weight, weight_scale, bias, residual, x_scale)):
+    if bias is not None:
+        if bias.shape != (total,) or bias.dtype not in (out_dtype, torch.float32):
+            raise ValueError(f"bias must be [{total}] of {out_dtype} or fp32; got {tuple(bias.shape)} {bias.dtype}")
+        if bias.device != device:
+            raise ValueError("x, weight, their scales, bias and residual must be on the same device.")
+    if residual is not None:
+        if list(residual.shape) != [*lead, n] or residual.dtype != out_dtype:
+            raise ValueError(f"residual must be {[*lead, n]} of {out_dtype}; got {tuple(residual.shape)} "
+                             f"{residual.dtype}")
+        if residual.device != device:
+            raise ValueError("x, weight, their scales, bias and residual must be on the same device.")
+    if weight.device != device or weight_scale.device != device:
         raise ValueError("x, weight, their scales, bias and residual must be on the same device.")
     _lib.require_gpu(x)
     _no_gradient("linear_int8", x, weight_scale, bias, residual, x_scale)
-    out = torch.empty(*x.shape[:-1], n, dtype=out_dtype, device=x.device)
+    out = torch.empty((*lead, n), dtype=out_dtype, device=device)
     if out.numel() == 0:
         return out
     x2, xs = _rows(x)
-    if x.dtype == torch.int8:
-        x2 = _integer_rows(x2, True)
-        k, xs, x_scale = x2.shape[1], x2.stride(0), x_scale.contiguous()
-    w = _integer_rows(weight, False, _FAR if not gated else min(_FAR, 0xFFF00000 // (n + 256)))
-    r2, rs = (None, 0) if residual is None else _rows(residual)
-    weight_scale = weight_scale.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    a = _lib.LikLinearInt8(
-        x2.data_ptr(), _lib.ptr(x_scale), w.data_ptr(), weight_scale.data_ptr(), _lib.ptr(bias), _lib.ptr(r2), xs,
-        w.stride(0), rs, x2.shape[0], k, n, _LIK_INT8 if x.dtype == torch.int8 else _lib.DTYPE_CODE[x.dtype],
-        _lib.DTYPE_CODE[out_dtype], 0 if bias is None else _lib.DTYPE_CODE[bias.dtype],
-        -1 if activation is None else ACTIVATIONS[activation], int(gated))
+    x_code = _LIK_INT8
+    if int8:
+        x2 = _integer_rows(x2, True, _FAR)
+        k, xs = x2.shape[1], x2.stride(0)
+        if not x_scale.is_contiguous():
+            x_scale = x_scale.contiguous()
+    else:
+        x_code = _lib.DTYPE_CODE[dtype]
+    # (a gated weight's up rows are n rows away from the gate's)
+    w = _integer_rows(weight, False, min(_FAR, 0xFFF00000 // (n + 256)) if gated else _FAR)
+    if not weight_scale.is_contiguous():
+        weight_scale = weight_scale.contiguous()
+    b_ptr = r_ptr = rs = b_code = 0
+    if bias is not None:
+        if not bias.is_contiguous():
+            bias = bias.contiguous()
+        b_ptr, b_code = bias.data_ptr(), _lib.DTYPE_CODE[bias.dtype]
+    if residual is not None:
+        r2, rs = _rows(residual)
+        r_ptr = r2.data_ptr()
+    a = _lib.pack_linear_int8(
+        x2.data_ptr(), x_scale.data_ptr() if int8 else 0, w.data_ptr(), weight_scale.data_ptr(), b_ptr, r_ptr, xs,
+        w.stride(0), rs, x2.shape[0], k, n, x_code, _lib.DTYPE_CODE[out_dtype], b_code,
+        -1 if activation is None else ACTIVATIONS[activation], gated)
     lib = _lib.load()
-    nbytes = lib.lik_linear_int8_workspace_size(ctypes.byref(a))
-    ws = _lib.workspace(nbytes, x.device)
-    with _lib.on_device(x.device):
-        rc = lib.lik_linear_int8(ctypes.byref(a), out.data_ptr(), _lib.ptr(ws), nbytes, _lib.stream_of(x))
+    nbytes = lib.lik_linear_int8_workspace_size(a)
+    ws = _lib.workspace(nbytes, device)
+    with _lib.on_device(device):
+        rc = lib.lik_linear_int8(a, out.data_ptr(), _lib.ptr(ws), nbytes, _lib.stream_of(x))
     _lib.check(rc, "lik_linear_int8")
     return out
 

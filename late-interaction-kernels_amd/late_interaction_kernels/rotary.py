@@ -9,7 +9,6 @@ differentiated again.
 
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
@@ -95,34 +94,41 @@ def rotary_frequencies(
 def _launch(q, k, frequencies, positions, cu, meta):
     """``(q', k')`` of the tensors that are not None."""
     offset, interleaved, amplitude, inverse = meta
-    x = q if q is not None else k
-    outs = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
-    if x.numel() == 0 and (k is None or k.numel() == 0):
-        return tuple(outs)
-
-    def strides(t):
-        if t is None:
-            return 0, 0, 0
-        s = t.stride()
-        return (0, s[0], s[1]) if t.dim() == 3 else s[:3]
-
-    if x.dim() == 3:
-        n, length = (1, x.shape[0]) if cu is None else (cu.numel() - 1, x.shape[0])
+    x = k if q is None else q
+    *lead, _, d = x.shape
+    outq = outk = None
+    hq = hk = qp = kp = qn = ql = qh = kn = kl = kh = pn = pl = pos = bits = 0
+    some = False
+    if q is not None:
+        outq = torch.empty_like(q, memory_format=torch.contiguous_format)
+        hq, qp, some = q.size(-2), q.data_ptr(), q.numel() != 0
+        *outer, ql, qh, _ = q.stride()
+        if outer:
+            qn = outer[0]
+    if k is not None:
+        outk = torch.empty_like(k, memory_format=torch.contiguous_format)
+        hk, kp, some = k.size(-2), k.data_ptr(), some or k.numel() != 0
+        *outer, kl, kh, _ = k.stride()
+        if outer:
+            kn = outer[0]
+    if not some:
+        return outq, outk
+    if len(lead) == 1:
+        n, length = 1 if cu is None else cu.numel() - 1, lead[0]
     else:
-        n, length = x.shape[:2]
-    pn = pl = 0
+        n, length = lead
     if positions is not None:
-        pn, pl = positions.stride() if positions.dim() == 2 else (0, positions.stride(0))
-    a = _lib.LikRotary(
-        _lib.ptr(q), _lib.ptr(k), _lib.DTYPE_CODE[x.dtype], 0 if q is None else q.shape[-2],
-        0 if k is None else k.shape[-2], x.shape[-1], n, length, *strides(q), *strides(k), _lib.ptr(cu),
-        _lib.ptr(positions), pn, pl, offset, frequencies.data_ptr(),
-        0 if positions is None else 8 * positions.element_size(), 8 * frequencies.element_size(), frequencies.numel(),
-        int(interleaved), int(inverse), amplitude)
+        pos, bits = positions.data_ptr(), 8 * positions.element_size()
+        *outer, pl = positions.stride()
+        if outer:
+            pn = outer[0]
+    a = _lib.pack_rotary(qp, kp, _lib.DTYPE_CODE[x.dtype], hq, hk, d, n, length, qn, ql, qh, kn, kl, kh,
+                         0 if cu is None else cu.data_ptr(), pos, pn, pl, offset, frequencies.data_ptr(), bits,
+                         8 * frequencies.element_size(), frequencies.numel(), interleaved, inverse, amplitude)
     with _lib.on_device(x.device):
-        rc = _lib.load().lik_rotary(ctypes.byref(a), _lib.ptr(outs[0]), _lib.ptr(outs[1]), _lib.stream_of(x))
+        rc = _lib.load().lik_rotary(a, _lib.ptr(outq), _lib.ptr(outk), _lib.stream_of(x))
     _lib.check(rc, "lik_rotary")
-    return tuple(outs)
+    return outq, outk
 
 
 def _unit(t):
@@ -141,9 +147,14 @@ class _RotaryFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, gq, gk):
         offset, interleaved, amplitude, inverse = ctx.meta
-        gq, gk = (g if need else None for g, need in zip((gq, gk), ctx.needs_input_grad))
+        need_q, need_k, *_ = ctx.needs_input_grad
+        gq, gk = gq if need_q else None, gk if need_k else None
         if gq is not None or gk is not None:
-            gq, gk = _RotaryFn.apply(gq, gk, *ctx.saved_tensors, (offset, interleaved, amplitude, not inverse))
+            meta = (offset, interleaved, amplitude, not inverse)
+            if torch.is_grad_enabled():
+                gq, gk = _RotaryFn.apply(gq, gk, *ctx.saved_tensors, meta)
+            else:
+                gq, gk = _launch(_unit(gq), _unit(gk), *ctx.saved_tensors, meta)
         return gq, gk, None, None, None, None
 
 
@@ -175,52 +186,66 @@ def rotary(
     Returns:
         ``q'`` of the shape and type of ``q``, or ``(q', k')``; contiguous.
     """
-    if q.dim() not in (3, 4):
-        raise ValueError(f"q must be [n, L, heads, d] or packed [tokens, heads, d]; got {tuple(q.shape)}")
-    if q.dtype not in _DTYPES:
-        raise TypeError(f"rotary takes fp16 / bf16 / fp32; got {q.dtype}")
-    d = q.shape[-1]
+    shape, dtype, device = q.shape, q.dtype, q.device
+    if len(shape) not in (3, 4):
+        raise ValueError(f"q must be [n, L, heads, d] or packed [tokens, heads, d]; got {tuple(shape)}")
+    if dtype not in _DTYPES:
+        raise TypeError(f"rotary takes fp16 / bf16 / fp32; got {dtype}")
+    *lead, heads, d = shape
     if k is not None:
-        if k.dtype != q.dtype:
-            raise TypeError(f"q and k must have one type; got {q.dtype} and {k.dtype}")
-        if k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != d:
-            raise ValueError(f"k must match q ({tuple(q.shape)}) but in its heads; got {tuple(k.shape)}")
+        *k_lead, k_heads, k_d = k.shape
+        if k.dtype != dtype:
+            raise TypeError(f"q and k must have one type; got {dtype} and {k.dtype}")
+        if k_lead != lead or k_d != d:
+            raise ValueError(f"k must match q ({tuple(shape)}) but in its heads; got {tuple(k.shape)}")
+        if k_heads > 65536:
+            raise ValueError("rotary takes at most 65536 heads")
+        if k.device != device:
+            raise ValueError("q, k, frequencies, positions and cu_seqlens must be on the same device.")
+    if heads > 65536:
+        raise ValueError("rotary takes at most 65536 heads")
     if not 2 <= d <= 1024:
         raise ValueError(f"rotary takes head dims of 2 to 1024; got {d}")
     if frequencies.dim() != 1 or not 1 <= frequencies.numel() <= d // 2:
         raise ValueError(f"frequencies must be [r / 2] with 2 <= r <= {d}; got {tuple(frequencies.shape)}")
     if frequencies.dtype not in (torch.float32, torch.float64):
         raise TypeError(f"frequencies must be fp32 or fp64; got {frequencies.dtype}")
-    if frequencies.requires_grad and torch.is_grad_enabled():
-        raise ValueError("rotary gives no gradient to its frequencies; pass frequencies.detach()")
-    if max(q.shape[-2], 0 if k is None else k.shape[-2]) > 65536:
-        raise ValueError("rotary takes at most 65536 heads")
+    if frequencies.requires_grad:
+        if torch.is_grad_enabled():
+            raise ValueError("rotary gives no gradient to its frequencies; pass frequencies.detach()")
+        frequencies = frequencies.detach()
+    if not isinstance(offset, int) or isinstance(offset, bool) or abs(offset) > 2**31:
+        raise ValueError(f"offset must be an int of at most 2^31; got {offset!r}")
     if positions is not None:
         if cu_seqlens is not None or offset != 0:
             raise ValueError("positions say everything: give them without cu_seqlens and offset")
         if positions.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"positions must be int32 or int64; got {positions.dtype}")
-        if tuple(positions.shape) not in ({q.shape[:1]} if q.dim() == 3 else {q.shape[:2], q.shape[1:2]}):
-            raise ValueError(f"positions must be {list(q.shape[:-2])}{' or [L]' if q.dim() == 4 else ''}; got "
+        if list(positions.shape) not in (lead, lead[1:] or lead):
+            raise ValueError(f"positions must be {lead}{' or [L]' if len(lead) == 2 else ''}; got "
                              f"{tuple(positions.shape)}")
-    if cu_seqlens is not None:
-        if q.dim() != 3:
+        if positions.device != device:
+            raise ValueError("q, k, frequencies, positions and cu_seqlens must be on the same device.")
+    elif cu_seqlens is not None:
+        if len(lead) != 1:
             raise ValueError("cu_seqlens go with packed [tokens, heads, d]")
         if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"cu_seqlens must be [s + 1] cumulative offsets; got {tuple(cu_seqlens.shape)} "
                              f"{cu_seqlens.dtype}")
-    elif q.dim() == 3 and positions is None:
+        if cu_seqlens.device != device:
+            raise ValueError("q, k, frequencies, positions and cu_seqlens must be on the same device.")
+    elif len(lead) == 1:
         raise ValueError("packed rows need cu_seqlens or positions")
-    if not isinstance(offset, int) or isinstance(offset, bool) or abs(offset) > 2**31:
-        raise ValueError(f"offset must be an int of at most 2^31; got {offset!r}")
     amplitude = float(amplitude)
     if not math.isfinite(amplitude):
         raise ValueError(f"amplitude must be finite; got {amplitude}")
-    if any(t is not None and t.device != q.device for t in (k, frequencies, positions, cu_seqlens)):
+    if frequencies.device != device:
         raise ValueError("q, k, frequencies, positions and cu_seqlens must be on the same device.")
     _lib.require_gpu(q)
-    frequencies, cu = frequencies.detach().contiguous(), _i32(cu_seqlens)
+    if not frequencies.is_contiguous():
+        frequencies = frequencies.contiguous()
     meta = (offset, bool(interleaved), amplitude, False)
+    cu = _i32(cu_seqlens)
     if _lib.differentiates(q, k):
         out = _RotaryFn.apply(q, k, frequencies, positions, cu, meta)
     else:
