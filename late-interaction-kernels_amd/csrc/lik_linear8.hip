@@ -18,16 +18,14 @@ struct LinP {
   const char* b;  // weight: int8 rows; GLU: gate rows, then up rows
   int64_t a_ld, b_ld;  // bytes
   int m, n, k;         // n: columns of the output
-  int tiles_n, full;   // the first `full` tiles are one workgroup's each,
-  int tail, splits;    // the `tail` others are `splits` workgroups' each,
-  int k_per;           // of k_per of k
-  int* part;           // their sums [tail][splits][a tile in the accumulators' order]
+  int tiles_n, tiles;  // tiles of a row of them, all
   const float* sx;
   const float* sw;
   const char* bias;    // null: none
   bool bias32;         // fp32 (else the output's type)
   const char* res;     // of the output's type; null: none
   int64_t res_ld;
+  bool res_near;       // its rows lie on 4 bytes and a tile's within a lane's 32-bit offset
   char* out;           // [m][n]
   bool rows16;         // whose rows start on 16 bytes
   int act;             // -1: none
@@ -132,7 +130,7 @@ struct Cols8 {
 };
 // Lane (m, h) of 16 columns' sums, c0 (GLU: of the gate) and c1 (GLU: of the up half), as it stores them: 16-byte
 // chunks, one or (fp32) two; r: the residual's.
-template <int OK, bool GLU>
+template <int OK, bool GLU, bool RES>
 __device__ __forceinline__ void group_outputs(const LinP& p, const int* c0, const int* c1, const Cols8& w0,
                                               const Cols8& w1, const u32x4* r, float sx, u32x4* out) {
   float v[8];
@@ -144,9 +142,9 @@ __device__ __forceinline__ void group_outputs(const LinP& p, const int* c0, cons
     for (int e = 0; e < 8; ++e) v[e] *= fmaf((float)c1[e], sx * w1.s[e / 4][e % 4], w1.b[e / 4][e % 4]);
   if constexpr (OK == EK_F32) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) out[e / 4][e % 4] = __float_as_uint(v[e] + __uint_as_float(r[e / 4][e % 4]));
+    for (int e = 0; e < 8; ++e) out[e / 4][e % 4] = __float_as_uint(RES ? v[e] + __uint_as_float(r[e / 4][e % 4]) : v[e]);
   } else {
-    if (p.res) {  // in the accumulators' order
+    if constexpr (RES) {  // in the accumulators' order
       const auto s0 = __builtin_amdgcn_permlane32_swap(r[0][0], r[0][2], false, false);
       const auto s1 = __builtin_amdgcn_permlane32_swap(r[0][1], r[0][3], false, false);
       const u32x4 x = {(uint32_t)s0[0], (uint32_t)s1[0], (uint32_t)s0[1], (uint32_t)s1[1]};
@@ -172,7 +170,7 @@ __device__ __forceinline__ void finish_block(const LinP& p, const i32x16& c0, co
 #pragma unroll
     for (int e = 0; e < 8; ++e) a0[e] = c0[8 * g + e], a1[e] = c1[8 * g + e];
     u32x4 o[C];
-    group_outputs<OK, GLU>(p, a0, a1, Cols8{{w0.s[2 * g], w0.s[2 * g + 1]}, {w0.b[2 * g], w0.b[2 * g + 1]}},
+    group_outputs<OK, GLU, true>(p, a0, a1, Cols8{{w0.s[2 * g], w0.s[2 * g + 1]}, {w0.b[2 * g], w0.b[2 * g + 1]}},
                            Cols8{{w1.s[2 * g], w1.s[2 * g + 1]}, {w1.b[2 * g], w1.b[2 * g + 1]}}, r.x + C * g, sx, o);
 #pragma unroll
     for (int j = 0; j < C; ++j) {
@@ -235,13 +233,10 @@ linear8_kernel(const LinP p) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wv % WM, wn = wv / WM;
-  const bool whole = (int)blockIdx.x < p.full;
-  const int at = (int)blockIdx.x - p.full, split = whole ? 0 : at / p.tail;
-  const uint32_t t = whole ? xcd_tile(blockIdx.x, (uint32_t)p.full) : (uint32_t)(p.full + at % p.tail);
+  const uint32_t t = xcd_tile(blockIdx.x, (uint32_t)p.tiles);
   const int tm = (int)(t / (uint32_t)p.tiles_n), tn = (int)(t % (uint32_t)p.tiles_n);
   const int m0 = tm * TM, n0 = tn * (TN / PAIR);
-  const int k0 = split * p.k_per, k1 = whole || k0 + p.k_per > p.k ? p.k : k0 + p.k_per;
-  const int steps = (k1 - k0 + BK - 1) / BK;
+  const int steps = (p.k + BK - 1) / BK;
 
   uint32_t offa[SA::NI], offb[SB::NI];
   SA::offsets(offa, wv, lane, p.a_ld, p.m - m0, false, 0);
@@ -254,8 +249,7 @@ linear8_kernel(const LinP p) {
   const char* b_at = p.b + (int64_t)n0 * p.b_ld;
   // a step past the end loads nothing but counts alike
   auto desc = [&](const char* at0, int i) {
-    const int k = k0 + i * BK;
-    return raw_desc(at0 + k, k < k1 ? 0xffffff00u : 0u);
+    return raw_desc(at0 + i * BK, i < steps ? 0xffffff00u : 0u);
   };
   u32x4 fa[2][MB], fb[2][NB];
   auto read = [&](int set, uint32_t lds, int ks, int j) {
@@ -295,7 +289,7 @@ linear8_kernel(const LinP p) {
   for (int i = 0; i < NS - 1; ++i) {
     const u32x4 da = desc(a_at, i), db = desc(b_at, i);
 #pragma unroll
-    for (int j = 0; j < NI; ++j) issue(j, lds0 + i * SBYTES, da, db, k1 - k0 - i * BK);
+    for (int j = 0; j < NI; ++j) issue(j, lds0 + i * SBYTES, da, db, p.k - i * BK);
   }
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 2) * NI) : "memory");
 #pragma unroll
@@ -303,7 +297,7 @@ linear8_kernel(const LinP p) {
   uint32_t cur = lds0, next = lds0 + SBYTES, into = lds0 + (NS - 1) * SBYTES;
   for (int i = 0; i < steps; ++i) {
     const u32x4 da = desc(a_at, i + NS - 1), db = desc(b_at, i + NS - 1);
-    const int left = k1 - k0 - (i + NS - 1) * BK;
+    const int left = p.k - (i + NS - 1) * BK;
     k_step(S0, cur, 1, ALL, [&](int j) { issue(j, into, da, db, left); });
     // the next step is complete in LDS, and every wavefront has read all of this one
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * NI) : "memory");
@@ -314,18 +308,6 @@ linear8_kernel(const LinP p) {
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load is in flight to LDS when the workgroup ends
 
-  if (!whole) {
-    int* out = p.part + (((int64_t)(at % p.tail) * p.splits + split) * NW + wv) * (NB * MB * 1024) + lane * 4;
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-#pragma unroll
-      for (int j = 0; j < MB; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *(i32x4*)(out + ((i * MB + j) * 4 + q) * 256) =
-              i32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-    return;
-  }
   const int l32 = lane & 31, h = lane >> 5;
   float sx[MB];
 #pragma unroll
@@ -366,16 +348,16 @@ __device__ __forceinline__ void each(F f) {
 // The waits count: a step waits for its own loads only, with all younger loads and stores in flight. So every
 // store is issued whatever its lanes hold (a lane without an output names an offset out of range), and column
 // edges, which store element by element, wait for everything.
-template <int OK, bool GLU, int TN, int DEF>
+template <int OK, bool GLU, bool RES, int TN, int DEF>
 __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) linear8_stream_kernel(const LinP p) {
-  constexpr int TM = 256, NW = 8, WM = 4, WN = 2, NS = 4;
+  constexpr int TM = 256, NW = 8, WM = 4, WN = 2, NS = TN == 192 ? 5 : 4;  // (as much as LDS holds)
   constexpr int MB = TM / WM / 32, NB = TN / WN / 32, PAIR = GLU ? 2 : 1;
   constexpr int PER = OK == EK_F32 ? 4 : 2;           // stores of a block
   constexpr int ALL = NB / PAIR * MB * PER, NOW = ALL - DEF;  // stores of a tile, and those at once
   using SA = Stage<TM, NW>;
   using SB = Stage<TN, NW>;
-  constexpr int SBYTES = SA::BYTES + SB::BYTES, NI = SA::NI + SB::NI;
-  constexpr bool SPARE = SB::LOADS % NW != 0;
+  constexpr int SBYTES = SA::BYTES + SB::BYTES, NL = SA::NI + SB::NI, NI = NL + RES;  // loads of a step
+  constexpr bool SPARE = RES || SB::LOADS % NW != 0;
   __shared__ __attribute__((aligned(1024))) char s_tile[NS * SBYTES + (SPARE ? 1024 : 0)];
   __shared__ float s_sx[2][TM];
   __shared__ __attribute__((aligned(16))) float s_sw[2][TN], s_b[2][TN];
@@ -384,7 +366,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int wm = wv % WM, wn = wv / WM;
   const int steps = (p.k + BK - 1) / BK;
   // tiles of this workgroup: t, t + stride, ..: its XCD's share, dealt round its workgroups
-  const uint32_t x = blockIdx.x & 7u, per = (uint32_t)p.full >> 3, extra = (uint32_t)p.full & 7u;
+  const uint32_t x = blockIdx.x & 7u, per = (uint32_t)p.tiles >> 3, extra = (uint32_t)p.tiles & 7u;
   const int end = (int)(x * per + (x < extra ? x : extra) + per + (x < extra ? 1 : 0));
   const int stride = ((int)gridDim.x - (int)x + 7) / 8;
   int t = end - (int)(per + (x < extra ? 1 : 0)) + (int)(blockIdx.x >> 3);
@@ -413,8 +395,22 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
     db = raw_desc(lb + ls * BK, size);
     left = p.k - ls * BK;
   };
+  // The residual of a tile is read ahead into L2, a few lines a step, since a burst of every CU's tile would come from
+  // memory with nothing else going on: lines at, at + 1, .. of this wavefront, 4 bytes of each to the spare KB.
+  constexpr int RL = TN / PAIR * El<OK>::B / 128;  // lines of a row
+  const int ahead = (TM * RL + NW * steps - 1) / (NW * steps);
+  int line = 0;
+  u32x4 dr;
+  auto read_ahead = [&]() {
+    const int at = line + wv * ahead + lane, row = at / RL, c = at % RL * (128 / El<OK>::B);
+    const int tm = t / p.tiles_n, m0 = tm * TM, n0 = (t - tm * p.tiles_n) * (TN / PAIR);
+    const bool on = lane < ahead && row < TM && m0 + row < p.m && n0 + c < p.n && p.res_near;
+    dma4(spare, on ? (uint32_t)(row * p.res_ld + c * El<OK>::B) : kOob, dr);
+    line += NW * ahead;
+  };
   auto issue = [&](int j) {
-    if (j < SA::NI) SA::issue(into, offa, j, wv, lane, da, left, spare);
+    if (RES && j == NL) read_ahead();
+    else if (j < SA::NI) SA::issue(into, offa, j, wv, lane, da, left, spare);
     else SB::issue(into + SA::BYTES, offb, j - SA::NI, wv, lane, db, left, spare);
   };
   auto advance = [&]() {
@@ -498,7 +494,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
   for (int i = 0; i < NS - 1; ++i) {
     aim();
 #pragma unroll
-    for (int j = 0; j < NI; ++j) issue(j);
+    for (int j = 0; j < NL; ++j) issue(j);
     advance();
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -530,6 +526,11 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
       for (int j = 0; j < MB; ++j) acc[i][j] = i32x16{};
     const int after = t + stride;
     if (after < end) load_tile_cols(after);
+    const int tm = t / p.tiles_n, m0 = tm * TM, n0 = (t - tm * p.tiles_n) * (TN / PAIR);
+    if constexpr (RES) {
+      dr = raw_desc(p.res + m0 * p.res_ld + n0 * El<OK>::B, 0xffffff00u);
+      line = 0;
+    }
     each<HEAD>([&](auto I) {
       if (decltype(I)::value < steps) step(I);
     });
@@ -539,7 +540,16 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         if (decltype(I)::value >= steps) put(integral_constant<int, NOW + decltype(I)::value>{}, later[decltype(I)::value]);
       });
 
-    const int tm = t / p.tiles_n, m0 = tm * TM, n0 = (t - tm * p.tiles_n) * (TN / PAIR);
+    // the residual's blocks are asked for one ahead
+    constexpr int RB = RES ? 2 : 1;
+    Res<OK> res[RB][MB];
+    auto ask_res = [&](auto I) {
+      constexpr int i = decltype(I)::value;
+#pragma unroll
+      for (int j = 0; j < MB; ++j)
+        load_res<OK>(p, res[i % RB][j], m0 + wm * (TM / WM) + j * 32 + l32, n0 + wn * (TN / WN / PAIR) + i * 32, h);
+    };
+    if constexpr (RES) ask_res(S0);
     const bool edge = !p.rows16 || n0 + TN / PAIR > p.n;
     const int64_t out_ld = (int64_t)p.n * El<OK>::B;
     out_desc = __builtin_amdgcn_make_buffer_rsrc(p.out + m0 * out_ld + n0 * El<OK>::B, (short)0, (int)0xffffff00u, 0x00020000);
@@ -559,9 +569,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
     each<NB / PAIR>([&](auto I) {
       constexpr int i = decltype(I)::value, C = PER / 2;
       const int n = n0 + wn * (TN / WN / PAIR) + i * 32;
-      Res<OK> res[MB];
-#pragma unroll
-      for (int j = 0; j < MB; ++j) load_res<OK>(p, res[j], m0 + wm * (TM / WM) + j * 32 + l32, n, h);
+      if constexpr (RES && i + 1 < NB / PAIR) ask_res(integral_constant<int, i + 1>{});
       u32x4 o[MB][PER];
       each<2>([&](auto G) {
         constexpr int g = decltype(G)::value;
@@ -578,7 +586,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
           int a0[8], a1[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) a0[e] = acc[i * PAIR][j][8 * g + e], a1[e] = acc[i * PAIR + PAIR - 1][j][8 * g + e];
-          group_outputs<OK, GLU>(p, a0, a1, w0, w1, res[j].x + C * g, sx[j], o[j] + C * g);
+          group_outputs<OK, GLU, RES>(p, a0, a1, w0, w1, res[i % RB][j].x + C * g, sx[j], o[j] + C * g);
           if (edge) {
             const int m = m0 + wm * (TM / WM) + j * 32 + l32;
 #pragma unroll
@@ -618,41 +626,6 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
       put(integral_constant<int, NOW + decltype(I)::value>{}, later[decltype(I)::value]);
     });
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load is in flight to LDS when the workgroup ends
-}
-
-// The tail's epilogue: a workgroup adds the splits of one block of every wavefront.
-template <int OK, bool GLU, int TM, int TN, int WM, int WN>
-__global__ void __launch_bounds__(WM* WN * 64) linear8_finish_kernel(const LinP p) {
-  constexpr int NW = WM * WN, MB = TM / WM / 32, NB = TN / WN / 32, PAIR = GLU ? 2 : 1;
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, wm = wv % WM, wn = wv / WM, h = lane >> 5;
-  int u = (int)blockIdx.x;
-  const int j = u % MB;
-  u /= MB;
-  const int i = u % (NB / PAIR) * PAIR;
-  u /= NB / PAIR;
-  const int t = p.full + u, tm = t / p.tiles_n, tn = t % p.tiles_n;
-  const int m = tm * TM + wm * (TM / WM) + j * 32 + (lane & 31);
-  const int n = tn * (TN / PAIR) + wn * (TN / WN / PAIR) + i / PAIR * 32;
-  Res<OK> r;
-  load_res<OK>(p, r, m, n, h);
-  Cols w0, w1;
-  load_cols<OK>(p, w0, n, 0, h);
-  if (GLU) load_cols<OK>(p, w1, n, p.n, h);
-  i32x16 c[PAIR];
-#pragma unroll
-  for (int b = 0; b < PAIR; ++b) c[b] = i32x16{};
-  const int* in = p.part + ((int64_t)u * p.splits * NW + wv) * (NB * MB * 1024) + lane * 4;
-#pragma unroll 2
-  for (int s = 0; s < p.splits; ++s, in += NW * NB * MB * 1024)
-#pragma unroll
-    for (int b = 0; b < PAIR; ++b)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const i32x4 x = *(const i32x4*)(in + (((i + b) * MB + j) * 4 + q) * 256);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c[b][4 * q + e] += x[e];
-      }
-  finish_block<OK, GLU>(p, c[0], c[PAIR - 1], w0, w1, r, m < p.m ? p.sx[m] : 0.f, m, n, h);
 }
 
 // Few rows: the weight is read once for all of them. A workgroup owns 16 weight rows (GLU: 8 gate and the 8 up rows of
@@ -828,6 +801,9 @@ __global__ void __launch_bounds__(512) few_rows8_kernel(const LinP p) {
   store4<OK>(p.out + m * ((int64_t)p.n * El<OK>::B), c, p.n, v);
 }
 
+// Deferred stores of a tile: as many as registers are left for.
+template <int OK, bool RES>
+constexpr int kDefer = OK == EK_F32 ? 0 : RES ? 4 : 8;
 constexpr int kCUs = 256;
 bool few_rows(int64_t m) { return m <= 64; }
 // Whether few_rows8_kernel quantises its rows itself: each workgroup does it for all of them, which costs more than a
@@ -837,51 +813,46 @@ bool quantise_within(int64_t m, int64_t k) { return (m <= 16 ? 16 : m <= 32 ? 32
 
 struct Shape {
   int tile;  // 256, 192: 256 x as many, walked; 1: 256 x 128; 0: small
-  int tiles_n, full, tail, splits, k_per;
+  int tiles_n, tiles;
 };
 // n: rows of the weight's tiles
-Shape shape_of(int64_t m, int64_t n, int64_t k, bool glu) {
+Shape shape_of(int64_t m, int64_t n, bool glu, bool res) {
   const int64_t rt = (m + 255) / 256;
   const auto rounds = [&](int64_t tn) { return (rt * ((n + tn - 1) / tn) + kCUs - 1) / kCUs; };
   int tile = rt * ((n + 127) / 128) >= kCUs ? 1 : 0;
-  if (rt * ((n + 255) / 256) >= kCUs) tile = glu || 4 * rounds(256) <= 3 * rounds(192) ? 256 : 192;
+  if (rt * ((n + 255) / 256) >= kCUs && !(glu && res))
+    tile = glu || (!res && 100 * rounds(256) <= 78 * rounds(192)) ? 256 : 192;
   const int64_t tm = tile ? 256 : glu ? 64 : 128, tn = tile > 1 ? tile : tile || glu ? 128 : 64;
-  const int64_t cols = (n + tn - 1) / tn;
-  return Shape{tile, (int)cols, (int)((m + tm - 1) / tm * cols), 0, 1, (int)k};
+  const int64_t cols = (n + tn - 1) / tn, tiles = (m + tm - 1) / tm * cols;
+  return Shape{tile, (int)cols, (int)tiles};
 }
 int64_t glu_rows(int64_t n) { return (n + 31) / 32 * 64; }  // (blocks of 32 gate and 32 up rows)
-size_t part_bytes(const Shape& s) { return (size_t)s.tail * s.splits * (s.tile ? 256 * 128 : 128 * 64) * 4; }
 
 template <int OK, bool GLU, int TM, int TN, int NS, int OCC>
 int launch_tiles(const LinP& p, hipStream_t s) {
-  const int groups = p.full + p.tail * p.splits;
-  launch_kernel(linear8_kernel<OK, GLU, TM, TN, 2, 2, NS, OCC>, dim3((unsigned)groups), dim3(256), 0u, s, p);
-  if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
-  if (p.tail) {
-    constexpr int blocks = TM / 64 * (TN / 64) / (GLU ? 2 : 1);
-    launch_kernel(linear8_finish_kernel<OK, GLU, TM, TN, 2, 2>, dim3((unsigned)(p.tail * blocks)), dim3(256), 0u, s, p);
-    if (hipGetLastError() != hipSuccess) return LIK_ERR_LAUNCH;
-  }
-  return LIK_OK;
+  launch_kernel(linear8_kernel<OK, GLU, TM, TN, 2, 2, NS, OCC>, dim3((unsigned)p.tiles), dim3(256), 0u, s, p);
+  return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;
+}
+template <int OK, bool GLU, bool RES>
+int launch_stream(const LinP& p, int tile, hipStream_t s) {
+  const unsigned groups = p.tiles < kCUs ? p.tiles : kCUs;
+  if constexpr (!GLU)
+    if (tile == 192) {
+      launch_kernel(linear8_stream_kernel<OK, GLU, RES, 192, kDefer<OK, RES>>, dim3(groups), dim3(512), 0u, s, p);
+      return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;
+    }
+  if constexpr (!RES)
+    launch_kernel(linear8_stream_kernel<OK, GLU, RES, 256, kDefer<OK, RES>>, dim3(groups), dim3(512), 0u, s, p);
+  return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;
 }
 template <int OK, bool GLU>
-int launch_gemm(LinP p, int* part, hipStream_t s) {
-  const Shape sh = shape_of(p.m, GLU ? glu_rows(p.n) : p.n, p.k, GLU);
+int launch_gemm(LinP p, hipStream_t s) {
+  const Shape sh = shape_of(p.m, GLU ? glu_rows(p.n) : p.n, GLU, p.res != nullptr);
   p.tiles_n = sh.tiles_n;
-  p.full = sh.full;
-  p.tail = sh.tail;
-  p.splits = sh.splits;
-  p.k_per = sh.k_per;
-  p.part = part;
-  if (sh.tile > 1) {
-    const unsigned groups = p.full < kCUs ? p.full : kCUs;
-    constexpr int DEF = OK == EK_F32 && !GLU ? 0 : 8;
-    if (GLU || sh.tile == 256)
-      launch_kernel(linear8_stream_kernel<OK, GLU, 256, DEF>, dim3(groups), dim3(512), 0u, s, p);
-    else if constexpr (!GLU)
-      launch_kernel(linear8_stream_kernel<OK, GLU, 192, OK == EK_F32 ? 0 : 8>, dim3(groups), dim3(512), 0u, s, p);
-    return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;
-  }
+  p.tiles = sh.tiles;
+  if constexpr (!GLU)
+    if (sh.tile > 1 && p.res) return launch_stream<OK, GLU, true>(p, sh.tile, s);
+  if (sh.tile > 1) return launch_stream<OK, GLU, false>(p, sh.tile, s);
   if (sh.tile) return launch_tiles<OK, GLU, 256, 128, 3, 2>(p, s);
   // (a wavefront has 32 columns of a 128 x 64 tile: gate and up blocks need 64)
   if constexpr (GLU) return launch_tiles<OK, GLU, 64, 128, 3, 3>(p, s);
@@ -920,7 +891,7 @@ int run(const lik_linear_int8_t* a, LinP p, char* ws, hipStream_t s) {
     p.a_ld = k16;
     p.sx = sx;
   }
-  return few ? launch_few<kInt8, OK, GLU>(p, s) : launch_gemm<OK, GLU>(p, (int*)ws, s);
+  return few ? launch_few<kInt8, OK, GLU>(p, s) : launch_gemm<OK, GLU>(p, s);
 }
 
 constexpr int64_t kFar = 0xfff00000ll;  // bytes that a lane's 32-bit offset reaches
@@ -934,13 +905,10 @@ int linear_check(const lik_linear_int8_t* a) {
   const int64_t groups = ((a->rows + 63) / 64) * ((2ll * a->out_features + 63) / 64);
   return groups < (1 << 24) ? LIK_OK : LIK_ERR_UNSUPPORTED;  // (a launch has less than 2^32 threads)
 }
+// Rows quantised in a launch of their own: the integers, then the scales.
 size_t linear_ws(const lik_linear_int8_t* a) {
-  const bool few = few_rows(a->rows);
-  size_t b = few ? 0
-                 : part_bytes(shape_of(a->rows, a->gated ? glu_rows(a->out_features) : a->out_features, a->in, a->gated != 0));
-  if (a->x_dtype != LIK_INT8 && !(few && quantise_within(a->rows, a->in)))
-    b += align256((size_t)(a->rows * (((int64_t)a->in + 15) / 16 * 16))) + align256((size_t)a->rows * 4);
-  return b ? b + 256 : 0;
+  if (a->x_dtype == LIK_INT8 || (few_rows(a->rows) && quantise_within(a->rows, a->in))) return 0;
+  return align256((size_t)(a->rows * (((int64_t)a->in + 15) / 16 * 16))) + align256((size_t)a->rows * 4) + 256;
 }
 
 }  // namespace
@@ -989,6 +957,7 @@ int lik_linear_int8(const lik_linear_int8_t* a, void* out, void* workspace, size
   p.bias32 = a->bias_dtype == LIK_F32;
   p.res = (const char*)a->residual;
   p.res_ld = a->residual_stride * ob;
+  p.res_near = ((uintptr_t)p.res | (uint64_t)p.res_ld) % 4 == 0 && p.res_ld >= 0 && 256 * p.res_ld < kFar;
   p.out = (char*)out;
   p.rows16 = (uintptr_t)out % 16 == 0 && (int64_t)p.n * ob % 16 == 0;
   p.act = a->activation;
