@@ -140,19 +140,6 @@ __device__ __forceinline__ void dma16(uint32_t lds, uint32_t voff, const u32x4& 
       : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(desc)
       : "memory");
 }
-// 64 lanes x 4 bytes, likewise.
-__device__ __forceinline__ void dma4(uint32_t lds, uint32_t voff, const u32x4& desc) {
-  uint32_t saved;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %1\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dword %2, %3, 0 offen lds\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(saved)
-      : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(desc)
-      : "memory");
-}
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
 }

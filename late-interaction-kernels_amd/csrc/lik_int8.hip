@@ -17,6 +17,7 @@ struct QuantP {
   int8_t* out;
   int64_t out_ld;
   float* scale;
+  bool stream;
 };
 
 template <int V>
@@ -34,7 +35,8 @@ __device__ __forceinline__ void store_int8(int8_t* row, int e, int end, const ui
 }
 
 // LPR lanes a row with NV chunks each in registers, U rows at once. Only a lane's last chunk can reach past the row.
-template <int EK, int LPR, int NV, int U>
+// NT: rows are read past the caches.
+template <int EK, int LPR, int NV, int U, bool NT>
 __global__ void __launch_bounds__(256) quantize_kernel(const QuantP p) {
   constexpr int V = El<EK>::V, RPW = 64 / LPR;
   const int lane = threadIdx.x % LPR, g = threadIdx.x % 64 / LPR;
@@ -49,9 +51,12 @@ __global__ void __launch_bounds__(256) quantize_kernel(const QuantP p) {
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
+          typedef u32x4 __attribute__((aligned(2))) u32x4_u;
           const int64_t r = r0 + u * RPW < p.rows ? r0 + u * RPW : p.rows - 1;
           const int c = j * LPR + lane;
-          chunk_load<EK, true>(p.x + r * p.x_ld, (j < NV - 1 || c < whole ? c : whole - 1) * V, p.dim, w[u][j]);
+          const u32x4_u* at = (const u32x4_u*)(p.x + r * p.x_ld) + (j < NV - 1 || c < whole ? c : whole - 1);
+          if constexpr (NT) w[u][j] = __builtin_nontemporal_load(at);
+          else w[u][j] = *at;
         }
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -117,12 +122,15 @@ unsigned groups(int64_t want) { return (unsigned)(want < (1 << 22) ? want : 1 <<
 template <int EK, int LPR, int NV, int U>
 void launch_rows(const QuantP& p, hipStream_t s) {
   const int64_t per = 4 * (64 / LPR) * U;
-  launch_kernel(quantize_kernel<EK, LPR, NV, U>, dim3(groups((p.rows + per - 1) / per)), dim3(256), 0u, s, p);
+  const dim3 grid(groups((p.rows + per - 1) / per));
+  if (p.stream) launch_kernel(quantize_kernel<EK, LPR, NV, U, true>, grid, dim3(256), 0u, s, p);
+  else launch_kernel(quantize_kernel<EK, LPR, NV, U, false>, grid, dim3(256), 0u, s, p);
 }
 template <int EK>
 int launch_quantize(const QuantP& p, hipStream_t s) {
   const int ch = (p.end + El<EK>::V - 1) / El<EK>::V;
-  // the fewest chunks a lane: all but its last are whole. Few rows: a wavefront each (32 rows of 768 bf16: .. us)
+  // the fewest chunks a lane: all but its last are whole. Few rows: a wavefront each (32 rows of 768 bf16: 3.5 us, two
+  // rows a wavefront 4.2 us)
   if (p.rows <= 1024 && ch <= 64) launch_rows<EK, 64, 1, 1>(p, s);
   else if (p.rows <= 1024 && ch <= 128) launch_rows<EK, 64, 2, 1>(p, s);
   else if (ch <= 16) launch_rows<EK, 16, 1, 4>(p, s);
@@ -192,6 +200,24 @@ int rows_check(int32_t dtype, int64_t rows, int32_t dim) {
 }
 
 }  // namespace
+
+int quantize_rows_int8(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int32_t dim, int8_t* out,
+                       int64_t out_stride, float* scale, bool stream, hipStream_t s) {
+  if (const int rc = rows_check(dtype, rows, dim)) return rc;
+  if (rows == 0) return LIK_OK;
+  if (!x || !out || !scale || out_stride < dim) return LIK_ERR_INVALID;
+  const int eb = dtype == LIK_F32 ? 4 : 2;
+  if ((uintptr_t)x % eb || (uintptr_t)scale % 4) return LIK_ERR_UNSUPPORTED;
+  const int64_t end = (dim + 15) / 16 * 16;
+  const QuantP p{(const char*)x, x_stride * eb, rows, dim, (int)(end < out_stride ? end : out_stride), out, out_stride,
+                 scale, stream};
+  switch (dtype) {
+    case LIK_BF16: return launch_quantize<EK_BF16>(p, s);
+    case LIK_F16: return launch_quantize<EK_F16>(p, s);
+    default: return launch_quantize<EK_F32>(p, s);
+  }
+}
+
 }  // namespace enc
 }  // namespace lik
 
@@ -202,20 +228,7 @@ extern "C" {
 
 int lik_quantize_int8(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int32_t dim, int8_t* out,
                       int64_t out_stride, float* scale, lik_stream_t stream) {
-  if (const int rc = rows_check(dtype, rows, dim)) return rc;
-  if (rows == 0) return LIK_OK;
-  if (!x || !out || !scale || out_stride < dim) return LIK_ERR_INVALID;
-  const int eb = dtype == LIK_F32 ? 4 : 2;
-  if ((uintptr_t)x % eb || (uintptr_t)scale % 4) return LIK_ERR_UNSUPPORTED;
-  const int64_t end = (dim + 15) / 16 * 16;
-  const QuantP p{(const char*)x, x_stride * eb, rows, dim, (int)(end < out_stride ? end : out_stride), out, out_stride,
-                 scale};
-  hipStream_t s = (hipStream_t)stream;
-  switch (dtype) {
-    case LIK_BF16: return launch_quantize<EK_BF16>(p, s);
-    case LIK_F16: return launch_quantize<EK_F16>(p, s);
-    default: return launch_quantize<EK_F32>(p, s);
-  }
+  return quantize_rows_int8(x, x_stride, dtype, rows, dim, out, out_stride, scale, true, (hipStream_t)stream);
 }
 
 int lik_dequantize_int8(const int8_t* x, int64_t x_stride, const float* scale, int32_t dtype, int64_t rows, int32_t dim,

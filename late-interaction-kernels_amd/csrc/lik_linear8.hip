@@ -25,7 +25,6 @@ struct LinP {
   bool bias32;         // fp32 (else the output's type)
   const char* res;     // of the output's type; null: none
   int64_t res_ld;
-  bool res_near;       // its rows lie on 4 bytes and a tile's within a lane's 32-bit offset
   char* out;           // [m][n]
   bool rows16;         // whose rows start on 16 bytes
   int act;             // -1: none
@@ -331,7 +330,6 @@ linear8_kernel(const LinP p) {
   }
 }
 
-constexpr int kNt = 2;  // a store's streaming hint
 // f(0), f(1), .. f(N - 1) as constants
 template <typename F, int... I>
 __device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F f) {
@@ -350,14 +348,14 @@ __device__ __forceinline__ void each(F f) {
 // edges, which store element by element, wait for everything.
 template <int OK, bool GLU, bool RES, int TN, int DEF>
 __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) linear8_stream_kernel(const LinP p) {
-  constexpr int TM = 256, NW = 8, WM = 4, WN = 2, NS = TN == 192 ? 5 : 4;  // (as much as LDS holds)
+  constexpr int TM = 256, NW = 8, WM = 4, WN = 2, NS = 4;
   constexpr int MB = TM / WM / 32, NB = TN / WN / 32, PAIR = GLU ? 2 : 1;
   constexpr int PER = OK == EK_F32 ? 4 : 2;           // stores of a block
   constexpr int ALL = NB / PAIR * MB * PER, NOW = ALL - DEF;  // stores of a tile, and those at once
   using SA = Stage<TM, NW>;
   using SB = Stage<TN, NW>;
-  constexpr int SBYTES = SA::BYTES + SB::BYTES, NL = SA::NI + SB::NI, NI = NL + RES;  // loads of a step
-  constexpr bool SPARE = RES || SB::LOADS % NW != 0;
+  constexpr int SBYTES = SA::BYTES + SB::BYTES, NI = SA::NI + SB::NI;  // loads of a step
+  constexpr bool SPARE = SB::LOADS % NW != 0;
   __shared__ __attribute__((aligned(1024))) char s_tile[NS * SBYTES + (SPARE ? 1024 : 0)];
   __shared__ float s_sx[2][TM];
   __shared__ __attribute__((aligned(16))) float s_sw[2][TN], s_b[2][TN];
@@ -395,22 +393,8 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
     db = raw_desc(lb + ls * BK, size);
     left = p.k - ls * BK;
   };
-  // The residual of a tile is read ahead into L2, a few lines a step, since a burst of every CU's tile would come from
-  // memory with nothing else going on: lines at, at + 1, .. of this wavefront, 4 bytes of each to the spare KB.
-  constexpr int RL = TN / PAIR * El<OK>::B / 128;  // lines of a row
-  const int ahead = (TM * RL + NW * steps - 1) / (NW * steps);
-  int line = 0;
-  u32x4 dr;
-  auto read_ahead = [&]() {
-    const int at = line + wv * ahead + lane, row = at / RL, c = at % RL * (128 / El<OK>::B);
-    const int tm = t / p.tiles_n, m0 = tm * TM, n0 = (t - tm * p.tiles_n) * (TN / PAIR);
-    const bool on = lane < ahead && row < TM && m0 + row < p.m && n0 + c < p.n && p.res_near;
-    dma4(spare, on ? (uint32_t)(row * p.res_ld + c * El<OK>::B) : kOob, dr);
-    line += NW * ahead;
-  };
   auto issue = [&](int j) {
-    if (RES && j == NL) read_ahead();
-    else if (j < SA::NI) SA::issue(into, offa, j, wv, lane, da, left, spare);
+    if (j < SA::NI) SA::issue(into, offa, j, wv, lane, da, left, spare);
     else SB::issue(into + SA::BYTES, offb, j - SA::NI, wv, lane, db, left, spare);
   };
   auto advance = [&]() {
@@ -480,11 +464,14 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
   for (int d = 0; d < (DEF ? DEF : 1); ++d) later[d] = u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
   for (int j = 0; j < MB; ++j) out_off[j][0] = out_off[j][1] = kOob;
+  // Streamed past the caches where that is faster (44801 x 768 -> 2304 with its quantising launch: fp16 120 against 139 us;
+  // 20000 rows to fp32: 92 against 84; with a residual no difference).
+  constexpr int NT = OK == EK_F32 || RES ? 0 : 2;
   // Store O of a tile, of block (O / PER / MB, O / PER % MB): 16 rows (the block's first or last) of 64 bytes, so that the
   // chunks of two lanes that are 16 apart have changed places.
   auto put = [&](auto O, const u32x4& v) {
     constexpr int o = decltype(O)::value, g = o % PER, j = o / PER % MB, i = o / PER / MB;
-    __builtin_amdgcn_raw_buffer_store_b128(v, out_desc, out_off[j][g & 1], i * 32 * El<OK>::B + g / 2 * 64, kNt);
+    __builtin_amdgcn_raw_buffer_store_b128(v, out_desc, out_off[j][g & 1], i * 32 * El<OK>::B + g / 2 * 64, NT);
   };
 
   load_tile_cols(t);
@@ -494,7 +481,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
   for (int i = 0; i < NS - 1; ++i) {
     aim();
 #pragma unroll
-    for (int j = 0; j < NL; ++j) issue(j);
+    for (int j = 0; j < NI; ++j) issue(j);
     advance();
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -527,10 +514,6 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
     const int after = t + stride;
     if (after < end) load_tile_cols(after);
     const int tm = t / p.tiles_n, m0 = tm * TM, n0 = (t - tm * p.tiles_n) * (TN / PAIR);
-    if constexpr (RES) {
-      dr = raw_desc(p.res + m0 * p.res_ld + n0 * El<OK>::B, 0xffffff00u);
-      line = 0;
-    }
     each<HEAD>([&](auto I) {
       if (decltype(I)::value < steps) step(I);
     });
@@ -801,9 +784,6 @@ __global__ void __launch_bounds__(512) few_rows8_kernel(const LinP p) {
   store4<OK>(p.out + m * ((int64_t)p.n * El<OK>::B), c, p.n, v);
 }
 
-// Deferred stores of a tile: as many as registers are left for.
-template <int OK, bool RES>
-constexpr int kDefer = OK == EK_F32 ? 0 : RES ? 4 : 8;
 constexpr int kCUs = 256;
 bool few_rows(int64_t m) { return m <= 64; }
 // Whether few_rows8_kernel quantises its rows itself: each workgroup does it for all of them, which costs more than a
@@ -835,14 +815,16 @@ int launch_tiles(const LinP& p, hipStream_t s) {
 }
 template <int OK, bool GLU, bool RES>
 int launch_stream(const LinP& p, int tile, hipStream_t s) {
+  // Deferred stores: with a residual they change nothing (105 us either way below), its reads are what takes the time.
+  constexpr int DEF = RES ? 0 : 8;
   const unsigned groups = p.tiles < kCUs ? p.tiles : kCUs;
   if constexpr (!GLU)
     if (tile == 192) {
-      launch_kernel(linear8_stream_kernel<OK, GLU, RES, 192, kDefer<OK, RES>>, dim3(groups), dim3(512), 0u, s, p);
+      launch_kernel(linear8_stream_kernel<OK, GLU, RES, 192, DEF>, dim3(groups), dim3(512), 0u, s, p);
       return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;
     }
   if constexpr (!RES)
-    launch_kernel(linear8_stream_kernel<OK, GLU, RES, 256, kDefer<OK, RES>>, dim3(groups), dim3(512), 0u, s, p);
+    launch_kernel(linear8_stream_kernel<OK, GLU, RES, 256, DEF>, dim3(groups), dim3(512), 0u, s, p);
   return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;
 }
 template <int OK, bool GLU>
@@ -885,8 +867,7 @@ int run(const lik_linear_int8_t* a, LinP p, char* ws, hipStream_t s) {
     ws += align256((size_t)(p.m * k16));
     float* sx = (float*)ws;
     ws += align256((size_t)p.m * 4);
-    if (const int rc = lik_quantize_int8(a->x, a->x_stride, a->x_dtype, a->rows, a->in, x8, k16, sx, (lik_stream_t)s))
-      return rc;
+    if (const int rc = quantize_rows_int8(a->x, a->x_stride, a->x_dtype, a->rows, a->in, x8, k16, sx, false, s)) return rc;
     p.a = (const char*)x8;
     p.a_ld = k16;
     p.sx = sx;
@@ -957,7 +938,6 @@ int lik_linear_int8(const lik_linear_int8_t* a, void* out, void* workspace, size
   p.bias32 = a->bias_dtype == LIK_F32;
   p.res = (const char*)a->residual;
   p.res_ld = a->residual_stride * ob;
-  p.res_near = ((uintptr_t)p.res | (uint64_t)p.res_ld) % 4 == 0 && p.res_ld >= 0 && 256 * p.res_ld < kFar;
   p.out = (char*)out;
   p.rows16 = (uintptr_t)out % 16 == 0 && (int64_t)p.n * ob % 16 == 0;
   p.act = a->activation;
