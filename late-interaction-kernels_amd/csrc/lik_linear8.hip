@@ -26,7 +26,7 @@ struct LinP {
   const char* res;     // of the output's type; null: none
   int64_t res_ld;
   char* out;           // [m][n]
-  bool rows16;         // whose rows start on 16 bytes
+  bool rows16;         // whose rows start on 16 bytes, 256 of them within a lane's 32-bit offset
   int act;             // -1: none
 };
 
@@ -793,7 +793,7 @@ bool quantise_within(int64_t m, int64_t k) { return (m <= 16 ? 16 : m <= 32 ? 32
 
 struct Shape {
   int tile;  // 256, 192: 256 x as many, walked; 1: 256 x 128; 0: small
-  int tiles_n, tiles;
+  int64_t tiles_n, tiles;
 };
 // n: rows of the weight's tiles
 Shape shape_of(int64_t m, int64_t n, bool glu, bool res) {
@@ -804,7 +804,7 @@ Shape shape_of(int64_t m, int64_t n, bool glu, bool res) {
     tile = glu || (!res && 100 * rounds(256) <= 78 * rounds(192)) ? 256 : 192;
   const int64_t tm = tile ? 256 : glu ? 64 : 128, tn = tile > 1 ? tile : tile || glu ? 128 : 64;
   const int64_t cols = (n + tn - 1) / tn, tiles = (m + tm - 1) / tm * cols;
-  return Shape{tile, (int)cols, (int)tiles};
+  return Shape{tile, cols, tiles};
 }
 int64_t glu_rows(int64_t n) { return (n + 31) / 32 * 64; }  // (blocks of 32 gate and 32 up rows)
 
@@ -830,8 +830,8 @@ int launch_stream(const LinP& p, int tile, hipStream_t s) {
 template <int OK, bool GLU>
 int launch_gemm(LinP p, hipStream_t s) {
   const Shape sh = shape_of(p.m, GLU ? glu_rows(p.n) : p.n, GLU, p.res != nullptr);
-  p.tiles_n = sh.tiles_n;
-  p.tiles = sh.tiles;
+  p.tiles_n = (int)sh.tiles_n;
+  p.tiles = (int)sh.tiles;
   if constexpr (!GLU)
     if (sh.tile > 1 && p.res) return launch_stream<OK, GLU, true>(p, sh.tile, s);
   if (sh.tile > 1) return launch_stream<OK, GLU, false>(p, sh.tile, s);
@@ -883,8 +883,9 @@ int linear_check(const lik_linear_int8_t* a) {
     return LIK_ERR_INVALID;
   if (a->bias && a->bias_dtype != a->out_dtype && a->bias_dtype != LIK_F32) return LIK_ERR_UNSUPPORTED;
   if (a->in > 131071 || a->rows > 0x7fffff00 || a->out_features > (1 << 24)) return LIK_ERR_UNSUPPORTED;
-  const int64_t groups = ((a->rows + 63) / 64) * ((2ll * a->out_features + 63) / 64);
-  return groups < (1 << 24) ? LIK_OK : LIK_ERR_UNSUPPORTED;  // (a launch has less than 2^32 threads)
+  // a launch has less than 2^32 threads; walked tiles are counted in 31 bits
+  const Shape sh = shape_of(a->rows, a->gated ? glu_rows(a->out_features) : a->out_features, a->gated != 0, a->residual);
+  return few_rows(a->rows) || sh.tiles < (sh.tile > 1 ? 1ll << 30 : 1ll << 24) ? LIK_OK : LIK_ERR_UNSUPPORTED;
 }
 // Rows quantised in a launch of their own: the integers, then the scales.
 size_t linear_ws(const lik_linear_int8_t* a) {
@@ -939,7 +940,7 @@ int lik_linear_int8(const lik_linear_int8_t* a, void* out, void* workspace, size
   p.res = (const char*)a->residual;
   p.res_ld = a->residual_stride * ob;
   p.out = (char*)out;
-  p.rows16 = (uintptr_t)out % 16 == 0 && (int64_t)p.n * ob % 16 == 0;
+  p.rows16 = (uintptr_t)out % 16 == 0 && (int64_t)p.n * ob % 16 == 0 && 256ll * p.n * ob < kFar;
   p.act = a->activation;
   char* ws = workspace ? align256(workspace) : nullptr;
   hipStream_t s = (hipStream_t)stream;
