@@ -6,7 +6,9 @@
 // Bound by HBM: every element is read once and written once. A workgroup owns T consecutive tokens and holds
 // their cosines and sines in LDS, since all heads of q and of k share them. theta is taken in turns and
 // reduced to less than one in 64 bits (an fp32 angle of position 10^5 is off by 0.004), sine and cosine of
-// what is left are fp32, and so is the turn; it is rounded once.
+// what is left are fp32, and so is the turn; it is rounded once. Measured (a large copy: 5.03 TB/s): 44928 packed
+// tokens of 24 heads of 64, bf16, 55 us (5.0 TB/s); 16480 tokens of 20 heads of 128 of which a half is turned 36 us
+// (4.7); 20000 of 16 heads of 96 fp32, a quarter turned, interleaved 49 us (5.0); one query of 32 tokens 3.5 us.
 #include "lik_enc.h"
 
 namespace lik {

@@ -18,7 +18,8 @@ Submodules mirror the reference: ``forward``, ``score_pairs``, ``padded``,
 ``plaid_index``, and ``reference`` (eager PyTorch ground truth for callers'
 own comparisons; no op here uses it). ``encoder`` adds the operators of the
 transformer encoder that makes the token vectors: ``attention``,
-``attention_varlen``, ``layer_norm`` and ``gated_ffn``, differentiable.
+``attention_varlen``, ``layer_norm``, ``gated_ffn`` and ``rotary``, differentiable, and
+linear layers on 8-bit integers for inference.
 """
 
 from importlib.metadata import PackageNotFoundError
