@@ -43,7 +43,7 @@ def quantize_int8_per_token(X: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor
     _lib.require_gpu(X)
     _no_gradient("quantize_int8_per_token", X)
     out = torch.empty_like(X, dtype=torch.int8, memory_format=torch.contiguous_format)
-    scale = torch.empty(X.shape[:-1], dtype=torch.float32, device=X.device)
+    scale = X.new_empty(X.shape[:-1], dtype=torch.float32)
     if X.numel():
         x2, xs = _rows(X)
         rows, d = x2.shape
@@ -174,7 +174,7 @@ def linear_int8(
         raise ValueError("x, weight, their scales, bias and residual must be on the same device.")
     _lib.require_gpu(x)
     _no_gradient("linear_int8", x, weight_scale, bias, residual, x_scale)
-    out = torch.empty((*lead, n), dtype=out_dtype, device=device)
+    out = x.new_empty((*lead, n), dtype=out_dtype)
     if out.numel() == 0:
         return out
     x2, xs = _rows(x)
