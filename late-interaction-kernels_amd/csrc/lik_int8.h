@@ -93,7 +93,7 @@ __device__ __forceinline__ void chunk_to_int8(const u32x4& w, float s, float inv
 }
 
 // lik_quantize_int8; `stream`: rows are read past the caches. Alone that is the faster way (1,030,001 rows of 128 fp16 there
-// and back 137 against 153 us); in front of a product that reads its integers from the caches the slower one (124 against 119).
+// and back 137 against 153 us when the way back took 74); in front of a product that reads its integers from the caches the slower one (124 against 119).
 int quantize_rows_int8(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int32_t dim, int8_t* out,
                        int64_t out_stride, float* scale, bool stream, hipStream_t s);
 

@@ -1,9 +1,9 @@
 // Token vectors as 8-bit integers with a scale each, and back (the definition: lik_int8.h).
 //
 // Bound by HBM: a row stays in the registers of its lanes between the maximum and the conversion, so each
-// element is read once and one byte written; rows past 4096 elements (fp32: 2048) are read twice, the second
-// time from L2. Measured: 1,030,001 rows of 128 fp16 to integers 65 us (6.1 TB/s), back 72 us (5.5); 44801 rows of 1152 bf16 to
-// integers 29 us (5.3); 32961 rows of 1027 fp32 40 us (4.2) and 58 us (2.9): their rows start off 16 bytes.
+// element is read once and one byte written; rows past 16384 elements (fp32: 8192) are read twice, the second
+// time from L2. Measured: 1,030,001 rows of 128 fp16 to integers 67 us (6.0 TB/s), back 68 us (5.9); 44801 rows of 1152 bf16 to
+// integers 29 us (5.3); 32961 rows of 1027 fp32, which start off 16 bytes, 40 us (4.2) and 27 us (6.2).
 #include "lik_int8.h"
 
 namespace lik {
@@ -88,7 +88,49 @@ __global__ void __launch_bounds__(256) quantize_kernel(const QuantP p) {
   }
 }
 
-// Wider rows: a workgroup each, read twice.
+// Wider rows: a workgroup each, NV chunks a thread in registers.
+template <int EK, int NV, bool NT>
+__global__ void __launch_bounds__(256) quantize_row_kernel(const QuantP p) {
+  constexpr int V = El<EK>::V;
+  typedef u32x4 __attribute__((aligned(2))) u32x4_u;
+  __shared__ uint32_t s_m[4];
+  const int whole = p.dim / V;
+  for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+    const char* row = p.x + r * p.x_ld;
+    u32x4 w[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = j * 256 + (int)threadIdx.x;
+      const u32x4_u* at = (const u32x4_u*)row + (c < whole ? c : whole - 1);
+      if constexpr (NT) w[j] = __builtin_nontemporal_load(at);
+      else w[j] = *at;
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = j * 256 + (int)threadIdx.x;
+      if (c >= whole) w[j] = u32x4{0u, 0u, 0u, 0u};
+      if (p.dim % V && c == whole) chunk_load<EK>(row, c * V, p.dim, w[j]);
+      m = absmax_bits<EK>(w[j], m);
+    }
+    m = absmax_lanes<EK, 64>(m);
+    if (threadIdx.x % 64 == 0) s_m[threadIdx.x / 64] = m;
+    __syncthreads();
+    m = absmax_join<EK>(absmax_join<EK>(s_m[0], s_m[1]), absmax_join<EK>(s_m[2], s_m[3]));
+    float s, inv;
+    row_scale<EK>(m, s, inv);
+    if (threadIdx.x == 0) p.scale[r] = s;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      uint32_t q[V / 4];
+      chunk_to_int8<EK>(w[j], s, inv, q);
+      store_int8<V>(p.out + r * p.out_ld, (j * 256 + (int)threadIdx.x) * V, p.end, q);
+    }
+    __syncthreads();  // (s_m is the next row's)
+  }
+}
+
+// Wider still: read twice.
 template <int EK>
 __global__ void __launch_bounds__(256) quantize_wide_kernel(const QuantP p) {
   constexpr int V = El<EK>::V;
@@ -127,6 +169,11 @@ void launch_rows(const QuantP& p, hipStream_t s) {
   if (p.stream) launch_kernel(quantize_kernel<EK, LPR, NV, U, true>, grid, dim3(256), 0u, s, p);
   else launch_kernel(quantize_kernel<EK, LPR, NV, U, false>, grid, dim3(256), 0u, s, p);
 }
+template <int EK, int NV>
+void launch_row(const QuantP& p, hipStream_t s) {
+  if (p.stream) launch_kernel(quantize_row_kernel<EK, NV, true>, dim3(groups(p.rows)), dim3(256), 0u, s, p);
+  else launch_kernel(quantize_row_kernel<EK, NV, false>, dim3(groups(p.rows)), dim3(256), 0u, s, p);
+}
 template <int EK>
 int launch_quantize(const QuantP& p, hipStream_t s) {
   const int ch = (p.end + El<EK>::V - 1) / El<EK>::V;
@@ -146,6 +193,8 @@ int launch_quantize(const QuantP& p, hipStream_t s) {
   else if (ch <= 384) launch_rows<EK, 64, 6, 1>(p, s);
   else if (ch <= 448) launch_rows<EK, 64, 7, 1>(p, s);
   else if (ch <= 512) launch_rows<EK, 64, 8, 1>(p, s);
+  else if (ch <= 1024) launch_row<EK, 4>(p, s);
+  else if (ch <= 2048) launch_row<EK, 8>(p, s);
   else launch_kernel(quantize_wide_kernel<EK>, dim3(groups(p.rows)), dim3(256), 0u, s, p);
   return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;
 }
@@ -159,7 +208,8 @@ struct DequantP {
 };
 
 // LPR lanes a row, U rows and NC chunks of V elements at once, so that neighbouring lanes write neighbouring 16 bytes.
-// (Stores past the caches: 188 us there and back instead of 137 for the million rows.)
+// (A thread with 16 elements of its own instead: 32961 x 1027 fp32 58 us, now 27; stores past the caches: the million rows
+// there and back 188 us instead of 154.)
 template <int EK, int LPR, int NC, int U>
 __global__ void __launch_bounds__(256) dequantize_kernel(const DequantP p) {
   constexpr int B = El<EK>::B, V = El<EK>::V, RPW = 64 / LPR, W = V / 4;
@@ -219,7 +269,7 @@ int launch_dequantize(const DequantP& p, hipStream_t s) {
   const int ch = (p.dim + El<EK>::V - 1) / El<EK>::V;
   if (ch <= 32)  // 4 rows a wavefront, 4 times
     launch_kernel(dequantize_kernel<EK, 16, 1, 4>, dim3(groups((p.rows + 63) / 64)), dim3(256), 0u, s, p);
-  else
+  else  // a wavefront each
     launch_kernel(dequantize_kernel<EK, 64, 4, 1>, dim3(groups((p.rows + 3) / 4)), dim3(256), 0u, s, p);
   return hipGetLastError() == hipSuccess ? LIK_OK : LIK_ERR_LAUNCH;
 }

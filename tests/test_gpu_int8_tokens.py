@@ -125,3 +125,10 @@ def test_other_stream_and_graph():
         graph.replay()
         wq, ws = quantize_int8_per_token(x)
         assert torch.equal(q, wq) and torch.equal(s, ws) and torch.equal(y, dequantize_int8_per_token(wq, ws, BF))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("d", [4095, 4097, 6001, 8191, 8193, 16383, 16385])
+def test_wide_rows(dtype, d):
+    q, s = _check(torch.randn(5, d + 3, device="cuda").to(dtype)[:, 1:d + 1])
+    assert torch.equal(dequantize_int8_per_token(q, s), q.float() * s[:, None])
