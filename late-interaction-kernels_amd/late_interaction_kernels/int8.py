@@ -18,7 +18,7 @@ _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 def _no_gradient(what, *tensors):
     """8-bit integers carry no gradient: a call that would drop one is refused."""
-    if _lib.differentiates(*tensors):
+    if _lib.differentiates(*tensors):  # (or forward-mode differentiation is active)
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or on detached tensors")
 
 
@@ -36,19 +36,21 @@ def quantize_int8_per_token(X: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor
         ``(X_int8, scale)``: int8 of the shape of ``X`` and fp32 ``X.shape[:-1]``. A weight ``[out, in]``
         gives what :func:`linear_int8` takes.
     """
-    if X.dim() < 1 or not 1 <= X.shape[-1] <= 1 << 24:
-        raise ValueError(f"X must be [..., d] with 1 <= d <= 2^24; got {tuple(X.shape)}")
-    if X.dtype not in _DTYPES:
-        raise TypeError(f"quantize_int8_per_token takes fp16 / bf16 / fp32; got {X.dtype}")
+    shape, dtype = X.shape, X.dtype
+    if not shape or not 1 <= shape[-1] <= 1 << 24:
+        raise ValueError(f"X must be [..., d] with 1 <= d <= 2^24; got {tuple(shape)}")
+    if dtype not in _DTYPES:
+        raise TypeError(f"quantize_int8_per_token takes fp16 / bf16 / fp32; got {dtype}")
     _lib.require_gpu(X)
     _no_gradient("quantize_int8_per_token", X)
     out = torch.empty_like(X, dtype=torch.int8, memory_format=torch.contiguous_format)
-    scale = X.new_empty(X.shape[:-1], dtype=torch.float32)
-    if X.numel():
-        x2, xs = _rows(X)
-        rows, d = x2.shape
-        with _lib.on_device(X.device):
-            rc = _lib.load().lik_quantize_int8(x2.data_ptr(), xs, _lib.DTYPE_CODE[X.dtype], rows, d, out.data_ptr(), d,
+    scale = X.new_empty(shape[:-1], dtype=torch.float32)
+    x2, xs = _rows(X)
+    rows, d = x2.shape
+    if rows:
+        device = X.device
+        with _lib.on_device(device):
+            rc = _lib.load().lik_quantize_int8(x2.data_ptr(), xs, _lib.DTYPE_CODE[dtype], rows, d, out.data_ptr(), d,
                                                scale.data_ptr(), _lib.stream_of(X))
         _lib.check(rc, "lik_quantize_int8")
     return out, scale
@@ -61,22 +63,25 @@ def dequantize_int8_per_token(
     ``X_int8.shape[:-1]``."""
     if X_int8.dtype != torch.int8 or scale.dtype != torch.float32:
         raise TypeError(f"X_int8 must be int8 and scale fp32; got {X_int8.dtype} and {scale.dtype}")
-    if X_int8.dim() < 1 or not 1 <= X_int8.shape[-1] <= 1 << 24:
-        raise ValueError(f"X_int8 must be [..., d] with 1 <= d <= 2^24; got {tuple(X_int8.shape)}")
-    if scale.shape != X_int8.shape[:-1]:
-        raise ValueError(f"scale must be {list(X_int8.shape[:-1])}; got {tuple(scale.shape)}")
+    shape = X_int8.shape
+    if not shape or not 1 <= shape[-1] <= 1 << 24:
+        raise ValueError(f"X_int8 must be [..., d] with 1 <= d <= 2^24; got {tuple(shape)}")
+    if scale.shape != shape[:-1]:
+        raise ValueError(f"scale must be {list(shape[:-1])}; got {tuple(scale.shape)}")
     if dtype not in _DTYPES:
         raise TypeError(f"dequantize_int8_per_token gives fp16 / bf16 / fp32; got {dtype}")
-    if scale.device != X_int8.device:
+    device = X_int8.device
+    if scale.device != device:
         raise ValueError("X_int8 and scale must be on the same device.")
     _lib.require_gpu(X_int8)
     _no_gradient("dequantize_int8_per_token", scale)
     out = torch.empty_like(X_int8, dtype=dtype, memory_format=torch.contiguous_format)
-    if out.numel():
-        (x2, xs), scale = _rows(X_int8), scale.contiguous()
-        with _lib.on_device(out.device):
-            rc = _lib.load().lik_dequantize_int8(x2.data_ptr(), xs, scale.data_ptr(), _lib.DTYPE_CODE[dtype],
-                                                 x2.shape[0], x2.shape[1], out.data_ptr(), _lib.stream_of(out))
+    (x2, xs), scale = _rows(X_int8), scale if scale.is_contiguous() else scale.contiguous()
+    rows, d = x2.shape
+    if rows:
+        with _lib.on_device(device):
+            rc = _lib.load().lik_dequantize_int8(x2.data_ptr(), xs, scale.data_ptr(), _lib.DTYPE_CODE[dtype], rows, d,
+                                                 out.data_ptr(), _lib.stream_of(out))
         _lib.check(rc, "lik_dequantize_int8")
     return out
 
