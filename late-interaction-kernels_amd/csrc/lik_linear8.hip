@@ -334,6 +334,9 @@ linear8_kernel(const LinP p) {
   }
 }
 
+constexpr int64_t kFar = 0xfff00000ll;      // bytes that a lane's 32-bit offset reaches
+constexpr uint32_t kNoRow = 0xfff80000u;    // a lane offset past them, also with a block's place in a tile's row added
+
 // f(0), f(1), .. f(N - 1) as constants
 template <typename F, int... I>
 __device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F f) {
@@ -469,15 +472,17 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
   for (int d = 0; d < (DEF ? DEF : 1); ++d) later[d] = u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
-  for (int j = 0; j < MB; ++j) out_off[j][0] = out_off[j][1] = kOob;
+  for (int j = 0; j < MB; ++j) out_off[j][0] = out_off[j][1] = kNoRow;
   // Streamed past the caches where that is faster (44801 x 768 -> 2304 with its quantising launch: fp16 120 against 139 us;
   // 20000 rows to fp32: 92 against 84; with a residual no difference).
   constexpr int NT = OK == EK_F32 || RES ? 0 : 2;
   // Store O of a tile, of block (O / PER / MB, O / PER % MB): 16 rows (the block's first or last) of 64 bytes, so that the
-  // chunks of two lanes that are 16 apart have changed places.
+  // chunks of two lanes that are 16 apart have changed places. The block's place is part of the lane's offset and no scalar
+  // register: a 16-byte store reads its last registers up to two wait states after it is issued, the compiler counts those
+  // for stores with a constant offset only, and with a register a conversion right behind one went to memory in its place.
   auto put = [&](auto O, const u32x4& v) {
     constexpr int o = decltype(O)::value, g = o % PER, j = o / PER % MB, i = o / PER / MB;
-    __builtin_amdgcn_raw_buffer_store_b128(v, out_desc, out_off[j][g & 1], i * 32 * El<OK>::B + g / 2 * 64, NT);
+    __builtin_amdgcn_raw_buffer_store_b128(v, out_desc, out_off[j][g & 1] + (i * 32 * El<OK>::B + g / 2 * 64), 0, NT);
   };
 
   load_tile_cols(t);
@@ -541,7 +546,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
     if constexpr (RES) ask_res(S0);
     const bool edge = !p.rows16 || n0 + TN / PAIR > p.n;
     const int64_t out_ld = (int64_t)p.n * El<OK>::B;
-    out_desc = __builtin_amdgcn_make_buffer_rsrc(p.out + m0 * out_ld + n0 * El<OK>::B, (short)0, (int)0xffffff00u, 0x00020000);
+    out_desc = __builtin_amdgcn_make_buffer_rsrc(p.out + m0 * out_ld + n0 * El<OK>::B, (short)0, (int)kFar, 0x00020000);
     float sx[MB];
 #pragma unroll
     for (int j = 0; j < MB; ++j) {
@@ -551,7 +556,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
       for (int g = 0; g < 2; ++g) {
         const int ro = wm * (TM / WM) + j * 32 + g * 16 + (lane & 15);
         out_off[j][g] = edge || m0 + ro >= p.m
-                            ? kOob
+                            ? kNoRow
                             : (uint32_t)(ro * out_ld + wn * (TN / WN / PAIR) * El<OK>::B + (lane & 16) * 2 + h * 16);
       }
     }
@@ -885,7 +890,6 @@ int run(const lik_linear_int8_t* a, LinP p, char* ws, hipStream_t s) {
   return few ? launch_few<kInt8, OK, GLU>(p, s) : launch_gemm<OK, GLU>(p, s);
 }
 
-constexpr int64_t kFar = 0xfff00000ll;  // bytes that a lane's 32-bit offset reaches
 int linear_check(const lik_linear_int8_t* a) {
   const auto is_float = [](int32_t t) { return t == LIK_BF16 || t == LIK_F16 || t == LIK_F32; };
   if (!is_float(a->out_dtype) || !(is_float(a->x_dtype) || a->x_dtype == LIK_INT8)) return LIK_ERR_UNSUPPORTED;
