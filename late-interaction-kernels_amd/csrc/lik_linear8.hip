@@ -86,11 +86,15 @@ __device__ __forceinline__ void store4(char* row, int n, int end, const float* v
     }
 }
 // n: the block's first column, `more`: rows of the weight before it (the up half: n hidden ones)
+__device__ __forceinline__ void load_scales(const LinP& p, f32x4* s, int n, int more, int h) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) s[q] = load4<EK_F32>((const char*)(p.sw + more), true, n + 8 * q + 4 * h, p.n);
+}
 template <int OK>
 __device__ __forceinline__ void load_cols(const LinP& p, Cols& c, int n, int more, int h) {
+  load_scales(p, c.s, n, more, h);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    c.s[q] = load4<EK_F32>((const char*)(p.sw + more), true, n + 8 * q + 4 * h, p.n);
     c.b[q] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (p.bias)
       c.b[q] = load4<OK>(p.bias + (int64_t)more * (OK == EK_F32 || p.bias32 ? 4 : 2), p.bias32, n + 8 * q + 4 * h, p.n);
@@ -127,6 +131,23 @@ __device__ __forceinline__ void activate(int act, float* v) {
   for (int e = 0; e < 8; ++e) v[e] = y[e];
 }
 
+// A sum is scaled as (sum * sx) * sw + b: the scales' own product may leave fp32's range where the result does not (1e-25 and
+// 1e-18: under 2^-126, which keeps a few bits; 1e20 and 1e20: an infinity, which a sum of zero makes NaN). The first product
+// is exact or normal, and finite unless sx is past 2^96 (sums reach 2^31). Such a token gives 2^64 of its scale to the
+// weights': near_scale for the token, lift_scales for copies of the weights' scales (past 2^63 the largest float will do: a
+// sum other than zero makes either infinite). Kernels ask once whether a wavefront has such rows, so that all others do without.
+__device__ __forceinline__ bool far_scale(float sx) { return fabsf(sx) > 0x1p96f; }
+__device__ __forceinline__ uint64_t far_rows(float sx) { return __builtin_amdgcn_ballot_w64(far_scale(sx)); }
+__device__ __forceinline__ float near_scale(float sx) { return far_scale(sx) ? sx * 0x1p-64f : sx; }
+template <int NQ>
+__device__ __forceinline__ void lift_scales(f32x4* sw, bool far) {
+#pragma unroll
+  for (int e = 0; e < 4 * NQ; ++e) {
+    const float w = sw[e / 4][e % 4], a = fabsf(w);
+    if (far) sw[e / 4][e % 4] = a > 0x1p63f && a < INFINITY ? copysignf(0x1.fffffep127f, w) : w * 0x1p64f;
+  }
+}
+
 // Weight scales and biases of a lane's columns in 16 of a block: two quads.
 struct Cols8 {
   f32x4 s[2], b[2];
@@ -138,11 +159,11 @@ __device__ __forceinline__ void group_outputs(const LinP& p, const int* c0, cons
                                               const Cols8& w1, const u32x4* r, float sx, u32x4* out) {
   float v[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = fmaf((float)c0[e], sx * w0.s[e / 4][e % 4], w0.b[e / 4][e % 4]);
+  for (int e = 0; e < 8; ++e) v[e] = fmaf((float)c0[e] * sx, w0.s[e / 4][e % 4], w0.b[e / 4][e % 4]);
   activate(p.act, v);
   if constexpr (GLU)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] *= fmaf((float)c1[e], sx * w1.s[e / 4][e % 4], w1.b[e / 4][e % 4]);
+    for (int e = 0; e < 8; ++e) v[e] *= fmaf((float)c1[e] * sx, w1.s[e / 4][e % 4], w1.b[e / 4][e % 4]);
   if constexpr (OK == EK_F32) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) out[e / 4][e % 4] = __float_as_uint(RES ? v[e] + __uint_as_float(r[e / 4][e % 4]) : v[e]);
@@ -240,6 +261,13 @@ linear8_kernel(const LinP p) {
   const int tm = (int)(t / (uint32_t)p.tiles_n), tn = (int)(t % (uint32_t)p.tiles_n);
   const int m0 = tm * TM, n0 = tn * (TN / PAIR);
   const int steps = (p.k + BK - 1) / BK;
+  const int l32 = lane & 31, h = lane >> 5;
+  float sx[MB];  // (first of all loads, which are waited for in order)
+#pragma unroll
+  for (int j = 0; j < MB; ++j) {
+    const int m = m0 + wm * (TM / WM) + j * 32 + l32;
+    sx[j] = m < p.m ? p.sx[m] : 0.f;
+  }
 
   uint32_t offa[SA::NI], offb[SB::NI];
   SA::offsets(offa, wv, lane, p.a_ld, p.m - m0, false, 0);
@@ -311,12 +339,11 @@ linear8_kernel(const LinP p) {
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load is in flight to LDS when the workgroup ends
 
-  const int l32 = lane & 31, h = lane >> 5;
-  float sx[MB];
+  uint64_t far = 0;
 #pragma unroll
   for (int j = 0; j < MB; ++j) {
-    const int m = m0 + wm * (TM / WM) + j * 32 + l32;
-    sx[j] = m < p.m ? p.sx[m] : 0.f;
+    far |= far_rows(sx[j]);
+    sx[j] = near_scale(sx[j]);
   }
 #pragma unroll
   for (int i = 0; i < NB; i += PAIR) {
@@ -327,6 +354,15 @@ linear8_kernel(const LinP p) {
 #pragma unroll
     for (int j = 0; j < MB; ++j) {
       const int m = m0 + wm * (TM / WM) + j * 32 + l32;
+      if (__builtin_expect(far != 0, false)) {  // (loaded again: the last rows' may be lifted)
+        const bool lift = m < p.m && far_scale(p.sx[m]);
+        load_scales(p, w0.s, n, 0, h);
+        lift_scales<4>(w0.s, lift);
+        if (GLU) {
+          load_scales(p, w1.s, n, p.n, h);
+          lift_scales<4>(w1.s, lift);
+        }
+      }
       Res<OK> r;
       load_res<OK>(p, r, m, n, h);
       finish_block<OK, GLU>(p, acc[i][j], acc[i + PAIR - 1][j], w0, w1, r, sx[j], m, n, h);
@@ -548,10 +584,12 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
     const int64_t out_ld = (int64_t)p.n * El<OK>::B;
     out_desc = __builtin_amdgcn_make_buffer_rsrc(p.out + m0 * out_ld + n0 * El<OK>::B, (short)0, (int)kFar, 0x00020000);
     float sx[MB];
+    uint64_t far = 0;
 #pragma unroll
     for (int j = 0; j < MB; ++j) {
       const int r = wm * (TM / WM) + j * 32 + l32;
-      sx[j] = s_sx[buf][r];
+      far |= far_rows(s_sx[buf][r]);
+      sx[j] = near_scale(s_sx[buf][r]);
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         const int ro = wm * (TM / WM) + j * 32 + g * 16 + (lane & 15);
@@ -577,6 +615,17 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         }
         each<MB>([&](auto J) {
           constexpr int j = decltype(J)::value;
+          if (__builtin_expect(far != 0, false)) {  // (loaded again: the last rows' may be lifted)
+            const bool lift = far_scale(s_sx[buf][wm * (TM / WM) + j * 32 + l32]);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const int at = wn * (TN / WN) + i * PAIR * 32 + 16 * g + 8 * q + 4 * h;
+              w0.s[q] = *(const f32x4*)&s_sw[buf][at];
+              if (GLU) w1.s[q] = *(const f32x4*)&s_sw[buf][at + 32];
+            }
+            lift_scales<2>(w0.s, lift);
+            if (GLU) lift_scales<2>(w1.s, lift);
+          }
           int a0[8], a1[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) a0[e] = acc[i * PAIR][j][8 * g + e], a1[e] = acc[i * PAIR + PAIR - 1][j][8 * g + e];
@@ -780,9 +829,12 @@ __global__ void __launch_bounds__(512) few_rows8_kernel(const LinP p) {
     sum += *(const i32x4*)s_sum[w][wv][lane];
     if (GLU) up += *(const i32x4*)s_sum[w][wv][lane + 32];
   }
+  lift_scales<1>(&s0, far_scale(s));
+  if (GLU) lift_scales<1>(&s1, far_scale(s));
+  s = near_scale(s);
   float v[8], y[8];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = v[e + 4] = fmaf((float)sum[e], s * s0[e], b0[e]);
+  for (int e = 0; e < 4; ++e) v[e] = v[e + 4] = fmaf((float)sum[e] * s, s0[e], b0[e]);
   if (p.act >= 0) {
     act8<false>(p.act, v, y, nullptr);
 #pragma unroll
@@ -790,7 +842,7 @@ __global__ void __launch_bounds__(512) few_rows8_kernel(const LinP p) {
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    if (GLU) v[e] *= fmaf((float)up[e], s * s1[e], b1[e]);
+    if (GLU) v[e] *= fmaf((float)up[e] * s, s1[e], b1[e]);
     v[e] += res[e];
   }
   store4<OK>(p.out + m * ((int64_t)p.n * El<OK>::B), c, p.n, v);
