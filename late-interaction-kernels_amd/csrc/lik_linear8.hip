@@ -85,16 +85,17 @@ __device__ __forceinline__ void store4(char* row, int n, int end, const float* v
       else ((uint16_t*)row)[n + e] = (uint16_t)f32_to_el<OK>(v[e]);
     }
 }
-// n: the block's first column, `more`: rows of the weight before it (the up half: n hidden ones)
-__device__ __forceinline__ void load_scales(const LinP& p, f32x4* s, int n, int more, int h) {
+// n: the block's first column, `more`: rows of the weight before it (the up half: n hidden ones). Of its two groups of 16
+// columns those from g on, ng of them (here and below).
+__device__ __forceinline__ void load_scales(const LinP& p, f32x4* s, int n, int more, int h, int g, int ng) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) s[q] = load4<EK_F32>((const char*)(p.sw + more), true, n + 8 * q + 4 * h, p.n);
+  for (int q = 2 * g; q < 2 * (g + ng); ++q) s[q] = load4<EK_F32>((const char*)(p.sw + more), true, n + 8 * q + 4 * h, p.n);
 }
 template <int OK>
-__device__ __forceinline__ void load_cols(const LinP& p, Cols& c, int n, int more, int h) {
-  load_scales(p, c.s, n, more, h);
+__device__ __forceinline__ void load_cols(const LinP& p, Cols& c, int n, int more, int h, int g, int ng) {
+  load_scales(p, c.s, n, more, h, g, ng);
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
+  for (int q = 2 * g; q < 2 * (g + ng); ++q) {
     c.b[q] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (p.bias)
       c.b[q] = load4<OK>(p.bias + (int64_t)more * (OK == EK_F32 || p.bias32 ? 4 : 2), p.bias32, n + 8 * q + 4 * h, p.n);
@@ -114,19 +115,22 @@ __device__ __forceinline__ int chunk_column(int j, int h) {
   return OK == EK_F32 ? 8 * j + 4 * h : 16 * j + 8 * h;
 }
 template <int OK>
-__device__ __forceinline__ void load_res(const LinP& p, Res<OK>& r, int m, int n, int h) {
+__device__ __forceinline__ void load_res(const LinP& p, Res<OK>& r, int m, int n, int h, int g = 0, int ng = 2) {
+  constexpr int C = kResChunks<OK> / 2;
 #pragma unroll
-  for (int j = 0; j < kResChunks<OK>; ++j) {
+  for (int j = C * g; j < C * (g + ng); ++j) {
     r.x[j] = u32x4{0u, 0u, 0u, 0u};
     const int c = n + chunk_column<OK>(j, h);
     if (p.res && m < p.m && c < p.n) chunk_load<OK>(p.res + m * p.res_ld, c, p.n, r.x[j]);
   }
 }
 
+template <int OK>
 __device__ __forceinline__ void activate(int act, float* v) {
   if (act < 0) return;
   float y[8];
-  act8<false>(act, v, y, nullptr);
+  if constexpr (OK == EK_F32) act8_f32(act, v, y);
+  else act8<false>(act, v, y, nullptr);
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = y[e];
 }
@@ -160,7 +164,7 @@ __device__ __forceinline__ void group_outputs(const LinP& p, const int* c0, cons
   float v[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = fmaf((float)c0[e] * sx, w0.s[e / 4][e % 4], w0.b[e / 4][e % 4]);
-  activate(p.act, v);
+  activate<OK>(p.act, v);
   if constexpr (GLU)
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] *= fmaf((float)c1[e] * sx, w1.s[e / 4][e % 4], w1.b[e / 4][e % 4]);
@@ -183,13 +187,13 @@ __device__ __forceinline__ void group_outputs(const LinP& p, const int* c0, cons
     out[0] = join_halves(pack2<OK>(v[0], v[1]), pack2<OK>(v[2], v[3]), pack2<OK>(v[4], v[5]), pack2<OK>(v[6], v[7]));
   }
 }
-template <int OK, bool GLU, int NJ = 2>
-__device__ __forceinline__ void finish_block(const LinP& p, const i32x16& c0, const i32x16& c1, const Cols& w0,
-                                             const Cols& w1, const Res<OK>& r, float sx, int m, int n, int h) {
+template <int OK, bool GLU>
+__device__ __forceinline__ void finish_block(const LinP& p, const i32x16& c0, const i32x16& c1, const Cols& w0, const Cols& w1,
+                                             const Res<OK>& r, float sx, int m, int n, int h, int g0, int ng) {
   constexpr int C = kResChunks<OK> / 2;  // chunks of a group
   char* row = p.out + m * ((int64_t)p.n * El<OK>::B);
 #pragma unroll
-  for (int g = 0; g < NJ; ++g) {
+  for (int g = g0; g < g0 + ng; ++g) {
     int a0[8], a1[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) a0[e] = c0[8 * g + e], a1[e] = c1[8 * g + e];
@@ -345,29 +349,32 @@ linear8_kernel(const LinP p) {
     far |= far_rows(sx[j]);
     sx[j] = near_scale(sx[j]);
   }
+  constexpr int NG = GLU && OK == EK_F32 ? 1 : 2;  // groups of columns at once, as many as the registers hold scales and biases of
 #pragma unroll
-  for (int i = 0; i < NB; i += PAIR) {
-    const int n = n0 + wn * (TN / WN / PAIR) + i / PAIR * 32;
-    Cols w0, w1;
-    load_cols<OK>(p, w0, n, 0, h);
-    if (GLU) load_cols<OK>(p, w1, n, p.n, h);
+  for (int i = 0; i < NB; i += PAIR)
 #pragma unroll
-    for (int j = 0; j < MB; ++j) {
-      const int m = m0 + wm * (TM / WM) + j * 32 + l32;
-      if (__builtin_expect(far != 0, false)) {  // (loaded again: the last rows' may be lifted)
-        const bool lift = m < p.m && far_scale(p.sx[m]);
-        load_scales(p, w0.s, n, 0, h);
-        lift_scales<4>(w0.s, lift);
-        if (GLU) {
-          load_scales(p, w1.s, n, p.n, h);
-          lift_scales<4>(w1.s, lift);
+    for (int g = 0; g < 2; g += NG) {
+      const int n = n0 + wn * (TN / WN / PAIR) + i / PAIR * 32;
+      Cols w0, w1;
+      load_cols<OK>(p, w0, n, 0, h, g, NG);
+      if (GLU) load_cols<OK>(p, w1, n, p.n, h, g, NG);
+#pragma unroll
+      for (int j = 0; j < MB; ++j) {
+        const int m = m0 + wm * (TM / WM) + j * 32 + l32;
+        if (__builtin_expect(far != 0, false)) {  // (loaded again: the last rows' may be lifted)
+          const bool lift = m < p.m && far_scale(p.sx[m]);
+          load_scales(p, w0.s, n, 0, h, g, NG);
+          lift_scales<2 * NG>(w0.s + 2 * g, lift);
+          if (GLU) {
+            load_scales(p, w1.s, n, p.n, h, g, NG);
+            lift_scales<2 * NG>(w1.s + 2 * g, lift);
+          }
         }
+        Res<OK> r;
+        load_res<OK>(p, r, m, n, h, g, NG);
+        finish_block<OK, GLU>(p, acc[i][j], acc[i + PAIR - 1][j], w0, w1, r, sx[j], m, n, h, g, NG);
       }
-      Res<OK> r;
-      load_res<OK>(p, r, m, n, h);
-      finish_block<OK, GLU>(p, acc[i][j], acc[i + PAIR - 1][j], w0, w1, r, sx[j], m, n, h);
     }
-  }
 }
 
 constexpr int64_t kFar = 0xfff00000ll;      // bytes that a lane's 32-bit offset reaches
@@ -832,14 +839,10 @@ __global__ void __launch_bounds__(512) few_rows8_kernel(const LinP p) {
   lift_scales<1>(&s0, far_scale(s));
   if (GLU) lift_scales<1>(&s1, far_scale(s));
   s = near_scale(s);
-  float v[8], y[8];
+  float v[8];
 #pragma unroll
   for (int e = 0; e < 4; ++e) v[e] = v[e + 4] = fmaf((float)sum[e] * s, s0[e], b0[e]);
-  if (p.act >= 0) {
-    act8<false>(p.act, v, y, nullptr);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = y[e];
-  }
+  activate<OK>(p.act, v);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     if (GLU) v[e] *= fmaf((float)up[e] * s, s1[e], b1[e]);
