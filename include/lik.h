@@ -639,7 +639,7 @@ int lik_dequantize_int8(const int8_t* x, int64_t x_stride, const float* scale, i
  * weight_scale and bias (null: none; of out_dtype or fp32) of as many elements; its rows start on 16 bytes and
  * are readable to the next multiple of 16 (what is there does not matter). activation -1: none,
  * else as in lik_gated_ffn. residual (null: none) is of out_dtype. Sums are exact
- * integers (in <= 131071); out is contiguous, of bf16 / fp16 / fp32, rounded once.
+ * integers (in <= 131071, or 131072 where x holds integers of which the last column is zeros); out is contiguous, of bf16 / fp16 / fp32, rounded once.
  */
 #define LIK_INT8 4
 typedef struct {

@@ -951,7 +951,8 @@ int linear_check(const lik_linear_int8_t* a) {
   if (a->rows < 0 || a->in < 1 || a->out_features < 1 || a->activation < -1 || a->activation > ACT_SILU)
     return LIK_ERR_INVALID;
   if (a->bias && a->bias_dtype != a->out_dtype && a->bias_dtype != LIK_F32) return LIK_ERR_UNSUPPORTED;
-  if (a->in > 131071 || a->rows > 0x7fffff00 || a->out_features > (1 << 24)) return LIK_ERR_UNSUPPORTED;
+  // (131072 integers: the caller's 131071 or fewer and zeros)
+  if (a->in > (a->x_dtype == LIK_INT8 ? 131072 : 131071) || a->rows > 0x7fffff00 || a->out_features > (1 << 24)) return LIK_ERR_UNSUPPORTED;
   // a launch has less than 2^32 threads; walked tiles are counted in 31 bits
   const Shape sh = shape_of(a->rows, a->gated ? glu_rows(a->out_features) : a->out_features, a->gated != 0, a->residual);
   return few_rows(a->rows) || sh.tiles < (sh.tile > 1 ? 1ll << 30 : 1ll << 24) ? LIK_OK : LIK_ERR_UNSUPPORTED;
