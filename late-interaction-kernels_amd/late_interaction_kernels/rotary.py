@@ -17,6 +17,7 @@ from . import _lib
 from ._core import _i32
 
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+_LARGEST = torch.finfo(torch.float32).max
 
 
 def rotary_frequencies(
@@ -237,8 +238,8 @@ def rotary(
     elif len(lead) == 1:
         raise ValueError("packed rows need cu_seqlens or positions")
     amplitude = float(amplitude)
-    if not math.isfinite(amplitude):
-        raise ValueError(f"amplitude must be finite; got {amplitude}")
+    if not abs(amplitude) <= _LARGEST:
+        raise ValueError(f"amplitude must be a finite fp32 number; got {amplitude}")
     if frequencies.device != device:
         raise ValueError("q, k, frequencies, positions and cu_seqlens must be on the same device.")
     _lib.require_gpu(q)
