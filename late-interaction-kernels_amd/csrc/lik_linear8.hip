@@ -859,19 +859,21 @@ bool few_rows(int64_t m) { return m <= 64; }
 bool quantise_within(int64_t m, int64_t k) { return (m <= 16 ? 16 : m <= 32 ? 32 : 64) * k <= 32 * 1024; }
 
 struct Shape {
-  // 256, 192: tiles of 256 x as many, walked, where those of 256 x 256 fill the CUs (their time is as the rounds by 1 to 0.78: 44801
-  // rows 768 -> 2304 99 us by 7 rounds of 256, 103 by 9 of 192; 1152 -> 768 73 us by 3 of 256, 61 by 3 of 192; a residual's
-  // registers leave only 192); 1: 256 x 128, where those fill the CUs; 0: 128 x 64 (gated: 64 x 128)
+  // 256, 192: tiles of 256 x as many, walked, where those of 256 x 256 fill the CUs. A round of 192 takes 0.78 of one of 256 at
+  // short k and 0.82 at longer (integers to bf16: 51200 x 768 -> 2304 120 us by 8 rounds of 256, 124 by 10 of 192; 88064 x 768 ->
+  // 1536 135 by 9, 143 by 11; 56320 x 768 -> 1152 73 by 5, 73 by 6; 56320 x 768 -> 1536 94 by 6, 91 by 7; with k = 384 the same
+  // four 85 and 80, 98 and 93, 54 and 50, 67 and 61, and 88064 x 384 -> 1152 73 by 7, 76 by 9). A residual's registers leave only
+  // 192. 1: 256 x 128, where those fill the CUs; 0: 128 x 64 (gated: 64 x 128)
   int tile;
   int64_t tiles_n, tiles;
 };
 // n: rows of the weight's tiles
-Shape shape_of(int64_t m, int64_t n, bool glu, bool res) {
+Shape shape_of(int64_t m, int64_t n, int64_t k, bool glu, bool res) {
   const int64_t rt = (m + 255) / 256;
   const auto rounds = [&](int64_t tn) { return (rt * ((n + tn - 1) / tn) + kCUs - 1) / kCUs; };
   int tile = rt * ((n + 127) / 128) >= kCUs ? 1 : 0;
   if (rt * ((n + 255) / 256) >= kCUs && !(glu && res))
-    tile = glu || (!res && 100 * rounds(256) <= 78 * rounds(192)) ? 256 : 192;
+    tile = glu || (!res && 100 * rounds(256) <= (k > 512 ? 82 : 78) * rounds(192)) ? 256 : 192;
   const int64_t tm = tile ? 256 : glu ? 64 : 128, tn = tile > 1 ? tile : tile || glu ? 128 : 64;
   const int64_t cols = (n + tn - 1) / tn, tiles = (m + tm - 1) / tm * cols;
   return Shape{tile, cols, tiles};
@@ -899,7 +901,7 @@ int launch_stream(const LinP& p, int tile, hipStream_t s) {
 }
 template <int OK, bool GLU>
 int launch_gemm(LinP p, hipStream_t s) {
-  const Shape sh = shape_of(p.m, GLU ? glu_rows(p.n) : p.n, GLU, p.res != nullptr);
+  const Shape sh = shape_of(p.m, GLU ? glu_rows(p.n) : p.n, p.k, GLU, p.res != nullptr);
   p.tiles_n = (int)sh.tiles_n;
   p.tiles = (int)sh.tiles;
   if constexpr (!GLU)
@@ -954,7 +956,7 @@ int linear_check(const lik_linear_int8_t* a) {
   // (131072 integers: the caller's 131071 or fewer and zeros)
   if (a->in > (a->x_dtype == LIK_INT8 ? 131072 : 131071) || a->rows > 0x7fffff00 || a->out_features > (1 << 24)) return LIK_ERR_UNSUPPORTED;
   // a launch has less than 2^32 threads; walked tiles are counted in 31 bits
-  const Shape sh = shape_of(a->rows, a->gated ? glu_rows(a->out_features) : a->out_features, a->gated != 0, a->residual);
+  const Shape sh = shape_of(a->rows, a->gated ? glu_rows(a->out_features) : a->out_features, a->in, a->gated != 0, a->residual);
   return few_rows(a->rows) || sh.tiles < (sh.tile > 1 ? 1ll << 30 : 1ll << 24) ? LIK_OK : LIK_ERR_UNSUPPORTED;
 }
 // Rows quantised in a launch of their own: the integers, then the scales.

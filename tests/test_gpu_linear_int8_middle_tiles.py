@@ -40,3 +40,10 @@ def test_integers_are_the_definitions(rows, k, xt):
     x = torch.randn(rows, k, device="cuda").to(xt)
     wq, ws = (t.cuda() for t in _want(torch.randn(96, k) * k**-0.5))
     _check(linear_int8(x, wq, ws), *_want(x), wq, ws)
+
+
+@pytest.mark.parametrize("k", [512, 528])
+@pytest.mark.parametrize("ot", [BF, FP])
+def test_both_sides_of_the_width_of_walked_tiles(k, ot):
+    """4 rounds of 256 columns or 5 of 192, by the number of steps."""
+    _run(65793, k, 768, ot, bias=True)
