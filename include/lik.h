@@ -626,7 +626,7 @@ int lik_rotary(const lik_rotary_t* a, void* q_out, void* k_out, lik_stream_t str
  */
 int lik_quantize_int8(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int32_t dim, int8_t* out,
                       int64_t out_stride, float* scale, lik_stream_t stream);
-/* And back: out [rows, dim], contiguous, of dtype = x * scale, rounded once. */
+/* And back: out [rows, dim], contiguous, of dtype = x * scale in fp32, then rounded to dtype. */
 int lik_dequantize_int8(const int8_t* x, int64_t x_stride, const float* scale, int32_t dtype, int64_t rows, int32_t dim,
                         void* out, lik_stream_t stream);
 
@@ -639,7 +639,9 @@ int lik_dequantize_int8(const int8_t* x, int64_t x_stride, const float* scale, i
  * weight_scale and bias (null: none; of out_dtype or fp32) of as many elements; its rows start on 16 bytes and
  * are readable to the next multiple of 16 (what is there does not matter). activation -1: none,
  * else as in lik_gated_ffn. residual (null: none) is of out_dtype. Sums are exact
- * integers (in <= 131071, or 131072 where x holds integers of which the last column is zeros); out is contiguous, of bf16 / fp16 / fp32, rounded once.
+ * integers (in <= 131071, or 131072 where x holds integers of which the last column is zeros), everything
+ * after them is fp32, rounded once to out_dtype; out is contiguous, of bf16 / fp16 / fp32. The erf gelu of 16-bit
+ * outputs is off by up to 1e-7 |v|, that of fp32 ones by fp32's roundings.
  */
 #define LIK_INT8 4
 typedef struct {

@@ -1,5 +1,6 @@
 // Device helpers shared by the encoder operators (layer norm, gated
-// feed-forward block, attention).
+// feed-forward block, attention, rotary positions, 8-bit tokens and linear
+// layers).
 #pragma once
 #include "lik_common.h"
 
@@ -7,7 +8,8 @@ namespace lik {
 namespace enc {
 
 // Element types of the encoder operators: 16-bit ones as the MFMA operands
-// name them, fp32 for the layer norm.
+// name them, fp32 for those that take or give it (norm, rotation, 8-bit
+// tokens and linear layers).
 template <int EK>
 struct El {
   static constexpr int B = EK == EK_F32 ? 4 : 2;  // bytes

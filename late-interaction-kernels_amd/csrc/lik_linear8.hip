@@ -248,8 +248,9 @@ struct Stage {
   }
 };
 
-// Fewer tiles than CUs: a workgroup of WM x WN wavefronts owns a TM x TN tile and walks k in steps of 64 bytes, NS of them in
-// LDS: the loads of step i + NS - 1 start while step i is multiplied. 300 rows 768 -> 2304 in 9 us with the host's part of the call.
+// Too few tiles for the walk below: a workgroup of WM x WN wavefronts owns a TM x TN tile and goes along k in steps of 64 bytes, NS of
+// them in LDS: the loads of step i + NS - 1 start while step i is multiplied. Tiles of 256 x 128 where those fill the CUs (16481 rows of
+// integers 768 -> 768 21 us), else of 128 x 64 (300 rows of bf16 768 -> 2304 10.3 us with their quantising), gated 64 x 128.
 template <int OK, bool GLU, int TM, int TN, int WM, int WN, int NS, int OCC>
 __global__ void __launch_bounds__(WM* WN * 64) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
 linear8_kernel(const LinP p) {
@@ -395,7 +396,7 @@ __device__ __forceinline__ void each(F f) {
 // registers for the next tile's steps, so that the writes of all CUs do not come in bursts with nothing else to do.
 // The waits count: a step waits for its own loads only, with all younger loads and stores in flight. So every
 // store is issued whatever its lanes hold (a lane without an output names an offset out of range), and column
-// edges, which store element by element, wait for everything. Two workgroups a CU with tiles of 256 x 128 instead
+// edges, which store element by element, wait for everything (44801 x 768 -> 2305 184 us). Two workgroups a CU with tiles of 256 x 128 instead
 // fall into step and do not overlap. 44801 rows 768 -> 2304 fp16 99 us (256 x 128 tiles: 134), 1152 -> 768 with a residual
 // 76 us (98), 16480 rows 1024 -> 2 x 2816 with silu 112 us (125).
 template <int OK, bool GLU, bool RES, int TN, int DEF>
@@ -683,7 +684,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
 // to registers as they lie, the eight sums meet in LDS. Rows that are no integers yet are quantised on the way, by every
 // workgroup for itself: the wavefronts' maxima meet in LDS first. 768 -> 2304 features of integers: 1 row 3.1 us, 32 rows 3.8, 64
 // rows 4.8 (32 weight rows a workgroup: 32 rows 9.8 us with quantising, now 7.3); 4096 -> 4096: 5.2, 8.4, 12.2.
-constexpr int kInt8 = EK_FP8;  // XK: 8-bit integers
+constexpr int kInt8 = 8;  // XK: 8-bit integers, next to the element types
 template <int XK, int OK, bool GLU, int MB>
 __global__ void __launch_bounds__(512) few_rows8_kernel(const LinP p) {
   constexpr int NW = 8, U = XK == kInt8 ? 4 : XK == EK_F32 ? 1 : 2;
@@ -887,7 +888,7 @@ int launch_tiles(const LinP& p, hipStream_t s) {
 }
 template <int OK, bool GLU, bool RES>
 int launch_stream(const LinP& p, int tile, hipStream_t s) {
-  // Deferred stores: with a residual they change nothing (105 us either way below), its reads are what takes the time.
+  // Deferred stores: with a residual they change nothing (44801 x 1152 -> 768 105 us either way), its reads are what takes the time.
   constexpr int DEF = RES ? 0 : 8;
   const unsigned groups = p.tiles < kCUs ? p.tiles : kCUs;
   if constexpr (!GLU)

@@ -59,8 +59,9 @@ def quantize_int8_per_token(X: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor
 def dequantize_int8_per_token(
     X_int8: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.float32
 ) -> torch.Tensor:
-    """``X_int8 * scale`` of each row, rounded once to ``dtype`` (fp16 / bf16 / fp32); ``scale`` is fp32
-    ``X_int8.shape[:-1]``."""
+    """``X_int8 * scale`` of each row in fp32, then rounded to ``dtype`` (fp16 / bf16 / fp32); ``scale`` is fp32
+    ``X_int8.shape[:-1]``. This is how an index or hidden states held in 8 bits get
+    back to the operators that read 16-bit or fp32 rows (MaxSim among them)."""
     if X_int8.dtype != torch.int8 or scale.dtype != torch.float32:
         raise TypeError(f"X_int8 must be int8 and scale fp32; got {X_int8.dtype} and {scale.dtype}")
     shape = X_int8.shape
@@ -131,9 +132,10 @@ def linear_int8(
         out_dtype: fp16 / bf16 / fp32; default the type of ``x`` (int8: bf16).
 
     Returns:
-        ``[..., out]``, everything after the integer sums in fp32 and rounded once. ``in`` is a multiple
-        of 16 in the kernels; a weight of another width (int8 ``x`` too) is padded in a copy per
-        call, unless its rows lie a multiple of 16 bytes apart (a slice of a wider one).
+        ``[..., out]``, everything after the integer sums in fp32 and rounded once ("gelu" of 16-bit
+        outputs is off by up to 1e-7 of its argument). ``in`` is a multiple of 16 in the kernels; a weight of another
+        width (int8 ``x`` too) is padded in a copy per call, unless its rows lie a multiple of 16 bytes apart (a
+        slice of a wider one).
     """
     if activation is not None and activation not in ACTIVATIONS:
         raise ValueError(f"activation must be None or one of {sorted(ACTIVATIONS)}; got {activation!r}")

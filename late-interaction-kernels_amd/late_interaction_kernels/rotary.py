@@ -45,7 +45,8 @@ def rotary_frequencies(
     - ``"yarn"`` (Peng et al., "YaRN: Efficient context window extension of large language
       models", 2023): the blend is linear in the pair's index, between the pairs that turn
       ``high`` (default 32, rounded down) and ``low`` (default 1, rounded up) times; the amplitude is
-      ``0.1 ln factor + 1``.
+      ``0.1 ln factor + 1``. As in the models that were trained so, and not in the paper, the last of them is at
+      most pair ``dim - 1``, and where both are one pair the blend takes 0.001 of an index.
 
     Returns:
         ``(frequencies, amplitude)``: fp64 ``[dim / 2]`` on ``device``, and 1.0 except for "yarn".
