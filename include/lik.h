@@ -584,7 +584,8 @@ int lik_attention_backward(const lik_attention_t* a, const void* out, const floa
  *   cu_seqlens[0] .. cu_seqlens[n] come out as zeros.
  * positions (32- or 64-bit integers, with strides; not with cu_seqlens): null counts from
  * offset at each sequence's start. frequencies [pairs] are 32- or 64-bit floats; the angle
- * is computed and reduced in 64 bits. q_out and k_out are contiguous.
+ * is computed and reduced in 64 bits. q_out and k_out are contiguous and overlap neither each
+ * other nor the inputs.
  */
 typedef struct {
   const void* q;
@@ -622,7 +623,8 @@ int lik_rotary(const lik_rotary_t* a, void* q_out, void* k_out, lik_stream_t str
  *   scale = max(fp32(max|x| / 127), 2^-126),  out = x / scale to the nearest integer, ties to even
  * (the rounding is that of the exact quotient). A row that holds an infinity or a NaN has the
  * scale NaN and zeros. out rows are out_stride bytes apart; bytes from dim to the next
- * multiple of 16 are written as zeros as far as out_stride has them.
+ * multiple of 16 are written as zeros as far as out_stride has them. Outputs do not overlap inputs
+ * (here and below).
  */
 int lik_quantize_int8(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int32_t dim, int8_t* out,
                       int64_t out_stride, float* scale, lik_stream_t stream);

@@ -291,6 +291,7 @@ int quantize_rows_int8(const void* x, int64_t x_stride, int32_t dtype, int64_t r
   if (!x || !out || !scale || out_stride < dim) return LIK_ERR_INVALID;
   const int eb = dtype == LIK_F32 ? 4 : 2;
   if ((uintptr_t)x % eb || (uintptr_t)scale % 4) return LIK_ERR_UNSUPPORTED;
+  if ((const void*)out == x) return LIK_ERR_INVALID;  // (a row's integers lie where others' elements do)
   const int64_t end = (dim + 15) / 16 * 16;
   const QuantP p{(const char*)x, x_stride * eb, rows, dim, (int)(end < out_stride ? end : out_stride), out, out_stride,
                  scale, stream};
@@ -320,6 +321,7 @@ int lik_dequantize_int8(const int8_t* x, int64_t x_stride, const float* scale, i
   if (rows == 0) return LIK_OK;
   if (!x || !out || !scale) return LIK_ERR_INVALID;
   if ((uintptr_t)out % (dtype == LIK_F32 ? 4 : 2) || (uintptr_t)scale % 4) return LIK_ERR_UNSUPPORTED;
+  if (out == (const void*)x) return LIK_ERR_INVALID;
   const DequantP p{x, x_stride, rows, scale, dim, (char*)out};
   hipStream_t s = (hipStream_t)stream;
   switch (dtype) {

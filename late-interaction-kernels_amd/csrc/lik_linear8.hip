@@ -998,6 +998,7 @@ int lik_linear_int8(const lik_linear_int8_t* a, void* out, void* workspace, size
   if (int8 && (a->in % 16 || a->x_stride % 16 || a->x_stride < 0 || 256 * a->x_stride >= kFar))
     return LIK_ERR_UNSUPPORTED;
   if (workspace_bytes < linear_ws(a) || (!workspace && linear_ws(a))) return LIK_ERR_WORKSPACE;
+  if (out == a->x || out == (const void*)a->weight) return LIK_ERR_INVALID;
   LinP p{};
   p.a = (const char*)a->x;
   p.a_ld = a->x_stride * (int8 ? 1 : xb);

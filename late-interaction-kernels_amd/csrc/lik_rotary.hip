@@ -186,6 +186,10 @@ extern "C" int lik_rotary(const lik_rotary_t* a, void* q_out, void* k_out, lik_s
       (uintptr_t)a->frequencies % (a->frequency_bits / 8) || (uintptr_t)a->cu_seqlens % 4 ||
       (a->positions && (uintptr_t)a->positions % (a->position_bits / 8)))
     return LIK_ERR_UNSUPPORTED;
+  // (elements near a chunk's end are read by two threads)
+  if ((heads && (q_out == a->q || q_out == a->k)) || (kv && (k_out == a->k || k_out == a->q)) ||
+      (heads && kv && q_out == k_out))
+    return LIK_ERR_INVALID;
   p.t[0] = {(const char*)a->q, (char*)q_out, a->q_stride_n * eb, a->q_stride_l * eb, a->q_stride_h * eb, heads};
   p.t[1] = {(const char*)a->k, (char*)k_out, a->k_stride_n * eb, a->k_stride_l * eb, a->k_stride_h * eb, kv};
   p.len = a->len;
