@@ -397,7 +397,7 @@ __device__ __forceinline__ void each(F f) {
 // The waits count: a step waits for its own loads only, with all younger loads and stores in flight. So every
 // store is issued whatever its lanes hold (a lane without an output names an offset out of range), and column
 // edges, which store element by element, wait for everything (44801 x 768 -> 2305 184 us). Two workgroups a CU with tiles of 256 x 128
-// instead fall into step and do not overlap. 44801 rows 768 -> 2304 fp16 99 to 103 us by box (256 x 128 tiles: 134), 1152 -> 768 with a
+// instead fall into step and do not overlap. 44801 rows 768 -> 2304 fp16 99 to 103 us by card (256 x 128 tiles: 134), 1152 -> 768 with a
 // residual 66 to 84 us by what is in the caches (98), 16480 rows 1024 -> 2 x 2816 with silu 112 to 116 us (125).
 template <int OK, bool GLU, bool RES, int TN, int DEF>
 __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) linear8_stream_kernel(const LinP p) {
